@@ -313,12 +313,119 @@ int nv4_qk_norm_rope_store(const void* qkv, const void* q_weight, const void* k_
                            void* k_cache, void* v_cache, int64_t tokens, int64_t num_heads, int64_t num_kv_heads,
                            int64_t head_dim, float eps, void* stream);
 
+/*
+ * The 4-bit KV cache: nv4_qk_norm_rope_store_kv4 writes it and
+ * nv4_paged_decode_attention_kv4 reads it (the counterparts of
+ * nv4_qk_norm_rope_store and nv4_paged_decode_attention; the reference keeps
+ * its cache in BF16 only).  For K and for V
+ *   codes   uint8 [pages, num_kv_heads, 256, 64]: two 4-bit codes a byte
+ *   scales  bf16  [pages, num_kv_heads, 256, 4]: one per 32 of the 128 channels
+ * With a the group's absolute maximum, the scale is s = bf16(a / 7) (1 for an
+ * all-zero group, at least the BF16 tiny; NaN when a value is not finite: the
+ * group then reads back as NaN) and the code of x is round-half-even(x / s)
+ * clamped to [-7, 7], held as code + 8; a value reads back as code * s.
+ * Four consecutive channels of a token are a 16-bit unit, the lowest channel in
+ * the lowest nibble.  With g = channel / 32 and r = channel % 32 a K unit lies
+ * at byte (r / 8) * 16 + g * 4 + (r % 8) / 4 * 2 of its token's 64 bytes, a V
+ * unit at byte ((r / 4) ^ (2 * (pair % 4))) * 16 + g * 4 + (token % 2) * 2 of
+ * the 128 bytes of its token pair (pair = token / 2).
+ *
+ * Store: per-head RMSNorm of q and k and rotary embedding of the fused QKV
+ * projection output, with one rounding at the end (BF16 for q, FP32 before the
+ * quantiser for k), K and V quantised into the cache rows slot_mapping[t].
+ *   qkv        bf16 [tokens, (num_heads + 2 * num_kv_heads) * 128]: q | k | v
+ *   cos_sin    float32 [max_position, 128]: cos in the first half, sin in the second
+ *   positions  int64 [tokens]; one outside [0, max_position) makes q and k NaN
+ *              and records error 8 (nv4_device_error)
+ *   slot_mapping int32 [tokens] or NULL (then no cache): < 0 stores nothing, a
+ *              slot beyond the cache stores nothing and records error 7; no slot may occur twice
+ *   q_out      bf16 [tokens, num_heads, 128]
+ *   k_out/v_out bf16 [tokens, num_kv_heads, 128] or NULL: the values that the
+ *              cache holds for the token (what a later read gives), for the
+ *              prefill's own attention
+ * All pointers 16-byte aligned (positions 8, slot_mapping 4).  head_dim == 128, page_size == 256.
+ */
+int nv4_qk_norm_rope_store_kv4(const void* qkv, const void* q_weight, const void* k_weight, const float* cos_sin,
+                               const int64_t* positions, const int32_t* slot_mapping, void* q_out, void* k_out,
+                               void* v_out, void* k_codes, void* k_scales, void* v_codes, void* v_scales,
+                               int64_t tokens, int64_t num_heads, int64_t num_kv_heads, int64_t head_dim,
+                               int64_t page_size, int64_t num_pages, int64_t max_position, double eps,
+                               void* stream);
+
+/*
+ * Decode attention over the 4-bit cache, one query token per sequence.
+ *   q, out        bf16 [batch, num_heads, 128]
+ *   block_tables  int32 [batch, max_pages]: page of each 256-token block; a page
+ *                 outside [0, num_pages) counts as absent and records error 6
+ *   context_lens  int32 [batch]: tokens of each sequence, the current one
+ *                 included; at most max_pages * 256 are read; 0 (or less) marks
+ *                 a padding row, whose output is zero
+ *   workspace     nv4_paged_attention_kv4_workspace_bytes(...) bytes of scratch;
+ *                 calls that may overlap need one each
+ * Grouped-query attention as nv4_paged_decode_attention (at most 8 query heads
+ * per KV head), scale > 0.  Statistics and sums in FP32, the products' operands
+ * in 16 bits.  All pointers 16-byte aligned (block_tables, context_lens 4).
+ */
+int64_t nv4_paged_attention_kv4_workspace_bytes(int64_t batch, int64_t num_heads, int64_t max_pages);
+int nv4_paged_decode_attention_kv4(const void* q, const void* k_codes, const void* k_scales, const void* v_codes,
+                                   const void* v_scales, const int32_t* block_tables, const int32_t* context_lens,
+                                   void* out, void* workspace, int64_t workspace_bytes, int64_t batch,
+                                   int64_t num_heads, int64_t num_kv_heads, int64_t head_dim, int64_t page_size,
+                                   int64_t num_pages, int64_t max_pages, float scale, void* stream);
+
+/*
+ * Step metadata of a batch from request lengths (the reference builds these
+ * lists on the host: nanovllm/engine/model_runner.py prepare_prefill /
+ * prepare_decode).  Request b has cached_lens[b] tokens in the cache and
+ * new_lens[b] to compute in this step, and owns the next
+ * ceil((cached + new) / page_size) entries of the flat list `pages`.
+ *   pages         int32 [num_listed]
+ *   block_tables  int32 [rows, max_pages]: the request's pages, then 0
+ *   context_lens  int32 [rows]: cached + new
+ *   query_starts  int32 [rows + 1]: first new token of each request; [batch] and beyond: their total
+ *   slot_mapping  int32 [tokens], positions int64 [tokens]: cache slot (page *
+ *                 page_size + offset) and position of every new token, in order;
+ *                 behind the last one slot -1 and position 0
+ * rows >= batch; rows behind the last request get context 0, pages 0.  Lengths
+ * below 0 count as 0.  A token whose page lies beyond `pages` or beyond
+ * max_pages, or is negative, gets slot -1, a table entry without a page 0, and
+ * error 6 is recorded; tokens beyond `tokens` are dropped.
+ * batch <= NV4_STEP_MAX_BATCH.  One launch, no workspace.
+ */
+#define NV4_STEP_MAX_BATCH 4096
+int nv4_step_tables(const int32_t* cached_lens, const int32_t* new_lens, const int32_t* pages,
+                    int32_t* block_tables, int32_t* context_lens, int32_t* query_starts, int32_t* slot_mapping,
+                    int64_t* positions, int64_t batch, int64_t rows, int64_t num_listed, int64_t tokens,
+                    int64_t max_pages, int64_t page_size, void* stream);
+
+/*
+ * Log-probabilities of given tokens (softmax over the vocabulary), their ranks,
+ * the entropy and the most likely alternatives.  The reference's sampler
+ * (nanovllm/layers/sampler.py) returns token ids only.
+ *   logits   bf16 (fp32 == 0) or float32 (fp32 == 1) [rows, vocab], rows row_stride elements apart
+ *   targets  int64 [rows]; one outside [0, vocab) is no token: logprob 0, rank 0
+ *   logprobs, entropy  float32 [rows] (natural logarithms)
+ *   ranks    int64 [rows]: 1 + the number of logits above the token's
+ *   top_logprobs float32, top_ids int64 [rows, top_k] (may be NULL when top_k is
+ *            0): by falling logit, ties to the lowest index.  A logit of -inf
+ *            (or NaN) is no alternative: where fewer than top_k are left, id -1 and -inf
+ * A row of nothing but -inf: logprob -inf, entropy 0.  A row that holds a NaN or
+ * +inf has no distribution: logprob, entropy and top_logprobs are NaN, ranks and
+ * ids go by the comparisons.  vocab <= NV4_LOGPROB_MAX_VOCAB, top_k <= NV4_LOGPROB_MAX_TOP.
+ */
+#define NV4_LOGPROB_MAX_VOCAB (1 << 24)
+#define NV4_LOGPROB_MAX_TOP 32
+int nv4_token_logprobs(const void* logits, int fp32, const int64_t* targets, float* logprobs, int64_t* ranks,
+                       float* entropy, float* top_logprobs, int64_t* top_ids, int64_t rows, int64_t vocab,
+                       int64_t row_stride, int64_t top_k, void* stream);
+
 /* Library metadata and error reporting. */
 int nv4_version(void);                      /* major*10000 + minor*100 + patch */
 const char* nv4_status_string(int status);  /* static string for a status code */
 int nv4_last_cuda_error(void);              /* cudaError_t of the last NV4_ERR_CUDA in this thread */
 /* Reads and clears the error word that bounded device-side waits set when they
- * give up (0 = none).  Synchronises the current device. */
+ * give up (1-5), and that the bounds checks on device-side indices set: 6 a page,
+ * 7 a cache slot, 8 a position (0 = none).  Synchronises the current device. */
 int nv4_device_error(int* code);
 
 #ifdef __cplusplus

@@ -447,5 +447,101 @@ int nv4_qk_norm_rope_store(const void* qkv, const void* q_weight, const void* k_
                                    v_cache, tokens, num_heads, num_kv_heads, eps, static_cast<cudaStream_t>(stream));
 }
 
+// ---- 4-bit KV cache, step tables, token log-probabilities
+int64_t nv4_paged_attention_kv4_workspace_bytes(int64_t batch, int64_t num_heads, int64_t max_pages) {
+  if (batch < 1 || num_heads < 1 || max_pages < 1) return 0;
+  return paged_attention_kv4_workspace_bytes(batch, num_heads, max_pages);
+}
+
+int nv4_paged_decode_attention_kv4(const void* q, const void* k_codes, const void* k_scales, const void* v_codes,
+                                   const void* v_scales, const int32_t* block_tables, const int32_t* context_lens,
+                                   void* out, void* workspace, int64_t workspace_bytes, int64_t batch,
+                                   int64_t num_heads, int64_t num_kv_heads, int64_t head_dim, int64_t page_size,
+                                   int64_t num_pages, int64_t max_pages, float scale, void* stream) {
+  if (!q || !k_codes || !k_scales || !v_codes || !v_scales || !block_tables || !context_lens || !out || !workspace)
+    return NV4_ERR_INVALID_ARGUMENT;
+  if (batch < 1 || batch > 65535 || num_kv_heads < 1 || num_kv_heads > 65535 || num_heads < num_kv_heads ||
+      num_heads % num_kv_heads || num_pages < 1 || num_pages > (int64_t(1) << 23) - 1 || max_pages < 1 ||
+      max_pages > 65535 || !(scale > 0.0f) || !(scale < 1e30f))
+    return NV4_ERR_INVALID_ARGUMENT;
+  if (head_dim != 128 || page_size != 256 || num_heads / num_kv_heads > 8) return NV4_ERR_UNSUPPORTED;
+  if (workspace_bytes < paged_attention_kv4_workspace_bytes(batch, num_heads, max_pages))
+    return NV4_ERR_INVALID_ARGUMENT;
+  if (!aligned(q, 16) || !aligned(k_codes, 16) || !aligned(k_scales, 16) || !aligned(v_codes, 16) ||
+      !aligned(v_scales, 16) || !aligned(out, 16) || !aligned(workspace, 16) || !aligned(block_tables, 4) ||
+      !aligned(context_lens, 4))
+    return NV4_ERR_ALIGNMENT;
+  if (!device_is_sm100()) return NV4_ERR_DEVICE;
+  return launch_paged_decode_attention_kv4(q, k_codes, k_scales, v_codes, v_scales, block_tables, context_lens, out,
+                                           workspace, batch, num_heads, num_kv_heads, num_pages, max_pages, scale,
+                                           static_cast<cudaStream_t>(stream));
+}
+
+int nv4_qk_norm_rope_store_kv4(const void* qkv, const void* q_weight, const void* k_weight, const float* cos_sin,
+                               const int64_t* positions, const int32_t* slot_mapping, void* q_out, void* k_out,
+                               void* v_out, void* k_codes, void* k_scales, void* v_codes, void* v_scales,
+                               int64_t tokens, int64_t num_heads, int64_t num_kv_heads, int64_t head_dim,
+                               int64_t page_size, int64_t num_pages, int64_t max_position, double eps,
+                               void* stream) {
+  if (!qkv || !q_weight || !k_weight || !cos_sin || !positions || !q_out) return NV4_ERR_INVALID_ARGUMENT;
+  const bool store = slot_mapping != nullptr;
+  if (store != (k_codes != nullptr) || store != (k_scales != nullptr) || store != (v_codes != nullptr) ||
+      store != (v_scales != nullptr) || (k_out != nullptr) != (v_out != nullptr))
+    return NV4_ERR_INVALID_ARGUMENT;
+  if (tokens < 1 || num_heads < 1 || num_kv_heads < 1 || tokens > (int64_t(1) << 31) - 1 ||
+      num_heads > 65535 || num_kv_heads > 65535 || tokens * (num_heads + 2 * num_kv_heads) > (int64_t(1) << 33) ||
+      max_position < 1 || !(eps >= 0.0) || !(eps < 1.0))
+    return NV4_ERR_INVALID_ARGUMENT;
+  if (store && (num_pages < 1 || num_pages > (int64_t(1) << 23) - 1)) return NV4_ERR_INVALID_ARGUMENT;
+  if (head_dim != 128 || (store && page_size != 256)) return NV4_ERR_UNSUPPORTED;
+  if (!aligned(qkv, 16) || !aligned(q_weight, 16) || !aligned(k_weight, 16) || !aligned(cos_sin, 16) ||
+      !aligned(positions, 8) || !aligned(slot_mapping, 4) || !aligned(q_out, 16) || !aligned(k_out, 16) ||
+      !aligned(v_out, 16) || !aligned(k_codes, 16) || !aligned(k_scales, 16) || !aligned(v_codes, 16) ||
+      !aligned(v_scales, 16))
+    return NV4_ERR_ALIGNMENT;
+  if (!device_is_sm100()) return NV4_ERR_DEVICE;
+  return launch_qk_norm_rope_store_kv4(qkv, q_weight, k_weight, cos_sin, positions, slot_mapping, q_out, k_out, v_out,
+                                       k_codes, k_scales, v_codes, v_scales, tokens, num_heads, num_kv_heads,
+                                       num_pages, max_position, eps, static_cast<cudaStream_t>(stream));
+}
+
+int nv4_step_tables(const int32_t* cached_lens, const int32_t* new_lens, const int32_t* pages,
+                    int32_t* block_tables, int32_t* context_lens, int32_t* query_starts, int32_t* slot_mapping,
+                    int64_t* positions, int64_t batch, int64_t rows, int64_t num_listed, int64_t tokens,
+                    int64_t max_pages, int64_t page_size, void* stream) {
+  if (!cached_lens || !new_lens || !block_tables || !context_lens || !query_starts || (num_listed && !pages) ||
+      (tokens && (!slot_mapping || !positions)))
+    return NV4_ERR_INVALID_ARGUMENT;
+  if (batch < 1 || rows < batch || rows > (int64_t(1) << 24) || num_listed < 0 || num_listed > (int64_t(1) << 30) ||
+      tokens < 0 || tokens > (int64_t(1) << 30) || max_pages < 1 || max_pages > (int64_t(1) << 24) || page_size < 1 ||
+      page_size > (int64_t(1) << 24))
+    return NV4_ERR_INVALID_ARGUMENT;
+  if (batch > NV4_STEP_MAX_BATCH) return NV4_ERR_UNSUPPORTED;
+  if (!aligned(cached_lens, 4) || !aligned(new_lens, 4) || !aligned(pages, 4) || !aligned(block_tables, 4) ||
+      !aligned(context_lens, 4) || !aligned(query_starts, 4) || !aligned(slot_mapping, 4) || !aligned(positions, 8))
+    return NV4_ERR_ALIGNMENT;
+  if (!device_is_sm100()) return NV4_ERR_DEVICE;
+  return launch_step_tables(cached_lens, new_lens, pages, block_tables, context_lens, query_starts, slot_mapping,
+                            positions, batch, rows, num_listed, tokens, max_pages, page_size,
+                            static_cast<cudaStream_t>(stream));
+}
+
+int nv4_token_logprobs(const void* logits, int fp32, const int64_t* targets, float* logprobs, int64_t* ranks,
+                       float* entropy, float* top_logprobs, int64_t* top_ids, int64_t rows, int64_t vocab,
+                       int64_t row_stride, int64_t top_k, void* stream) {
+  if (!logits || !targets || !logprobs || !ranks || !entropy || (fp32 != 0 && fp32 != 1))
+    return NV4_ERR_INVALID_ARGUMENT;
+  if (rows < 1 || rows > (int64_t(1) << 31) - 1 || vocab < 1 || row_stride < (rows > 1 ? vocab : 0) || top_k < 0 ||
+      (top_k > 0 && (!top_logprobs || !top_ids)))
+    return NV4_ERR_INVALID_ARGUMENT;
+  if (vocab > NV4_LOGPROB_MAX_VOCAB || top_k > NV4_LOGPROB_MAX_TOP) return NV4_ERR_UNSUPPORTED;
+  if (!aligned(logits, fp32 ? 4 : 2) || !aligned(targets, 8) || !aligned(logprobs, 4) || !aligned(ranks, 8) ||
+      !aligned(entropy, 4) || !aligned(top_logprobs, 4) || !aligned(top_ids, 8))
+    return NV4_ERR_ALIGNMENT;
+  if (!device_is_sm100()) return NV4_ERR_DEVICE;
+  return launch_token_logprobs(logits, fp32, targets, logprobs, ranks, entropy, top_logprobs, top_ids, rows, vocab,
+                               row_stride, top_k, static_cast<cudaStream_t>(stream));
+}
+
 }  // extern "C"
 #pragma GCC visibility pop

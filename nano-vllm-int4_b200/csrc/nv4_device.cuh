@@ -29,13 +29,18 @@ constexpr float kBf16Tiny = 0x1.0p-126f;
 constexpr int kMagicBits = 0x4B400000;
 constexpr float kMagic = 12582912.0f;
 
-// Error words written by bounded waits (one per device, read/cleared by host).
+// Error words written by bounded waits and by the bounds checks on indices read
+// from device memory (one per device, read/cleared by host).
 enum DeviceError : int {
   kErrNone = 0,
   kErrTimeoutFull = 1,      // consumer waited too long for a loaded stage
   kErrTimeoutEmpty = 2,     // producer waited too long for a free stage
   kErrTimeoutMma = 3,       // tensor-core pipeline wait timed out
   kErrTimeoutDrain = 4,     // wait for in-flight copies at exit timed out
+                            // (5: a peer rank, see peer_common.cuh)
+  kErrBadPage = 6,          // a page index outside the cache, or more pages needed than listed
+  kErrBadSlot = 7,          // a cache slot outside the cache
+  kErrBadPosition = 8,      // a position outside the rotary table
 };
 
 // Defined here: the library is one translation unit (nv4_unity.cu).

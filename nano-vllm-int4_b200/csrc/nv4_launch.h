@@ -96,6 +96,27 @@ int launch_qk_norm_rope_store(const void* qkv, const void* q_weight, const void*
                               const int64_t* positions, const int* slot_mapping, void* q_out, void* k_out,
                               void* k_cache, void* v_cache, int64_t tokens, int64_t num_heads, int64_t num_kv_heads,
                               float eps, cudaStream_t stream);
+// The 4-bit KV cache (kv4_cache.cu).
+int64_t paged_attention_kv4_workspace_bytes(int64_t batch, int64_t num_heads, int64_t max_pages);
+int launch_paged_decode_attention_kv4(const void* q, const void* k_codes, const void* k_scales, const void* v_codes,
+                                      const void* v_scales, const int* block_tables, const int* context_lens,
+                                      void* out, void* workspace, int64_t batch, int64_t num_heads,
+                                      int64_t num_kv_heads, int64_t num_pages, int64_t max_pages, float scale,
+                                      cudaStream_t stream);
+int launch_qk_norm_rope_store_kv4(const void* qkv, const void* q_weight, const void* k_weight, const float* cos_sin,
+                                  const int64_t* positions, const int* slot_mapping, void* q_out, void* k_out,
+                                  void* v_out, void* k_codes, void* k_scales, void* v_codes, void* v_scales,
+                                  int64_t tokens, int64_t num_heads, int64_t num_kv_heads, int64_t num_pages,
+                                  int64_t max_position, double eps, cudaStream_t stream);
+// Step metadata from request lengths (step_tables.cu).
+int launch_step_tables(const int* cached, const int* fresh, const int* pages, int* block_tables, int* context_lens,
+                       int* query_starts, int* slot_mapping, int64_t* positions, int64_t batch, int64_t rows,
+                       int64_t num_listed, int64_t tokens, int64_t max_pages, int64_t page_size,
+                       cudaStream_t stream);
+// Token log-probabilities (token_logprobs.cu).
+int launch_token_logprobs(const void* logits, int fp32, const int64_t* targets, float* logprobs, int64_t* ranks,
+                          float* entropy, float* top_logprobs, int64_t* top_ids, int64_t rows, int64_t vocab,
+                          int64_t row_stride, int64_t top_k, cudaStream_t stream);
 // Peer mode of the stream GEMM (row-parallel layers): the launcher fills in the
 // tile geometry the matching tile reduce needs.
 // Launch plan of the decode stream GEMM (w4a4_gemm.cu); the C ABI exports it

@@ -38,7 +38,9 @@ EXPORTS = ("nv4_rht_quant_pack", "nv4_rht_quant_i8", "nv4_w4a4_grouped_gemm", "n
            "nv4_peer_buffer_open", "nv4_peer_buffer_close", "nv4_peer_buffer_free", "nv4_peer_allreduce_bf16",
            "nv4_w4a4_gemm_peer_allreduce_bf16", "nv4_silu_mul_rht_quant_i8",
            "nv4_add_rmsnorm_rht_quant_i8", "nv4_w4a4_stream_plan", "nv4_paged_attention_workspace_bytes",
-           "nv4_paged_decode_attention", "nv4_qk_norm_rope_store", "nv4_w4a16_plan")
+           "nv4_paged_decode_attention", "nv4_qk_norm_rope_store", "nv4_w4a16_plan",
+           "nv4_qk_norm_rope_store_kv4", "nv4_paged_attention_kv4_workspace_bytes",
+           "nv4_paged_decode_attention_kv4", "nv4_step_tables", "nv4_token_logprobs")
 
 
 class NativeLibraryError(RuntimeError):
@@ -132,6 +134,16 @@ def load(path: str | None = None) -> ctypes.CDLL:
         lib.nv4_qk_norm_rope_store.argtypes = [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64,
                                                _i64, ctypes.c_float, _vp]
         lib.nv4_qk_norm_rope_store.restype = _int
+        lib.nv4_qk_norm_rope_store_kv4.argtypes = [_vp] * 13 + [_i64] * 7 + [ctypes.c_double, _vp]
+        lib.nv4_qk_norm_rope_store_kv4.restype = _int
+        lib.nv4_paged_attention_kv4_workspace_bytes.argtypes = [_i64, _i64, _i64]
+        lib.nv4_paged_attention_kv4_workspace_bytes.restype = _i64
+        lib.nv4_paged_decode_attention_kv4.argtypes = [_vp] * 9 + [_i64] * 8 + [ctypes.c_float, _vp]
+        lib.nv4_paged_decode_attention_kv4.restype = _int
+        lib.nv4_step_tables.argtypes = [_vp] * 8 + [_i64] * 6 + [_vp]
+        lib.nv4_step_tables.restype = _int
+        lib.nv4_token_logprobs.argtypes = [_vp, _int] + [_vp] * 6 + [_i64] * 4 + [_vp]
+        lib.nv4_token_logprobs.restype = _int
         lib.nv4_status_string.argtypes = [_int]
         lib.nv4_status_string.restype = ctypes.c_char_p
         lib.nv4_device_error.argtypes = [ctypes.POINTER(_int)]
@@ -383,3 +395,60 @@ def qk_norm_rope_store(qkv, q_weight, k_weight, cos_sin, positions, slot_mapping
                                             opt(slot_mapping), ptr(q_out), opt(k_out), opt(k_cache), opt(v_cache), t,
                                             num_heads, num_kv_heads, q_out.shape[-1], float(eps), stream_of(qkv)),
               "nv4_qk_norm_rope_store")
+
+
+# ---------------------------------------------------------------- 4-bit KV cache, step tables, log-probabilities
+def _addr(t) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+def paged_attention_kv4_workspace_bytes(batch: int, num_heads: int, max_pages: int) -> int:
+    return int(load().nv4_paged_attention_kv4_workspace_bytes(batch, num_heads, max_pages))
+
+
+def paged_decode_attention_kv4(q, k_codes, k_scales, v_codes, v_scales, block_tables, context_lens, out, workspace,
+                               scale: float) -> None:
+    """nv4_paged_decode_attention_kv4: q, out [B, Hq, 128], codes [pages, Hkv, 256, 64], scales [pages, Hkv, 256, 4]."""
+    b, hq, d = q.shape
+    pages, hkv, page_size = k_codes.shape[:3]
+    with torch.cuda.device(q.device):
+        check(load().nv4_paged_decode_attention_kv4(
+            q.data_ptr(), k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr(),
+            block_tables.data_ptr(), context_lens.data_ptr(), out.data_ptr(), workspace.data_ptr(),
+            workspace.numel() * workspace.element_size(), b, hq, hkv, d, page_size, pages, block_tables.shape[1],
+            scale, stream_of(q)), "nv4_paged_decode_attention_kv4")
+
+
+def qk_norm_rope_store_kv4(qkv, q_weight, k_weight, cos_sin, positions, slot_mapping, q_out, k_out, v_out, k_codes,
+                           k_scales, v_codes, v_scales, num_heads: int, num_kv_heads: int, eps: float) -> None:
+    """nv4_qk_norm_rope_store_kv4 (k_out with v_out, and slot_mapping with the four cache tensors, may be None)."""
+    pages, page_size = (k_codes.shape[0], k_codes.shape[2]) if k_codes is not None else (0, 256)
+    with torch.cuda.device(qkv.device):
+        check(load().nv4_qk_norm_rope_store_kv4(
+            qkv.data_ptr(), q_weight.data_ptr(), k_weight.data_ptr(), cos_sin.data_ptr(), positions.data_ptr(),
+            _addr(slot_mapping), q_out.data_ptr(), _addr(k_out), _addr(v_out), _addr(k_codes), _addr(k_scales),
+            _addr(v_codes), _addr(v_scales), qkv.shape[0], num_heads, num_kv_heads, q_out.shape[-1], page_size, pages,
+            cos_sin.shape[0], eps, stream_of(qkv)), "nv4_qk_norm_rope_store_kv4")
+
+
+def step_tables(cached_lens, new_lens, pages, block_tables, context_lens, query_starts, slot_mapping, positions,
+                page_size: int) -> None:
+    """nv4_step_tables; the outputs' shapes give rows, max_pages and tokens."""
+    rows, max_pages = block_tables.shape
+    with torch.cuda.device(cached_lens.device):
+        check(load().nv4_step_tables(
+            cached_lens.data_ptr(), new_lens.data_ptr(), pages.data_ptr(), block_tables.data_ptr(),
+            context_lens.data_ptr(), query_starts.data_ptr(), slot_mapping.data_ptr(), positions.data_ptr(),
+            cached_lens.shape[0], rows, pages.shape[0], slot_mapping.shape[0], max_pages, page_size,
+            stream_of(cached_lens)), "nv4_step_tables")
+
+
+def token_logprobs(logits, targets, logprobs, ranks, entropy, top_logprobs, top_ids) -> None:
+    """nv4_token_logprobs (top_logprobs and top_ids None: no alternatives)."""
+    rows, vocab = logits.shape
+    top_k = 0 if top_ids is None else top_ids.shape[1]
+    with torch.cuda.device(logits.device):
+        check(load().nv4_token_logprobs(
+            logits.data_ptr(), 1 if logits.dtype == torch.float32 else 0, targets.data_ptr(), logprobs.data_ptr(),
+            ranks.data_ptr(), entropy.data_ptr(), _addr(top_logprobs), _addr(top_ids), rows, vocab, logits.stride(0),
+            top_k, stream_of(logits)), "nv4_token_logprobs")
