@@ -202,11 +202,48 @@ int launch_qk_norm_rope_store_kv4(const void* qkv, const void* q_weight, const v
 }
 
 // ------------------------------------------------------------ decode attention
-// One CTA per (page of the context, KV head, sequence), a warp per token: a
-// lane holds four channels of q for every query head of the group, the dot
-// products are summed over the warp, and each warp keeps its own running
-// maximum, sum and output, merged at the end of the page into a partial that a
-// second kernel joins.
+// o[h] = sum_t softmax_t(scale q[h].k_t) v_t over a sequence's tokens, for the G
+// query heads that share a KV head.  Per token and KV head 144 bytes are read
+// and 256 codes widened; at HBM rate an SM has about 6 cycles for that, so the
+// work per code is what the kernel is arranged around.
+//
+// Split: the tokens of all (sequence, KV head) jobs form one line of 128-token
+// units, cut evenly over a fixed grid (two CTAs an SM), so ragged lengths cost
+// nothing.  The lengths live on the device: every CTA makes the prefix sum
+// itself.  A job that lies within one CTA is finished there; else each CTA
+// writes an unnormalised partial to the workspace (two slots a CTA: the job
+// that it continues, the job that it leaves) and a second kernel joins them in
+// order.  A producer warp copies units into a ring with bulk copies (a unit of
+// a page is contiguous), eight consumer warps take 16 tokens of each.
+//
+// Arithmetic, per 16 tokens and warp, on mma.sync m16n8k16:
+//   S^T [16 tokens x 8 heads]: A = K codes widened to BF16, B = q.  A nibble u
+//     becomes 128 + u with one mask-and-or (u is in the low mantissa bits of
+//     128); the excess 136 = 128 + 8 over the code c = u - 8 leaves through
+//     the accumulator's start -136 sum(q), so K needs no subtraction.  The
+//     scale is one per token and 32 channels: two MMAs, then one FMA.
+//   O^T [128 channels x 8 heads]: A = V codes (c exactly, BF16), B = p * scale,
+//     rounded to BF16: the probability's only rounding.  Accumulated over the
+//     whole context, so here the excess is subtracted before the product.
+// p reaches its B fragment with movmatrix.  The running maximum is moved only
+// when a score exceeds it by 2^8 (p and its sum are at most 2^8 larger then).
+constexpr int kKv4Warps = 8;
+constexpr int kKv4Threads = (kKv4Warps + 1) * 32;
+constexpr int kKv4Unit = kKv4Warps * 16;  // tokens of a unit; divides the page
+constexpr int kKv4Stages = 4;
+constexpr int kKv4CodeBytes = kKv4Unit * kKv4RowBytes;       // of K or V, a unit
+constexpr int kKv4ScaleBytes = kKv4Unit * kKv4Groups * 2;
+constexpr int kKv4QBytes = kKv4MaxGroup * kKv4D * 2;
+constexpr int kKv4StageBytes = 2 * kKv4CodeBytes + 2 * kKv4ScaleBytes + kKv4QBytes;
+constexpr int kKv4RedStride = kKv4D + 4;  // floats; conflict-free stores of the fragments
+constexpr int kKv4RedBytes = kKv4Warps * kKv4MaxGroup * kKv4RedStride * 4;
+constexpr int kKv4Smem = kKv4Stages * kKv4StageBytes + kKv4RedBytes;
+constexpr int kKv4CtasPerSm = 2;
+constexpr int kKv4MaxCtas = 2 * 160;
+constexpr int kKv4SlotFloats = kKv4MaxGroup * (kKv4D + 2);  // a partial: outputs, then (max, sum) per head
+constexpr float kKv4NoMax = -1e30f;
+constexpr float kKv4Slack = 8.0f;  // log2 units by which a score may pass the running maximum
+
 struct Kv4AttnArgs {
   const uint16_t* q;  // [B, Hq, 128]
   const uint8_t* k_codes;
@@ -215,109 +252,410 @@ struct Kv4AttnArgs {
   const uint16_t* v_scales;
   const int* block_tables;  // [B, max_pages]
   const int* context_lens;
-  float* o_part;   // [B, Hq, max_pages, 128]
-  float* ml_part;  // [B, Hq, max_pages, 2]
+  uint16_t* out;
+  float* partials;   // [2 * CTAs][kKv4SlotFloats]
+  int64_t* starts;   // [B + 1]: first unit of each sequence, per KV head
   int64_t num_pages;
-  int Hq, Hkv, max_pages;
+  int B, Hq, Hkv, max_pages;
   float scale_log2;
 };
 
-__global__ void __launch_bounds__(128) paged_decode_attention_kv4_kernel(const Kv4AttnArgs p) {
-  __shared__ float red[4][kKv4MaxGroup][kKv4D];
-  __shared__ float ml[4][kKv4MaxGroup][2];
-  const int pi = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
-  const int ctx = p.context_lens[b];
-  if (pi * kKv4Page >= ctx) return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+struct Kv4Meta {  // of a unit in the ring
+  int job;     // b * Hkv + h
+  int tokens;  // valid tokens, 0 for an absent page
+  int first;   // first unit of the job in this CTA
+  int last;    // 0, or 1 + where the result goes: 1 the output, 2 / 3 partial slot 0 / 1
+};
+
+__device__ __forceinline__ int kv4_context(const Kv4AttnArgs& p, int b) {
+  return min(max(p.context_lens[b], 0), p.max_pages * kKv4Page);
+}
+__device__ __forceinline__ int kv4_units(int ctx) { return (ctx + kKv4Unit - 1) / kKv4Unit; }
+
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Transpose of an 8x8 matrix of 16-bit elements held as mma fragments.
+__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+__device__ __forceinline__ void mma_bf16_from(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                              uint32_t b0, uint32_t b1, float c0, float c1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%10, %11, %10, %11};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
+}
+__device__ __forceinline__ void mma_bf16_acc(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                             uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Nibble i of both halves of w as BF16: 128 + u.
+template <int I>
+__device__ __forceinline__ uint32_t nibbles_plus128(uint32_t w) {
+  return ((w >> (4 * I)) & 0x000F000Fu) | 0x43004300u;
+}
+// The same as codes: (128 + u) - 136, exact in BF16.
+template <int I>
+__device__ __forceinline__ uint32_t nibbles_code(uint32_t w) {
+  const uint32_t v = nibbles_plus128<I>(w);
+  __nv_bfloat162 x = *reinterpret_cast<const __nv_bfloat162*>(&v);
+  x = __hsub2(x, __floats2bfloat162_rn(136.0f, 136.0f));
+  return *reinterpret_cast<uint32_t*>(&x);
+}
+
+// First unit of CTA i of n over `total` units.
+__device__ __forceinline__ int64_t kv4_cut(int64_t total, int i, int n) { return total * i / n; }
+
+__global__ void __launch_bounds__(kKv4Threads, kKv4CtasPerSm) paged_decode_attention_kv4_kernel(const Kv4AttnArgs p) {
+  extern __shared__ __align__(128) uint8_t smem_kv4[];
+  __shared__ uint64_t full[kKv4Stages], empty[kKv4Stages], red_full, red_free;
+  __shared__ Kv4Meta meta[kKv4Stages];
+  __shared__ int64_t sums[kKv4Threads / 32];
+  __shared__ int64_t start_of_b;
+  __shared__ int start_b;
+  __shared__ float red_ml[kKv4Warps][kKv4MaxGroup][2];
+  float* red = reinterpret_cast<float*>(smem_kv4 + kKv4Stages * kKv4StageBytes);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int G = p.Hq / p.Hkv;
-  int ntok = min(kKv4Page, ctx - pi * kKv4Page);
-  const int page = p.block_tables[static_cast<int64_t>(b) * p.max_pages + pi];
-  if (page < 0 || page >= p.num_pages) {  // its tokens count as absent
-    if (threadIdx.x == 0) record_error(kErrBadPage);
-    ntok = 0;
-  }
-  const int64_t tile = static_cast<int64_t>(page) * p.Hkv + kvh;
-  const uint8_t* kc = p.k_codes + tile * (kKv4Page * kKv4RowBytes);
-  const uint8_t* vc = p.v_codes + tile * (kKv4Page * kKv4RowBytes);
-  const uint16_t* ks = p.k_scales + tile * (kKv4Page * kKv4Groups);
-  const uint16_t* vs = p.v_scales + tile * (kKv4Page * kKv4Groups);
-  float q[kKv4MaxGroup][4], o[kKv4MaxGroup][4], m[kKv4MaxGroup], l[kKv4MaxGroup];
-#pragma unroll
-  for (int h = 0; h < kKv4MaxGroup; ++h) {
-    m[h] = -1e30f;
-    l[h] = 0.0f;
-    const uint2 raw = h < G ? *reinterpret_cast<const uint2*>(
-                                  p.q + (static_cast<int64_t>(b) * p.Hq + kvh * G + h) * kKv4D + lane * 4)
-                            : make_uint2(0, 0);
-    q[h][0] = bf16lo_to_f32(raw.x), q[h][1] = bf16hi_to_f32(raw.x);
-    q[h][2] = bf16lo_to_f32(raw.y), q[h][3] = bf16hi_to_f32(raw.y);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o[h][i] = 0.0f;
-  }
-  for (int t = warp; t < ntok; t += 4) {
-    const uint32_t ku = *reinterpret_cast<const uint16_t*>(kc + t * kKv4RowBytes + kv4_k_unit(lane));
-    const uint32_t vu = *reinterpret_cast<const uint16_t*>(vc + kv4_v_unit(t, lane));
-    const float ksc = bf16_bits_to_f32(ks[t * kKv4Groups + (lane >> 3)]);
-    const float vsc = bf16_bits_to_f32(vs[t * kKv4Groups + (lane >> 3)]);
-    float k[4], v[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      k[i] = ksc * static_cast<float>(static_cast<int>((ku >> (4 * i)) & 15) - 8);
-      v[i] = vsc * static_cast<float>(static_cast<int>((vu >> (4 * i)) & 15) - 8);
+
+  if (tid == 0) {
+    for (int i = 0; i < kKv4Stages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], kKv4Warps);
     }
-#pragma unroll
-    for (int h = 0; h < kKv4MaxGroup; ++h) {
-      if (h >= G) break;
-      float s = q[h][0] * k[0] + q[h][1] * k[1] + q[h][2] * k[2] + q[h][3] * k[3];
-#pragma unroll
-      for (int x = 16; x >= 1; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-      s *= p.scale_log2;
-      const float mn = fmaxf(m[h], s), alpha = exp2f(m[h] - mn), e = exp2f(s - mn);
-      m[h] = mn;
-      l[h] = l[h] * alpha + e;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[h][i] = o[h][i] * alpha + e * v[i];
-    }
+    mbar_init(&red_full, kKv4Warps);
+    mbar_init(&red_free, kKv4Warps);
+    fence_mbar_init();
   }
+  // Units of all sequences, and the sequence of this CTA's first unit: each
+  // thread takes a run of sequences.
+  const int per = (p.B + kKv4Threads - 1) / kKv4Threads;
+  const int b_lo = min(tid * per, p.B), b_hi = min(b_lo + per, p.B);
+  int64_t mine = 0;
+  for (int b = b_lo; b < b_hi; ++b) mine += kv4_units(kv4_context(p, b));
+  int64_t incl = mine;
 #pragma unroll
-  for (int h = 0; h < kKv4MaxGroup; ++h) {
-    if (h >= G) break;
-    *reinterpret_cast<float4*>(&red[warp][h][lane * 4]) = make_float4(o[h][0], o[h][1], o[h][2], o[h][3]);
-    if (lane == 0) ml[warp][h][0] = m[h], ml[warp][h][1] = l[h];
+  for (int m = 1; m < 32; m <<= 1) {
+    const int64_t o = __shfl_up_sync(0xffffffffu, incl, m);
+    if (lane >= m) incl += o;
+  }
+  if (lane == 31) sums[warp] = incl;
+  __syncthreads();
+  int64_t total = 0, before = 0;
+  for (int w = 0; w < kKv4Threads / 32; ++w) {
+    if (w < warp) before += sums[w];
+    total += sums[w];
+  }
+  const int ctas = static_cast<int>(min(total * p.Hkv, static_cast<int64_t>(gridDim.x)));  // a unit each at least
+  const bool working = static_cast<int>(blockIdx.x) < ctas;
+  const int64_t u0 = working ? kv4_cut(total * p.Hkv, blockIdx.x, ctas) : -1;
+  const int64_t u1 = working ? kv4_cut(total * p.Hkv, blockIdx.x + 1, ctas) : -1;
+  {
+    int64_t at = before + incl - mine;
+    for (int b = b_lo; b < b_hi; ++b) {
+      const int n = kv4_units(kv4_context(p, b));
+      if (u0 >= at * p.Hkv && u0 < (at + n) * p.Hkv) start_b = b, start_of_b = at;
+      if (blockIdx.x == 0) p.starts[b] = at;
+      at += n;
+    }
+    if (blockIdx.x == 0 && tid == 0) p.starts[p.B] = total;
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < G * kKv4D; i += 128) {
-    const int h = i / kKv4D, d = i % kKv4D;
-    float M = -1e30f, L = 0.0f, acc = 0.0f;
-    for (int w = 0; w < 4; ++w) M = fmaxf(M, ml[w][h][0]);
-    for (int w = 0; w < 4; ++w) {
-      const float f = exp2f(ml[w][h][0] - M);
-      acc += f * red[w][h][d];
-      L += f * ml[w][h][1];
+  grid_dependents_launch();
+  if (!working) return;
+
+  if (warp == kKv4Warps) {  // ---- producer
+    int b = start_b;
+    int64_t rest = u0 - start_of_b * p.Hkv;  // units into this sequence
+    int ctx = kv4_context(p, b), n = kv4_units(ctx);
+    int h = static_cast<int>(rest / n), k = static_cast<int>(rest - static_cast<int64_t>(h) * n);
+    int ids_b = -1, ids_first = 0, ids = 0;  // page ids held by the lanes
+    bool ok = true;
+    int64_t issued = 0;
+    for (int64_t u = u0; u < u1; ++u, ++issued) {
+      const int pi = k / (kKv4Page / kKv4Unit);
+      if (b != ids_b || pi < ids_first || pi >= ids_first + 32) {
+        ids_b = b, ids_first = pi & ~31;
+        const int at = ids_first + lane;
+        ids = at < p.max_pages ? p.block_tables[static_cast<int64_t>(b) * p.max_pages + at] : 0;
+      }
+      const int page = __shfl_sync(0xffffffffu, ids, pi - ids_first);
+      const int st = static_cast<int>(issued % kKv4Stages);
+      if (issued >= kKv4Stages) {
+        ok = mbar_wait(&empty[st], static_cast<uint32_t>(issued / kKv4Stages - 1) & 1, kErrTimeoutEmpty);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+      }
+      if (lane == 0) {
+        int tokens = min(kKv4Unit, ctx - k * kKv4Unit);
+        const bool first = u == u0 || k == 0, last = u + 1 == u1 || k + 1 == n;
+        const bool whole = k + 1 == n && u - k >= u0;  // the job began and ends in this CTA
+        if (page < 0 || page >= p.num_pages) {
+          record_error(kErrBadPage);
+          tokens = 0;
+        }
+        meta[st].job = b * p.Hkv + h;
+        meta[st].tokens = tokens;
+        meta[st].first = first;
+        meta[st].last = !last ? 0 : whole ? 1 : u - k <= u0 ? 2 : 3;
+        const uint32_t rows = (tokens + 15) & ~15;
+        const uint32_t q_bytes = first ? G * kKv4D * 2 : 0;
+        mbar_arrive_expect_tx(&full[st], rows * (2 * kKv4RowBytes + 4 * kKv4Groups) + q_bytes);
+        uint8_t* dst = smem_kv4 + st * kKv4StageBytes;
+        if (q_bytes)
+          bulk_load(dst + 2 * kKv4CodeBytes + 2 * kKv4ScaleBytes,
+                    p.q + (static_cast<int64_t>(b) * p.Hq + h * G) * kKv4D, q_bytes, &full[st]);
+        if (rows) {
+          const int64_t row = (static_cast<int64_t>(page) * p.Hkv + h) * kKv4Page +
+                              (k % (kKv4Page / kKv4Unit)) * kKv4Unit;
+          bulk_load(dst, p.k_codes + row * kKv4RowBytes, rows * kKv4RowBytes, &full[st]);
+          bulk_load(dst + 2 * kKv4CodeBytes, p.k_scales + row * kKv4Groups, rows * kKv4Groups * 2, &full[st]);
+          bulk_load(dst + kKv4CodeBytes, p.v_codes + row * kKv4RowBytes, rows * kKv4RowBytes, &full[st]);
+          bulk_load(dst + 2 * kKv4CodeBytes + kKv4ScaleBytes, p.v_scales + row * kKv4Groups, rows * kKv4Groups * 2,
+                    &full[st]);
+        }
+      }
+      if (++k == n) {
+        k = 0;
+        if (++h == p.Hkv) {
+          h = 0;
+          if (u + 1 < u1) {
+            do {
+              ctx = kv4_context(p, ++b);
+              n = kv4_units(ctx);
+            } while (n == 0);
+          }
+        }
+      }
     }
-    const int64_t part = (static_cast<int64_t>(b) * p.Hq + kvh * G + h) * p.max_pages + pi;
-    p.o_part[part * kKv4D + d] = acc;
-    if (d == 0) p.ml_part[part * 2] = M, p.ml_part[part * 2 + 1] = L;
+    // The CTA's shared memory must outlive its copies.
+    if (!ok)
+      for (int64_t i = issued > kKv4Stages ? issued - kKv4Stages : 0; i < issued; ++i)
+        mbar_wait(&full[i % kKv4Stages], static_cast<uint32_t>(i / kKv4Stages) & 1, kErrTimeoutDrain);
+    return;
+  }
+
+  // ---- consumers
+  const int gid = lane >> 2, tig = lane & 3;
+  uint32_t qb[4][4];     // B fragments of q: group, then nibble order
+  float start[4][2];     // -136 sum of q over a group, of heads 2 tig and 2 tig + 1
+  float o[8][4];
+  float m[2], l[2], top[2];  // running maximum (log2 units), sum, score limit of this maximum
+  uint32_t merges = 0;
+  const int64_t units = u1 - u0;
+  for (int64_t it = 0; it < units; ++it) {
+    const int st = static_cast<int>(it % kKv4Stages);
+    if (!mbar_wait(&full[st], static_cast<uint32_t>(it / kKv4Stages) & 1, kErrTimeoutFull)) return;
+    const uint8_t* buf = smem_kv4 + st * kKv4StageBytes;
+    const Kv4Meta mt = meta[st];
+    if (mt.first) {
+      const uint16_t* qs = reinterpret_cast<const uint16_t*>(buf + 2 * kKv4CodeBytes + 2 * kKv4ScaleBytes);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint4 w = make_uint4(0, 0, 0, 0);
+        if (gid < G) w = *reinterpret_cast<const uint4*>(qs + gid * kKv4D + j * 32 + tig * 8);
+        qb[j][0] = __byte_perm(w.x, w.z, 0x5410);  // channels (0, 4), (1, 5), (2, 6), (3, 7)
+        qb[j][1] = __byte_perm(w.x, w.z, 0x7632);
+        qb[j][2] = __byte_perm(w.y, w.w, 0x5410);
+        qb[j][3] = __byte_perm(w.y, w.w, 0x7632);
+        float s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s += bf16lo_to_f32(qb[j][i]) + bf16hi_to_f32(qb[j][i]);
+        s += __shfl_xor_sync(0xffffffffu, s, 1);
+        s += __shfl_xor_sync(0xffffffffu, s, 2);
+        start[j][0] = -136.0f * __shfl_sync(0xffffffffu, s, 8 * tig);
+        start[j][1] = -136.0f * __shfl_sync(0xffffffffu, s, 8 * tig + 4);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[i][e] = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) m[e] = kKv4NoMax, l[e] = 0.0f, top[e] = kKv4NoMax;
+    }
+    const int t0 = warp * 16;
+    if (t0 < mt.tokens) {
+      // scores of tokens t0 + gid (s[0], s[1]: heads 2 tig, 2 tig + 1) and t0 + gid + 8 (s[2], s[3])
+      const uint4 ka = *reinterpret_cast<const uint4*>(buf + (t0 + gid) * kKv4RowBytes + tig * 16);
+      const uint4 kb = *reinterpret_cast<const uint4*>(buf + (t0 + gid + 8) * kKv4RowBytes + tig * 16);
+      const uint2 sa = *reinterpret_cast<const uint2*>(buf + 2 * kKv4CodeBytes + (t0 + gid) * 8);
+      const uint2 sb = *reinterpret_cast<const uint2*>(buf + 2 * kKv4CodeBytes + (t0 + gid + 8) * 8);
+      const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
+      const float fa[4] = {bf16lo_to_f32(sa.x), bf16hi_to_f32(sa.x), bf16lo_to_f32(sa.y), bf16hi_to_f32(sa.y)};
+      const float fb[4] = {bf16lo_to_f32(sb.x), bf16hi_to_f32(sb.x), bf16lo_to_f32(sb.y), bf16hi_to_f32(sb.y)};
+      float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float acc[4];
+        mma_bf16_from(acc, nibbles_plus128<0>(wa[j]), nibbles_plus128<0>(wb[j]), nibbles_plus128<1>(wa[j]),
+                      nibbles_plus128<1>(wb[j]), qb[j][0], qb[j][1], start[j][0], start[j][1]);
+        mma_bf16_acc(acc, nibbles_plus128<2>(wa[j]), nibbles_plus128<2>(wb[j]), nibbles_plus128<3>(wa[j]),
+                     nibbles_plus128<3>(wb[j]), qb[j][2], qb[j][3]);
+        s[0] = fmaf(fa[j], acc[0], s[0]);
+        s[1] = fmaf(fa[j], acc[1], s[1]);
+        s[2] = fmaf(fb[j], acc[2], s[2]);
+        s[3] = fmaf(fb[j], acc[3], s[3]);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[e] *= p.scale_log2;
+      const uint2 ua = *reinterpret_cast<const uint2*>(buf + 2 * kKv4CodeBytes + kKv4ScaleBytes + (t0 + gid) * 8);
+      const uint2 ub = *reinterpret_cast<const uint2*>(buf + 2 * kKv4CodeBytes + kKv4ScaleBytes + (t0 + gid + 8) * 8);
+      float ga[4] = {bf16lo_to_f32(ua.x), bf16hi_to_f32(ua.x), bf16lo_to_f32(ua.y), bf16hi_to_f32(ua.y)};
+      float gb[4] = {bf16lo_to_f32(ub.x), bf16hi_to_f32(ub.x), bf16lo_to_f32(ub.y), bf16hi_to_f32(ub.y)};
+      if (t0 + 16 > mt.tokens) {  // rows behind the last token hold anything, NaN scales among it
+        if (t0 + gid >= mt.tokens) {
+          s[0] = s[1] = -INFINITY;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) ga[j] = 0.0f;
+        }
+        if (t0 + gid + 8 >= mt.tokens) {
+          s[2] = s[3] = -INFINITY;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) gb[j] = 0.0f;
+        }
+      }
+      const bool above = s[0] > top[0] || s[2] > top[0] || s[1] > top[1] || s[3] > top[1];
+      if (__any_sync(0xffffffffu, above)) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float mx = fmaxf(fmaxf(s[e], s[e + 2]), m[e]);
+#pragma unroll
+          for (int x = 4; x <= 16; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+          const float alpha = ex2(m[e] - mx);
+          m[e] = mx;
+          top[e] = mx + kKv4Slack;
+          l[e] *= alpha;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) o[i][e] *= alpha, o[i][e + 2] *= alpha;
+        }
+      }
+      float pr[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) pr[e] = ex2(s[e] - m[e & 1]);
+      l[0] += pr[0] + pr[2];
+      l[1] += pr[1] + pr[3];
+      const uint4 va = *reinterpret_cast<const uint4*>(buf + kKv4CodeBytes + (t0 / 2 + tig) * 128 +
+                                                       ((gid ^ (2 * tig)) * 16));
+      const uint4 vb = *reinterpret_cast<const uint4*>(buf + kKv4CodeBytes + (t0 / 2 + 4 + tig) * 128 +
+                                                       ((gid ^ (2 * tig)) * 16));
+      const uint32_t xa[4] = {va.x, va.y, va.z, va.w}, xb[4] = {vb.x, vb.y, vb.z, vb.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t b0 = movmatrix_trans(pack_bf16x2(pr[0] * ga[j], pr[1] * ga[j]));
+        const uint32_t b1 = movmatrix_trans(pack_bf16x2(pr[2] * gb[j], pr[3] * gb[j]));
+        mma_bf16_acc(o[2 * j], nibbles_code<0>(xa[j]), nibbles_code<1>(xa[j]), nibbles_code<0>(xb[j]),
+                     nibbles_code<1>(xb[j]), b0, b1);
+        mma_bf16_acc(o[2 * j + 1], nibbles_code<2>(xa[j]), nibbles_code<3>(xa[j]), nibbles_code<2>(xb[j]),
+                     nibbles_code<3>(xb[j]), b0, b1);
+      }
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&empty[st]);
+
+    if (mt.last) {  // join the warps
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int x = 4; x <= 16; x <<= 1) l[e] += __shfl_xor_sync(0xffffffffu, l[e], x);
+      if (merges > 0 && !mbar_wait(&red_free, (merges - 1) & 1, kErrTimeoutEmpty)) return;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int head = 2 * tig + e;
+        if (head < G) {
+          float* dst = red + (warp * kKv4MaxGroup + head) * kKv4RedStride + gid * 4;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            *reinterpret_cast<float4*>(dst + 32 * j) =
+                make_float4(o[2 * j][e], o[2 * j][e + 2], o[2 * j + 1][e], o[2 * j + 1][e + 2]);
+          if (gid == 0) red_ml[warp][head][0] = m[e], red_ml[warp][head][1] = l[e];
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&red_full);
+      if (!mbar_wait(&red_full, merges & 1, kErrTimeoutFull)) return;
+      const int b = mt.job / p.Hkv, h0 = (mt.job - b * p.Hkv) * G;
+      float* slot = p.partials + (2 * static_cast<int64_t>(blockIdx.x) + (mt.last == 3)) * kKv4SlotFloats;
+      for (int i = tid; i < G * kKv4D; i += kKv4Warps * 32) {
+        const int head = i / kKv4D, d = i % kKv4D;
+        float M = kKv4NoMax, L = 0.0f, acc = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kKv4Warps; ++w) M = fmaxf(M, red_ml[w][head][0]);
+#pragma unroll
+        for (int w = 0; w < kKv4Warps; ++w) {
+          const float f = ex2(red_ml[w][head][0] - M);
+          L = fmaf(f, red_ml[w][head][1], L);
+          acc = fmaf(f, red[(w * kKv4MaxGroup + head) * kKv4RedStride + d], acc);
+        }
+        if (mt.last == 1) {
+          p.out[(static_cast<int64_t>(b) * p.Hq + h0 + head) * kKv4D + d] =
+              __bfloat16_as_ushort(__float2bfloat16_rn(L == 0.0f ? 0.0f : acc / L));
+        } else {
+          slot[i] = acc;
+          if (d == 0) slot[kKv4MaxGroup * kKv4D + 2 * head] = M, slot[kKv4MaxGroup * kKv4D + 2 * head + 1] = L;
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&red_free);
+      ++merges;
+    }
   }
 }
 
-__global__ void __launch_bounds__(128) kv4_merge_kernel(const Kv4AttnArgs p, uint16_t* __restrict__ out) {
-  const int64_t bh = blockIdx.x;
-  const int b = static_cast<int>(bh / p.Hq), d = threadIdx.x;
-  const int np = min(p.max_pages, (max(p.context_lens[b], 0) + kKv4Page - 1) / kKv4Page);
-  const int64_t base = bh * p.max_pages;
-  float M = -1e30f, L = 0.0f, acc = 0.0f;
-  for (int i = 0; i < np; ++i) M = fmaxf(M, p.ml_part[(base + i) * 2]);
-  for (int i = 0; i < np; ++i) {
-    const float f = exp2f(p.ml_part[(base + i) * 2] - M);
-    acc += f * p.o_part[(base + i) * kKv4D + d];
-    L += f * p.ml_part[(base + i) * 2 + 1];
+// Joins the partials of the jobs that several CTAs hold, in CTA order, and
+// writes the zeros of empty sequences.  One CTA per job.
+__global__ void __launch_bounds__(kKv4D) kv4_merge_kernel(const Kv4AttnArgs p, int grid) {
+  const int job = blockIdx.x, b = job / p.Hkv, G = p.Hq / p.Hkv, d = threadIdx.x;
+  grid_dependency_wait();
+  const int64_t first = p.starts[b], n = p.starts[b + 1] - first, total = p.starts[p.B] * p.Hkv;
+  uint16_t* out = p.out + (static_cast<int64_t>(b) * p.Hq + (job - b * p.Hkv) * G) * kKv4D + d;
+  const int ctas = static_cast<int>(min(total, static_cast<int64_t>(grid)));
+  if (n == 0) {
+    for (int g = 0; g < G; ++g) out[g * kKv4D] = 0;
+    return;
   }
-  out[bh * kKv4D + d] = __bfloat16_as_ushort(__float2bfloat16_rn(L == 0.0f ? 0.0f : acc / L));
+  const int64_t a = first * p.Hkv + (job - b * p.Hkv) * n, e = a + n;
+  // the CTA of a unit u is the largest i whose cut is at or before it
+  const int c0 = static_cast<int>(((a + 1) * ctas + total - 1) / total) - 1;
+  const int c1 = static_cast<int>((e * ctas + total - 1) / total) - 1;
+  if (c0 == c1) return;
+  // c0 holds its part in slot 0 when the job is the first of its units, the others always do
+  const float* s0 = p.partials + (2 * static_cast<int64_t>(c0) + (kv4_cut(total, c0, ctas) < a)) * kKv4SlotFloats;
+  for (int g = 0; g < G; ++g) {
+    const int ml = kKv4MaxGroup * kKv4D + 2 * g;
+    float M = s0[ml];
+    for (int c = c0 + 1; c <= c1; ++c) M = fmaxf(M, p.partials[2 * static_cast<int64_t>(c) * kKv4SlotFloats + ml]);
+    float f = ex2(s0[ml] - M), L = f * s0[ml + 1], acc = f * s0[g * kKv4D + d];
+#pragma unroll 4
+    for (int c = c0 + 1; c <= c1; ++c) {
+      const float* s = p.partials + 2 * static_cast<int64_t>(c) * kKv4SlotFloats;
+      f = ex2(s[ml] - M);
+      L = fmaf(f, s[ml + 1], L);
+      acc = fmaf(f, s[g * kKv4D + d], acc);
+    }
+    out[g * kKv4D] = __bfloat16_as_ushort(__float2bfloat16_rn(L == 0.0f ? 0.0f : acc / L));
+  }
 }
 
+static int64_t kv4_starts_bytes(int64_t batch) { return (batch + 1) * 8 + 15 & ~int64_t(15); }
+static int64_t kv4_max_ctas(int64_t batch, int64_t num_heads, int64_t max_pages) {
+  return std::min<int64_t>(kKv4MaxCtas, batch * num_heads * max_pages * (kKv4Page / kKv4Unit));
+}
 int64_t paged_attention_kv4_workspace_bytes(int64_t batch, int64_t num_heads, int64_t max_pages) {
-  return batch * num_heads * max_pages * (kKv4D + 2) * 4;
+  return kv4_starts_bytes(batch) + kv4_max_ctas(batch, num_heads, max_pages) * 2 * kKv4SlotFloats * 4;
 }
 
 int launch_paged_decode_attention_kv4(const void* q, const void* k_codes, const void* k_scales, const void* v_codes,
@@ -325,6 +663,9 @@ int launch_paged_decode_attention_kv4(const void* q, const void* k_codes, const 
                                       void* out, void* workspace, int64_t batch, int64_t num_heads,
                                       int64_t num_kv_heads, int64_t num_pages, int64_t max_pages, float scale,
                                       cudaStream_t stream) {
+  static int done[64] = {};
+  int rc = ensure_smem_attr(reinterpret_cast<const void*>(&paged_decode_attention_kv4_kernel), kKv4Smem, done);
+  if (rc != NV4_OK) return rc;
   Kv4AttnArgs a;
   a.q = static_cast<const uint16_t*>(q);
   a.k_codes = static_cast<const uint8_t*>(k_codes);
@@ -333,19 +674,22 @@ int launch_paged_decode_attention_kv4(const void* q, const void* k_codes, const 
   a.v_scales = static_cast<const uint16_t*>(v_scales);
   a.block_tables = block_tables;
   a.context_lens = context_lens;
-  a.o_part = static_cast<float*>(workspace);
-  a.ml_part = a.o_part + batch * num_heads * max_pages * kKv4D;
+  a.out = static_cast<uint16_t*>(out);
+  a.starts = static_cast<int64_t*>(workspace);
+  a.partials = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kv4_starts_bytes(batch));
   a.num_pages = num_pages;
+  a.B = static_cast<int>(batch);
   a.Hq = static_cast<int>(num_heads);
   a.Hkv = static_cast<int>(num_kv_heads);
   a.max_pages = static_cast<int>(max_pages);
   a.scale_log2 = scale * 1.4426950408889634f;
-  const dim3 grid(static_cast<unsigned>(max_pages), static_cast<unsigned>(num_kv_heads),
-                  static_cast<unsigned>(batch));
-  const int rc = launch_kernel(paged_decode_attention_kv4_kernel, grid, dim3(128), 0, stream, false, a);
+  // no more CTAs than there can be units
+  const int ctas = static_cast<int>(std::min<int64_t>(
+      kv4_max_ctas(batch, num_kv_heads, max_pages), kKv4CtasPerSm * static_cast<int64_t>(device_sm_count())));
+  rc = launch_kernel(paged_decode_attention_kv4_kernel, dim3(ctas), dim3(kKv4Threads), kKv4Smem, stream, false, a);
   if (rc != NV4_OK) return rc;
-  return launch_kernel(kv4_merge_kernel, dim3(static_cast<unsigned>(batch * num_heads)), dim3(kKv4D), 0, stream,
-                       false, a, static_cast<uint16_t*>(out));
+  return launch_kernel(kv4_merge_kernel, dim3(static_cast<unsigned>(batch * num_kv_heads)), dim3(kKv4D), 0, stream,
+                       true, a, ctas);
 }
 
 }  // namespace nv4
