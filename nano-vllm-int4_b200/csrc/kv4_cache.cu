@@ -227,10 +227,10 @@ int launch_qk_norm_rope_store_kv4(const void* qkv, const void* q_weight, const v
 //     whole context, so here the excess is subtracted before the product.
 // p reaches its B fragment with movmatrix.  The running maximum is moved only
 // when a score exceeds it by 2^8 (p and its sum are at most 2^8 larger then).
-constexpr int kKv4Warps = 8;
+constexpr int kKv4Warps = 4;
 constexpr int kKv4Threads = (kKv4Warps + 1) * 32;
 constexpr int kKv4Unit = kKv4Warps * 16;  // tokens of a unit; divides the page
-constexpr int kKv4Stages = 4;
+constexpr int kKv4Stages = 5;
 constexpr int kKv4CodeBytes = kKv4Unit * kKv4RowBytes;       // of K or V, a unit
 constexpr int kKv4ScaleBytes = kKv4Unit * kKv4Groups * 2;
 constexpr int kKv4QBytes = kKv4MaxGroup * kKv4D * 2;
@@ -238,8 +238,8 @@ constexpr int kKv4StageBytes = 2 * kKv4CodeBytes + 2 * kKv4ScaleBytes + kKv4QByt
 constexpr int kKv4RedStride = kKv4D + 4;  // floats; conflict-free stores of the fragments
 constexpr int kKv4RedBytes = kKv4Warps * kKv4MaxGroup * kKv4RedStride * 4;
 constexpr int kKv4Smem = kKv4Stages * kKv4StageBytes + kKv4RedBytes;
-constexpr int kKv4CtasPerSm = 2;
-constexpr int kKv4MaxCtas = 2 * 160;
+constexpr int kKv4CtasPerSm = 3;
+constexpr int kKv4MaxCtas = 3 * 160;
 constexpr int kKv4SlotFloats = kKv4MaxGroup * (kKv4D + 2);  // a partial: outputs, then (max, sum) per head
 constexpr float kKv4NoMax = -1e30f;
 constexpr float kKv4Slack = 8.0f;  // log2 units by which a score may pass the running maximum
