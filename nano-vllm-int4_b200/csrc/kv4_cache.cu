@@ -216,33 +216,36 @@ int launch_qk_norm_rope_store_kv4(const void* qkv, const void* q_weight, const v
 // order.  A producer warp copies units into a ring with bulk copies (a unit of
 // a page is contiguous), eight consumer warps take 16 tokens of each.
 //
-// Arithmetic, per 16 tokens and warp, on mma.sync m16n8k16:
-//   S^T [16 tokens x 8 heads]: A = K codes widened to BF16, B = q.  A nibble u
-//     becomes 128 + u with one mask-and-or (u is in the low mantissa bits of
-//     128); the excess 136 = 128 + 8 over the code c = u - 8 leaves through
-//     the accumulator's start -136 sum(q), so K needs no subtraction.  The
-//     scale is one per token and 32 channels: two MMAs, then one FMA.
-//   O^T [128 channels x 8 heads]: A = V codes (c exactly, BF16), B = p * scale,
-//     rounded to BF16: the probability's only rounding.  Accumulated over the
-//     whole context, so here the excess is subtracted before the product.
+// Arithmetic, per 16 tokens and warp, on mma.sync:
+//   S^T [16 tokens x 8 heads], m16n8k16 in BF16: A = K codes as 128 + u (the nibble
+//     u = c + 8 in the low mantissa bits of 128: one mask-and-or), B = q. The
+//     excess of 136 leaves through the accumulator's start, -136 sum(q), so K needs no
+//     subtraction. The scale is one per token and 32 channels: two MMAs, one FMA.
+//   O^T [128 channels x 8 heads], likewise: A = V codes, exactly (accumulated over
+//     the whole context, so the excess is subtracted first), B = p * scale,
+//     rounded to BF16: the probability's only rounding.
 // p reaches its B fragment with movmatrix.  The running maximum is moved only
 // when a score exceeds it by 2^8 (p and its sum are at most 2^8 larger then).
 constexpr int kKv4Warps = 4;
 constexpr int kKv4Threads = (kKv4Warps + 1) * 32;
-constexpr int kKv4Unit = kKv4Warps * 16;  // tokens of a unit; divides the page
-constexpr int kKv4Stages = 5;
+constexpr int kKv4Tiles = 2;                          // 16-token tiles a warp takes of a unit
+constexpr int kKv4Unit = kKv4Warps * kKv4Tiles * 16;  // tokens of a unit; divides the page
+constexpr int kKv4Stages = 2;  // what four CTAs an SM leave room for
 constexpr int kKv4CodeBytes = kKv4Unit * kKv4RowBytes;       // of K or V, a unit
 constexpr int kKv4ScaleBytes = kKv4Unit * kKv4Groups * 2;
-constexpr int kKv4QBytes = kKv4MaxGroup * kKv4D * 2;
-constexpr int kKv4StageBytes = 2 * kKv4CodeBytes + 2 * kKv4ScaleBytes + kKv4QBytes;
 constexpr int kKv4RedStride = kKv4D + 4;  // floats; conflict-free stores of the fragments
-constexpr int kKv4RedBytes = kKv4Warps * kKv4MaxGroup * kKv4RedStride * 4;
-constexpr int kKv4Smem = kKv4Stages * kKv4StageBytes + kKv4RedBytes;
-constexpr int kKv4CtasPerSm = 3;
-constexpr int kKv4MaxCtas = 3 * 160;
+constexpr int kKv4CtasPerSm = 4;
+constexpr int kKv4MaxCtas = kKv4CtasPerSm * 160;
 constexpr int kKv4SlotFloats = kKv4MaxGroup * (kKv4D + 2);  // a partial: outputs, then (max, sum) per head
 constexpr float kKv4NoMax = -1e30f;
 constexpr float kKv4Slack = 8.0f;  // log2 units by which a score may pass the running maximum
+
+// Shared memory: the stages (K, V, K scales, V scales, q), then the warps' outputs
+// of four heads at a time.
+constexpr int kKv4QAt = 2 * kKv4CodeBytes + 2 * kKv4ScaleBytes;
+constexpr int kKv4StageBytes = kKv4QAt + kKv4MaxGroup * kKv4D * 2;
+constexpr int kKv4RedAt = kKv4Stages * kKv4StageBytes;
+constexpr int kKv4Smem = kKv4RedAt + kKv4Warps * 4 * kKv4RedStride * 4;
 
 struct Kv4AttnArgs {
   const uint16_t* q;  // [B, Hq, 128]
@@ -303,15 +306,19 @@ __device__ __forceinline__ void mma_bf16_acc(float (&d)[4], uint32_t a0, uint32_
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// Nibble i of both halves of w as BF16: 128 + u.
+// Nibble I of both halves of w as BF16: 128 + u. magic = 0x43004300 (128, 128),
+// in a register that the compiler does not know: with two constants it makes two
+// logic operations of (w & mask) | magic.
 template <int I>
-__device__ __forceinline__ uint32_t nibbles_plus128(uint32_t w) {
-  return ((w >> (4 * I)) & 0x000F000Fu) | 0x43004300u;
+__device__ __forceinline__ uint32_t nibbles_plus128(uint32_t w, uint32_t magic) {
+  uint32_t v;
+  asm("lop3.b32 %0, %1, 0x000F000F, %2, 0xEA;" : "=r"(v) : "r"(w >> (4 * I)), "r"(magic));
+  return v;
 }
-// The same as codes: (128 + u) - 136, exact in BF16.
+// The same as codes: (128 + u) - 136, exact.
 template <int I>
-__device__ __forceinline__ uint32_t nibbles_code(uint32_t w) {
-  const uint32_t v = nibbles_plus128<I>(w);
+__device__ __forceinline__ uint32_t nibbles_code(uint32_t w, uint32_t magic) {
+  const uint32_t v = nibbles_plus128<I>(w, magic);
   __nv_bfloat162 x = *reinterpret_cast<const __nv_bfloat162*>(&v);
   x = __hsub2(x, __floats2bfloat162_rn(136.0f, 136.0f));
   return *reinterpret_cast<uint32_t*>(&x);
@@ -327,12 +334,14 @@ __global__ void __launch_bounds__(kKv4Threads, kKv4CtasPerSm) paged_decode_atten
   __shared__ int64_t sums[kKv4Threads / 32];
   __shared__ int64_t start_of_b;
   __shared__ int start_b;
+  __shared__ uint32_t magic_word;
   __shared__ float red_ml[kKv4Warps][kKv4MaxGroup][2];
-  float* red = reinterpret_cast<float*>(smem_kv4 + kKv4Stages * kKv4StageBytes);
+  float* red = reinterpret_cast<float*>(smem_kv4 + kKv4RedAt);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int G = p.Hq / p.Hkv;
 
   if (tid == 0) {
+    magic_word = 0x43004300u;
     for (int i = 0; i < kKv4Stages; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], kKv4Warps);
@@ -378,92 +387,103 @@ __global__ void __launch_bounds__(kKv4Threads, kKv4CtasPerSm) paged_decode_atten
   grid_dependents_launch();
   if (!working) return;
 
-  if (warp == kKv4Warps) {  // ---- producer
+  if (warp == kKv4Warps) {  // ---- producer: one thread
+    if (lane != 0) return;
+    constexpr int kPerPage = kKv4Page / kKv4Unit;
     int b = start_b;
-    int64_t rest = u0 - start_of_b * p.Hkv;  // units into this sequence
+    const int64_t rest = u0 - start_of_b * p.Hkv;  // units into this sequence
     int ctx = kv4_context(p, b), n = kv4_units(ctx);
     int h = static_cast<int>(rest / n), k = static_cast<int>(rest - static_cast<int64_t>(h) * n);
-    int ids_b = -1, ids_first = 0, ids = 0;  // page ids held by the lanes
+    const int* table = p.block_tables + static_cast<int64_t>(b) * p.max_pages;
+    int next = table[k / kPerPage];  // the page of the next unit that begins one
+    bool first = true;         // of the job in this CTA
+    bool begun = k == 0;       // the job began in this CTA
+    bool there = true;         // the page exists
     bool ok = true;
-    int64_t issued = 0;
-    for (int64_t u = u0; u < u1; ++u, ++issued) {
-      const int pi = k / (kKv4Page / kKv4Unit);
-      if (b != ids_b || pi < ids_first || pi >= ids_first + 32) {
-        ids_b = b, ids_first = pi & ~31;
-        const int at = ids_first + lane;
-        ids = at < p.max_pages ? p.block_tables[static_cast<int64_t>(b) * p.max_pages + at] : 0;
+    int st = 0, filled = 0;    // ring position; stages filled so far, at most kKv4Stages
+    uint32_t round = 0;        // parity of the ring's current round
+    const uint8_t *kc = nullptr, *vc = nullptr, *ks = nullptr, *vs = nullptr;
+    for (int64_t left = u1 - u0; left > 0; --left) {
+      if (first || k % kPerPage == 0) {
+        const int page = next;
+        there = page >= 0 && page < p.num_pages;
+        if (!there) record_error(kErrBadPage);
+        const int64_t row = (static_cast<int64_t>(page) * p.Hkv + h) * kKv4Page + (k % kPerPage) * kKv4Unit;
+        kc = p.k_codes + row * kKv4RowBytes;
+        vc = p.v_codes + row * kKv4RowBytes;
+        ks = reinterpret_cast<const uint8_t*>(p.k_scales + row * kKv4Groups);
+        vs = reinterpret_cast<const uint8_t*>(p.v_scales + row * kKv4Groups);
+        // the page after it, of this job or the first of the next head's
+        const int pi = k / kPerPage + 1;
+        next = table[pi * kPerPage < n ? pi : 0];
       }
-      const int page = __shfl_sync(0xffffffffu, ids, pi - ids_first);
-      const int st = static_cast<int>(issued % kKv4Stages);
-      if (issued >= kKv4Stages) {
-        ok = mbar_wait(&empty[st], static_cast<uint32_t>(issued / kKv4Stages - 1) & 1, kErrTimeoutEmpty);
-        ok = __all_sync(0xffffffffu, ok);
+      if (filled == kKv4Stages) {
+        ok = mbar_wait(&empty[st], round ^ 1, kErrTimeoutEmpty);
         if (!ok) break;
+      } else {
+        ++filled;
       }
-      if (lane == 0) {
-        int tokens = min(kKv4Unit, ctx - k * kKv4Unit);
-        const bool first = u == u0 || k == 0, last = u + 1 == u1 || k + 1 == n;
-        const bool whole = k + 1 == n && u - k >= u0;  // the job began and ends in this CTA
-        if (page < 0 || page >= p.num_pages) {
-          record_error(kErrBadPage);
-          tokens = 0;
-        }
-        meta[st].job = b * p.Hkv + h;
-        meta[st].tokens = tokens;
-        meta[st].first = first;
-        meta[st].last = !last ? 0 : whole ? 1 : u - k <= u0 ? 2 : 3;
-        const uint32_t rows = (tokens + 15) & ~15;
-        const uint32_t q_bytes = first ? G * kKv4D * 2 : 0;
-        mbar_arrive_expect_tx(&full[st], rows * (2 * kKv4RowBytes + 4 * kKv4Groups) + q_bytes);
-        uint8_t* dst = smem_kv4 + st * kKv4StageBytes;
-        if (q_bytes)
-          bulk_load(dst + 2 * kKv4CodeBytes + 2 * kKv4ScaleBytes,
-                    p.q + (static_cast<int64_t>(b) * p.Hq + h * G) * kKv4D, q_bytes, &full[st]);
-        if (rows) {
-          const int64_t row = (static_cast<int64_t>(page) * p.Hkv + h) * kKv4Page +
-                              (k % (kKv4Page / kKv4Unit)) * kKv4Unit;
-          bulk_load(dst, p.k_codes + row * kKv4RowBytes, rows * kKv4RowBytes, &full[st]);
-          bulk_load(dst + 2 * kKv4CodeBytes, p.k_scales + row * kKv4Groups, rows * kKv4Groups * 2, &full[st]);
-          bulk_load(dst + kKv4CodeBytes, p.v_codes + row * kKv4RowBytes, rows * kKv4RowBytes, &full[st]);
-          bulk_load(dst + 2 * kKv4CodeBytes + kKv4ScaleBytes, p.v_scales + row * kKv4Groups, rows * kKv4Groups * 2,
-                    &full[st]);
-        }
+      const int tokens = there ? min(kKv4Unit, ctx - k * kKv4Unit) : 0;
+      const bool ends = k + 1 == n, last = left == 1 || ends;
+      Kv4Meta mt;
+      mt.job = b * p.Hkv + h;
+      mt.tokens = tokens;
+      mt.first = first;
+      // the slot of a job that goes on from the CTA before is 0, as is that of one that begins with the CTA
+      mt.last = !last ? 0 : begun && ends ? 1 : begun && u1 - left - k > u0 ? 3 : 2;
+      meta[st] = mt;
+      const uint32_t rows = (tokens + 15) & ~15;
+      const uint32_t q_bytes = first ? G * kKv4D * 2 : 0;
+      mbar_arrive_expect_tx(&full[st], rows * (2 * kKv4RowBytes + 4 * kKv4Groups) + q_bytes);
+      uint8_t* dst = smem_kv4 + st * kKv4StageBytes;
+      if (first) bulk_load(dst + kKv4QAt, p.q + (static_cast<int64_t>(b) * p.Hq + h * G) * kKv4D, q_bytes, &full[st]);
+      if (rows) {
+        bulk_load(dst, kc, rows * kKv4RowBytes, &full[st]);
+        bulk_load(dst + 2 * kKv4CodeBytes, ks, rows * kKv4Groups * 2, &full[st]);
+        bulk_load(dst + kKv4CodeBytes, vc, rows * kKv4RowBytes, &full[st]);
+        bulk_load(dst + 2 * kKv4CodeBytes + kKv4ScaleBytes, vs, rows * kKv4Groups * 2, &full[st]);
       }
+      kc += kKv4CodeBytes, vc += kKv4CodeBytes, ks += kKv4ScaleBytes, vs += kKv4ScaleBytes;
+      if (++st == kKv4Stages) st = 0, round ^= 1;
+      first = false;
       if (++k == n) {
-        k = 0;
+        k = 0, first = begun = true;
         if (++h == p.Hkv) {
           h = 0;
-          if (u + 1 < u1) {
+          if (left > 1) {
             do {
               ctx = kv4_context(p, ++b);
               n = kv4_units(ctx);
             } while (n == 0);
+            table = p.block_tables + static_cast<int64_t>(b) * p.max_pages;
+            next = table[0];
           }
         }
       }
     }
     // The CTA's shared memory must outlive its copies.
-    if (!ok)
-      for (int64_t i = issued > kKv4Stages ? issued - kKv4Stages : 0; i < issued; ++i)
-        mbar_wait(&full[i % kKv4Stages], static_cast<uint32_t>(i / kKv4Stages) & 1, kErrTimeoutDrain);
+    if (!ok)  // stages at and behind st were last filled in the round before
+      for (int i = 0; i < filled; ++i) mbar_wait(&full[i], i < st ? round : round ^ 1, kErrTimeoutDrain);
     return;
   }
 
   // ---- consumers
+  uint32_t magic;
+  asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(magic) : "r"(smem_u32(&magic_word)));
   const int gid = lane >> 2, tig = lane & 3;
-  uint32_t qb[4][4];     // B fragments of q: group, then nibble order
-  float start[4][2];     // -136 sum of q over a group, of heads 2 tig and 2 tig + 1
+  uint32_t qb[4][4];         // B fragments of q, per 32 channels
+  float start[4][2];         // -136 sum of q over 32 channels, of heads 2 tig and 2 tig + 1
   float o[8][4];
   float m[2], l[2], top[2];  // running maximum (log2 units), sum, score limit of this maximum
   uint32_t merges = 0;
-  const int64_t units = u1 - u0;
-  for (int64_t it = 0; it < units; ++it) {
-    const int st = static_cast<int>(it % kKv4Stages);
-    if (!mbar_wait(&full[st], static_cast<uint32_t>(it / kKv4Stages) & 1, kErrTimeoutFull)) return;
+  int st = 0;
+  uint32_t round = 0;
+  for (int64_t left = u1 - u0; left > 0; --left) {
+    if (!mbar_wait(&full[st], round, kErrTimeoutFull)) return;
     const uint8_t* buf = smem_kv4 + st * kKv4StageBytes;
     const Kv4Meta mt = meta[st];
     if (mt.first) {
-      const uint16_t* qs = reinterpret_cast<const uint16_t*>(buf + 2 * kKv4CodeBytes + 2 * kKv4ScaleBytes);
+      const uint16_t* qs = reinterpret_cast<const uint16_t*>(buf + kKv4QAt);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         uint4 w = make_uint4(0, 0, 0, 0);
@@ -472,28 +492,29 @@ __global__ void __launch_bounds__(kKv4Threads, kKv4CtasPerSm) paged_decode_atten
         qb[j][1] = __byte_perm(w.x, w.z, 0x7632);
         qb[j][2] = __byte_perm(w.y, w.w, 0x5410);
         qb[j][3] = __byte_perm(w.y, w.w, 0x7632);
-        float s = 0.0f;
+        float sum = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s += bf16lo_to_f32(qb[j][i]) + bf16hi_to_f32(qb[j][i]);
-        s += __shfl_xor_sync(0xffffffffu, s, 1);
-        s += __shfl_xor_sync(0xffffffffu, s, 2);
-        start[j][0] = -136.0f * __shfl_sync(0xffffffffu, s, 8 * tig);
-        start[j][1] = -136.0f * __shfl_sync(0xffffffffu, s, 8 * tig + 4);
+        for (int i = 0; i < 4; ++i) sum += bf16lo_to_f32(qb[j][i]) + bf16hi_to_f32(qb[j][i]);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        start[j][0] = -136.0f * __shfl_sync(0xffffffffu, sum, 8 * tig);
+        start[j][1] = -136.0f * __shfl_sync(0xffffffffu, sum, 8 * tig + 4);
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[i][e] = 0.0f;
+        for (int x = 0; x < 4; ++x) o[i][x] = 0.0f;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) m[e] = kKv4NoMax, l[e] = 0.0f, top[e] = kKv4NoMax;
+      for (int x = 0; x < 2; ++x) m[x] = kKv4NoMax, l[x] = 0.0f, top[x] = kKv4NoMax;
     }
-    const int t0 = warp * 16;
-    if (t0 < mt.tokens) {
-      // scores of tokens t0 + gid (s[0], s[1]: heads 2 tig, 2 tig + 1) and t0 + gid + 8 (s[2], s[3])
-      const uint4 ka = *reinterpret_cast<const uint4*>(buf + (t0 + gid) * kKv4RowBytes + tig * 16);
-      const uint4 kb = *reinterpret_cast<const uint4*>(buf + (t0 + gid + 8) * kKv4RowBytes + tig * 16);
-      const uint2 sa = *reinterpret_cast<const uint2*>(buf + 2 * kKv4CodeBytes + (t0 + gid) * 8);
-      const uint2 sb = *reinterpret_cast<const uint2*>(buf + 2 * kKv4CodeBytes + (t0 + gid + 8) * 8);
+    // tiles warp, warp + 4, ...: a short unit is spread over all warps
+#pragma unroll 1
+    for (int t = warp * 16; t < mt.tokens; t += kKv4Warps * 16) {
+      // scores of tokens t + gid (s[0], s[1]: heads 2 tig, 2 tig + 1) and t + gid + 8 (s[2], s[3])
+      const uint4 ka = *reinterpret_cast<const uint4*>(buf + (t + gid) * kKv4RowBytes + tig * 16);
+      const uint4 kb = *reinterpret_cast<const uint4*>(buf + (t + gid + 8) * kKv4RowBytes + tig * 16);
+      const uint2 sa = *reinterpret_cast<const uint2*>(buf + 2 * kKv4CodeBytes + (t + gid) * 8);
+      const uint2 sb = *reinterpret_cast<const uint2*>(buf + 2 * kKv4CodeBytes + (t + gid + 8) * 8);
       const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
       const float fa[4] = {bf16lo_to_f32(sa.x), bf16hi_to_f32(sa.x), bf16lo_to_f32(sa.y), bf16hi_to_f32(sa.y)};
       const float fb[4] = {bf16lo_to_f32(sb.x), bf16hi_to_f32(sb.x), bf16lo_to_f32(sb.y), bf16hi_to_f32(sb.y)};
@@ -501,38 +522,27 @@ __global__ void __launch_bounds__(kKv4Threads, kKv4CtasPerSm) paged_decode_atten
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         float acc[4];
-        mma_bf16_from(acc, nibbles_plus128<0>(wa[j]), nibbles_plus128<0>(wb[j]), nibbles_plus128<1>(wa[j]),
-                      nibbles_plus128<1>(wb[j]), qb[j][0], qb[j][1], start[j][0], start[j][1]);
-        mma_bf16_acc(acc, nibbles_plus128<2>(wa[j]), nibbles_plus128<2>(wb[j]), nibbles_plus128<3>(wa[j]),
-                     nibbles_plus128<3>(wb[j]), qb[j][2], qb[j][3]);
-        s[0] = fmaf(fa[j], acc[0], s[0]);
-        s[1] = fmaf(fa[j], acc[1], s[1]);
-        s[2] = fmaf(fb[j], acc[2], s[2]);
-        s[3] = fmaf(fb[j], acc[3], s[3]);
+        mma_bf16_from(acc, nibbles_plus128<0>(wa[j], magic), nibbles_plus128<0>(wb[j], magic),
+                      nibbles_plus128<1>(wa[j], magic), nibbles_plus128<1>(wb[j], magic), qb[j][0], qb[j][1],
+                      start[j][0], start[j][1]);
+        mma_bf16_acc(acc, nibbles_plus128<2>(wa[j], magic), nibbles_plus128<2>(wb[j], magic),
+                     nibbles_plus128<3>(wa[j], magic), nibbles_plus128<3>(wb[j], magic), qb[j][2], qb[j][3]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[i] = fmaf(i < 2 ? fa[j] : fb[j], acc[i], s[i]);
       }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[e] *= p.scale_log2;
-      const uint2 ua = *reinterpret_cast<const uint2*>(buf + 2 * kKv4CodeBytes + kKv4ScaleBytes + (t0 + gid) * 8);
-      const uint2 ub = *reinterpret_cast<const uint2*>(buf + 2 * kKv4CodeBytes + kKv4ScaleBytes + (t0 + gid + 8) * 8);
-      float ga[4] = {bf16lo_to_f32(ua.x), bf16hi_to_f32(ua.x), bf16lo_to_f32(ua.y), bf16hi_to_f32(ua.y)};
-      float gb[4] = {bf16lo_to_f32(ub.x), bf16hi_to_f32(ub.x), bf16lo_to_f32(ub.y), bf16hi_to_f32(ub.y)};
-      if (t0 + 16 > mt.tokens) {  // rows behind the last token hold anything, NaN scales among it
-        if (t0 + gid >= mt.tokens) {
-          s[0] = s[1] = -INFINITY;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) ga[j] = 0.0f;
-        }
-        if (t0 + gid + 8 >= mt.tokens) {
-          s[2] = s[3] = -INFINITY;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) gb[j] = 0.0f;
-        }
+      for (int i = 0; i < 4; ++i) s[i] *= p.scale_log2;
+      uint2 ua = *reinterpret_cast<const uint2*>(buf + 2 * kKv4CodeBytes + kKv4ScaleBytes + (t + gid) * 8);
+      uint2 ub = *reinterpret_cast<const uint2*>(buf + 2 * kKv4CodeBytes + kKv4ScaleBytes + (t + gid + 8) * 8);
+      if (t + 16 > mt.tokens) {  // rows behind the last token hold anything: a probability of 0 does not undo a NaN
+        if (t + gid >= mt.tokens) s[0] = s[1] = -INFINITY, ua = make_uint2(0, 0);
+        if (t + gid + 8 >= mt.tokens) s[2] = s[3] = -INFINITY, ub = make_uint2(0, 0);
       }
       const bool above = s[0] > top[0] || s[2] > top[0] || s[1] > top[1] || s[3] > top[1];
       if (__any_sync(0xffffffffu, above)) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float mx = fmaxf(fmaxf(s[e], s[e + 2]), m[e]);
+          float mx = fmaxf(m[e], fmaxf(s[e], s[e + 2]));
 #pragma unroll
           for (int x = 4; x <= 16; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
           const float alpha = ex2(m[e] - mx);
@@ -545,109 +555,130 @@ __global__ void __launch_bounds__(kKv4Threads, kKv4CtasPerSm) paged_decode_atten
       }
       float pr[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) pr[e] = ex2(s[e] - m[e & 1]);
+      for (int i = 0; i < 4; ++i) pr[i] = ex2(s[i] - m[i & 1]);
       l[0] += pr[0] + pr[2];
       l[1] += pr[1] + pr[3];
-      const uint4 va = *reinterpret_cast<const uint4*>(buf + kKv4CodeBytes + (t0 / 2 + tig) * 128 +
-                                                       ((gid ^ (2 * tig)) * 16));
-      const uint4 vb = *reinterpret_cast<const uint4*>(buf + kKv4CodeBytes + (t0 / 2 + 4 + tig) * 128 +
-                                                       ((gid ^ (2 * tig)) * 16));
+      const float ga[4] = {bf16lo_to_f32(ua.x), bf16hi_to_f32(ua.x), bf16lo_to_f32(ua.y), bf16hi_to_f32(ua.y)};
+      const float gb[4] = {bf16lo_to_f32(ub.x), bf16hi_to_f32(ub.x), bf16lo_to_f32(ub.y), bf16hi_to_f32(ub.y)};
+      const uint8_t* vt = buf + kKv4CodeBytes + (t / 2 + tig) * 128 + ((gid ^ (2 * tig)) * 16);
+      const uint4 va = *reinterpret_cast<const uint4*>(vt), vb = *reinterpret_cast<const uint4*>(vt + 4 * 128);
       const uint32_t xa[4] = {va.x, va.y, va.z, va.w}, xb[4] = {vb.x, vb.y, vb.z, vb.w};
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const uint32_t b0 = movmatrix_trans(pack_bf16x2(pr[0] * ga[j], pr[1] * ga[j]));
         const uint32_t b1 = movmatrix_trans(pack_bf16x2(pr[2] * gb[j], pr[3] * gb[j]));
-        mma_bf16_acc(o[2 * j], nibbles_code<0>(xa[j]), nibbles_code<1>(xa[j]), nibbles_code<0>(xb[j]),
-                     nibbles_code<1>(xb[j]), b0, b1);
-        mma_bf16_acc(o[2 * j + 1], nibbles_code<2>(xa[j]), nibbles_code<3>(xa[j]), nibbles_code<2>(xb[j]),
-                     nibbles_code<3>(xb[j]), b0, b1);
+        mma_bf16_acc(o[2 * j], nibbles_code<0>(xa[j], magic), nibbles_code<1>(xa[j], magic),
+                     nibbles_code<0>(xb[j], magic), nibbles_code<1>(xb[j], magic), b0, b1);
+        mma_bf16_acc(o[2 * j + 1], nibbles_code<2>(xa[j], magic), nibbles_code<3>(xa[j], magic),
+                     nibbles_code<2>(xb[j], magic), nibbles_code<3>(xb[j], magic), b0, b1);
       }
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(&empty[st]);
+    if (++st == kKv4Stages) st = 0, round ^= 1;
 
     if (mt.last) {  // join the warps
 #pragma unroll
       for (int e = 0; e < 2; ++e)
 #pragma unroll
         for (int x = 4; x <= 16; x <<= 1) l[e] += __shfl_xor_sync(0xffffffffu, l[e], x);
-      if (merges > 0 && !mbar_wait(&red_free, (merges - 1) & 1, kErrTimeoutEmpty)) return;
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int head = 2 * tig + e;
-        if (head < G) {
-          float* dst = red + (warp * kKv4MaxGroup + head) * kKv4RedStride + gid * 4;
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            *reinterpret_cast<float4*>(dst + 32 * j) =
-                make_float4(o[2 * j][e], o[2 * j][e + 2], o[2 * j + 1][e], o[2 * j + 1][e + 2]);
-          if (gid == 0) red_ml[warp][head][0] = m[e], red_ml[warp][head][1] = l[e];
-        }
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&red_full);
-      if (!mbar_wait(&red_full, merges & 1, kErrTimeoutFull)) return;
       const int b = mt.job / p.Hkv, h0 = (mt.job - b * p.Hkv) * G;
       float* slot = p.partials + (2 * static_cast<int64_t>(blockIdx.x) + (mt.last == 3)) * kKv4SlotFloats;
-      for (int i = tid; i < G * kKv4D; i += kKv4Warps * 32) {
-        const int head = i / kKv4D, d = i % kKv4D;
-        float M = kKv4NoMax, L = 0.0f, acc = 0.0f;
+      for (int g0 = 0; g0 < G; g0 += 4, ++merges) {  // four heads at a time
+        if (merges > 0 && !mbar_wait(&red_free, (merges - 1) & 1, kErrTimeoutEmpty)) return;
 #pragma unroll
-        for (int w = 0; w < kKv4Warps; ++w) M = fmaxf(M, red_ml[w][head][0]);
+        for (int e = 0; e < 2; ++e) {
+          const int head = 2 * tig + e;
+          if (head >= g0 && head < min(G, g0 + 4)) {
+            float* dst = red + (warp * 4 + head - g0) * kKv4RedStride + gid * 4;
 #pragma unroll
-        for (int w = 0; w < kKv4Warps; ++w) {
-          const float f = ex2(red_ml[w][head][0] - M);
-          L = fmaf(f, red_ml[w][head][1], L);
-          acc = fmaf(f, red[(w * kKv4MaxGroup + head) * kKv4RedStride + d], acc);
+            for (int j = 0; j < 4; ++j)
+              *reinterpret_cast<float4*>(dst + 32 * j) =
+                  make_float4(o[2 * j][e], o[2 * j][e + 2], o[2 * j + 1][e], o[2 * j + 1][e + 2]);
+            if (gid == 0) red_ml[warp][head][0] = m[e], red_ml[warp][head][1] = l[e];
+          }
         }
-        if (mt.last == 1) {
-          p.out[(static_cast<int64_t>(b) * p.Hq + h0 + head) * kKv4D + d] =
-              __bfloat16_as_ushort(__float2bfloat16_rn(L == 0.0f ? 0.0f : acc / L));
-        } else {
-          slot[i] = acc;
-          if (d == 0) slot[kKv4MaxGroup * kKv4D + 2 * head] = M, slot[kKv4MaxGroup * kKv4D + 2 * head + 1] = L;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&red_full);
+        if (!mbar_wait(&red_full, merges & 1, kErrTimeoutFull)) return;
+        const int d = tid;  // a channel a thread: kKv4Warps * 32 == kKv4D
+        for (int head = g0; head < min(G, g0 + 4); ++head) {
+          float M = kKv4NoMax, S = 0.0f, acc = 0.0f;
+#pragma unroll
+          for (int w = 0; w < kKv4Warps; ++w) M = fmaxf(M, red_ml[w][head][0]);
+#pragma unroll
+          for (int w = 0; w < kKv4Warps; ++w) {
+            const float f = ex2(red_ml[w][head][0] - M);
+            S = fmaf(f, red_ml[w][head][1], S);
+            acc = fmaf(f, red[(w * 4 + head - g0) * kKv4RedStride + d], acc);
+          }
+          if (mt.last == 1) {
+            p.out[(static_cast<int64_t>(b) * p.Hq + h0 + head) * kKv4D + d] =
+                __bfloat16_as_ushort(__float2bfloat16_rn(S == 0.0f ? 0.0f : acc / S));
+          } else {
+            slot[head * kKv4D + d] = acc;
+            if (d == 0) *reinterpret_cast<float2*>(slot + kKv4MaxGroup * kKv4D + 2 * head) = make_float2(M, S);
+          }
         }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&red_free);
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&red_free);
-      ++merges;
     }
   }
 }
+static_assert(kKv4Warps * 32 == kKv4D, "the join takes a channel a thread");
 
 // Joins the partials of the jobs that several CTAs hold, in CTA order, and
-// writes the zeros of empty sequences.  One CTA per job.
+// writes the zeros of empty sequences.  One CTA per (sequence, query head), a
+// thread per channel.  Latency bound, so three rounds of loads: the cuts, the
+// maxima and sums (one part a lane), the outputs (eight in flight).
 __global__ void __launch_bounds__(kKv4D) kv4_merge_kernel(const Kv4AttnArgs p, int grid) {
-  const int job = blockIdx.x, b = job / p.Hkv, G = p.Hq / p.Hkv, d = threadIdx.x;
+  const int b = blockIdx.x / p.Hq, hq = blockIdx.x - b * p.Hq, G = p.Hq / p.Hkv, h = hq / G, g = hq - h * G;
+  const int d = threadIdx.x, lane = d & 31;
   grid_dependency_wait();
   const int64_t first = p.starts[b], n = p.starts[b + 1] - first, total = p.starts[p.B] * p.Hkv;
-  uint16_t* out = p.out + (static_cast<int64_t>(b) * p.Hq + (job - b * p.Hkv) * G) * kKv4D + d;
-  const int ctas = static_cast<int>(min(total, static_cast<int64_t>(grid)));
+  uint16_t* out = p.out + static_cast<int64_t>(blockIdx.x) * kKv4D + d;
   if (n == 0) {
-    for (int g = 0; g < G; ++g) out[g * kKv4D] = 0;
+    *out = 0;
     return;
   }
-  const int64_t a = first * p.Hkv + (job - b * p.Hkv) * n, e = a + n;
+  const int ctas = static_cast<int>(min(total, static_cast<int64_t>(grid)));
+  const int64_t a = first * p.Hkv + h * n, e = a + n;
   // the CTA of a unit u is the largest i whose cut is at or before it
   const int c0 = static_cast<int>(((a + 1) * ctas + total - 1) / total) - 1;
   const int c1 = static_cast<int>((e * ctas + total - 1) / total) - 1;
   if (c0 == c1) return;
   // c0 holds its part in slot 0 when the job is the first of its units, the others always do
-  const float* s0 = p.partials + (2 * static_cast<int64_t>(c0) + (kv4_cut(total, c0, ctas) < a)) * kKv4SlotFloats;
-  for (int g = 0; g < G; ++g) {
-    const int ml = kKv4MaxGroup * kKv4D + 2 * g;
-    float M = s0[ml];
-    for (int c = c0 + 1; c <= c1; ++c) M = fmaxf(M, p.partials[2 * static_cast<int64_t>(c) * kKv4SlotFloats + ml]);
-    float f = ex2(s0[ml] - M), L = f * s0[ml + 1], acc = f * s0[g * kKv4D + d];
-#pragma unroll 4
-    for (int c = c0 + 1; c <= c1; ++c) {
-      const float* s = p.partials + 2 * static_cast<int64_t>(c) * kKv4SlotFloats;
-      f = ex2(s[ml] - M);
-      L = fmaf(f, s[ml + 1], L);
-      acc = fmaf(f, s[g * kKv4D + d], acc);
+  const int slot0 = kv4_cut(total, c0, ctas) < a ? 1 : 0;
+  float M = kKv4NoMax, S = 0.0f, acc = 0.0f;
+  for (int c = c0; c <= c1; c += 32) {
+    const int parts = min(32, c1 - c + 1);
+    const float* at = p.partials + static_cast<int64_t>(c) * 2 * kKv4SlotFloats;  // part i at 2 i slots, but for slot0
+    float2 ml = make_float2(kKv4NoMax, 0.0f);
+    const int skew = c == c0 ? slot0 : 0;
+    if (lane < parts)
+      ml = *reinterpret_cast<const float2*>(at + (2 * lane + (lane == 0 ? skew : 0)) * kKv4SlotFloats +
+                                            kKv4MaxGroup * kKv4D + 2 * g);
+    float mx = fmaxf(ml.x, M);
+#pragma unroll
+    for (int x = 16; x >= 1; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+    const float keep = ex2(M - mx), f = ex2(ml.x - mx);
+    M = mx;
+    float fs = f * ml.y;
+#pragma unroll
+    for (int x = 16; x >= 1; x >>= 1) fs += __shfl_xor_sync(0xffffffffu, fs, x);
+    S = fmaf(S, keep, fs);
+    acc *= keep;
+    for (int i = 0; i < parts; i += 8) {
+      float v[8];
+#pragma unroll
+      for (int x = 0; x < 8; ++x)
+        v[x] = i + x < parts ? at[(2 * (i + x) + (i + x == 0 ? skew : 0)) * kKv4SlotFloats + g * kKv4D + d] : 0.0f;
+#pragma unroll
+      for (int x = 0; x < 8; ++x) acc = fmaf(__shfl_sync(0xffffffffu, f, (i + x) & 31), v[x], acc);
     }
-    out[g * kKv4D] = __bfloat16_as_ushort(__float2bfloat16_rn(L == 0.0f ? 0.0f : acc / L));
   }
+  *out = __bfloat16_as_ushort(__float2bfloat16_rn(S == 0.0f ? 0.0f : acc / S));
 }
 
 static int64_t kv4_starts_bytes(int64_t batch) { return (batch + 1) * 8 + 15 & ~int64_t(15); }
@@ -688,7 +719,7 @@ int launch_paged_decode_attention_kv4(const void* q, const void* k_codes, const 
       kv4_max_ctas(batch, num_kv_heads, max_pages), kKv4CtasPerSm * static_cast<int64_t>(device_sm_count())));
   rc = launch_kernel(paged_decode_attention_kv4_kernel, dim3(ctas), dim3(kKv4Threads), kKv4Smem, stream, false, a);
   if (rc != NV4_OK) return rc;
-  return launch_kernel(kv4_merge_kernel, dim3(static_cast<unsigned>(batch * num_kv_heads)), dim3(kKv4D), 0, stream,
+  return launch_kernel(kv4_merge_kernel, dim3(static_cast<unsigned>(batch * num_heads)), dim3(kKv4D), 0, stream,
                        true, a, ctas);
 }
 

@@ -48,7 +48,8 @@ def page_bytes(num_kv_heads: int) -> int:
     return 2 * num_kv_heads * PAGE_TOKENS * (HEAD_DIM // 2 + HEAD_DIM // GROUP_CHANNELS * 2)
 
 
-def _check_cache(cache: Kv4Cache, device) -> tuple[int, int]:
+def _check_cache(cache: Kv4Cache) -> int:
+    """Number of KV heads of a well-formed cache."""
     codes = cache.k_codes.shape
     if len(codes) != 4 or codes[0] < 1 or codes[1] < 1 or codes[2:] != (PAGE_TOKENS, HEAD_DIM // 2):
         raise ValueError("Expected codes[pages,Hkv,256,64]")
@@ -59,10 +60,7 @@ def _check_cache(cache: Kv4Cache, device) -> tuple[int, int]:
         raise TypeError("Codes must be UINT8")
     if cache.k_scales.dtype != torch.bfloat16 or cache.v_scales.dtype != torch.bfloat16:
         raise TypeError("Cache scales must be BF16")
-    for t in cache:
-        if t.device != device or not t.is_contiguous():
-            raise ValueError("The cache must be contiguous on the input's device")
-    return codes[0], codes[1]
+    return codes[1]
 
 
 def qk_norm_rope_store_kv4(qkv, q_weight, k_weight, cos_sin, positions, slot_mapping, cache: Kv4Cache | None, *,
@@ -84,7 +82,7 @@ def qk_norm_rope_store_kv4(qkv, q_weight, k_weight, cos_sin, positions, slot_map
     if qkv.ndim != 2 or qkv.dtype != torch.bfloat16 or qkv.shape[0] < 1 \
             or qkv.shape[1] != (num_heads + 2 * num_kv_heads) * HEAD_DIM:
         raise ValueError("Expected BF16 qkv[T,(Hq+2Hkv)*128], T>0")
-    t, device = qkv.shape[0], qkv.device
+    t = qkv.shape[0]
     if q_weight.shape != (HEAD_DIM,) or k_weight.shape != (HEAD_DIM,) or q_weight.dtype != torch.bfloat16 \
             or k_weight.dtype != torch.bfloat16:
         raise ValueError("Expected BF16 q_weight[128] and k_weight[128]")
@@ -96,21 +94,19 @@ def qk_norm_rope_store_kv4(qkv, q_weight, k_weight, cos_sin, positions, slot_map
         raise ValueError("slot_mapping and cache go together")
     if slot_mapping is not None and (slot_mapping.shape != (t,) or slot_mapping.dtype != torch.int32):
         raise ValueError("Expected INT32 slot_mapping[T]")
-    if not qkv.is_cuda:
-        raise ValueError("All tensors must be contiguous on one CUDA device")
+    if cache is not None and _check_cache(cache) != num_kv_heads:
+        raise ValueError("The cache has another number of KV heads")
     if q_out is None:
-        q_out = torch.empty((t, num_heads, HEAD_DIM), dtype=torch.bfloat16, device=device)
+        q_out = qkv.new_empty((t, num_heads, HEAD_DIM))
     elif q_out.shape != (t, num_heads, HEAD_DIM) or q_out.dtype != torch.bfloat16:
         raise ValueError("Expected BF16 q_out[T,Hq,128]")
-    for x in (qkv, q_weight, k_weight, cos_sin, positions, slot_mapping, q_out):
-        if x is not None and (x.device != device or not x.is_contiguous()):
-            raise ValueError("All tensors must be contiguous on one CUDA device")
-    if cache is not None and _check_cache(cache, device)[1] != num_kv_heads:
-        raise ValueError("The cache has another number of KV heads")
+    if not _native.on_one_device(qkv.get_device(), qkv, q_weight, k_weight, cos_sin, positions, slot_mapping, q_out,
+                                 *(cache or ())):
+        raise ValueError("All tensors must be contiguous on one CUDA device")
     k_out = v_out = None
     if return_values:
-        k_out = torch.empty((t, num_kv_heads, HEAD_DIM), dtype=torch.bfloat16, device=device)
-        v_out = torch.empty_like(k_out)
+        k_out = qkv.new_empty((t, num_kv_heads, HEAD_DIM))
+        v_out = qkv.new_empty((t, num_kv_heads, HEAD_DIM))
     _native.qk_norm_rope_store_kv4(qkv, q_weight, k_weight, cos_sin, positions, slot_mapping, q_out, k_out, v_out,
                                    *(cache or (None,) * 4), num_heads, num_kv_heads, eps)
     return (q_out, k_out, v_out) if return_values else q_out
@@ -136,10 +132,7 @@ def paged_decode_attention_kv4(q, cache: Kv4Cache, block_tables, context_lens, *
     if q.ndim != 3 or q.dtype != torch.bfloat16 or q.shape[0] < 1 or q.shape[2] != HEAD_DIM:
         raise ValueError("Expected BF16 q[B,Hq,128], B>0")
     b, hq, _ = q.shape
-    device = q.device
-    if not q.is_cuda:
-        raise ValueError("All tensors must be contiguous on one CUDA device")
-    _, hkv = _check_cache(cache, device)
+    hkv = _check_cache(cache)
     if hq < hkv or hq % hkv or hq // hkv > 8:
         raise ValueError("Expected query heads to be 1 to 8 times the KV heads")
     if block_tables.ndim != 2 or block_tables.shape[0] != b or block_tables.shape[1] < 1 \
@@ -150,13 +143,13 @@ def paged_decode_attention_kv4(q, cache: Kv4Cache, block_tables, context_lens, *
     if not scale > 0:
         raise ValueError("scale must be positive")
     if out is None:
-        out = torch.empty_like(q)
+        out = q.new_empty(q.shape)
     elif out.shape != q.shape or out.dtype != torch.bfloat16:
         raise ValueError("Expected BF16 out[B,Hq,128]")
     if workspace is None:
-        workspace = kv4_attention_workspace(b, hq, block_tables.shape[1], device)
-    for x in (q, block_tables, context_lens, out, workspace):
-        if x.device != device or not x.is_contiguous():
-            raise ValueError("All tensors must be contiguous on one CUDA device")
+        nbytes = _native.paged_attention_kv4_workspace_bytes(b, hq, block_tables.shape[1])
+        workspace = q.new_empty(nbytes, dtype=torch.uint8)
+    if not _native.on_one_device(q.get_device(), q, block_tables, context_lens, out, workspace, *cache):
+        raise ValueError("All tensors must be contiguous on one CUDA device")
     _native.paged_decode_attention_kv4(q, *cache, block_tables, context_lens, out, workspace, scale)
     return out

@@ -22,14 +22,15 @@ class StepTables(NamedTuple):
 
 
 def alloc_step_tables(rows: int, tokens: int, max_pages: int, device) -> StepTables:
-    """Output buffers, for instance a captured graph's static ones.  They are
-    carved from one allocation (the INT64 positions first)."""
+    """Output buffers, for instance a captured graph's static ones."""
     if rows < 1 or tokens < 0 or max_pages < 1:
         raise ValueError("Expected rows>0, tokens>=0, max_pages>0")
-    sizes = (rows * max_pages, rows, tokens, rows + 1)
-    buf = torch.empty(2 * tokens + sum(sizes), dtype=torch.int32, device=device)
-    tables, lens, slots, starts = buf[2 * tokens:].split(sizes)
-    return StepTables(tables.view(rows, max_pages), lens, slots, buf[:2 * tokens].view(torch.int64), starts)
+    return _like(torch.empty(0, dtype=torch.int32, device=device), rows, tokens, max_pages)
+
+
+def _like(x, rows: int, tokens: int, max_pages: int) -> StepTables:
+    return StepTables(x.new_empty((rows, max_pages)), x.new_empty(rows), x.new_empty(tokens),
+                      x.new_empty(tokens, dtype=torch.int64), x.new_empty(rows + 1))
 
 
 def build_step_tables(cached_lens, new_lens, pages, *, num_tokens: int, max_pages: int, page_size: int = 256,
@@ -49,17 +50,15 @@ def build_step_tables(cached_lens, new_lens, pages, *, num_tokens: int, max_page
     if cached_lens.ndim != 1 or cached_lens.shape[0] < 1 or cached_lens.dtype != torch.int32 \
             or new_lens.shape != cached_lens.shape or new_lens.dtype != torch.int32:
         raise ValueError("Expected INT32 cached_lens[B] and new_lens[B], B>0")
-    b, device = cached_lens.shape[0], cached_lens.device
+    b = cached_lens.shape[0]
     if b > MAX_BATCH:
         raise ValueError(f"Expected at most {MAX_BATCH} requests")
     if pages.ndim != 1 or pages.dtype != torch.int32:
         raise ValueError("Expected INT32 pages[P]")
     if num_tokens < 0 or max_pages < 1 or page_size < 1:
         raise ValueError("Expected num_tokens>=0, max_pages>0, page_size>0")
-    if not cached_lens.is_cuda:
-        raise ValueError("All tensors must be contiguous on one CUDA device")
     if out is None:
-        out = alloc_step_tables(b, num_tokens, max_pages, device)
+        out = _like(cached_lens, b, num_tokens, max_pages)
     else:
         rows = out.block_tables.shape[0]
         if out.block_tables.shape != (rows, max_pages) or rows < b or out.context_lens.shape != (rows,) \
@@ -71,9 +70,8 @@ def build_step_tables(cached_lens, new_lens, pages, *, num_tokens: int, max_page
                 x.dtype != torch.int32 for x in (out.block_tables, out.context_lens, out.slot_mapping,
                                                  out.query_starts)):
             raise TypeError("Expected INT64 positions and INT32 other outputs")
-    for x in (cached_lens, new_lens, pages, *out):
-        if x.device != device or not x.is_contiguous():
-            raise ValueError("All tensors must be contiguous on one CUDA device")
+    if not _native.on_one_device(cached_lens.get_device(), cached_lens, new_lens, pages, *out):
+        raise ValueError("All tensors must be contiguous on one CUDA device")
     _native.step_tables(cached_lens, new_lens, pages, out.block_tables, out.context_lens, out.query_starts,
                         out.slot_mapping, out.positions, page_size)
     return out

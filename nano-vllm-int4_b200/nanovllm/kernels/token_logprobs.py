@@ -39,17 +39,14 @@ def token_logprobs(logits, targets, *, top_k: int = 0) -> TokenLogprobs:
         raise ValueError("Expected INT64 targets[T]")
     if not 0 <= top_k <= MAX_TOP_K:
         raise ValueError(f"top_k must be in 0..{MAX_TOP_K}")
-    device = logits.device
-    if not logits.is_cuda or targets.device != device or not targets.is_contiguous():
+    if not logits.is_cuda or not _native.on_one_device(logits.get_device(), targets):
         raise ValueError("All tensors must be on one CUDA device, targets contiguous")
     if (v > 1 and logits.stride(1) != 1) or (t > 1 and logits.stride(0) < v):
         raise ValueError("The logits of a row must be contiguous, and rows must not overlap")
-    # one allocation for the outputs: two 64-bit ones first
-    buf = torch.empty(t * (4 + 3 * top_k), dtype=torch.float32, device=device)
-    wide = buf[:2 * t * (1 + top_k)].view(torch.int64)
-    rest = buf[2 * t * (1 + top_k):]
-    out = TokenLogprobs(rest[:t], wide[:t], rest[t:2 * t], rest[2 * t:].view(t, top_k) if top_k else None,
-                        wide[t:].view(t, top_k) if top_k else None)
+    new = logits.new_empty
+    out = TokenLogprobs(new(t, dtype=torch.float32), new(t, dtype=torch.int64), new(t, dtype=torch.float32),
+                        new((t, top_k), dtype=torch.float32) if top_k else None,
+                        new((t, top_k), dtype=torch.int64) if top_k else None)
     if t:
-        _native.token_logprobs(logits, targets, *out[:3], *out[3:])
+        _native.token_logprobs(logits, targets, *out)
     return out
