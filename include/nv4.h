@@ -409,15 +409,20 @@ int nv4_step_tables(const int32_t* cached_lens, const int32_t* new_lens, const i
  *   top_logprobs float32, top_ids int64 [rows, top_k] (may be NULL when top_k is
  *            0): by falling logit, ties to the lowest index.  A logit of -inf
  *            (or NaN) is no alternative: where fewer than top_k are left, id -1 and -inf
+ *   workspace  nv4_token_logprobs_workspace_bytes(...) bytes of scratch, 8-byte
+ *              aligned (may be NULL when that is 0, as it is for many rows);
+ *              calls that may overlap need one each
  * A row of nothing but -inf: logprob -inf, entropy 0.  A row that holds a NaN or
  * +inf has no distribution: logprob, entropy and top_logprobs are NaN, ranks and
  * ids go by the comparisons.  vocab <= NV4_LOGPROB_MAX_VOCAB, top_k <= NV4_LOGPROB_MAX_TOP.
  */
 #define NV4_LOGPROB_MAX_VOCAB (1 << 24)
 #define NV4_LOGPROB_MAX_TOP 32
+int64_t nv4_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int64_t top_k);
 int nv4_token_logprobs(const void* logits, int fp32, const int64_t* targets, float* logprobs, int64_t* ranks,
-                       float* entropy, float* top_logprobs, int64_t* top_ids, int64_t rows, int64_t vocab,
-                       int64_t row_stride, int64_t top_k, void* stream);
+                       float* entropy, float* top_logprobs, int64_t* top_ids, void* workspace,
+                       int64_t workspace_bytes, int64_t rows, int64_t vocab, int64_t row_stride, int64_t top_k,
+                       void* stream);
 
 /* Library metadata and error reporting. */
 int nv4_version(void);                      /* major*10000 + minor*100 + patch */

@@ -526,21 +526,31 @@ int nv4_step_tables(const int32_t* cached_lens, const int32_t* new_lens, const i
                             static_cast<cudaStream_t>(stream));
 }
 
+int64_t nv4_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int64_t top_k) {
+  if (rows < 1 || rows > (int64_t(1) << 31) - 1 || vocab < 1 || vocab > NV4_LOGPROB_MAX_VOCAB || top_k < 0 ||
+      top_k > NV4_LOGPROB_MAX_TOP)
+    return 0;
+  return token_logprobs_workspace_bytes(rows, vocab, top_k);
+}
+
 int nv4_token_logprobs(const void* logits, int fp32, const int64_t* targets, float* logprobs, int64_t* ranks,
-                       float* entropy, float* top_logprobs, int64_t* top_ids, int64_t rows, int64_t vocab,
-                       int64_t row_stride, int64_t top_k, void* stream) {
+                       float* entropy, float* top_logprobs, int64_t* top_ids, void* workspace,
+                       int64_t workspace_bytes, int64_t rows, int64_t vocab, int64_t row_stride, int64_t top_k,
+                       void* stream) {
   if (!logits || !targets || !logprobs || !ranks || !entropy || (fp32 != 0 && fp32 != 1))
     return NV4_ERR_INVALID_ARGUMENT;
   if (rows < 1 || rows > (int64_t(1) << 31) - 1 || vocab < 1 || row_stride < (rows > 1 ? vocab : 0) || top_k < 0 ||
       (top_k > 0 && (!top_logprobs || !top_ids)))
     return NV4_ERR_INVALID_ARGUMENT;
   if (vocab > NV4_LOGPROB_MAX_VOCAB || top_k > NV4_LOGPROB_MAX_TOP) return NV4_ERR_UNSUPPORTED;
-  if (!aligned(logits, fp32 ? 4 : 2) || !aligned(targets, 8) || !aligned(logprobs, 4) || !aligned(ranks, 8) ||
+  const int64_t scratch = token_logprobs_workspace_bytes(rows, vocab, top_k);
+  if (scratch > 0 && (!workspace || workspace_bytes < scratch)) return NV4_ERR_INVALID_ARGUMENT;
+  if (!aligned(workspace, 8) || !aligned(logits, fp32 ? 4 : 2) || !aligned(targets, 8) || !aligned(logprobs, 4) || !aligned(ranks, 8) ||
       !aligned(entropy, 4) || !aligned(top_logprobs, 4) || !aligned(top_ids, 8))
     return NV4_ERR_ALIGNMENT;
   if (!device_is_sm100()) return NV4_ERR_DEVICE;
-  return launch_token_logprobs(logits, fp32, targets, logprobs, ranks, entropy, top_logprobs, top_ids, rows, vocab,
-                               row_stride, top_k, static_cast<cudaStream_t>(stream));
+  return launch_token_logprobs(logits, fp32, targets, logprobs, ranks, entropy, top_logprobs, top_ids, workspace,
+                               rows, vocab, row_stride, top_k, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

@@ -115,8 +115,9 @@ int launch_step_tables(const int* cached, const int* fresh, const int* pages, in
                        cudaStream_t stream);
 // Token log-probabilities (token_logprobs.cu).
 int launch_token_logprobs(const void* logits, int fp32, const int64_t* targets, float* logprobs, int64_t* ranks,
-                          float* entropy, float* top_logprobs, int64_t* top_ids, int64_t rows, int64_t vocab,
-                          int64_t row_stride, int64_t top_k, cudaStream_t stream);
+                          float* entropy, float* top_logprobs, int64_t* top_ids, void* workspace, int64_t rows,
+                          int64_t vocab, int64_t row_stride, int64_t top_k, cudaStream_t stream);
+int64_t token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int64_t top_k);
 // Peer mode of the stream GEMM (row-parallel layers): the launcher fills in the
 // tile geometry the matching tile reduce needs.
 // Launch plan of the decode stream GEMM (w4a4_gemm.cu); the C ABI exports it

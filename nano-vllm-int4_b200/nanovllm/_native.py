@@ -40,7 +40,8 @@ EXPORTS = ("nv4_rht_quant_pack", "nv4_rht_quant_i8", "nv4_w4a4_grouped_gemm", "n
            "nv4_add_rmsnorm_rht_quant_i8", "nv4_w4a4_stream_plan", "nv4_paged_attention_workspace_bytes",
            "nv4_paged_decode_attention", "nv4_qk_norm_rope_store", "nv4_w4a16_plan",
            "nv4_qk_norm_rope_store_kv4", "nv4_paged_attention_kv4_workspace_bytes",
-           "nv4_paged_decode_attention_kv4", "nv4_step_tables", "nv4_token_logprobs")
+           "nv4_paged_decode_attention_kv4", "nv4_step_tables", "nv4_token_logprobs",
+           "nv4_token_logprobs_workspace_bytes")
 
 
 class NativeLibraryError(RuntimeError):
@@ -142,7 +143,9 @@ def load(path: str | None = None) -> ctypes.CDLL:
         lib.nv4_paged_decode_attention_kv4.restype = _int
         lib.nv4_step_tables.argtypes = [_vp] * 8 + [_i64] * 6 + [_vp]
         lib.nv4_step_tables.restype = _int
-        lib.nv4_token_logprobs.argtypes = [_vp, _int] + [_vp] * 6 + [_i64] * 4 + [_vp]
+        lib.nv4_token_logprobs_workspace_bytes.argtypes = [_i64, _i64, _i64]
+        lib.nv4_token_logprobs_workspace_bytes.restype = _i64
+        lib.nv4_token_logprobs.argtypes = [_vp, _int] + [_vp] * 7 + [_i64] * 5 + [_vp]
         lib.nv4_token_logprobs.restype = _int
         lib.nv4_status_string.argtypes = [_int]
         lib.nv4_status_string.restype = ctypes.c_char_p
@@ -461,10 +464,13 @@ def step_tables(cached_lens, new_lens, pages, block_tables, context_lens, query_
 
 
 def token_logprobs(logits, targets, logprobs, ranks, entropy, top_logprobs, top_ids) -> None:
-    """nv4_token_logprobs (top_logprobs and top_ids None: no alternatives)."""
+    """nv4_token_logprobs (top_logprobs and top_ids None: no alternatives); the
+    workspace comes from torch's allocator."""
     rows, vocab = logits.shape
     top_k = 0 if top_ids is None else top_ids.shape[1]
+    nbytes = load().nv4_token_logprobs_workspace_bytes(rows, vocab, top_k)
+    workspace = logits.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     _call(load().nv4_token_logprobs, "nv4_token_logprobs", logits.get_device(),
           logits.data_ptr(), 1 if logits.dtype == torch.float32 else 0, targets.data_ptr(), logprobs.data_ptr(),
-          ranks.data_ptr(), entropy.data_ptr(), _addr(top_logprobs), _addr(top_ids), rows, vocab, logits.stride(0),
-          top_k)
+          ranks.data_ptr(), entropy.data_ptr(), _addr(top_logprobs), _addr(top_ids), _addr(workspace), nbytes, rows,
+          vocab, logits.stride(0), top_k)

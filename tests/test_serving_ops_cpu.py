@@ -89,21 +89,22 @@ def test_step_tables_pointers(i):
 
 
 def logprobs(ptrs=(), **over):
-    a = dict(fp32=1, rows=3, vocab=100, stride=100, k=2) | over
-    p = [P] * 7
+    a = dict(fp32=1, rows=3, vocab=100000, stride=100000, k=2, ws=1 << 30) | over
+    p = [P] * 8
     for i, x in dict(ptrs).items():
         p[i] = x
-    return _native.load().nv4_token_logprobs(p[0], a["fp32"], *p[1:], a["rows"], a["vocab"], a["stride"], a["k"], None)
+    return _native.load().nv4_token_logprobs(p[0], a["fp32"], *p[1:], a["ws"], a["rows"], a["vocab"], a["stride"],
+                                             a["k"], None)
 
 
 @pytest.mark.parametrize("over,status", [
-    (dict(fp32=2), INVALID), (dict(rows=0), INVALID), (dict(vocab=0), INVALID), (dict(stride=99), INVALID),
-    (dict(k=-1), INVALID), (dict(k=33), UNSUPPORTED), (dict(vocab=(1 << 24) + 1, stride=1 << 25), UNSUPPORTED)])
+    (dict(fp32=2), INVALID), (dict(rows=0), INVALID), (dict(vocab=0), INVALID), (dict(stride=99999), INVALID),
+    (dict(k=-1), INVALID), (dict(ws=100), INVALID), (dict(k=33), UNSUPPORTED), (dict(vocab=(1 << 24) + 1, stride=1 << 25), UNSUPPORTED)])
 def test_logprob_refusals(over, status):
     assert logprobs(**over) == status
 
 
-@pytest.mark.parametrize("i", range(7))
+@pytest.mark.parametrize("i", range(8))
 def test_logprob_pointers(i):
     assert logprobs(ptrs={i: None}) == INVALID
     assert logprobs(ptrs={i: V(256 + 1)}) == ALIGNMENT
@@ -169,3 +170,11 @@ def test_reference_packing_round_trip():
     assert torch.equal(ref.read_k(cache), codes.double()) and torch.equal(ref.read_v(cache), codes.double())
     for byte in (ref.K_BYTE, ref.V_BYTE):
         assert torch.equal((byte * 2 + ref.SHIFT // 4).flatten().sort().values, torch.arange(256 * 128))
+
+
+def test_logprob_workspace():
+    """None once the rows alone fill the GPU; a part for every CTA of a row else."""
+    size = _native.load().nv4_token_logprobs_workspace_bytes
+    assert size(1024, 151936, 20) == 0 and size(1, 100, 5) == 0
+    assert size(1, 151936, 0) > 0 and size(1, 151936, 20) - size(1, 151936, 0) == 64 * 20 * 8
+    assert size(1024, 1 << 24, 0) > 0 and size(0, 100, 5) == 0 and size(1, 100, 33) == 0
