@@ -1,16 +1,22 @@
 // Log-probabilities of given tokens from their logits, with the tokens' ranks,
 // the distribution's entropy and the k most likely alternatives.
 //
-// For a row x of V logits with maximum m, S = sum exp(x - m) and W = sum
-// exp(x - m) (x - m):
-//   logprob(t) = x_t - m - log S          rank(t) = 1 + #{x > x_t}
-//   entropy    = log S - W / S            (both terms >= 0: nothing cancels)
+// For a row x of V logits, with a reference m at most 1 below the maximum, d = x -
+// m, S = sum exp(d) and W = sum exp(d) d:
+//   logprob(t) = d_t - log S      rank(t) = 1 + #{x > x_t}
+//   entropy    = log S - W / S
+// (a reference far below the maximum would cost precision: both terms of the
+// entropy grow with the distance.  Folding x log2(e) - m log2(e) into one FMA
+// saves 3% on 1024 rows but the maximum's own exponential is then not 1.)
 // Alternatives are ordered by logit, ties to the lowest index.
 //
-// One pass over the logits, bound by HBM where there are many rows.  A warp
-// takes chunks of 256 contiguous logits, eight a lane; every lane keeps its own
-// running (m, S, W).  The rank costs one comparison with the chunk's maximum
-// unless that exceeds the token's logit.  The alternatives cost one maximum per
+// One pass over the logits, bound by HBM where there are many rows, with the
+// exponential unit (16 a cycle and SM) next.  A warp takes chunks of 256
+// contiguous logits, eight a lane, and moves its reference when a chunk's maximum
+// exceeds it by more than 1: that happens a few times a row for the warp, while
+// every lane's own maximum would move in most chunks for some lane.  The rank
+// costs one comparison with the chunk's maximum unless that exceeds the token's
+// logit.  The alternatives cost one maximum per
 // chunk in that pass: the k largest elements lie in the k chunks with the largest
 // maxima (for any other chunk there are k elements above all of it), so after the
 // pass a threshold is found among the maxima, the few chunks that reach it are
@@ -18,6 +24,8 @@
 //
 // With few rows a row is split over several CTAs, whose results a second kernel
 // joins.
+#include <cfloat>
+
 #include "nv4_device.cuh"
 #include "nv4_launch.h"
 
@@ -46,7 +54,9 @@ struct LogprobArgs {
   int rows, vocab, top_k, splits;
 };
 
-// Statistics of a set of logits: m = -inf and S = W = 0 for none above -inf.
+// Statistics of a set of logits relative to m; m = -inf and S = W = 0 for none
+// above -inf.  From |m| = 2^40 on, neighbouring numbers differ by more than any
+// exponential shows: S is then the number of logits equal to the maximum m, W 0.
 struct LogprobStat {
   float m, s, w;
   int above;
@@ -126,23 +136,20 @@ __device__ __forceinline__ void unpack_chunk(const uint4 (&raw)[LaneOf<T>::kVecs
   }
 }
 
-// The statistics of a joined with those of b.
-__device__ __forceinline__ LogprobStat join_stats(const LogprobStat& a, const LogprobStat& b) {
-  LogprobStat r;
-  r.m = fmaxf(a.m, b.m);
-  r.above = a.above + b.above;
-  r.s = r.w = 0.0f;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const LogprobStat& t = i ? b : a;
-    if (t.m == r.m) {
-      r.s += t.s, r.w += t.w;
-    } else if (t.m > -INFINITY) {
-      const float d = t.m - r.m, f = exp2f(d * kLog2e);
-      if (f > 0.0f) r.s = fmaf(f, t.s, r.s), r.w = fmaf(f, fmaf(d, t.s, t.w), r.w);
-    }
-  }
-  return r;
+__device__ __forceinline__ bool is_big(float m) { return fabsf(m) >= 0x1p40f; }
+
+// Moves statistics from their reference to the larger m.
+__device__ __forceinline__ void move_stat(float& s, float& w, float from, float m) {
+  if (from == m) return;
+  const float d = from - m, f = is_big(from) || is_big(m) ? 0.0f : ex2(d * kLog2e);
+  w = f > 0.0f ? f * fmaf(d, s, w) : 0.0f;
+  s = f > 0.0f ? f * s : 0.0f;
+}
+__device__ __forceinline__ LogprobStat join_stats(LogprobStat a, LogprobStat b) {
+  const float m = fmaxf(a.m, b.m);
+  move_stat(a.s, a.w, a.m, m);
+  move_stat(b.s, b.w, b.m, m);
+  return {m, a.s + b.s, a.w + b.w, a.above + b.above};
 }
 __device__ __forceinline__ LogprobStat warp_join(LogprobStat t) {
 #pragma unroll
@@ -178,42 +185,37 @@ __device__ __forceinline__ uint64_t list_merge(uint64_t a, uint64_t b, int lane)
 // A row's results from its statistics and its list of keys (one warp).
 __device__ __forceinline__ void finish_row(const LogprobArgs& p, int64_t row, float xt, bool given,
                                            const LogprobStat& t, bool nan, uint64_t list, int lane) {
-  const bool empty = t.m == -INFINITY && !nan;
-  const float m = nan ? NAN : t.m, log_s = logf(t.s);
+  const bool none = nan || t.m == INFINITY, empty = t.m == -INFINITY;
+  const float log_s = logf(t.s);
   if (lane == 0) {
-    p.logprobs[row] = !given ? 0.0f : empty ? -INFINITY : (xt - m) - log_s;
+    p.logprobs[row] = !given ? 0.0f : none ? NAN : empty ? -INFINITY : (xt - t.m) - log_s;
     p.ranks[row] = given ? t.above + 1 : 0;
-    p.entropy[row] = empty ? 0.0f : nan ? NAN : log_s - t.w / t.s;
+    p.entropy[row] = none ? NAN : empty ? 0.0f : log_s - t.w / t.s;
   }
   if (lane < p.top_k) {
-    p.top_logprobs[row * p.top_k + lane] = list ? (key_logit(list) - m) - log_s : -INFINITY;
+    p.top_logprobs[row * p.top_k + lane] = !list ? -INFINITY : none ? NAN : (key_logit(list) - t.m) - log_s;
     p.top_ids[row * p.top_k + lane] = list ? static_cast<int64_t>(0xFFFFFFFFu - static_cast<uint32_t>(list)) : -1;
   }
 }
 
-// A logit below which exp(x - m) is 0 in FP32 whatever it is, so that clamping to
-// it keeps x - m finite (0 * -inf would be NaN); below m where m - 110 is m.
-// -inf where there is none (m is the type's lowest value).
+// The statistics that a warp gathers: the reference is the warp's, the sums and the
+// count are the lanes'.
 template <typename T>
-__device__ __forceinline__ float logit_floor(float m) {
-  float l = m - 110.0f;
-  if constexpr (sizeof(T) == 4) {
-    return l < m ? l : nextafterf(m, -INFINITY);
-  } else {
-    l = __bfloat162float(__float2bfloat16_rd(l));
-    if (l < m) return l;
-    const uint32_t bits = __float_as_uint(m) >> 16;  // |m| is large: the BF16 number below it
-    return __uint_as_float((m > 0.0f ? bits - 1 : bits + 1) << 16);
+struct WarpStat {
+  float m, limit, floor;  // reference, m + 1; m - 110 or less, whose exponential is 0
+  float s = 0.0f, w = 0.0f;
+  float above = 0.0f;  // whole numbers below 2^24
+  bool nan = false;
+
+  __device__ __forceinline__ WarpStat() { refer(sizeof(T) == 4 ? -FLT_MAX : -0x1.fep127f); }  // the lowest value
+  __device__ __forceinline__ void refer(float to) {
+    m = to;
+    limit = to + 1.0f;
+    floor = to - 110.0f;
+    if constexpr (sizeof(T) == 2) floor = __bfloat162float(__float2bfloat16_rd(floor));
   }
-}
 
-template <typename T>
-struct LaneStat {
-  LogprobStat t;
-  float floor;  // of t.m
-  bool nan;
-
-  // The chunk's eight logits; returns their maximum (NaN aside).
+  // The chunk's logits; returns the lane's maximum (NaN aside).
   __device__ __forceinline__ float add(uint4 (&raw)[LaneOf<T>::kVecs], float xt) {
     float x[8], top;
     if constexpr (sizeof(T) == 2) {
@@ -228,54 +230,61 @@ struct LaneStat {
 #pragma unroll
       for (int e = 1; e < 8; ++e) asm("max.NaN.f32 %0, %1, %2;" : "=f"(top) : "f"(top), "f"(x[e]));
     }
-    if (top != top) {
-      nan = true;
-      unpack_chunk<T>(raw, x);
-      top = -INFINITY;
+    if (__any_sync(0xffffffffu, !(top <= limit))) {
+      if (top != top) {
+        nan = true;
+        unpack_chunk<T>(raw, x);
+        top = -INFINITY;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) top = fmaxf(top, x[e]);
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, x[e]);
+      }
+      const uint32_t order = __reduce_max_sync(0xffffffffu, logit_order(top));
+      const float most = key_logit(static_cast<uint64_t>(order) << 32);
+      if (order != 0 && most > m) {
+        move_stat(s, w, m, most);
+        refer(most);
+      }
     }
     if (top > xt) {
-      unpack_chunk<T>(raw, x);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) t.above += x[e] > xt;
-    }
-    if (top > t.m) {
-      if (t.m > -INFINITY) {
-        const float d = t.m - top, f = exp2f(d * kLog2e);
-        if (f > 0.0f) t.w = f * fmaf(d, t.s, t.w), t.s *= f;
-        else t.w = t.s = 0.0f;
-      }
-      t.m = top;
-      floor = logit_floor<T>(top);
-    }
-    if (t.m == -INFINITY) return top;
-    if (floor > -INFINITY) {
       if constexpr (sizeof(T) == 2) {
-        const uint32_t f = __float_as_uint(floor), ff = f | (f >> 16);  // floor is a BF16 number
-        uint32_t* w = reinterpret_cast<uint32_t*>(&raw[0]);
+        const uint32_t t = __float_as_uint(xt), tt = t | (t >> 16);
+        const uint32_t v[4] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w};
+        uint32_t n[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) asm("max.bf16x2 %0, %0, %1;" : "+r"(w[i]) : "r"(ff));
-        unpack_chunk<T>(raw, x);
+        for (int i = 0; i < 4; ++i)  // 1.0 or 0.0 in either half
+          asm("set.gt.bf16x2.bf16x2 %0, %1, %2;" : "=r"(n[i]) : "r"(v[i]), "r"(tt));
+        asm("add.bf16x2 %0, %0, %1;" : "+r"(n[0]) : "r"(n[1]));
+        asm("add.bf16x2 %0, %0, %1;" : "+r"(n[2]) : "r"(n[3]));
+        asm("add.bf16x2 %0, %0, %1;" : "+r"(n[0]) : "r"(n[2]));
+        above += bf16lo_to_f32(n[0]) + bf16hi_to_f32(n[0]);
       } else {
+        float n = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = fmaxf(x[e], floor);
+        for (int e = 0; e < 8; ++e) n += x[e] > xt ? 1.0f : 0.0f;
+        above += n;
       }
-      float s0 = 0.0f, s1 = 0.0f, w0 = 0.0f, w1 = 0.0f;
-#pragma unroll
-      for (int e = 0; e < 8; e += 2) {
-        const float d0 = x[e] - t.m, d1 = x[e + 1] - t.m;
-        const float e0 = ex2(d0 * kLog2e), e1 = ex2(d1 * kLog2e);
-        s0 += e0, s1 += e1;
-        w0 = fmaf(e0, d0, w0), w1 = fmaf(e1, d1, w1);
-      }
-      t.s += s0 + s1;
-      t.w += w0 + w1;
-    } else {  // the maximum is the type's lowest value: the others are it or -inf
-      unpack_chunk<T>(raw, x);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) t.s += x[e] == t.m ? 1.0f : 0.0f;
     }
+    // Clamped to the floor, d stays finite (0 * -inf would be NaN) and its exponential 0.
+    if constexpr (sizeof(T) == 2) {
+      const uint32_t f = __float_as_uint(floor), ff = f | (f >> 16);  // floor is a BF16 number
+      uint32_t* v = reinterpret_cast<uint32_t*>(&raw[0]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) asm("max.bf16x2 %0, %0, %1;" : "+r"(v[i]) : "r"(ff));
+      unpack_chunk<T>(raw, x);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = fmaxf(x[e], floor);
+    }
+    float s0 = 0.0f, s1 = 0.0f, w0 = 0.0f, w1 = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      const float d0 = x[e] - m, d1 = x[e + 1] - m;
+      const float e0 = ex2(d0 * kLog2e), e1 = ex2(d1 * kLog2e);
+      s0 += e0, s1 += e1;
+      w0 = fmaf(e0, d0, w0), w1 = fmaf(e1, d1, w1);
+    }
+    s += s0 + s1;
+    w += w0 + w1;
     return top;
   }
 };
@@ -306,27 +315,55 @@ __global__ void __launch_bounds__(kLpThreads, kLpCtasPerSm) token_logprobs_kerne
   const bool tops = p.top_k > 0;
   if (tid == 0) bound = 0, num_picked = 0;
 
-  LaneStat<T> st;
-  st.t.m = -INFINITY, st.t.s = st.t.w = 0.0f, st.t.above = 0;
-  st.floor = -INFINITY;
-  st.nan = false;
-  for (int c = c0 + warp; c < c1; c += kLpWarps * kAhead) {
+  WarpStat<T> st;
+  const auto take = [&](uint4 (&raw)[kVecs], int c) {
+    const float top = st.add(raw, xt);
+    if (tops) {
+      const uint32_t most = __reduce_max_sync(0xffffffffu, logit_order(top));
+      if (lane == 0) maxima[c - c0] = most;
+    }
+  };
+  // Only the row's first and last chunk can lie partly outside it.
+  const int in0 = c0 * kLpChunk >= lo ? c0 : c0 + 1, in1 = c1 * kLpChunk <= hi ? c1 : c1 - 1;
+  for (int c = in0 + warp; c < in1; c += kLpWarps * kAhead) {
     uint4 raw[kAhead][kVecs];
+    const T* at = base + static_cast<int64_t>(c) * kLpChunk + lane * kVec;
 #pragma unroll
     for (int u = 0; u < kAhead; ++u)
-      if (c + u * kLpWarps < c1) load_chunk<T>(base, c + u * kLpWarps, lane, lo, hi, raw[u]);
+      if (c + u * kLpWarps < in1)
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      if (c + u * kLpWarps >= c1) break;
-      const float top = st.add(raw[u], xt);
-      if (tops) {
-        const uint32_t most = __reduce_max_sync(0xffffffffu, logit_order(top));
-        if (lane == 0) maxima[c + u * kLpWarps - c0] = most;
-      }
-    }
+        for (int v = 0; v < kVecs; ++v)
+          raw[u][v] = __ldg(reinterpret_cast<const uint4*>(at + u * kLpWarps * kLpChunk + v * 32 * kVec));
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (c + u * kLpWarps < in1) take(raw[u], c + u * kLpWarps);
   }
-  st.t = warp_join(st.t);
-  if (lane == 0) stats[warp] = st.t;
+  // The first by warp 0, the last by warp 1 (by warp 0 if it is the first as well).
+  int end = -1;
+  if (warp == 0 && in0 > c0) end = c0;
+  else if (in1 < c1 && warp == (c1 - 1 == c0 ? 0 : 1)) end = c1 - 1;
+  if (end >= 0) {
+    uint4 raw[kVecs];
+    load_chunk<T>(base, end, lane, lo, hi, raw);
+    take(raw, end);
+  }
+  if (is_big(st.m)) {  // the lowest value, if nothing was above it; else the maximum: count what equals it
+    st.s = st.w = 0.0f;
+    for (int c = in0 + warp; c < in1 + kLpWarps; c += kLpWarps) {
+      const int own = c < in1 ? c : end;
+      if (own < 0) break;
+      uint4 raw[kVecs];
+      float v[8];
+      load_chunk<T>(base, own, lane, lo, hi, raw);
+      unpack_chunk<T>(raw, v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) st.s += v[e] == st.m ? 1.0f : 0.0f;
+      if (own == end) break;
+    }
+    if (!__any_sync(0xffffffffu, st.s > 0.0f)) st.m = -INFINITY;
+  }
+  const LogprobStat mine = warp_join({st.m, st.s, st.w, static_cast<int>(st.above)});
+  if (lane == 0) stats[warp] = mine;
   const bool nan = __syncthreads_or(st.nan);
 
   uint64_t list = 0;
