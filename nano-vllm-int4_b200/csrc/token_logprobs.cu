@@ -37,6 +37,7 @@ constexpr int kLpChunk = 256;
 constexpr int kLpMaxTop = NV4_LOGPROB_MAX_TOP;
 constexpr int kLpMaxChunks = 2048;    // of a CTA: their maxima are held in shared memory
 constexpr int kLpCtasPerSm = 4;
+constexpr int kLpRingBytes = 4096;    // of a warp: 8 BF16 or 4 FP32 chunks in flight
 constexpr int kLpMaxSplits = 64;      // but for rows whose chunks need more
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -198,12 +199,36 @@ __device__ __forceinline__ void finish_row(const LogprobArgs& p, int64_t row, fl
   }
 }
 
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t a, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(a));
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
 // The statistics that a warp gathers: the reference is the warp's, the sums and the
 // count are the lanes'.
 template <typename T>
 struct WarpStat {
   float m, limit, floor;  // reference, m + 1; m - 110 or less, whose exponential is 0
-  float s = 0.0f, w = 0.0f;
+  uint64_t s = 0, w = 0;  // pairs of FP32: even and odd elements
   float above = 0.0f;  // whole numbers below 2^24
   bool nan = false;
 
@@ -241,7 +266,13 @@ struct WarpStat {
       const uint32_t order = __reduce_max_sync(0xffffffffu, logit_order(top));
       const float most = key_logit(static_cast<uint64_t>(order) << 32);
       if (order != 0 && most > m) {
-        move_stat(s, w, m, most);
+        float s0, s1, w0, w1;
+        unpair(s, s0, s1);
+        unpair(w, w0, w1);
+        move_stat(s0, w0, m, most);
+        move_stat(s1, w1, m, most);
+        s = pair(s0, s1);
+        w = pair(w0, w1);
         refer(most);
       }
     }
@@ -275,31 +306,35 @@ struct WarpStat {
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[e] = fmaxf(x[e], floor);
     }
-    float s0 = 0.0f, s1 = 0.0f, w0 = 0.0f, w1 = 0.0f;
+    // Two at a time: the packed FP32 operations halve the issue slots.
+    const uint64_t minus_m = pair(-m, -m), log2e = pair(kLog2e, kLog2e);
 #pragma unroll
     for (int e = 0; e < 8; e += 2) {
-      const float d0 = x[e] - m, d1 = x[e + 1] - m;
-      const float e0 = ex2(d0 * kLog2e), e1 = ex2(d1 * kLog2e);
-      s0 += e0, s1 += e1;
-      w0 = fmaf(e0, d0, w0), w1 = fmaf(e1, d1, w1);
+      const uint64_t d = add2(pair(x[e], x[e + 1]), minus_m);
+      float y0, y1;
+      unpair(mul2(d, log2e), y0, y1);
+      const uint64_t g = pair(ex2(y0), ex2(y1));
+      s = add2(s, g);
+      w = fma2(g, d, w);
     }
-    s += s0 + s1;
-    w += w0 + w1;
     return top;
   }
 };
 
 template <typename T>
 __global__ void __launch_bounds__(kLpThreads, kLpCtasPerSm) token_logprobs_kernel(const LogprobArgs p) {
+  // The warps' rings of chunks in flight; after the pass the picked chunks and the lists.
+  __shared__ __align__(16) uint8_t ring[kLpWarps * kLpRingBytes];
   __shared__ uint32_t maxima[kLpMaxChunks];
-  __shared__ int picked[kLpMaxChunks];
-  __shared__ uint64_t lists[kLpWarps][32];
+  int* picked = reinterpret_cast<int*>(ring);
+  uint64_t(*lists)[32] = reinterpret_cast<uint64_t(*)[32]>(ring + kLpMaxChunks * sizeof(int));
+  static_assert(kLpMaxChunks * sizeof(int) + kLpWarps * 32 * 8 <= kLpWarps * kLpRingBytes, "they fit");
   __shared__ uint32_t sorted[kLpWarps][32];
   __shared__ LogprobStat stats[kLpWarps];
   __shared__ uint32_t bound;
   __shared__ int num_picked;
   constexpr int kVecs = LaneOf<T>::kVecs, kVec = LaneOf<T>::kVec;
-  constexpr int kAhead = 4 / kVecs;  // chunks a warp loads ahead: 64 bytes a lane
+  constexpr int kDepth = kLpRingBytes / (kLpChunk * sizeof(T));
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t row = blockIdx.x / p.splits;
   const int split = static_cast<int>(blockIdx.x - row * p.splits);
@@ -325,18 +360,32 @@ __global__ void __launch_bounds__(kLpThreads, kLpCtasPerSm) token_logprobs_kerne
   };
   // Only the row's first and last chunk can lie partly outside it.
   const int in0 = c0 * kLpChunk >= lo ? c0 : c0 + 1, in1 = c1 * kLpChunk <= hi ? c1 : c1 - 1;
-  for (int c = in0 + warp; c < in1; c += kLpWarps * kAhead) {
-    uint4 raw[kAhead][kVecs];
-    const T* at = base + static_cast<int64_t>(c) * kLpChunk + lane * kVec;
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u)
-      if (c + u * kLpWarps < in1)
+  // A lane copies into the ring what it reads back itself, so no barrier is needed.
+  {
+    const int n = (in1 - in0 - warp + kLpWarps - 1) / kLpWarps;
+    uint8_t* slot = ring + warp * kLpRingBytes + lane * 16;
+    const T* at = base + static_cast<int64_t>(in0 + warp) * kLpChunk + lane * kVec;
+    const auto issue = [&](int i) {
+      if (i < n)
 #pragma unroll
         for (int v = 0; v < kVecs; ++v)
-          raw[u][v] = __ldg(reinterpret_cast<const uint4*>(at + u * kLpWarps * kLpChunk + v * 32 * kVec));
+          cp_async16(smem_u32(slot + (i % kDepth * kVecs + v) * 512),
+                     at + static_cast<int64_t>(i) * kLpWarps * kLpChunk + v * 32 * kVec, 16);
+      cp_async_commit();
+    };
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u)
-      if (c + u * kLpWarps < in1) take(raw[u], c + u * kLpWarps);
+    for (int i = 0; i < kDepth; ++i) issue(i);
+#pragma unroll 1
+    for (int i = 0; i < n; ++i) {
+      cp_async_wait<kDepth - 1>();
+      uint4 raw[kVecs];
+#pragma unroll
+      for (int v = 0; v < kVecs; ++v)
+        raw[v] = *reinterpret_cast<const uint4*>(slot + (i % kDepth * kVecs + v) * 512);
+      take(raw, in0 + warp + i * kLpWarps);
+      issue(i + kDepth);
+    }
+    cp_async_wait<0>();
   }
   // The first by warp 0, the last by warp 1 (by warp 0 if it is the first as well).
   int end = -1;
@@ -347,8 +396,13 @@ __global__ void __launch_bounds__(kLpThreads, kLpCtasPerSm) token_logprobs_kerne
     load_chunk<T>(base, end, lane, lo, hi, raw);
     take(raw, end);
   }
+  float s, w, s1, w1;
+  unpair(st.s, s, s1);
+  unpair(st.w, w, w1);
+  s += s1;
+  w += w1;
   if (is_big(st.m)) {  // the lowest value, if nothing was above it; else the maximum: count what equals it
-    st.s = st.w = 0.0f;
+    s = w = 0.0f;
     for (int c = in0 + warp; c < in1 + kLpWarps; c += kLpWarps) {
       const int own = c < in1 ? c : end;
       if (own < 0) break;
@@ -357,12 +411,12 @@ __global__ void __launch_bounds__(kLpThreads, kLpCtasPerSm) token_logprobs_kerne
       load_chunk<T>(base, own, lane, lo, hi, raw);
       unpack_chunk<T>(raw, v);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) st.s += v[e] == st.m ? 1.0f : 0.0f;
+      for (int e = 0; e < 8; ++e) s += v[e] == st.m ? 1.0f : 0.0f;
       if (own == end) break;
     }
-    if (!__any_sync(0xffffffffu, st.s > 0.0f)) st.m = -INFINITY;
+    if (!__any_sync(0xffffffffu, s > 0.0f)) st.m = -INFINITY;
   }
-  const LogprobStat mine = warp_join({st.m, st.s, st.w, static_cast<int>(st.above)});
+  const LogprobStat mine = warp_join({st.m, s, w, static_cast<int>(st.above)});
   if (lane == 0) stats[warp] = mine;
   const bool nan = __syncthreads_or(st.nan);
 
