@@ -11,16 +11,16 @@
 // Alternatives are ordered by logit, ties to the lowest index.
 //
 // One pass over the logits, bound by HBM where there are many rows, with the
-// exponential unit (16 a cycle and SM) next.  A warp takes chunks of 256
-// contiguous logits, eight a lane, and moves its reference when a chunk's maximum
+// exponential unit (16 a cycle and SM) next.  A warp takes chunks of 512
+// contiguous logits, 16 a lane, and moves its reference when a chunk's maximum
 // exceeds it by more than 1: that happens a few times a row for the warp, while
 // every lane's own maximum would move in most chunks for some lane.  The rank
 // costs one comparison with the chunk's maximum unless that exceeds the token's
-// logit.  The alternatives cost one maximum per
-// chunk in that pass: the k largest elements lie in the k chunks with the largest
-// maxima (for any other chunk there are k elements above all of it), so after the
-// pass a threshold is found among the maxima, the few chunks that reach it are
-// read again (from L2) and their elements above it sorted.
+// logit.  The alternatives cost a
+// maximum per chunk and per lane in that pass: the k-th largest of the lanes'
+// maxima bounds the k-th largest logit from below (k logits reach it), so the few
+// chunks whose maximum reaches it are read again (from L2) and their logits that
+// do are sorted.
 //
 // With few rows a row is split over several CTAs, whose results a second kernel
 // joins.
@@ -33,11 +33,12 @@ namespace nv4 {
 
 constexpr int kLpThreads = 256;
 constexpr int kLpWarps = kLpThreads / 32;
-constexpr int kLpChunk = 256;
+constexpr int kLpChunk = 512;
+constexpr int kLpLane = kLpChunk / 32;  // logits of a chunk that a lane takes
 constexpr int kLpMaxTop = NV4_LOGPROB_MAX_TOP;
 constexpr int kLpMaxChunks = 2048;    // of a CTA: their maxima are held in shared memory
 constexpr int kLpCtasPerSm = 4;
-constexpr int kLpRingBytes = 4096;    // of a warp: 8 BF16 or 4 FP32 chunks in flight
+constexpr int kLpRingBytes = 4096;    // of a warp: 4 BF16 or 2 FP32 chunks in flight
 constexpr int kLpMaxSplits = 64;      // but for rows whose chunks need more
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -82,15 +83,15 @@ __device__ __forceinline__ float key_logit(uint64_t key) {
   return __uint_as_float((order & 0x80000000u) ? (order & 0x7FFFFFFFu) : ~order);
 }
 
-// The eight logits of a lane in a chunk: 8 consecutive BF16 or twice 4 FP32
-// elements.  `base` is the row's start rounded down to 16 bytes, the row's own
+// The 16 logits of a lane in a chunk: twice 8 consecutive BF16 or four times 4
+// FP32 elements.  `base` is the row's start rounded down to 16 bytes, the row's own
 // elements are base[lo .. hi); what lies outside is not read and counts as -inf.
 __device__ __forceinline__ float load_logit(const float* p) { return __ldg(p); }
 __device__ __forceinline__ float load_logit(const uint16_t* p) { return bf16_bits_to_f32(__ldg(p)); }
 
 template <typename T>
 struct LaneOf {
-  static constexpr int kVec = 16 / sizeof(T), kVecs = 8 / kVec;
+  static constexpr int kVec = 16 / sizeof(T), kVecs = kLpLane / kVec;
   static __device__ __forceinline__ int offset(int lane, int e) {  // of element e of a lane within the chunk
     return (e / kVec) * 32 * kVec + lane * kVec + e % kVec;
   }
@@ -123,17 +124,19 @@ __device__ __forceinline__ void load_chunk(const T* base, int chunk, int lane, i
   }
 }
 template <typename T>
-__device__ __forceinline__ void unpack_chunk(const uint4 (&raw)[LaneOf<T>::kVecs], float (&x)[8]) {
-  if constexpr (sizeof(T) == 4) {
+__device__ __forceinline__ void unpack_chunk(const uint4 (&raw)[LaneOf<T>::kVecs], float (&x)[kLpLane]) {
 #pragma unroll
-    for (int v = 0; v < 2; ++v) {
-      x[4 * v] = __uint_as_float(raw[v].x), x[4 * v + 1] = __uint_as_float(raw[v].y);
-      x[4 * v + 2] = __uint_as_float(raw[v].z), x[4 * v + 3] = __uint_as_float(raw[v].w);
+  for (int v = 0; v < LaneOf<T>::kVecs; ++v) {
+    const uint32_t w[4] = {raw[v].x, raw[v].y, raw[v].z, raw[v].w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        x[4 * v + i] = __uint_as_float(w[i]);
+      } else {
+        x[8 * v + 2 * i] = bf16lo_to_f32(w[i]);
+        x[8 * v + 2 * i + 1] = bf16hi_to_f32(w[i]);
+      }
     }
-  } else {
-    const uint32_t w[4] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[2 * i] = bf16lo_to_f32(w[i]), x[2 * i + 1] = bf16hi_to_f32(w[i]);
   }
 }
 
@@ -242,18 +245,19 @@ struct WarpStat {
 
   // The chunk's logits; returns the lane's maximum (NaN aside).
   __device__ __forceinline__ float add(uint4 (&raw)[LaneOf<T>::kVecs], float xt) {
-    float x[8], top;
+    constexpr int kWords = 4 * LaneOf<T>::kVecs;
+    uint32_t* word = reinterpret_cast<uint32_t*>(&raw[0]);
+    float x[kLpLane], top;
     if constexpr (sizeof(T) == 2) {
-      uint32_t a, b;
-      asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(a) : "r"(raw[0].x), "r"(raw[0].y));
-      asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(b) : "r"(raw[0].z), "r"(raw[0].w));
-      asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(a) : "r"(a), "r"(b));
+      uint32_t a = word[0];
+#pragma unroll
+      for (int i = 1; i < kWords; ++i) asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(a) : "r"(word[i]));
       asm("max.NaN.f32 %0, %1, %2;" : "=f"(top) : "f"(bf16lo_to_f32(a)), "f"(bf16hi_to_f32(a)));
     } else {
       unpack_chunk<T>(raw, x);
       top = x[0];
 #pragma unroll
-      for (int e = 1; e < 8; ++e) asm("max.NaN.f32 %0, %1, %2;" : "=f"(top) : "f"(top), "f"(x[e]));
+      for (int e = 1; e < kLpLane; ++e) asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(x[e]));
     }
     if (__any_sync(0xffffffffu, !(top <= limit))) {
       if (top != top) {
@@ -261,7 +265,7 @@ struct WarpStat {
         unpack_chunk<T>(raw, x);
         top = -INFINITY;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) top = fmaxf(top, x[e]);
+        for (int e = 0; e < kLpLane; ++e) top = fmaxf(top, x[e]);
       }
       const uint32_t order = __reduce_max_sync(0xffffffffu, logit_order(top));
       const float most = key_logit(static_cast<uint64_t>(order) << 32);
@@ -279,37 +283,35 @@ struct WarpStat {
     if (top > xt) {
       if constexpr (sizeof(T) == 2) {
         const uint32_t t = __float_as_uint(xt), tt = t | (t >> 16);
-        const uint32_t v[4] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w};
-        uint32_t n[4];
+        uint32_t n = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)  // 1.0 or 0.0 in either half
-          asm("set.gt.bf16x2.bf16x2 %0, %1, %2;" : "=r"(n[i]) : "r"(v[i]), "r"(tt));
-        asm("add.bf16x2 %0, %0, %1;" : "+r"(n[0]) : "r"(n[1]));
-        asm("add.bf16x2 %0, %0, %1;" : "+r"(n[2]) : "r"(n[3]));
-        asm("add.bf16x2 %0, %0, %1;" : "+r"(n[0]) : "r"(n[2]));
-        above += bf16lo_to_f32(n[0]) + bf16hi_to_f32(n[0]);
+        for (int i = 0; i < kWords; ++i) {
+          uint32_t g;  // 1.0 or 0.0 in either half
+          asm("set.gt.bf16x2.bf16x2 %0, %1, %2;" : "=r"(g) : "r"(word[i]), "r"(tt));
+          asm("add.bf16x2 %0, %0, %1;" : "+r"(n) : "r"(g));
+        }
+        above += bf16lo_to_f32(n) + bf16hi_to_f32(n);
       } else {
         float n = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) n += x[e] > xt ? 1.0f : 0.0f;
+        for (int e = 0; e < kLpLane; ++e) n += x[e] > xt ? 1.0f : 0.0f;
         above += n;
       }
     }
     // Clamped to the floor, d stays finite (0 * -inf would be NaN) and its exponential 0.
     if constexpr (sizeof(T) == 2) {
       const uint32_t f = __float_as_uint(floor), ff = f | (f >> 16);  // floor is a BF16 number
-      uint32_t* v = reinterpret_cast<uint32_t*>(&raw[0]);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) asm("max.bf16x2 %0, %0, %1;" : "+r"(v[i]) : "r"(ff));
+      for (int i = 0; i < kWords; ++i) asm("max.bf16x2 %0, %0, %1;" : "+r"(word[i]) : "r"(ff));
       unpack_chunk<T>(raw, x);
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = fmaxf(x[e], floor);
+      for (int e = 0; e < kLpLane; ++e) x[e] = fmaxf(x[e], floor);
     }
     // Two at a time: the packed FP32 operations halve the issue slots.
     const uint64_t minus_m = pair(-m, -m), log2e = pair(kLog2e, kLog2e);
 #pragma unroll
-    for (int e = 0; e < 8; e += 2) {
+    for (int e = 0; e < kLpLane; e += 2) {
       const uint64_t d = add2(pair(x[e], x[e + 1]), minus_m);
       float y0, y1;
       unpair(mul2(d, log2e), y0, y1);
@@ -351,9 +353,11 @@ __global__ void __launch_bounds__(kLpThreads, kLpCtasPerSm) token_logprobs_kerne
   if (tid == 0) bound = 0, num_picked = 0;
 
   WarpStat<T> st;
+  float largest = -INFINITY;  // of the lane's logits
   const auto take = [&](uint4 (&raw)[kVecs], int c) {
     const float top = st.add(raw, xt);
     if (tops) {
+      largest = fmaxf(largest, top);
       const uint32_t most = __reduce_max_sync(0xffffffffu, logit_order(top));
       if (lane == 0) maxima[c - c0] = most;
     }
@@ -362,28 +366,37 @@ __global__ void __launch_bounds__(kLpThreads, kLpCtasPerSm) token_logprobs_kerne
   const int in0 = c0 * kLpChunk >= lo ? c0 : c0 + 1, in1 = c1 * kLpChunk <= hi ? c1 : c1 - 1;
   // A lane copies into the ring what it reads back itself, so no barrier is needed.
   {
+    constexpr int kBytes = kLpChunk * sizeof(T), kDepth = kLpRingBytes / kBytes;
+    constexpr int64_t kStep = static_cast<int64_t>(kLpWarps) * kLpChunk;
     const int n = (in1 - in0 - warp + kLpWarps - 1) / kLpWarps;
-    uint8_t* slot = ring + warp * kLpRingBytes + lane * 16;
+    const uint32_t slots = smem_u32(ring) + warp * kLpRingBytes + lane * 16;
     const T* at = base + static_cast<int64_t>(in0 + warp) * kLpChunk + lane * kVec;
-    const auto issue = [&](int i) {
-      if (i < n)
+    const auto issue = [&](uint32_t slot) {
 #pragma unroll
-        for (int v = 0; v < kVecs; ++v)
-          cp_async16(smem_u32(slot + (i % kDepth * kVecs + v) * 512),
-                     at + static_cast<int64_t>(i) * kLpWarps * kLpChunk + v * 32 * kVec, 16);
-      cp_async_commit();
+      for (int v = 0; v < kVecs; ++v) cp_async16(slot + v * 512, at + v * 32 * kVec, 16);
+      at += kStep;
     };
 #pragma unroll
-    for (int i = 0; i < kDepth; ++i) issue(i);
+    for (int i = 0; i < kDepth; ++i) {
+      if (i < n) issue(slots + i * kBytes);
+      cp_async_commit();
+    }
+    uint32_t slot = slots, turn = slots + kLpRingBytes;
 #pragma unroll 1
     for (int i = 0; i < n; ++i) {
       cp_async_wait<kDepth - 1>();
       uint4 raw[kVecs];
 #pragma unroll
       for (int v = 0; v < kVecs; ++v)
-        raw[v] = *reinterpret_cast<const uint4*>(slot + (i % kDepth * kVecs + v) * 512);
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(raw[v].x), "=r"(raw[v].y), "=r"(raw[v].z), "=r"(raw[v].w)
+                     : "r"(slot + v * 512)
+                     : "memory");
       take(raw, in0 + warp + i * kLpWarps);
-      issue(i + kDepth);
+      if (i + kDepth < n) issue(slot);
+      cp_async_commit();
+      slot += kBytes;
+      if (slot == turn) slot = slots;
     }
     cp_async_wait<0>();
   }
@@ -407,11 +420,11 @@ __global__ void __launch_bounds__(kLpThreads, kLpCtasPerSm) token_logprobs_kerne
       const int own = c < in1 ? c : end;
       if (own < 0) break;
       uint4 raw[kVecs];
-      float v[8];
+      float v[kLpLane];
       load_chunk<T>(base, own, lane, lo, hi, raw);
       unpack_chunk<T>(raw, v);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) s += v[e] == st.m ? 1.0f : 0.0f;
+      for (int e = 0; e < kLpLane; ++e) s += v[e] == st.m ? 1.0f : 0.0f;
       if (own == end) break;
     }
     if (!__any_sync(0xffffffffu, s > 0.0f)) st.m = -INFINITY;
@@ -422,10 +435,9 @@ __global__ void __launch_bounds__(kLpThreads, kLpCtasPerSm) token_logprobs_kerne
 
   uint64_t list = 0;
   if (tops) {
-    // The top_k-th largest of the threads' largest maxima bounds that of the row from
-    // below.  Each warp sorts its 32; a key's rank is its lane plus what the others hold above it.
-    uint32_t key = 0;
-    for (int i = tid; i < c1 - c0; i += kLpThreads) key = max(key, maxima[i]);
+    // The top_k-th largest of the lanes' maxima.  Each warp sorts its 32; a key's rank
+    // is its lane plus the number of the other warps' keys before it.
+    uint32_t key = logit_order(largest);
 #pragma unroll
     for (int k = 2; k <= 32; k <<= 1)
 #pragma unroll
@@ -461,10 +473,10 @@ __global__ void __launch_bounds__(kLpThreads, kLpCtasPerSm) token_logprobs_kerne
       const int c = c0 + picked[i];
       uint4 raw[kVecs];
       load_chunk<T>(base, c, lane, lo, hi, raw);
-      float v[8];
+      float v[kLpLane];
       unpack_chunk<T>(raw, v);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
+      for (int e = 0; e < kLpLane; ++e) {
         const uint32_t order = logit_order(v[e]);
         const uint64_t k = logit_key(order, c * kLpChunk + LaneOf<T>::offset(lane, e) - lo);
         uint32_t todo = __ballot_sync(0xffffffffu, order >= least && k > last);
