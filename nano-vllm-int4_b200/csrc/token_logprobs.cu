@@ -17,10 +17,11 @@
 // every lane's own maximum would move in most chunks for some lane.  The rank
 // costs one comparison with the chunk's maximum unless that exceeds the token's
 // logit.  The alternatives cost a
-// maximum per chunk and per lane in that pass: the k-th largest of the lanes'
-// maxima bounds the k-th largest logit from below (k logits reach it), so the few
-// chunks whose maximum reaches it are read again (from L2) and their logits that
-// do are sorted.
+// maximum per chunk and per lane in that pass: the k-th largest maximum of 64
+// groups of lanes bounds the k-th largest logit from below (k logits reach it), so
+// the few chunks whose maximum reaches it are read again (from L2), the logits
+// that do are collected (about k, unless many are equal) and each one's rank is
+// counted.
 //
 // With few rows a row is split over several CTAs, whose results a second kernel
 // joins.
@@ -39,7 +40,9 @@ constexpr int kLpMaxTop = NV4_LOGPROB_MAX_TOP;
 constexpr int kLpMaxChunks = 2048;    // of a CTA: their maxima are held in shared memory
 constexpr int kLpCtasPerSm = 4;
 constexpr int kLpRingBytes = 4096;    // of a warp: 4 BF16 or 2 FP32 chunks in flight
-constexpr int kLpMaxSplits = 64;      // but for rows whose chunks need more
+constexpr int kLpMaxFound = 512;      // logits that reach the alternatives' threshold; more take another way
+constexpr int kLpMaxSplits = 64;
+static_assert(NV4_LOGPROB_MAX_VOCAB / kLpChunk / kLpMaxChunks < kLpMaxSplits, "the longest row's parts");
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct LogprobArgs {
@@ -155,9 +158,9 @@ __device__ __forceinline__ LogprobStat join_stats(LogprobStat a, LogprobStat b) 
   move_stat(b.s, b.w, b.m, m);
   return {m, a.s + b.s, a.w + b.w, a.above + b.above};
 }
-__device__ __forceinline__ LogprobStat warp_join(LogprobStat t) {
-#pragma unroll
-  for (int o = 16; o >= 1; o >>= 1) {
+// Joins the lanes' statistics (in lane 0); `lanes` of them, a power of two.
+__device__ __forceinline__ LogprobStat warp_join(LogprobStat t, int lanes) {
+  for (int o = lanes >> 1; o >= 1; o >>= 1) {
     LogprobStat u;
     u.m = __shfl_xor_sync(0xffffffffu, t.m, o);
     u.s = __shfl_xor_sync(0xffffffffu, t.s, o);
@@ -174,16 +177,45 @@ __device__ __forceinline__ void list_insert(uint64_t& list, uint64_t key, int la
   const uint64_t up = __shfl_up_sync(0xffffffffu, list, 1);
   list = lane < pos ? list : lane == pos ? key : up;
 }
-// The 32 largest of two such lists.
-__device__ __forceinline__ uint64_t list_merge(uint64_t a, uint64_t b, int lane) {
-  const uint64_t r = __shfl_sync(0xffffffffu, b, 31 - lane);
-  a = a > r ? a : r;  // bitonic
+__device__ __forceinline__ float warp_max(float x) {
+  float d;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(d) : "f"(x));
+  return d;
+}
+
+// The k largest of n keys in shared memory, falling, to `out` (left as it is
+// where there are fewer): every thread counts the keys above its own.  Keys differ, but for 0.
+__device__ __forceinline__ void rank_keys(const uint64_t* keys, int n, int k, uint64_t* out, int tid) {
+  for (int i = tid; i < n; i += kLpThreads) {
+    const uint64_t mine = keys[i];
+    int rank = 0;
+    int j = 0;
+    for (; j + 8 <= n; j += 8)
 #pragma unroll
-  for (int o = 16; o >= 1; o >>= 1) {
-    const uint64_t t = __shfl_xor_sync(0xffffffffu, a, o);
-    a = ((lane & o) == 0) == (a > t) ? a : t;
+      for (int u = 0; u < 8; ++u) rank += keys[j + u] > mine;
+    for (; j < n; ++j) rank += keys[j] > mine;
+    if (mine != 0 && rank < k) out[rank] = mine;
   }
-  return a;
+}
+
+// The k largest keys of n <= 64 falling lists of k keys, `stride` apart in shared
+// memory, as a warp's list: k times the largest of the lists' heads.
+__device__ __forceinline__ uint64_t select_top(const uint64_t* lists, int stride, int n, int k, int lane) {
+  const uint64_t *a = lists + lane * stride, *b = a + 32 * stride;
+  uint64_t head_a = lane < n ? *a : 0, head_b = lane + 32 < n ? *b : 0, list = 0;
+  const uint64_t *end_a = a + k, *end_b = b + k;
+  for (int i = 0; i < k; ++i) {
+    const uint64_t head = head_a > head_b ? head_a : head_b;
+    const uint32_t high = __reduce_max_sync(0xffffffffu, static_cast<uint32_t>(head >> 32));
+    const uint32_t low =
+        __reduce_max_sync(0xffffffffu, static_cast<uint32_t>(head >> 32) == high ? static_cast<uint32_t>(head) : 0);
+    const uint64_t key = static_cast<uint64_t>(high) << 32 | low;
+    if (key == 0) break;
+    if (lane == i) list = key;
+    if (head_a == key) head_a = ++a < end_a ? *a : 0;
+    else if (head_b == key) head_b = ++b < end_b ? *b : 0;
+  }
+  return list;
 }
 
 // A row's results from its statistics and its list of keys (one warp).
@@ -325,16 +357,18 @@ struct WarpStat {
 
 template <typename T>
 __global__ void __launch_bounds__(kLpThreads, kLpCtasPerSm) token_logprobs_kernel(const LogprobArgs p) {
-  // The warps' rings of chunks in flight; after the pass the picked chunks and the lists.
+  // The warps' rings of chunks in flight; after the pass the collected keys and the lists.
   __shared__ __align__(16) uint8_t ring[kLpWarps * kLpRingBytes];
-  __shared__ uint32_t maxima[kLpMaxChunks];
-  int* picked = reinterpret_cast<int*>(ring);
-  uint64_t(*lists)[32] = reinterpret_cast<uint64_t(*)[32]>(ring + kLpMaxChunks * sizeof(int));
-  static_assert(kLpMaxChunks * sizeof(int) + kLpWarps * 32 * 8 <= kLpWarps * kLpRingBytes, "they fit");
-  __shared__ uint32_t sorted[kLpWarps][32];
+  __shared__ float maxima[kLpMaxChunks];
+  uint64_t* found = reinterpret_cast<uint64_t*>(ring);                           // [kLpMaxFound]
+  uint64_t(*lists)[32] = reinterpret_cast<uint64_t(*)[32]>(found + kLpMaxFound);  // [kLpWarps]
+  uint64_t* sorted = lists[kLpWarps];                                            // [kLpMaxTop]
+  static_assert((kLpMaxFound + (kLpWarps + 1) * 32) * 8 <= kLpWarps * kLpRingBytes, "they fit");
+  __shared__ float lane_max[kLpWarps][32];
+  __shared__ float group_max[64];
   __shared__ LogprobStat stats[kLpWarps];
-  __shared__ uint32_t bound;
-  __shared__ int num_picked;
+  __shared__ float bound;
+  __shared__ int num_found;
   constexpr int kVecs = LaneOf<T>::kVecs, kVec = LaneOf<T>::kVec;
   constexpr int kDepth = kLpRingBytes / (kLpChunk * sizeof(T));
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -346,19 +380,19 @@ __global__ void __launch_bounds__(kLpThreads, kLpCtasPerSm) token_logprobs_kerne
   const int chunks = (hi + kLpChunk - 1) / kLpChunk;
   const int c0 = static_cast<int>(static_cast<int64_t>(chunks) * split / p.splits);
   const int c1 = static_cast<int>(static_cast<int64_t>(chunks) * (split + 1) / p.splits);
-  const int64_t target = p.targets[row];
-  const bool given = target >= 0 && target < p.vocab;
-  const float xt = given ? load_logit(x + target) : INFINITY;
   const bool tops = p.top_k > 0;
-  if (tid == 0) bound = 0, num_picked = 0;
+  if (tid == 0) num_found = 0;
 
+  int64_t target;
+  bool given;
+  float xt;
   WarpStat<T> st;
   float largest = -INFINITY;  // of the lane's logits
   const auto take = [&](uint4 (&raw)[kVecs], int c) {
     const float top = st.add(raw, xt);
     if (tops) {
       largest = fmaxf(largest, top);
-      const uint32_t most = __reduce_max_sync(0xffffffffu, logit_order(top));
+      const float most = warp_max(top);
       if (lane == 0) maxima[c - c0] = most;
     }
   };
@@ -381,6 +415,9 @@ __global__ void __launch_bounds__(kLpThreads, kLpCtasPerSm) token_logprobs_kerne
       if (i < n) issue(slots + i * kBytes);
       cp_async_commit();
     }
+    target = p.targets[row];  // these two loads follow one another: behind the copies
+    given = target >= 0 && target < p.vocab;
+    xt = given ? load_logit(x + target) : INFINITY;
     uint32_t slot = slots, turn = slots + kLpRingBytes;
 #pragma unroll 1
     for (int i = 0; i < n; ++i) {
@@ -429,76 +466,84 @@ __global__ void __launch_bounds__(kLpThreads, kLpCtasPerSm) token_logprobs_kerne
     }
     if (!__any_sync(0xffffffffu, s > 0.0f)) st.m = -INFINITY;
   }
-  const LogprobStat mine = warp_join({st.m, s, w, static_cast<int>(st.above)});
-  if (lane == 0) stats[warp] = mine;
+  int above = static_cast<int>(st.above);
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) {  // one reference a warp: plain sums
+    s += __shfl_xor_sync(0xffffffffu, s, o);
+    w += __shfl_xor_sync(0xffffffffu, w, o);
+    above += __shfl_xor_sync(0xffffffffu, above, o);
+  }
+  if (lane == 0) stats[warp] = {st.m, s, w, above};
+  if (tops) lane_max[warp][lane] = largest;
   const bool nan = __syncthreads_or(st.nan);
 
   uint64_t list = 0;
   if (tops) {
-    // The top_k-th largest of the lanes' maxima.  Each warp sorts its 32; a key's rank
-    // is its lane plus the number of the other warps' keys before it.
-    uint32_t key = logit_order(largest);
+    // The top_k-th largest of 64 maxima, each of a lane of four warps.
+    if (tid < kLpMaxTop) sorted[tid] = 0;
+    if (tid < 64) {
+      float g = lane_max[warp * 4][lane];
 #pragma unroll
-    for (int k = 2; k <= 32; k <<= 1)
+      for (int i = 1; i < 4; ++i) g = fmaxf(g, lane_max[warp * 4 + i][lane]);
+      group_max[tid] = g;
+      named_barrier_sync(1, 64);
+      int rank = 0;
 #pragma unroll
-      for (int o = k >> 1; o >= 1; o >>= 1) {
-        const uint32_t other = __shfl_xor_sync(0xffffffffu, key, o);
-        const bool larger = ((lane & o) == 0) == ((lane & k) == 0);  // falling over the lanes
-        key = larger ? max(key, other) : min(key, other);
-      }
-    sorted[warp][lane] = key;
-    __syncthreads();
-    int rank = lane;
-#pragma unroll
-    for (int w = 0; w < kLpWarps; ++w) {
-      if (w == warp) continue;
-      int n = 0;  // keys of warp w before this one: above it, or equal and of an earlier warp
-#pragma unroll
-      for (int o = 16; o >= 1; o >>= 1) {
-        const uint32_t other = sorted[w][n + o - 1];
-        if (other > key || (other == key && w < warp)) n += o;
-      }
-      if (n == 31) n += sorted[w][31] > key || (sorted[w][31] == key && w < warp);
-      rank += n;
+      for (int i = 0; i < 64; ++i) rank += group_max[i] > g || (group_max[i] == g && i < tid);
+      if (rank == p.top_k - 1) bound = fmaxf(g, -FLT_MAX);  // -inf: no alternative
     }
-    if (rank == p.top_k - 1) bound = key;
     __syncthreads();
-    const uint32_t least = max(bound, 1u);  // 0: chunks of nothing but -inf
-    for (int i = tid; i < c1 - c0; i += kLpThreads)
-      if (maxima[i] >= least) picked[atomicAdd(&num_picked, 1)] = i;  // in any order: the keys are ordered
-    __syncthreads();
-    const int n = num_picked;
-    uint64_t last = 0;  // the warp's top_k-th key
-    for (int i = warp; i < n; i += kLpWarps) {
-      const int c = c0 + picked[i];
-      uint4 raw[kVecs];
-      load_chunk<T>(base, c, lane, lo, hi, raw);
-      float v[kLpLane];
-      unpack_chunk<T>(raw, v);
+    // The warp's own chunks that reach it.
+    const float least = bound;
+    const auto each_picked = [&](const auto& use) {
+      for (int i0 = 0; i0 < c1 - c0; i0 += 32 * kLpWarps) {
+        const int i = i0 + lane * kLpWarps + warp;
+        uint32_t todo = __ballot_sync(0xffffffffu, i < c1 - c0 && maxima[i] >= least);
+        for (; todo; todo &= todo - 1) {
+          const int c = c0 + i0 + (__ffs(todo) - 1) * kLpWarps + warp;
+          uint4 raw[kVecs];
+          float v[kLpLane];
+          load_chunk<T>(base, c, lane, lo, hi, raw);
+          unpack_chunk<T>(raw, v);
 #pragma unroll
-      for (int e = 0; e < kLpLane; ++e) {
-        const uint32_t order = logit_order(v[e]);
-        const uint64_t k = logit_key(order, c * kLpChunk + LaneOf<T>::offset(lane, e) - lo);
-        uint32_t todo = __ballot_sync(0xffffffffu, order >= least && k > last);
+          for (int e = 0; e < kLpLane; ++e) use(v[e], c * kLpChunk + LaneOf<T>::offset(lane, e) - lo);
+        }
+      }
+    };
+    each_picked([&](float v, int index) {
+      if (v >= least) {
+        const int at = atomicAdd(&num_found, 1);  // in any order: the keys are ordered
+        if (at < kLpMaxFound) found[at] = logit_key(logit_order(v), index);
+      }
+    });
+    __syncthreads();
+    if (num_found <= kLpMaxFound) {
+      rank_keys(found, num_found, p.top_k, sorted, tid);
+      __syncthreads();
+    } else {  // many equal logits: a sorted list per warp, then the lists' heads
+      uint64_t last = 0;  // the warp's top_k-th key
+      each_picked([&](float v, int index) {
+        const uint64_t k = logit_key(logit_order(v), index);
+        uint32_t todo = __ballot_sync(0xffffffffu, v >= least && k > last);
         while (todo) {
-          const int from = __ffs(todo) - 1;
-          list_insert(list, __shfl_sync(0xffffffffu, k, from), lane);
+          list_insert(list, __shfl_sync(0xffffffffu, k, __ffs(todo) - 1), lane);
           last = __shfl_sync(0xffffffffu, list, p.top_k - 1);
           todo &= todo - 1;
           todo &= __ballot_sync(0xffffffffu, k > last);
         }
+      });
+      lists[warp][lane] = list;
+      __syncthreads();
+      if (warp == 0) {
+        list = select_top(lists[0], 32, kLpWarps, p.top_k, lane);
+        sorted[lane] = list;
+        __syncwarp();
       }
     }
-    lists[warp][lane] = list;
-    __syncthreads();
+    list = lane < p.top_k ? sorted[lane] : 0;
   }
   if (warp != 0) return;
-  if (tops)
-    for (int w = 1; w < kLpWarps; ++w) list = list_merge(list, lists[w][lane], lane);
-  LogprobStat t;
-  t.m = -INFINITY, t.s = t.w = 0.0f, t.above = 0;
-  if (lane < kLpWarps) t = stats[lane];
-  t = warp_join(t);
+  const LogprobStat t = warp_join(stats[lane & (kLpWarps - 1)], kLpWarps);
   if (p.splits == 1) {
     finish_row(p, row, xt, given, t, nan, list, lane);
   } else {
@@ -510,37 +555,57 @@ __global__ void __launch_bounds__(kLpThreads, kLpCtasPerSm) token_logprobs_kerne
 // Joins the parts of a row; one CTA per row.
 template <typename T>
 __global__ void __launch_bounds__(kLpThreads) token_logprobs_join_kernel(const LogprobArgs p) {
-  __shared__ uint64_t lists[kLpWarps][32];
+  __shared__ uint64_t lists[kLpMaxSplits * kLpMaxTop], found[kLpMaxFound], sorted[kLpMaxTop];
+  __shared__ int num_found;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t row = blockIdx.x;
   const T* x = static_cast<const T*>(p.logits) + row * p.row_stride;
   const int64_t target = p.targets[row];
   const bool given = target >= 0 && target < p.vocab;
   const float xt = given ? load_logit(x + target) : INFINITY;
+  if (threadIdx.x == 0) num_found = 0;
+  if (threadIdx.x < kLpMaxTop) sorted[threadIdx.x] = 0;
   grid_dependency_wait();
+  const uint64_t* keys = p.part_keys + row * p.splits * p.top_k;
+  for (int i = threadIdx.x; i < p.splits * p.top_k; i += kLpThreads) lists[i] = keys[i];
+  LogprobStat t = {-INFINITY, 0.0f, 0.0f, 0};
+  bool nan = false;
+  if (warp == 0) {
+    for (int i = lane; i < p.splits; i += 32) {
+      const LogprobPart part = p.parts[row * p.splits + i];
+      t = join_stats(t, part.st);
+      nan |= part.nan != 0;
+    }
+    nan = __any_sync(0xffffffffu, nan);
+    t = warp_join(t, 32);
+  }
+  __syncthreads();
   uint64_t list = 0;
   if (p.top_k > 0) {
-    for (int i = warp; i < p.splits; i += kLpWarps) {
-      const uint64_t k = lane < p.top_k ? p.part_keys[(row * p.splits + i) * p.top_k + lane] : 0;
-      list = i == warp ? k : list_merge(list, k, lane);
-    }
-    lists[warp][lane] = list;
+    // The top_k-th largest of the first few keys of every list (twice as many as
+    // wanted) bounds the row's from below; the keys that reach it are ranked.
+    const int k = p.top_k, each = min(k, (2 * k + p.splits - 1) / p.splits), n = each * p.splits;
+    if (threadIdx.x < n)  // at most 2 k + splits
+      found[threadIdx.x] = lists[threadIdx.x / each * k + threadIdx.x % each];
     __syncthreads();
+    rank_keys(found, n, k, sorted, threadIdx.x);
+    __syncthreads();
+    const uint64_t least = max(sorted[k - 1], uint64_t(1));
+    for (int i = threadIdx.x; i < p.splits * k; i += kLpThreads)
+      if (lists[i] >= least) {
+        const int at = atomicAdd(&num_found, 1);
+        if (at < kLpMaxFound) found[at] = lists[i];
+      }
+    __syncthreads();
+    if (num_found <= kLpMaxFound) {
+      rank_keys(found, num_found, k, sorted, threadIdx.x);
+    } else if (warp == 0) {
+      sorted[lane] = select_top(lists, k, p.splits, k, lane);
+    }
+    __syncthreads();
+    if (lane < k) list = sorted[lane];
   }
-  if (warp != 0) return;
-  if (p.top_k > 0)
-    for (int w = 1; w < kLpWarps; ++w) list = list_merge(list, lists[w][lane], lane);
-  LogprobStat t;
-  t.m = -INFINITY, t.s = t.w = 0.0f, t.above = 0;
-  bool nan = false;
-  for (int i = lane; i < p.splits; i += 32) {
-    const LogprobPart& part = p.parts[row * p.splits + i];
-    t = join_stats(t, part.st);
-    nan |= part.nan != 0;
-  }
-  nan = __any_sync(0xffffffffu, nan);
-  t = warp_join(t);
-  finish_row(p, row, xt, given, t, nan, list, lane);
+  if (warp == 0) finish_row(p, row, xt, given, t, nan, list, lane);
 }
 
 // CTAs of a row: one where the rows alone fill the SMs, else so many that all do,

@@ -88,6 +88,16 @@ def test_hard_rows(cuda_device, dtype, kind):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_many_equal_logits_over_many_parts(cuda_device, dtype):
+    """Every part of a split row holds more candidates than are ranked at once."""
+    v, k = 1000003, 32
+    x = torch.zeros(2, v, dtype=dtype)
+    x[1, 500000:] = 1.0
+    targets = torch.tensor([v - 1, 3])
+    check(token_logprobs(x.to(cuda_device), targets.to(cuda_device), top_k=k), x, targets, k)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_masks(cuda_device, dtype):
     """-inf and the type's lowest value, few or no tokens left, targets masked or outside."""
     v, k = 5003, 20
