@@ -27,18 +27,11 @@ constexpr int kKv4RowBytes = 64;    // codes of a token
 constexpr int kKv4Groups = 4;       // scales of a token
 constexpr int kKv4MaxGroup = 8;     // query heads per KV head
 
-// Byte of the unit of channels 4 * lane .. 4 * lane + 3 within a token's K row.
-__device__ __forceinline__ int kv4_k_unit(int lane) {
-  return ((lane & 7) >> 1) * 16 + (lane >> 3) * 4 + (lane & 1) * 2;
-}
-// Byte of that unit of token t within its (page, head) tile of V codes.
-__device__ __forceinline__ int kv4_v_unit(int t, int lane) {
-  const int pair = t >> 1;
-  return pair * 128 + ((lane & 7) ^ (2 * (pair & 3))) * 16 + (lane >> 3) * 4 + (t & 1) * 2;
-}
-
 // ------------------------------------------------------------ store
-// One warp per (token, head) of the fused QKV output, four channels a lane.
+// Half a warp per (token, head) of the fused QKV output, eight channels a lane.
+// Bound by HBM for long prompts: a row is read and written once, cos and sin
+// come from L1.
+//
 // K is normalised and rotated in 64 bits and rounded once to FP32 before it is
 // quantised: a code depends on which side of a border x / s lies, and with
 // FP32 sums it would depend on the order of the sum.  x / s itself is an IEEE
@@ -64,111 +57,115 @@ struct Kv4StoreArgs {
   int T, Hq, Hkv;
 };
 
-// Quantises a lane's four values with its group (8 lanes): the unit of codes
-// and the group's scale.
-__device__ __forceinline__ uint32_t kv4_quantise(const float (&x)[4], uint16_t& scale_bits, float (&value)[4]) {
-  uint32_t top = 0;  // as bits: an infinity or NaN is above every number
+__device__ __forceinline__ void unpack8(const uint4& raw, float (&x)[8]) {
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+  for (int i = 0; i < 4; ++i) x[2 * i] = bf16lo_to_f32(w[i]), x[2 * i + 1] = bf16hi_to_f32(w[i]);
+}
+__device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
+  return make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]),
+                    pack_bf16x2(x[6], x[7]));
+}
+
+// RMSNorm and rotary embedding of a head over the 16 lanes of `mask`, in F.  Lane
+// l of the 16 holds channels 8 l .. 8 l + 7; channel i is rotated with i + 64, eight lanes on.
+template <typename F>
+__device__ __forceinline__ void norm_rope8(float (&x)[8], const float (&w)[8], const float (&c)[8],
+                                           const float (&s)[8], double eps, uint32_t mask, bool first_half) {
+  F ss = 0;
 #pragma unroll
-  for (int m = 1; m <= 4; m <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, m));
-  float s = __bfloat162float(__float2bfloat16_rn(__fdiv_rn(__uint_as_float(top), 7.0f)));
-  s = fmaxf(s, kBf16Tiny);
-  if (top == 0) s = 1.0f;
-  if (top >= 0x7F800000u) s = __uint_as_float(0x7FC00000u);
-  scale_bits = static_cast<uint16_t>(__float_as_uint(s) >> 16);
-  uint32_t unit = 0;
+  for (int i = 0; i < 8; ++i) ss += static_cast<F>(x[i] * x[i]);  // 16 significant bits: exact in FP32
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float c = fminf(fmaxf(rintf(__fdiv_rn(x[i], s)), -7.0f), 7.0f);
-    unit |= static_cast<uint32_t>(static_cast<int>(c) + 8) << (4 * i);
-    value[i] = c * s;
+  for (int m = 8; m >= 1; m >>= 1) ss += __shfl_xor_sync(mask, ss, m);
+  F r;
+  if constexpr (sizeof(F) == 8) r = rsqrt(ss * (1.0 / kKv4D) + eps);
+  else r = rsqrtf(ss * (1.0f / kKv4D) + static_cast<float>(eps));
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const F n = static_cast<F>(x[i]) * r * static_cast<F>(w[i]);
+    const F o = __shfl_xor_sync(mask, n, 8);
+    const F turned = o * static_cast<F>(s[i]);
+    x[i] = static_cast<float>(n * static_cast<F>(c[i]) + (first_half ? -turned : turned));
   }
-  return unit;
 }
 
 __global__ void __launch_bounds__(256) qk_norm_rope_store_kv4_kernel(const Kv4StoreArgs p) {
   const int heads = p.Hq + 2 * p.Hkv;
-  const int64_t gw = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (gw >= static_cast<int64_t>(p.T) * heads) return;
-  const int t = static_cast<int>(gw / heads), h = static_cast<int>(gw - static_cast<int64_t>(t) * heads);
-  const uint2 raw = *reinterpret_cast<const uint2*>(p.qkv + gw * kKv4D + lane * 4);
-  const float x[4] = {bf16lo_to_f32(raw.x), bf16hi_to_f32(raw.x), bf16lo_to_f32(raw.y), bf16hi_to_f32(raw.y)};
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 16 + (threadIdx.x >> 4);
+  const int lane = threadIdx.x & 15;
+  const uint32_t mask = threadIdx.x & 16 ? 0xFFFF0000u : 0x0000FFFFu;  // the two halves go their own ways
+  if (row >= static_cast<int64_t>(p.T) * heads) return;
+  const int t = static_cast<int>(row / heads), h = static_cast<int>(row - static_cast<int64_t>(t) * heads);
+  float x[8];
+  unpack8(__ldg(reinterpret_cast<const uint4*>(p.qkv + row * kKv4D) + lane), x);
 
-  float y[4];
   if (h < p.Hq + p.Hkv) {
-    const uint2 wr = *reinterpret_cast<const uint2*>((h < p.Hq ? p.q_weight : p.k_weight) + lane * 4);
-    const float w[4] = {bf16lo_to_f32(wr.x), bf16hi_to_f32(wr.x), bf16lo_to_f32(wr.y), bf16hi_to_f32(wr.y)};
+    float w[8], c[8], s[8];
+    unpack8(__ldg(reinterpret_cast<const uint4*>(h < p.Hq ? p.q_weight : p.k_weight) + lane), w);
     const int64_t pos = p.positions[t];
-    float4 c4 = make_float4(NAN, NAN, NAN, NAN), s4 = c4;  // a position beyond the table: NaN, and an error
     if (pos >= 0 && pos < p.max_position) {
-      const float* cs = p.cos_sin + pos * kKv4D + (lane & 15) * 4;
-      c4 = *reinterpret_cast<const float4*>(cs);
-      s4 = *reinterpret_cast<const float4*>(cs + kKv4D / 2);
-    } else if (lane == 0) {
-      record_error(kErrBadPosition);
+      const float4* cs = reinterpret_cast<const float4*>(p.cos_sin + pos * kKv4D) + (lane & 7) * 2;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        *reinterpret_cast<float4*>(c + 4 * i) = __ldg(cs + i);
+        *reinterpret_cast<float4*>(s + 4 * i) = __ldg(cs + kKv4D / 8 + i);
+      }
+    } else {  // beyond the table: NaN, and an error
+#pragma unroll
+      for (int i = 0; i < 8; ++i) c[i] = s[i] = NAN;
+      if (lane == 0) record_error(kErrBadPosition);
     }
-    const float c[4] = {c4.x, c4.y, c4.z, c4.w}, s[4] = {s4.x, s4.y, s4.z, s4.w};
     if (h < p.Hq) {
-      float ss = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) ss = fmaf(x[i], x[i], ss);
-#pragma unroll
-      for (int m = 16; m >= 1; m >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
-      const float r = rsqrtf(ss * (1.0f / kKv4D) + static_cast<float>(p.eps));
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float n = x[i] * r * w[i];
-        const float o = __shfl_xor_sync(0xffffffffu, n, 16);
-        y[i] = lane < 16 ? n * c[i] - o * s[i] : n * c[i] + o * s[i];
-      }
-    } else {
-      double ss = 0.0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) ss += static_cast<double>(x[i] * x[i]);  // 16 significant bits: exact in FP32
-#pragma unroll
-      for (int m = 16; m >= 1; m >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
-      const double r = rsqrt(ss * (1.0 / kKv4D) + p.eps);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const double n = static_cast<double>(x[i]) * r * static_cast<double>(w[i]);
-        const double o = __shfl_xor_sync(0xffffffffu, n, 16);
-        const double cd = c[i], sd = s[i];
-        y[i] = static_cast<float>(lane < 16 ? n * cd - o * sd : n * cd + o * sd);
-      }
+      norm_rope8<float>(x, w, c, s, p.eps, mask, lane < 8);
+      reinterpret_cast<uint4*>(p.q_out + (static_cast<int64_t>(t) * p.Hq + h) * kKv4D)[lane] = pack8(x);
+      return;
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) y[i] = x[i];
+    norm_rope8<double>(x, w, c, s, p.eps, mask, lane < 8);
   }
-  if (h < p.Hq) {
-    *reinterpret_cast<uint2*>(p.q_out + (static_cast<int64_t>(t) * p.Hq + h) * kKv4D + lane * 4) =
-        make_uint2(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]));
-    return;
-  }
+
+  // The scale of the group (four lanes), the codes and the values that they stand for.
   const bool is_k = h < p.Hq + p.Hkv;
   const int kvh = is_k ? h - p.Hq : h - p.Hq - p.Hkv;
-  uint16_t scale;
-  float value[4];
-  const uint32_t unit = kv4_quantise(y, scale, value);
+  uint32_t top = 0;  // as bits: an infinity or NaN is above every number
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+  top = max(top, __shfl_xor_sync(mask, top, 1));
+  top = max(top, __shfl_xor_sync(mask, top, 2));
+  float scale = __bfloat162float(__float2bfloat16_rn(__fdiv_rn(__uint_as_float(top), 7.0f)));
+  scale = fmaxf(scale, kBf16Tiny);
+  if (top == 0) scale = 1.0f;
+  if (top >= 0x7F800000u) scale = __uint_as_float(0x7FC00000u);
+  uint32_t word = 0;  // nibble i: channel i of the lane's eight
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float c = fminf(fmaxf(rintf(__fdiv_rn(x[i], scale)), -7.0f), 7.0f);
+    word |= static_cast<uint32_t>(static_cast<int>(c) + 8) << (4 * i);
+    x[i] = c * scale;
+  }
   uint16_t* values = is_k ? p.k_out : p.v_out;
   if (values != nullptr)
-    *reinterpret_cast<uint2*>(values + (static_cast<int64_t>(t) * p.Hkv + kvh) * kKv4D + lane * 4) =
-        make_uint2(pack_bf16x2(value[0], value[1]), pack_bf16x2(value[2], value[3]));
+    reinterpret_cast<uint4*>(values + (static_cast<int64_t>(t) * p.Hkv + kvh) * kKv4D)[lane] = pack8(x);
   const int slot = p.slot_mapping != nullptr ? p.slot_mapping[t] : -1;
   if (slot < 0) return;
   if (slot >= p.num_slots) {
     if (lane == 0) record_error(kErrBadSlot);
     return;
   }
-  const int row = slot % kKv4Page;
+  const int token = slot % kKv4Page, g = lane >> 2;
   const int64_t tile = static_cast<int64_t>(slot / kKv4Page) * p.Hkv + kvh;
-  uint8_t* codes = (is_k ? p.k_codes : p.v_codes) + tile * (kKv4Page * kKv4RowBytes);
-  uint16_t* scales = (is_k ? p.k_scales : p.v_scales) + (tile * kKv4Page + row) * kKv4Groups;
-  const int at = is_k ? row * kKv4RowBytes + kv4_k_unit(lane) : kv4_v_unit(row, lane);
-  *reinterpret_cast<uint16_t*>(codes + at) = static_cast<uint16_t>(unit);
-  if ((lane & 7) == 0) scales[lane >> 3] = scale;
+  if (is_k) {  // the lane's two units are a word
+    uint8_t* codes = p.k_codes + (tile * kKv4Page + token) * kKv4RowBytes;
+    *reinterpret_cast<uint32_t*>(codes + (lane & 3) * 16 + g * 4) = word;
+  } else {
+    const int pair = token >> 1, turn = 2 * (pair & 3);
+    uint8_t* codes = p.v_codes + tile * (kKv4Page * kKv4RowBytes) + pair * 128 + g * 4 + (token & 1) * 2;
+    const int run = (lane & 3) * 2;  // of four channels, within the group
+    *reinterpret_cast<uint16_t*>(codes + (run ^ turn) * 16) = static_cast<uint16_t>(word);
+    *reinterpret_cast<uint16_t*>(codes + ((run + 1) ^ turn) * 16) = static_cast<uint16_t>(word >> 16);
+  }
+  if ((lane & 3) == 0)
+    (is_k ? p.k_scales : p.v_scales)[(tile * kKv4Page + token) * kKv4Groups + g] =
+        static_cast<uint16_t>(__float_as_uint(scale) >> 16);
 }
 
 int launch_qk_norm_rope_store_kv4(const void* qkv, const void* q_weight, const void* k_weight, const float* cos_sin,
@@ -196,8 +193,8 @@ int launch_qk_norm_rope_store_kv4(const void* qkv, const void* q_weight, const v
   a.T = static_cast<int>(tokens);
   a.Hq = static_cast<int>(num_heads);
   a.Hkv = static_cast<int>(num_kv_heads);
-  const int64_t warps = tokens * (num_heads + 2 * num_kv_heads);
-  return launch_kernel(qk_norm_rope_store_kv4_kernel, dim3(static_cast<unsigned>((warps + 7) / 8)), dim3(256), 0,
+  const int64_t rows = tokens * (num_heads + 2 * num_kv_heads);
+  return launch_kernel(qk_norm_rope_store_kv4_kernel, dim3(static_cast<unsigned>((rows + 15) / 16)), dim3(256), 0,
                        stream, false, a);
 }
 
