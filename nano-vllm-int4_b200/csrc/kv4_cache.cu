@@ -16,6 +16,8 @@
 //   K: byte (r / 8) * 16 + g * 4 + (r % 8) / 4 * 2 of the token's 64 bytes;
 //   V: byte ((r / 4) ^ (2 * (pair % 4))) * 16 + g * 4 + (t % 2) * 2 of the 128
 //      bytes of the token pair t / 2.
+#include <numeric>
+
 #include "nv4_device.cuh"
 #include "nv4_launch.h"
 
@@ -28,16 +30,20 @@ constexpr int kKv4Groups = 4;       // scales of a token
 constexpr int kKv4MaxGroup = 8;     // query heads per KV head
 
 // ------------------------------------------------------------ store
-// Half a warp per (token, head) of the fused QKV output, eight channels a lane.
-// Bound by HBM for long prompts: a row is read and written once, cos and sin
-// come from L1.
+// Half a warp per row ((token, head) of the fused QKV output), eight channels a
+// lane: four and the four that the rotation pairs them with.  The half warps of a
+// full grid walk the rows; their number is coprime to the heads, so that each
+// takes q, K and V rows in turn (a K row costs four times a q row).  The next
+// row, its cos and sin and the position after it are on their way meanwhile.
+// Bound by HBM for long prompts: a row is read and written once.
 //
-// K is normalised and rotated in 64 bits and rounded once to FP32 before it is
-// quantised: a code depends on which side of a border x / s lies, and with
-// FP32 sums it would depend on the order of the sum.  x / s itself is an IEEE
-// FP32 quotient: for a 24-bit x and an 8-bit s it never rounds onto a
-// half-integer that the exact quotient does not hit, so the code is the exact
-// quotient's.  q needs no such care: FP32, rounded once to BF16.
+// A K code depends on which side of a border x / s lies, and with FP32 sums that
+// would depend on the order of the sum.  So K is computed beyond FP32 and rounded
+// once to it: the sum of squares and its root in 64 bits, norm weight and
+// rotation as unevaluated sums of two FP32 numbers (k = r (P c -+ P' s) with P = x w
+// exact; about 2^-46 off before the rounding).  That is 18 FP32 operations a
+// value; in FP64 the conversions alone took twice the time.  q needs no such
+// care: FP32, rounded once to BF16.
 struct Kv4StoreArgs {
   const uint16_t* qkv;
   const uint16_t* q_weight;
@@ -55,117 +61,186 @@ struct Kv4StoreArgs {
   int64_t max_position, num_slots;
   double eps;
   int T, Hq, Hkv;
+  int walkers;                  // half warps that walk the rows, each by as many rows
+  int walk_tokens, walk_heads;  // that many rows, as tokens and heads
 };
 
-__device__ __forceinline__ void unpack8(const uint4& raw, float (&x)[8]) {
-  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+// A lane's channels 4 l .. 4 l + 3 and 64 on, of the 16 lanes of a row.
+struct Row8 {
+  uint2 lo, hi;
+};
+__device__ __forceinline__ Row8 load_row(const uint16_t* row, int lane) {
+  const uint2* p = reinterpret_cast<const uint2*>(row) + lane;
+  return {__ldg(p), __ldg(p + 16)};
+}
+__device__ __forceinline__ void store_row(uint16_t* row, int lane, const float (&x)[8]) {
+  uint2* p = reinterpret_cast<uint2*>(row) + lane;
+  __stcs(p, make_uint2(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3])));
+  __stcs(p + 16, make_uint2(pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7])));
+}
+__device__ __forceinline__ void unpack_row(const Row8& r, float (&x)[8]) {
+  const uint32_t w[4] = {r.lo.x, r.lo.y, r.hi.x, r.hi.y};
 #pragma unroll
   for (int i = 0; i < 4; ++i) x[2 * i] = bf16lo_to_f32(w[i]), x[2 * i + 1] = bf16hi_to_f32(w[i]);
 }
-__device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
-  return make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]),
-                    pack_bf16x2(x[6], x[7]));
-}
 
-// RMSNorm and rotary embedding of a head over the 16 lanes of `mask`, in F.  Lane
-// l of the 16 holds channels 8 l .. 8 l + 7; channel i is rotated with i + 64, eight lanes on.
-template <typename F>
-__device__ __forceinline__ void norm_rope8(float (&x)[8], const float (&w)[8], const float (&c)[8],
-                                           const float (&s)[8], double eps, uint32_t mask, bool first_half) {
-  F ss = 0;
+// RMSNorm and rotary embedding over the 16 lanes of `mask`.
+__device__ __forceinline__ void norm_rope_q(float (&x)[8], const float (&w)[8], const float (&c)[4],
+                                            const float (&s)[4], float eps, uint32_t mask) {
+  float ss = 0.0f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) ss += static_cast<F>(x[i] * x[i]);  // 16 significant bits: exact in FP32
+  for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
 #pragma unroll
   for (int m = 8; m >= 1; m >>= 1) ss += __shfl_xor_sync(mask, ss, m);
-  F r;
-  if constexpr (sizeof(F) == 8) r = rsqrt(ss * (1.0 / kKv4D) + eps);
-  else r = rsqrtf(ss * (1.0f / kKv4D) + static_cast<float>(eps));
+  const float r = rsqrtf(ss * (1.0f / kKv4D) + eps);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float a = x[i] * r * w[i], b = x[i + 4] * r * w[i + 4];
+    x[i] = fmaf(a, c[i], -(b * s[i]));
+    x[i + 4] = fmaf(b, c[i], a * s[i]);
+  }
+}
+// r (a c + b s) of exact a, b, with r = rh + rl.
+__device__ __forceinline__ float turn_k(float a, float b, float c, float s, float rh, float rl) {
+  const float ac = a * c, bs = b * s;
+  const float low = fmaf(a, c, -ac) + fmaf(b, s, -bs);
+  const float sum = ac + bs, z = sum - ac;  // and the sum's own rounding error:
+  const float rest = ((ac - (sum - z)) + (bs - z)) + low;
+  const float y = sum * rh;
+  return y + fmaf(rest, rh, fmaf(sum, rl, fmaf(sum, rh, -y)));
+}
+__device__ __forceinline__ void norm_rope_k(float (&x)[8], const float (&w)[8], const float (&c)[4],
+                                            const float (&s)[4], double eps, uint32_t mask) {
+  double ss = 0.0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const F n = static_cast<F>(x[i]) * r * static_cast<F>(w[i]);
-    const F o = __shfl_xor_sync(mask, n, 8);
-    const F turned = o * static_cast<F>(s[i]);
-    x[i] = static_cast<float>(n * static_cast<F>(c[i]) + (first_half ? -turned : turned));
+    const double d = x[i];
+    ss = fma(d, d, ss);
+  }
+#pragma unroll
+  for (int m = 8; m >= 1; m >>= 1) ss += __shfl_xor_sync(mask, ss, m);
+  const double r = rsqrt(ss * (1.0 / kKv4D) + eps);
+  const float rh = static_cast<float>(r), rl = static_cast<float>(r - static_cast<double>(rh));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float a = x[i] * w[i], b = x[i + 4] * w[i + 4];  // 16 significant bits: exact
+    x[i] = turn_k(a, -b, c[i], s[i], rh, rl);
+    x[i + 4] = turn_k(b, a, c[i], s[i], rh, rl);
   }
 }
 
-__global__ void __launch_bounds__(256) qk_norm_rope_store_kv4_kernel(const Kv4StoreArgs p) {
-  const int heads = p.Hq + 2 * p.Hkv;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 16 + (threadIdx.x >> 4);
-  const int lane = threadIdx.x & 15;
-  const uint32_t mask = threadIdx.x & 16 ? 0xFFFF0000u : 0x0000FFFFu;  // the two halves go their own ways
-  if (row >= static_cast<int64_t>(p.T) * heads) return;
-  const int t = static_cast<int>(row / heads), h = static_cast<int>(row - static_cast<int64_t>(t) * heads);
-  float x[8];
-  unpack8(__ldg(reinterpret_cast<const uint4*>(p.qkv + row * kKv4D) + lane), x);
-
-  if (h < p.Hq + p.Hkv) {
-    float w[8], c[8], s[8];
-    unpack8(__ldg(reinterpret_cast<const uint4*>(h < p.Hq ? p.q_weight : p.k_weight) + lane), w);
-    const int64_t pos = p.positions[t];
-    if (pos >= 0 && pos < p.max_position) {
-      const float4* cs = reinterpret_cast<const float4*>(p.cos_sin + pos * kKv4D) + (lane & 7) * 2;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        *reinterpret_cast<float4*>(c + 4 * i) = __ldg(cs + i);
-        *reinterpret_cast<float4*>(s + 4 * i) = __ldg(cs + kKv4D / 8 + i);
-      }
-    } else {  // beyond the table: NaN, and an error
-#pragma unroll
-      for (int i = 0; i < 8; ++i) c[i] = s[i] = NAN;
-      if (lane == 0) record_error(kErrBadPosition);
-    }
-    if (h < p.Hq) {
-      norm_rope8<float>(x, w, c, s, p.eps, mask, lane < 8);
-      reinterpret_cast<uint4*>(p.q_out + (static_cast<int64_t>(t) * p.Hq + h) * kKv4D)[lane] = pack8(x);
-      return;
-    }
-    norm_rope8<double>(x, w, c, s, p.eps, mask, lane < 8);
-  }
-
-  // The scale of the group (four lanes), the codes and the values that they stand for.
-  const bool is_k = h < p.Hq + p.Hkv;
-  const int kvh = is_k ? h - p.Hq : h - p.Hq - p.Hkv;
+// Quantises four values of a lane with their group (eight lanes): the unit of codes
+// and the scale; x becomes the values that the codes stand for.
+__device__ __forceinline__ uint32_t kv4_quantise(float* x, float& scale, uint32_t mask) {
   uint32_t top = 0;  // as bits: an infinity or NaN is above every number
 #pragma unroll
-  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
-  top = max(top, __shfl_xor_sync(mask, top, 1));
-  top = max(top, __shfl_xor_sync(mask, top, 2));
-  float scale = __bfloat162float(__float2bfloat16_rn(__fdiv_rn(__uint_as_float(top), 7.0f)));
+  for (int i = 0; i < 4; ++i) top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+#pragma unroll
+  for (int m = 1; m <= 4; m <<= 1) top = max(top, __shfl_xor_sync(mask, top, m));
+  scale = __bfloat162float(__float2bfloat16_rn(__fdiv_rn(__uint_as_float(top), 7.0f)));
   scale = fmaxf(scale, kBf16Tiny);
   if (top == 0) scale = 1.0f;
   if (top >= 0x7F800000u) scale = __uint_as_float(0x7FC00000u);
-  uint32_t word = 0;  // nibble i: channel i of the lane's eight
+  // x / s to the last bit or next to it: q + (x - q s) / s, the remainder exact.
+  // That rounds to the exact quotient's integer: s has 8 significant bits, so a
+  // quotient off a half-integer h is off by more than 2^-24 (1 + 2^-8) h, above
+  // half a unit of h by 2^-33 h, and the error is 2^-47 h; h itself comes out
+  // exactly.  Below 2^-80 the remainder would underflow: an IEEE division.
+  const float inv = __frcp_rn(scale);
+  uint32_t unit = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float c = fminf(fmaxf(rintf(__fdiv_rn(x[i], scale)), -7.0f), 7.0f);
-    word |= static_cast<uint32_t>(static_cast<int>(c) + 8) << (4 * i);
-    x[i] = c * scale;
+  for (int i = 0; i < 4; ++i) {
+    float q = x[i] * inv;
+    q = fmaf(fmaf(-q, scale, x[i]), inv, q);
+    if (scale < 0x1p-80f) q = __fdiv_rn(x[i], scale);
+    // rounded to even in the last place of 1.5 * 2^23; + 8 makes the nibble
+    const float z = fminf(fmaxf(q, -7.0f), 7.0f) + 12582920.0f;
+    unit |= (__float_as_uint(z) & 15u) << (4 * i);
+    x[i] = (z - 12582920.0f) * scale;
   }
-  uint16_t* values = is_k ? p.k_out : p.v_out;
-  if (values != nullptr)
-    reinterpret_cast<uint4*>(values + (static_cast<int64_t>(t) * p.Hkv + kvh) * kKv4D)[lane] = pack8(x);
-  const int slot = p.slot_mapping != nullptr ? p.slot_mapping[t] : -1;
-  if (slot < 0) return;
-  if (slot >= p.num_slots) {
-    if (lane == 0) record_error(kErrBadSlot);
-    return;
+  return unit;
+}
+
+__global__ void __launch_bounds__(256, 4) qk_norm_rope_store_kv4_kernel(const Kv4StoreArgs p) {
+  const int heads = p.Hq + 2 * p.Hkv, lane = threadIdx.x & 15;
+  const uint32_t mask = threadIdx.x & 16 ? 0xFFFF0000u : 0x0000FFFFu;  // the two halves go their own ways
+  const int first = blockIdx.x * 16 + (threadIdx.x >> 4);
+  int t = first / heads, h = first - t * heads;
+  if (first >= p.walkers || t >= p.T) return;
+  const uint16_t* src = p.qkv + static_cast<int64_t>(first) * kKv4D;
+  const int64_t stride = static_cast<int64_t>(p.walkers) * kKv4D;
+
+  // cos and sin of a position; NaN beyond the table, and an error
+  const auto load_turn = [&](int64_t pos, int head, float4& c, float4& s) {
+    if (head >= p.Hq + p.Hkv) return;  // V
+    if (pos >= 0 && pos < p.max_position) {
+      const float4* cs = reinterpret_cast<const float4*>(p.cos_sin + pos * kKv4D) + lane;
+      c = __ldg(cs);
+      s = __ldg(cs + 16);
+    } else {
+      c = s = make_float4(NAN, NAN, NAN, NAN);
+      if (lane == 0) record_error(kErrBadPosition);
+    }
+  };
+  Row8 raw = load_row(src, lane);
+  float4 c4 = {}, s4 = {};
+  load_turn(p.positions[t], h, c4, s4);
+  int t1 = t + p.walk_tokens, h1 = h + p.walk_heads;  // the row after this one
+  if (h1 >= heads) h1 -= heads, ++t1;
+  int64_t pos1 = t1 < p.T ? p.positions[t1] : 0;
+  while (true) {
+    float x[8];
+    unpack_row(raw, x);
+    const float c[4] = {c4.x, c4.y, c4.z, c4.w}, s[4] = {s4.x, s4.y, s4.z, s4.w};
+    const int row_t = t, row_h = h;
+    t = t1, h = h1;
+    const bool more = t < p.T;
+    if (more) {
+      src += stride;
+      raw = load_row(src, lane);
+      load_turn(pos1, h, c4, s4);
+      t1 = t + p.walk_tokens, h1 = h + p.walk_heads;
+      if (h1 >= heads) h1 -= heads, ++t1;
+      pos1 = t1 < p.T ? p.positions[t1] : 0;
+    }
+    const bool is_q = row_h < p.Hq, is_k = !is_q && row_h < p.Hq + p.Hkv;
+    if (is_q || is_k) {
+      float w[8];
+      unpack_row(load_row(is_q ? p.q_weight : p.k_weight, lane), w);
+      if (is_q) norm_rope_q(x, w, c, s, static_cast<float>(p.eps), mask);
+      else norm_rope_k(x, w, c, s, p.eps, mask);
+    }
+    if (is_q) {
+      store_row(p.q_out + (static_cast<int64_t>(row_t) * p.Hq + row_h) * kKv4D, lane, x);
+    } else {
+      const int kvh = row_h - (is_k ? p.Hq : p.Hq + p.Hkv);
+      float scale[2];
+      uint32_t unit[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) unit[i] = kv4_quantise(x + 4 * i, scale[i], mask);
+      uint16_t* values = is_k ? p.k_out : p.v_out;
+      if (values != nullptr)
+        store_row(values + (static_cast<int64_t>(row_t) * p.Hkv + kvh) * kKv4D, lane, x);
+      const int slot = p.slot_mapping != nullptr ? p.slot_mapping[row_t] : -1;
+      if (slot >= 0 && slot < p.num_slots) {
+        const int token = slot % kKv4Page, quad = lane & 7;  // within groups lane / 8 and 2 + lane / 8
+        const int64_t tile = static_cast<int64_t>(slot / kKv4Page) * p.Hkv + kvh;
+        uint8_t* codes = (is_k ? p.k_codes : p.v_codes) + tile * (kKv4Page * kKv4RowBytes) + (lane >> 3) * 4;
+        codes += is_k ? token * kKv4RowBytes + (quad >> 1) * 16 + (quad & 1) * 2
+                      : (token >> 1) * 128 + (quad ^ (2 * ((token >> 1) & 3))) * 16 + (token & 1) * 2;
+        *reinterpret_cast<uint16_t*>(codes) = static_cast<uint16_t>(unit[0]);
+        *reinterpret_cast<uint16_t*>(codes + 8) = static_cast<uint16_t>(unit[1]);
+        if (quad == 0) {
+          uint16_t* scales = (is_k ? p.k_scales : p.v_scales) + (tile * kKv4Page + token) * kKv4Groups + (lane >> 3);
+          scales[0] = static_cast<uint16_t>(__float_as_uint(scale[0]) >> 16);
+          scales[2] = static_cast<uint16_t>(__float_as_uint(scale[1]) >> 16);
+        }
+      } else if (slot >= 0 && lane == 0) {
+        record_error(kErrBadSlot);
+      }
+    }
+    if (!more) return;
   }
-  const int token = slot % kKv4Page, g = lane >> 2;
-  const int64_t tile = static_cast<int64_t>(slot / kKv4Page) * p.Hkv + kvh;
-  if (is_k) {  // the lane's two units are a word
-    uint8_t* codes = p.k_codes + (tile * kKv4Page + token) * kKv4RowBytes;
-    *reinterpret_cast<uint32_t*>(codes + (lane & 3) * 16 + g * 4) = word;
-  } else {
-    const int pair = token >> 1, turn = 2 * (pair & 3);
-    uint8_t* codes = p.v_codes + tile * (kKv4Page * kKv4RowBytes) + pair * 128 + g * 4 + (token & 1) * 2;
-    const int run = (lane & 3) * 2;  // of four channels, within the group
-    *reinterpret_cast<uint16_t*>(codes + (run ^ turn) * 16) = static_cast<uint16_t>(word);
-    *reinterpret_cast<uint16_t*>(codes + ((run + 1) ^ turn) * 16) = static_cast<uint16_t>(word >> 16);
-  }
-  if ((lane & 3) == 0)
-    (is_k ? p.k_scales : p.v_scales)[(tile * kKv4Page + token) * kKv4Groups + g] =
-        static_cast<uint16_t>(__float_as_uint(scale) >> 16);
 }
 
 int launch_qk_norm_rope_store_kv4(const void* qkv, const void* q_weight, const void* k_weight, const float* cos_sin,
@@ -193,9 +268,16 @@ int launch_qk_norm_rope_store_kv4(const void* qkv, const void* q_weight, const v
   a.T = static_cast<int>(tokens);
   a.Hq = static_cast<int>(num_heads);
   a.Hkv = static_cast<int>(num_kv_heads);
-  const int64_t rows = tokens * (num_heads + 2 * num_kv_heads);
-  return launch_kernel(qk_norm_rope_store_kv4_kernel, dim3(static_cast<unsigned>((rows + 15) / 16)), dim3(256), 0,
-                       stream, false, a);
+  // as many CTAs of 16 half warps as run at once, or as there are rows for
+  const int64_t heads = num_heads + 2 * num_kv_heads, rows = tokens * heads;
+  const int64_t ctas = std::min<int64_t>((rows + 15) / 16, 4 * static_cast<int64_t>(device_sm_count()));
+  int64_t walkers = ctas * 16;
+  while (walkers > 1 && std::gcd(walkers, heads) != 1) --walkers;
+  if (rows <= ctas * 16) walkers = ctas * 16;  // one row each
+  a.walkers = static_cast<int>(walkers);
+  a.walk_tokens = static_cast<int>(walkers / heads);
+  a.walk_heads = static_cast<int>(walkers % heads);
+  return launch_kernel(qk_norm_rope_store_kv4_kernel, dim3(static_cast<unsigned>(ctas)), dim3(256), 0, stream, false, a);
 }
 
 // ------------------------------------------------------------ decode attention

@@ -488,7 +488,7 @@ int nv4_qk_norm_rope_store_kv4(const void* qkv, const void* q_weight, const void
   if (store != (k_codes != nullptr) || store != (k_scales != nullptr) || store != (v_codes != nullptr) ||
       store != (v_scales != nullptr) || (k_out != nullptr) != (v_out != nullptr))
     return NV4_ERR_INVALID_ARGUMENT;
-  if (tokens < 1 || num_heads < 1 || num_kv_heads < 1 || tokens > (int64_t(1) << 31) - 1 ||
+  if (tokens < 1 || num_heads < 1 || num_kv_heads < 1 || tokens > (int64_t(1) << 30) ||
       num_heads > 65535 || num_kv_heads > 65535 || tokens * (num_heads + 2 * num_kv_heads) > (int64_t(1) << 33) ||
       max_position < 1 || !(eps >= 0.0) || !(eps < 1.0))
     return NV4_ERR_INVALID_ARGUMENT;
