@@ -73,68 +73,86 @@ __device__ __forceinline__ Row8 load_row(const uint16_t* row, int lane) {
   const uint2* p = reinterpret_cast<const uint2*>(row) + lane;
   return {__ldg(p), __ldg(p + 16)};
 }
-__device__ __forceinline__ void store_row(uint16_t* row, int lane, const float (&x)[8]) {
-  uint2* p = reinterpret_cast<uint2*>(row) + lane;
-  __stcs(p, make_uint2(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3])));
-  __stcs(p + 16, make_uint2(pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7])));
-}
-__device__ __forceinline__ void unpack_row(const Row8& r, float (&x)[8]) {
+// The lane's values as pairs of FP32: channels (0, 1), (2, 3), then 64 on.
+__device__ __forceinline__ void unpack_row(const Row8& r, uint64_t (&x)[4]) {
   const uint32_t w[4] = {r.lo.x, r.lo.y, r.hi.x, r.hi.y};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) x[2 * i] = bf16lo_to_f32(w[i]), x[2 * i + 1] = bf16hi_to_f32(w[i]);
+  for (int i = 0; i < 4; ++i) x[i] = pair(bf16lo_to_f32(w[i]), bf16hi_to_f32(w[i]));
+}
+__device__ __forceinline__ uint32_t pack_pair(uint64_t x) {
+  float lo, hi;
+  unpair(x, lo, hi);
+  return pack_bf16x2(lo, hi);
+}
+__device__ __forceinline__ void store_row(uint16_t* row, int lane, const uint64_t (&x)[4]) {
+  uint2* p = reinterpret_cast<uint2*>(row) + lane;
+  __stcs(p, make_uint2(pack_pair(x[0]), pack_pair(x[1])));
+  __stcs(p + 16, make_uint2(pack_pair(x[2]), pack_pair(x[3])));
 }
 
-// RMSNorm and rotary embedding over the 16 lanes of `mask`.
-__device__ __forceinline__ void norm_rope_q(float (&x)[8], const float (&w)[8], const float (&c)[4],
-                                            const float (&s)[4], float eps, uint32_t mask) {
-  float ss = 0.0f;
+// RMSNorm and rotary embedding over the 16 lanes of `mask`; c, s: cos and sin of
+// the lane's four channels.
+__device__ __forceinline__ void norm_rope_q(uint64_t (&x)[4], const uint64_t (&w)[4], const uint64_t (&c)[2],
+                                            const uint64_t (&s)[2], float eps, uint32_t mask) {
+  uint64_t s2 = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
+  for (int i = 0; i < 4; ++i) s2 = fma2(x[i], x[i], s2);
+  float ss, other;
+  unpair(s2, ss, other);
+  ss += other;
 #pragma unroll
   for (int m = 8; m >= 1; m >>= 1) ss += __shfl_xor_sync(mask, ss, m);
   const float r = rsqrtf(ss * (1.0f / kKv4D) + eps);
+  const uint64_t rr = pair(r, r);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float a = x[i] * r * w[i], b = x[i + 4] * r * w[i + 4];
-    x[i] = fmaf(a, c[i], -(b * s[i]));
-    x[i + 4] = fmaf(b, c[i], a * s[i]);
+  for (int i = 0; i < 2; ++i) {
+    const uint64_t a = mul2(mul2(x[i], rr), w[i]), b = mul2(mul2(x[i + 2], rr), w[i + 2]);
+    x[i] = sub2(mul2(a, c[i]), mul2(b, s[i]));
+    x[i + 2] = fma2(b, c[i], mul2(a, s[i]));
   }
 }
-// r (a c + b s) of exact a, b, with r = rh + rl.
-__device__ __forceinline__ float turn_k(float a, float b, float c, float s, float rh, float rl) {
-  const float ac = a * c, bs = b * s;
-  const float low = fmaf(a, c, -ac) + fmaf(b, s, -bs);
-  const float sum = ac + bs, z = sum - ac;  // and the sum's own rounding error:
-  const float rest = ((ac - (sum - z)) + (bs - z)) + low;
-  const float y = sum * rh;
-  return y + fmaf(rest, rh, fmaf(sum, rl, fmaf(sum, rh, -y)));
+// r (a c + b s) of exact a, b, with r = rh + rl: both products and their sum with
+// what rounding takes from them.
+__device__ __forceinline__ uint64_t turn_k(uint64_t a, uint64_t b, uint64_t c, uint64_t s, uint64_t rh, uint64_t rl) {
+  const uint64_t ac = mul2(a, c), bs = mul2(b, s);
+  const uint64_t low = add2(fma2(a, c, sub2(0, ac)), fma2(b, s, sub2(0, bs)));
+  const uint64_t sum = add2(ac, bs), z = sub2(sum, ac);
+  const uint64_t rest = add2(add2(sub2(ac, sub2(sum, z)), sub2(bs, z)), low);
+  const uint64_t y = mul2(sum, rh);
+  return add2(y, fma2(rest, rh, fma2(sum, rl, fma2(sum, rh, sub2(0, y)))));
 }
-__device__ __forceinline__ void norm_rope_k(float (&x)[8], const float (&w)[8], const float (&c)[4],
-                                            const float (&s)[4], double eps, uint32_t mask) {
+__device__ __forceinline__ void norm_rope_k(uint64_t (&x)[4], const uint64_t (&w)[4], const uint64_t (&c)[2],
+                                            const uint64_t (&s)[2], double eps, uint32_t mask) {
   double ss = 0.0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const double d = x[i];
-    ss = fma(d, d, ss);
+  for (int i = 0; i < 4; ++i) {
+    float lo, hi;
+    unpair(x[i], lo, hi);
+    ss = fma(static_cast<double>(lo), static_cast<double>(lo), ss);
+    ss = fma(static_cast<double>(hi), static_cast<double>(hi), ss);
   }
 #pragma unroll
   for (int m = 8; m >= 1; m >>= 1) ss += __shfl_xor_sync(mask, ss, m);
   const double r = rsqrt(ss * (1.0 / kKv4D) + eps);
-  const float rh = static_cast<float>(r), rl = static_cast<float>(r - static_cast<double>(rh));
+  const float h = static_cast<float>(r), l = static_cast<float>(r - static_cast<double>(h));
+  const uint64_t rh = pair(h, h), rl = pair(l, l);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float a = x[i] * w[i], b = x[i + 4] * w[i + 4];  // 16 significant bits: exact
-    x[i] = turn_k(a, -b, c[i], s[i], rh, rl);
-    x[i + 4] = turn_k(b, a, c[i], s[i], rh, rl);
+  for (int i = 0; i < 2; ++i) {
+    const uint64_t a = mul2(x[i], w[i]), b = mul2(x[i + 2], w[i + 2]);  // 16 significant bits: exact
+    x[i] = turn_k(a, sub2(0, b), c[i], s[i], rh, rl);
+    x[i + 2] = turn_k(b, a, c[i], s[i], rh, rl);
   }
 }
 
 // Quantises four values of a lane with their group (eight lanes): the unit of codes
 // and the scale; x becomes the values that the codes stand for.
-__device__ __forceinline__ uint32_t kv4_quantise(float* x, float& scale, uint32_t mask) {
+__device__ __forceinline__ uint32_t kv4_quantise(uint64_t* x, float& scale, uint32_t mask) {
+  float v[4];
+  unpair(x[0], v[0], v[1]);
+  unpair(x[1], v[2], v[3]);
   uint32_t top = 0;  // as bits: an infinity or NaN is above every number
 #pragma unroll
-  for (int i = 0; i < 4; ++i) top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+  for (int i = 0; i < 4; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
 #pragma unroll
   for (int m = 1; m <= 4; m <<= 1) top = max(top, __shfl_xor_sync(mask, top, m));
   scale = __bfloat162float(__float2bfloat16_rn(__fdiv_rn(__uint_as_float(top), 7.0f)));
@@ -147,18 +165,31 @@ __device__ __forceinline__ uint32_t kv4_quantise(float* x, float& scale, uint32_
   // half a unit of h by 2^-33 h, and the error is 2^-47 h; h itself comes out
   // exactly.  Below 2^-80 the remainder would underflow: an IEEE division.
   const float inv = __frcp_rn(scale);
+  const uint64_t ii = pair(inv, inv), minus = pair(-scale, -scale);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint64_t q = mul2(x[i], ii);
+    unpair(fma2(fma2(q, minus, x[i]), ii, q), v[2 * i], v[2 * i + 1]);
+  }
+  if (scale < 0x1p-80f)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      unpair(x[i], v[2 * i], v[2 * i + 1]);
+      v[2 * i] = __fdiv_rn(v[2 * i], scale);
+      v[2 * i + 1] = __fdiv_rn(v[2 * i + 1], scale);
+    }
+  // Rounded to even in the last place of 1.5 * 2^23, whose low 16 bits are 0; + 8
+  // makes the nibble.
   uint32_t unit = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float q = x[i] * inv;
-    q = fmaf(fmaf(-q, scale, x[i]), inv, q);
-    if (scale < 0x1p-80f) q = __fdiv_rn(x[i], scale);
-    // rounded to even in the last place of 1.5 * 2^23; + 8 makes the nibble
-    const float z = fminf(fmaxf(q, -7.0f), 7.0f) + 12582920.0f;
-    unit |= (__float_as_uint(z) & 15u) << (4 * i);
-    x[i] = (z - 12582920.0f) * scale;
+  for (int i = 3; i >= 0; --i) {
+    v[i] = fminf(fmaxf(v[i], -7.0f), 7.0f) + 12582920.0f;
+    unit = unit * 16 + __float_as_uint(v[i]);
   }
-  return unit;
+  const uint64_t ss = pair(scale, scale), magic = pair(12582920.0f, 12582920.0f);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) x[i] = mul2(sub2(pair(v[2 * i], v[2 * i + 1]), magic), ss);
+  return unit & 0xFFFFu;
 }
 
 __global__ void __launch_bounds__(256, 4) qk_norm_rope_store_kv4_kernel(const Kv4StoreArgs p) {
@@ -173,7 +204,7 @@ __global__ void __launch_bounds__(256, 4) qk_norm_rope_store_kv4_kernel(const Kv
   // cos and sin of a position; NaN beyond the table, and an error
   const auto load_turn = [&](int64_t pos, int head, float4& c, float4& s) {
     if (head >= p.Hq + p.Hkv) return;  // V
-    if (pos >= 0 && pos < p.max_position) {
+    if (static_cast<uint64_t>(pos) < static_cast<uint64_t>(p.max_position)) {
       const float4* cs = reinterpret_cast<const float4*>(p.cos_sin + pos * kKv4D) + lane;
       c = __ldg(cs);
       s = __ldg(cs + 16);
@@ -189,9 +220,9 @@ __global__ void __launch_bounds__(256, 4) qk_norm_rope_store_kv4_kernel(const Kv
   if (h1 >= heads) h1 -= heads, ++t1;
   int64_t pos1 = t1 < p.T ? p.positions[t1] : 0;
   while (true) {
-    float x[8];
+    uint64_t x[4];
     unpack_row(raw, x);
-    const float c[4] = {c4.x, c4.y, c4.z, c4.w}, s[4] = {s4.x, s4.y, s4.z, s4.w};
+    const uint64_t c[2] = {pair(c4.x, c4.y), pair(c4.z, c4.w)}, s[2] = {pair(s4.x, s4.y), pair(s4.z, s4.w)};
     const int row_t = t, row_h = h;
     t = t1, h = h1;
     const bool more = t < p.T;
@@ -205,7 +236,7 @@ __global__ void __launch_bounds__(256, 4) qk_norm_rope_store_kv4_kernel(const Kv
     }
     const bool is_q = row_h < p.Hq, is_k = !is_q && row_h < p.Hq + p.Hkv;
     if (is_q || is_k) {
-      float w[8];
+      uint64_t w[4];
       unpack_row(load_row(is_q ? p.q_weight : p.k_weight, lane), w);
       if (is_q) norm_rope_q(x, w, c, s, static_cast<float>(p.eps), mask);
       else norm_rope_k(x, w, c, s, p.eps, mask);
@@ -217,7 +248,7 @@ __global__ void __launch_bounds__(256, 4) qk_norm_rope_store_kv4_kernel(const Kv
       float scale[2];
       uint32_t unit[2];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) unit[i] = kv4_quantise(x + 4 * i, scale[i], mask);
+      for (int i = 0; i < 2; ++i) unit[i] = kv4_quantise(x + 2 * i, scale[i], mask);
       uint16_t* values = is_k ? p.k_out : p.v_out;
       if (values != nullptr)
         store_row(values + (static_cast<int64_t>(row_t) * p.Hkv + kvh) * kKv4D, lane, x);
