@@ -30,12 +30,13 @@ constexpr int kKv4Groups = 4;       // scales of a token
 constexpr int kKv4MaxGroup = 8;     // query heads per KV head
 
 // ------------------------------------------------------------ store
-// Half a warp per row ((token, head) of the fused QKV output), eight channels a
-// lane: four and the four that the rotation pairs them with.  The half warps of a
-// full grid walk the rows; their number is coprime to the heads, so that each
-// takes q, K and V rows in turn (a K row costs four times a q row).  The next
-// row, its cos and sin and the position after it are on their way meanwhile.
-// Bound by HBM for long prompts: a row is read and written once.
+// Eight lanes per row ((token, head) of the fused QKV output), 16 channels a lane:
+// eight and the eight that the rotation pairs them with (with half as many a
+// lane, what every row costs besides its values made it 1.4 times slower).  The
+// octets of a full grid walk the rows; their number is coprime to the heads, so
+// that each takes q, K and V rows in turn (a K row costs four times a q row).
+// The next row is on its way meanwhile.  Bound by HBM for long prompts: a row is
+// read and written once.
 //
 // A K code depends on which side of a border x / s lies, and with FP32 sums that
 // would depend on the order of the sum.  So K is computed beyond FP32 and rounded
@@ -61,54 +62,55 @@ struct Kv4StoreArgs {
   int64_t max_position, num_slots;
   double eps;
   int T, Hq, Hkv;
-  int walkers;                  // half warps that walk the rows, each by as many rows
+  int walkers;                  // octets that walk the rows, each by as many rows
   int walk_tokens, walk_heads;  // that many rows, as tokens and heads
 };
 
-// A lane's channels 4 l .. 4 l + 3 and 64 on, of the 16 lanes of a row.
-struct Row8 {
-  uint2 lo, hi;
+// A lane's channels 8 l .. 8 l + 7 and 64 on, of the 8 lanes of a row.
+constexpr int kKv4RowLanes = 8;
+struct RowPart {
+  uint4 lo, hi;
 };
-__device__ __forceinline__ Row8 load_row(const uint16_t* row, int lane) {
-  const uint2* p = reinterpret_cast<const uint2*>(row) + lane;
-  return {__ldg(p), __ldg(p + 16)};
+__device__ __forceinline__ RowPart load_row(const uint16_t* row, int lane) {
+  const uint4* p = reinterpret_cast<const uint4*>(row) + lane;
+  return {__ldg(p), __ldg(p + 8)};
 }
-// The lane's values as pairs of FP32: channels (0, 1), (2, 3), then 64 on.
-__device__ __forceinline__ void unpack_row(const Row8& r, uint64_t (&x)[4]) {
-  const uint32_t w[4] = {r.lo.x, r.lo.y, r.hi.x, r.hi.y};
+// The lane's values as pairs of FP32: channels (0, 1), ..., (6, 7), then 64 on.
+__device__ __forceinline__ void unpack_row(const RowPart& r, uint64_t (&x)[8]) {
+  const uint32_t w[8] = {r.lo.x, r.lo.y, r.lo.z, r.lo.w, r.hi.x, r.hi.y, r.hi.z, r.hi.w};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) x[i] = pair(bf16lo_to_f32(w[i]), bf16hi_to_f32(w[i]));
+  for (int i = 0; i < 8; ++i) x[i] = pair(bf16lo_to_f32(w[i]), bf16hi_to_f32(w[i]));
 }
 __device__ __forceinline__ uint32_t pack_pair(uint64_t x) {
   float lo, hi;
   unpair(x, lo, hi);
   return pack_bf16x2(lo, hi);
 }
-__device__ __forceinline__ void store_row(uint16_t* row, int lane, const uint64_t (&x)[4]) {
-  uint2* p = reinterpret_cast<uint2*>(row) + lane;
-  __stcs(p, make_uint2(pack_pair(x[0]), pack_pair(x[1])));
-  __stcs(p + 16, make_uint2(pack_pair(x[2]), pack_pair(x[3])));
+__device__ __forceinline__ void store_row(uint16_t* row, int lane, const uint64_t (&x)[8]) {
+  uint4* p = reinterpret_cast<uint4*>(row) + lane;
+  __stcs(p, make_uint4(pack_pair(x[0]), pack_pair(x[1]), pack_pair(x[2]), pack_pair(x[3])));
+  __stcs(p + 8, make_uint4(pack_pair(x[4]), pack_pair(x[5]), pack_pair(x[6]), pack_pair(x[7])));
 }
 
-// RMSNorm and rotary embedding over the 16 lanes of `mask`; c, s: cos and sin of
-// the lane's four channels.
-__device__ __forceinline__ void norm_rope_q(uint64_t (&x)[4], const uint64_t (&w)[4], const uint64_t (&c)[2],
-                                            const uint64_t (&s)[2], float eps, uint32_t mask) {
+// RMSNorm and rotary embedding over the lanes of `mask`; c, s: cos and sin of the
+// lane's eight channels.
+__device__ __forceinline__ void norm_rope_q(uint64_t (&x)[8], const uint64_t (&w)[8], const uint64_t (&c)[4],
+                                            const uint64_t (&s)[4], float eps, uint32_t mask) {
   uint64_t s2 = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) s2 = fma2(x[i], x[i], s2);
+  for (int i = 0; i < 8; ++i) s2 = fma2(x[i], x[i], s2);
   float ss, other;
   unpair(s2, ss, other);
   ss += other;
 #pragma unroll
-  for (int m = 8; m >= 1; m >>= 1) ss += __shfl_xor_sync(mask, ss, m);
+  for (int m = kKv4RowLanes / 2; m >= 1; m >>= 1) ss += __shfl_xor_sync(mask, ss, m);
   const float r = rsqrtf(ss * (1.0f / kKv4D) + eps);
   const uint64_t rr = pair(r, r);
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const uint64_t a = mul2(mul2(x[i], rr), w[i]), b = mul2(mul2(x[i + 2], rr), w[i + 2]);
+  for (int i = 0; i < 4; ++i) {
+    const uint64_t a = mul2(mul2(x[i], rr), w[i]), b = mul2(mul2(x[i + 4], rr), w[i + 4]);
     x[i] = sub2(mul2(a, c[i]), mul2(b, s[i]));
-    x[i + 2] = fma2(b, c[i], mul2(a, s[i]));
+    x[i + 4] = fma2(b, c[i], mul2(a, s[i]));
   }
 }
 // r (a c + b s) of exact a, b, with r = rh + rl: both products and their sum with
@@ -121,40 +123,40 @@ __device__ __forceinline__ uint64_t turn_k(uint64_t a, uint64_t b, uint64_t c, u
   const uint64_t y = mul2(sum, rh);
   return add2(y, fma2(rest, rh, fma2(sum, rl, fma2(sum, rh, sub2(0, y)))));
 }
-__device__ __forceinline__ void norm_rope_k(uint64_t (&x)[4], const uint64_t (&w)[4], const uint64_t (&c)[2],
-                                            const uint64_t (&s)[2], double eps, uint32_t mask) {
+__device__ __forceinline__ void norm_rope_k(uint64_t (&x)[8], const uint64_t (&w)[8], const uint64_t (&c)[4],
+                                            const uint64_t (&s)[4], double eps, uint32_t mask) {
   double ss = 0.0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < 8; ++i) {
     float lo, hi;
     unpair(x[i], lo, hi);
     ss = fma(static_cast<double>(lo), static_cast<double>(lo), ss);
     ss = fma(static_cast<double>(hi), static_cast<double>(hi), ss);
   }
 #pragma unroll
-  for (int m = 8; m >= 1; m >>= 1) ss += __shfl_xor_sync(mask, ss, m);
+  for (int m = kKv4RowLanes / 2; m >= 1; m >>= 1) ss += __shfl_xor_sync(mask, ss, m);
   const double r = rsqrt(ss * (1.0 / kKv4D) + eps);
   const float h = static_cast<float>(r), l = static_cast<float>(r - static_cast<double>(h));
   const uint64_t rh = pair(h, h), rl = pair(l, l);
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const uint64_t a = mul2(x[i], w[i]), b = mul2(x[i + 2], w[i + 2]);  // 16 significant bits: exact
+  for (int i = 0; i < 4; ++i) {
+    const uint64_t a = mul2(x[i], w[i]), b = mul2(x[i + 4], w[i + 4]);  // 16 significant bits: exact
     x[i] = turn_k(a, sub2(0, b), c[i], s[i], rh, rl);
-    x[i + 2] = turn_k(b, a, c[i], s[i], rh, rl);
+    x[i + 4] = turn_k(b, a, c[i], s[i], rh, rl);
   }
 }
 
-// Quantises four values of a lane with their group (eight lanes): the unit of codes
-// and the scale; x becomes the values that the codes stand for.
+// Quantises eight values of a lane with their group (four lanes): the codes, a
+// nibble a channel, and the scale; x becomes the values that the codes stand for.
 __device__ __forceinline__ uint32_t kv4_quantise(uint64_t* x, float& scale, uint32_t mask) {
-  float v[4];
-  unpair(x[0], v[0], v[1]);
-  unpair(x[1], v[2], v[3]);
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) unpair(x[i], v[2 * i], v[2 * i + 1]);
   uint32_t top = 0;  // as bits: an infinity or NaN is above every number
 #pragma unroll
-  for (int i = 0; i < 4; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-#pragma unroll
-  for (int m = 1; m <= 4; m <<= 1) top = max(top, __shfl_xor_sync(mask, top, m));
+  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+  top = max(top, __shfl_xor_sync(mask, top, 1));
+  top = max(top, __shfl_xor_sync(mask, top, 2));
   scale = __bfloat162float(__float2bfloat16_rn(__fdiv_rn(__uint_as_float(top), 7.0f)));
   scale = fmaxf(scale, kBf16Tiny);
   if (top == 0) scale = 1.0f;
@@ -166,78 +168,73 @@ __device__ __forceinline__ uint32_t kv4_quantise(uint64_t* x, float& scale, uint
   // exactly.  Below 2^-80 the remainder would underflow: an IEEE division.
   const float inv = __frcp_rn(scale);
   const uint64_t ii = pair(inv, inv), minus = pair(-scale, -scale);
+  if (scale >= 0x1p-80f) {
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const uint64_t q = mul2(x[i], ii);
-    unpair(fma2(fma2(q, minus, x[i]), ii, q), v[2 * i], v[2 * i + 1]);
-  }
-  if (scale < 0x1p-80f)
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      unpair(x[i], v[2 * i], v[2 * i + 1]);
-      v[2 * i] = __fdiv_rn(v[2 * i], scale);
-      v[2 * i + 1] = __fdiv_rn(v[2 * i + 1], scale);
+    for (int i = 0; i < 4; ++i) {
+      const uint64_t q = mul2(x[i], ii);
+      unpair(fma2(fma2(q, minus, x[i]), ii, q), v[2 * i], v[2 * i + 1]);
     }
-  // Rounded to even in the last place of 1.5 * 2^23, whose low 16 bits are 0; + 8
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __fdiv_rn(v[i], scale);
+  }
+  // Rounded to even in the last place of 1.5 * 2^23, whose low 22 bits are 0; + 8
   // makes the nibble.
-  uint32_t unit = 0;
+  uint32_t low = 0, high = 0;
 #pragma unroll
   for (int i = 3; i >= 0; --i) {
     v[i] = fminf(fmaxf(v[i], -7.0f), 7.0f) + 12582920.0f;
-    unit = unit * 16 + __float_as_uint(v[i]);
+    v[i + 4] = fminf(fmaxf(v[i + 4], -7.0f), 7.0f) + 12582920.0f;
+    low = low * 16 + __float_as_uint(v[i]);
+    high = high * 16 + __float_as_uint(v[i + 4]);
   }
   const uint64_t ss = pair(scale, scale), magic = pair(12582920.0f, 12582920.0f);
 #pragma unroll
-  for (int i = 0; i < 2; ++i) x[i] = mul2(sub2(pair(v[2 * i], v[2 * i + 1]), magic), ss);
-  return unit & 0xFFFFu;
+  for (int i = 0; i < 4; ++i) x[i] = mul2(sub2(pair(v[2 * i], v[2 * i + 1]), magic), ss);
+  return __byte_perm(low, high, 0x5410);
 }
 
-__global__ void __launch_bounds__(256, 4) qk_norm_rope_store_kv4_kernel(const Kv4StoreArgs p) {
-  const int heads = p.Hq + 2 * p.Hkv, lane = threadIdx.x & 15;
-  const uint32_t mask = threadIdx.x & 16 ? 0xFFFF0000u : 0x0000FFFFu;  // the two halves go their own ways
-  const int first = blockIdx.x * 16 + (threadIdx.x >> 4);
+constexpr int kKv4StoreThreads = 128, kKv4StoreCtas = 6;  // an SM
+__global__ void __launch_bounds__(kKv4StoreThreads, kKv4StoreCtas)
+    qk_norm_rope_store_kv4_kernel(const Kv4StoreArgs p) {
+  const int heads = p.Hq + 2 * p.Hkv, lane = threadIdx.x & 7;
+  const uint32_t mask = 0xFFu << (threadIdx.x & 24);  // the octets go their own ways
+  const int first = blockIdx.x * (kKv4StoreThreads / kKv4RowLanes) + (threadIdx.x >> 3);
   int t = first / heads, h = first - t * heads;
   if (first >= p.walkers || t >= p.T) return;
   const uint16_t* src = p.qkv + static_cast<int64_t>(first) * kKv4D;
   const int64_t stride = static_cast<int64_t>(p.walkers) * kKv4D;
-
-  // cos and sin of a position; NaN beyond the table, and an error
-  const auto load_turn = [&](int64_t pos, int head, float4& c, float4& s) {
-    if (head >= p.Hq + p.Hkv) return;  // V
-    if (static_cast<uint64_t>(pos) < static_cast<uint64_t>(p.max_position)) {
-      const float4* cs = reinterpret_cast<const float4*>(p.cos_sin + pos * kKv4D) + lane;
-      c = __ldg(cs);
-      s = __ldg(cs + 16);
-    } else {
-      c = s = make_float4(NAN, NAN, NAN, NAN);
-      if (lane == 0) record_error(kErrBadPosition);
-    }
-  };
-  Row8 raw = load_row(src, lane);
-  float4 c4 = {}, s4 = {};
-  load_turn(p.positions[t], h, c4, s4);
-  int t1 = t + p.walk_tokens, h1 = h + p.walk_heads;  // the row after this one
-  if (h1 >= heads) h1 -= heads, ++t1;
-  int64_t pos1 = t1 < p.T ? p.positions[t1] : 0;
+  RowPart raw = load_row(src, lane);
+  int64_t pos = p.positions[t];
   while (true) {
-    uint64_t x[4];
+    uint64_t x[8];
     unpack_row(raw, x);
-    const uint64_t c[2] = {pair(c4.x, c4.y), pair(c4.z, c4.w)}, s[2] = {pair(s4.x, s4.y), pair(s4.z, s4.w)};
     const int row_t = t, row_h = h;
-    t = t1, h = h1;
+    const int64_t row_pos = pos;
+    t += p.walk_tokens, h += p.walk_heads;  // the row after this one
+    if (h >= heads) h -= heads, ++t;
     const bool more = t < p.T;
     if (more) {
       src += stride;
       raw = load_row(src, lane);
-      load_turn(pos1, h, c4, s4);
-      t1 = t + p.walk_tokens, h1 = h + p.walk_heads;
-      if (h1 >= heads) h1 -= heads, ++t1;
-      pos1 = t1 < p.T ? p.positions[t1] : 0;
+      pos = p.positions[t];
     }
     const bool is_q = row_h < p.Hq, is_k = !is_q && row_h < p.Hq + p.Hkv;
     if (is_q || is_k) {
-      uint64_t w[4];
+      uint64_t w[8], c[4], s[4];
       unpack_row(load_row(is_q ? p.q_weight : p.k_weight, lane), w);
+      if (static_cast<uint64_t>(row_pos) < static_cast<uint64_t>(p.max_position)) {
+        const ulonglong2* cs = reinterpret_cast<const ulonglong2*>(p.cos_sin + row_pos * kKv4D) + lane * 2;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const ulonglong2 cc = __ldg(cs + i), sn = __ldg(cs + 16 + i);
+          c[2 * i] = cc.x, c[2 * i + 1] = cc.y, s[2 * i] = sn.x, s[2 * i + 1] = sn.y;
+        }
+      } else {  // beyond the table: NaN, and an error
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c[i] = s[i] = pair(NAN, NAN);
+        if (lane == 0) record_error(kErrBadPosition);
+      }
       if (is_q) norm_rope_q(x, w, c, s, static_cast<float>(p.eps), mask);
       else norm_rope_k(x, w, c, s, p.eps, mask);
     }
@@ -246,23 +243,31 @@ __global__ void __launch_bounds__(256, 4) qk_norm_rope_store_kv4_kernel(const Kv
     } else {
       const int kvh = row_h - (is_k ? p.Hq : p.Hq + p.Hkv);
       float scale[2];
-      uint32_t unit[2];
+      uint32_t word[2];  // of groups lane / 4 and 2 + lane / 4
 #pragma unroll
-      for (int i = 0; i < 2; ++i) unit[i] = kv4_quantise(x + 2 * i, scale[i], mask);
+      for (int i = 0; i < 2; ++i) word[i] = kv4_quantise(x + 4 * i, scale[i], mask);
       uint16_t* values = is_k ? p.k_out : p.v_out;
-      if (values != nullptr)
-        store_row(values + (static_cast<int64_t>(row_t) * p.Hkv + kvh) * kKv4D, lane, x);
+      if (values != nullptr) store_row(values + (static_cast<int64_t>(row_t) * p.Hkv + kvh) * kKv4D, lane, x);
       const int slot = p.slot_mapping != nullptr ? p.slot_mapping[row_t] : -1;
       if (slot >= 0 && slot < p.num_slots) {
-        const int token = slot % kKv4Page, quad = lane & 7;  // within groups lane / 8 and 2 + lane / 8
+        const int token = slot % kKv4Page, g = lane >> 2, run = lane & 3;
         const int64_t tile = static_cast<int64_t>(slot / kKv4Page) * p.Hkv + kvh;
-        uint8_t* codes = (is_k ? p.k_codes : p.v_codes) + tile * (kKv4Page * kKv4RowBytes) + (lane >> 3) * 4;
-        codes += is_k ? token * kKv4RowBytes + (quad >> 1) * 16 + (quad & 1) * 2
-                      : (token >> 1) * 128 + (quad ^ (2 * ((token >> 1) & 3))) * 16 + (token & 1) * 2;
-        *reinterpret_cast<uint16_t*>(codes) = static_cast<uint16_t>(unit[0]);
-        *reinterpret_cast<uint16_t*>(codes + 8) = static_cast<uint16_t>(unit[1]);
-        if (quad == 0) {
-          uint16_t* scales = (is_k ? p.k_scales : p.v_scales) + (tile * kKv4Page + token) * kKv4Groups + (lane >> 3);
+        if (is_k) {
+          uint8_t* codes = p.k_codes + (tile * kKv4Page + token) * kKv4RowBytes + run * 16 + g * 4;
+          *reinterpret_cast<uint32_t*>(codes) = word[0];
+          *reinterpret_cast<uint32_t*>(codes + 8) = word[1];
+        } else {
+          uint8_t* codes = p.v_codes + tile * (kKv4Page * kKv4RowBytes) + (token >> 1) * 128 + g * 4 + (token & 1) * 2;
+          const int turn = 2 * ((token >> 1) & 3);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            uint8_t* at = codes + ((2 * run + i) ^ turn) * 16;
+            *reinterpret_cast<uint16_t*>(at) = static_cast<uint16_t>(word[0] >> (16 * i));
+            *reinterpret_cast<uint16_t*>(at + 8) = static_cast<uint16_t>(word[1] >> (16 * i));
+          }
+        }
+        if (run == 0) {
+          uint16_t* scales = (is_k ? p.k_scales : p.v_scales) + (tile * kKv4Page + token) * kKv4Groups + g;
           scales[0] = static_cast<uint16_t>(__float_as_uint(scale[0]) >> 16);
           scales[2] = static_cast<uint16_t>(__float_as_uint(scale[1]) >> 16);
         }
@@ -299,16 +304,19 @@ int launch_qk_norm_rope_store_kv4(const void* qkv, const void* q_weight, const v
   a.T = static_cast<int>(tokens);
   a.Hq = static_cast<int>(num_heads);
   a.Hkv = static_cast<int>(num_kv_heads);
-  // as many CTAs of 16 half warps as run at once, or as there are rows for
+  // as many CTAs as run at once, or as there are rows for
+  constexpr int64_t kRows = kKv4StoreThreads / kKv4RowLanes;
   const int64_t heads = num_heads + 2 * num_kv_heads, rows = tokens * heads;
-  const int64_t ctas = std::min<int64_t>((rows + 15) / 16, 4 * static_cast<int64_t>(device_sm_count()));
-  int64_t walkers = ctas * 16;
-  while (walkers > 1 && std::gcd(walkers, heads) != 1) --walkers;
-  if (rows <= ctas * 16) walkers = ctas * 16;  // one row each
+  const int64_t ctas =
+      std::min<int64_t>((rows + kRows - 1) / kRows, kKv4StoreCtas * static_cast<int64_t>(device_sm_count()));
+  int64_t walkers = ctas * kRows;
+  if (rows > walkers)
+    while (walkers > 1 && std::gcd(walkers, heads) != 1) --walkers;
   a.walkers = static_cast<int>(walkers);
   a.walk_tokens = static_cast<int>(walkers / heads);
   a.walk_heads = static_cast<int>(walkers % heads);
-  return launch_kernel(qk_norm_rope_store_kv4_kernel, dim3(static_cast<unsigned>(ctas)), dim3(256), 0, stream, false, a);
+  return launch_kernel(qk_norm_rope_store_kv4_kernel, dim3(static_cast<unsigned>(ctas)),
+                       dim3(kKv4StoreThreads), 0, stream, false, a);
 }
 
 // ------------------------------------------------------------ decode attention
