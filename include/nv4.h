@@ -392,7 +392,7 @@ int nv4_paged_decode_attention_kv4(const void* q, const void* k_codes, const voi
  * error 6 is recorded; tokens beyond `tokens` are dropped.
  * batch <= NV4_STEP_MAX_BATCH.  One launch, no workspace.
  */
-#define NV4_STEP_MAX_BATCH 4096
+#define NV4_STEP_MAX_BATCH 28672
 int nv4_step_tables(const int32_t* cached_lens, const int32_t* new_lens, const int32_t* pages,
                     int32_t* block_tables, int32_t* context_lens, int32_t* query_starts, int32_t* slot_mapping,
                     int64_t* positions, int64_t batch, int64_t rows, int64_t num_listed, int64_t tokens,

@@ -6,8 +6,8 @@
 // the next ceil((cached + new) / page_size) entries of the flat page list.  So
 // the first page of a request and its first token are two prefix sums over the
 // batch, and each output element follows from them by itself.  One launch:
-// every CTA makes both sums in shared memory (a few KB, read from L2) and
-// takes its share of the outputs.  Bound by latency: two loads in a row, the
+// every CTA makes both sums in shared memory (eight bytes a request, which limits
+// the batch) and takes its share of the outputs.  Bound by latency: two loads in a row, the
 // scan, a binary search.
 #include "nv4_device.cuh"
 #include "nv4_launch.h"
@@ -15,7 +15,6 @@
 namespace nv4 {
 
 constexpr int kStepThreads = 256;
-constexpr int kStepMaxBatch = 4096;  // two int32 prefix sums in shared memory: 32 KB
 
 struct StepTablesArgs {
   const int* cached;
@@ -130,8 +129,15 @@ int launch_step_tables(const int* cached, const int* fresh, const int* pages, in
   a.page_size = static_cast<int>(page_size);
   const int64_t items = std::max(std::max(rows * max_pages, tokens), rows + 1);
   const int64_t ctas = std::min<int64_t>((items + kStepThreads - 1) / kStepThreads, 2 * device_sm_count());
+  static int done[64] = {};
+  const int smem = 2 * (a.batch + 1) * static_cast<int>(sizeof(int));
+  if (smem > 48 * 1024) {
+    const int rc = ensure_smem_attr(reinterpret_cast<const void*>(&step_tables_kernel),
+                                    2 * (NV4_STEP_MAX_BATCH + 1) * sizeof(int), done);
+    if (rc != NV4_OK) return rc;
+  }
   return launch_kernel(step_tables_kernel, dim3(static_cast<unsigned>(ctas)), dim3(kStepThreads),
-                       2 * (batch + 1) * sizeof(int), stream, false, a);
+                       smem, stream, false, a);
 }
 
 }  // namespace nv4

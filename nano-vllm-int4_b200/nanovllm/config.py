@@ -1,6 +1,6 @@
 """Engine configuration (the reference's ``nanovllm/config.py:8-35`` semantics).
 
-Same fields, defaults and checks as the reference, with two differences:
+Same fields, defaults and checks as the reference, with two differences and one addition:
 
 * tensor parallelism is allowed for W4A4 (the reference refuses it,
   ``config.py:32-33``): the W4A4 linears shard along N / group-aligned K;
@@ -8,7 +8,10 @@ Same fields, defaults and checks as the reference, with two differences:
   reading a checkpoint (no weights are available offline; the benchmark's
   end-to-end configuration is a random-init Qwen3-8B).  With it,
   ``w4a4_checkpoint="random"`` selects random W4A4 weights (block128 layout,
-  codes in [-8, 7]) without a manifest on disk.
+  codes in [-8, 7]) without a manifest on disk;
+* ``kv_cache_dtype="int4"`` keeps the KV cache in 4 bits (one BF16 scale per 32
+  channels: 144 bytes per token and KV head instead of 512), with any of the
+  linear flavours.
 
 ``model`` is a directory with the Hugging Face ``config.json`` (and, unless
 the load format is dummy, safetensors weights).
@@ -39,6 +42,7 @@ class Config:
 
     use_w4a16: bool = False
     w4a4_checkpoint: str | None = None
+    kv_cache_dtype: str = "bf16"
     load_format: str = "auto"
     seed: int = 0
 
@@ -47,6 +51,8 @@ class Config:
             raise ValueError("kvcache_block_size must be 256 (the decode attention kernel's page)")
         if not 1 <= self.tensor_parallel_size <= 8:
             raise ValueError("tensor_parallel_size must be in 1..8")
+        if self.kv_cache_dtype not in ("bf16", "int4"):
+            raise ValueError("kv_cache_dtype must be 'bf16' or 'int4'")
         if self.load_format not in ("auto", "dummy"):
             raise ValueError("load_format must be 'auto' or 'dummy'")
         self.hf_config = AutoConfig.from_pretrained(self.model)

@@ -74,6 +74,9 @@ class LLMEngine:
         seqs, is_prefill = self.scheduler.schedule()
         computed = sum(len(s) for s in seqs) if is_prefill else len(seqs)
         tokens = self.runner.run(seqs, is_prefill)
+        for seq, found in zip(seqs, self.runner.logprobs):
+            if found is not None:
+                seq.logprobs.append(found)
         done = self.scheduler.postprocess(seqs, tokens)
         return seqs, is_prefill, computed, done
 
@@ -104,7 +107,12 @@ class LLMEngine:
         for s in seqs:
             ids = s.completion_token_ids
             text = self.tokenizer.decode(ids) if self.tokenizer is not None else ""
-            out.append({"text": text, "token_ids": ids})
+            result = {"text": text, "token_ids": ids}
+            if s.top_logprobs is not None:
+                result["logprobs"] = s.logprobs
+            if s.top_prompt_logprobs is not None:
+                result["prompt_logprobs"] = s.prompt_logprobs
+            out.append(result)
         return out
 
     def exit(self):

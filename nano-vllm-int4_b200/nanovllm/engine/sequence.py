@@ -32,6 +32,10 @@ class Sequence:
         self.temperature = params.temperature
         self.max_tokens = params.max_tokens
         self.ignore_eos = params.ignore_eos
+        self.top_logprobs = params.logprobs                 # alternatives asked for, or None
+        self.top_prompt_logprobs = params.prompt_logprobs
+        self.logprobs: list[dict] = []                      # of the generated tokens
+        self.prompt_logprobs: list[dict] | None = None      # of the prompt's tokens after the first
 
     def __len__(self) -> int:
         return len(self.token_ids)

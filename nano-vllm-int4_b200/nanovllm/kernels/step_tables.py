@@ -10,7 +10,7 @@ import torch
 
 from nanovllm import _native
 
-MAX_BATCH = 4096
+MAX_BATCH = 28672
 
 
 class StepTables(NamedTuple):
@@ -38,7 +38,7 @@ def build_step_tables(cached_lens, new_lens, pages, *, num_tokens: int, max_page
     """Block tables, context lengths, slots and positions of a step.
 
     Request b has ``cached_lens[b]`` tokens in the cache and ``new_lens[b]`` to
-    compute (INT32 [B], B <= 4096); it owns the next ceil((cached + new) /
+    compute (INT32 [B], B <= 28672); it owns the next ceil((cached + new) /
     page_size) entries of the flat list ``pages`` (INT32).  ``num_tokens`` is the
     number of new tokens.  ``out`` may have more rows and tokens than the step
     (the padding of a captured batch): rows behind the last request get context

@@ -77,7 +77,7 @@ def tables(ptrs=(), **over):
 
 @pytest.mark.parametrize("over,status", [
     (dict(batch=0), INVALID), (dict(rows=2), INVALID), (dict(listed=-1), INVALID), (dict(tokens=-1), INVALID),
-    (dict(max_pages=0), INVALID), (dict(page=0), INVALID), (dict(batch=4097, rows=4097), UNSUPPORTED)])
+    (dict(max_pages=0), INVALID), (dict(page=0), INVALID), (dict(batch=28673, rows=28673), UNSUPPORTED)])
 def test_step_tables_refusals(over, status):
     assert tables(**over) == status
 
@@ -138,7 +138,7 @@ def test_python_refusals():
     one = torch.ones(2, dtype=torch.int32)
     for bad, over, match in (((one.long(), one, one), {}, "cached"), ((one, one[:1], one), {}, "cached"), ((one, one, one[None]), {}, "pages"),
                              ((one, one, one), dict(num_tokens=-1), "num_tokens"), ((one, one, one), dict(max_pages=0), "max_pages"),
-                             ((one, one, one), {}, "CUDA"), ((torch.ones(4097, dtype=torch.int32),) * 2 + (one,), {}, "4096")):
+                             ((one, one, one), {}, "CUDA"), ((torch.ones(28673, dtype=torch.int32),) * 2 + (one,), {}, "28672")):
         with pytest.raises(ValueError, match=match):
             build_step_tables(*bad, **(dict(num_tokens=2, max_pages=1) | over))
     assert alloc_step_tables(2, 3, 4, "cpu").positions.shape == (3,)
@@ -176,5 +176,22 @@ def test_logprob_workspace():
     """None once the rows alone fill the GPU; a part for every CTA of a row else."""
     size = _native.load().nv4_token_logprobs_workspace_bytes
     assert size(1024, 151936, 20) == 0 and size(1, 100, 5) == 0
-    assert size(1, 151936, 0) > 0 and size(1, 151936, 20) - size(1, 151936, 0) == 64 * 20 * 8
+    assert size(1, 151936, 0) > 0 and size(1, 151936, 20) - size(1, 151936, 0) == 37 * 20 * 8  # 297 chunks, 8 a part
     assert size(1024, 1 << 24, 0) > 0 and size(0, 100, 5) == 0 and size(1, 100, 33) == 0
+
+
+def test_engine_parameters(tmp_path):
+    from nanovllm.config import Config
+    from nanovllm.engine.sequence import Sequence
+    from nanovllm.sampling_params import SamplingParams
+    from nanovllm.utils import synthetic
+    model = synthetic.write_qwen3_config(str(tmp_path), num_hidden_layers=1)
+    assert Config(model).kv_cache_dtype == "bf16" and Config(model, kv_cache_dtype="int4").kv_cache_dtype == "int4"
+    with pytest.raises(ValueError, match="kv_cache_dtype"):
+        Config(model, kv_cache_dtype="fp8")
+    for bad in (dict(logprobs=-1), dict(logprobs=33), dict(prompt_logprobs=33)):
+        with pytest.raises(ValueError, match="logprobs"):
+            SamplingParams(**bad)
+    s = Sequence([1, 2], SamplingParams(logprobs=0, prompt_logprobs=4))
+    assert s.top_logprobs == 0 and s.top_prompt_logprobs == 4 and s.logprobs == [] and s.prompt_logprobs is None
+    assert Sequence([1]).top_logprobs is None

@@ -38,7 +38,7 @@ CASES = [  # cached, new, page_size
     ([0], [1], 256), ([255], [1], 256), ([256], [1], 256), ([0], [257], 256), ([5, 0, 0, 300], [1, 0, 700, 1], 256),
     ([0, 0, 0], [0, 0, 0], 256), ([7, 9, 0], [3, 0, 5], 1), ([100, 3], [28, 61], 16), ([10, 20, 30], [5, 5, 5], 7),
     ([(37 * i) % 2000 for i in range(513)], [1] * 513, 256), ([0] * 1000, [(13 * i) % 40 for i in range(1000)], 256),
-    ([3 * i for i in range(4096)], [i % 3 for i in range(4096)], 256)]
+    ([3 * i for i in range(4097)], [i % 3 for i in range(4097)], 256), ([i % 700 for i in range(28672)], [1] * 28672, 256)]
 
 
 @pytest.mark.parametrize("cached,new,page_size", CASES, ids=range(len(CASES)))
