@@ -331,8 +331,9 @@ int launch_qk_norm_rope_store_kv4(const void* qkv, const void* q_weight, const v
 // itself.  A job that lies within one CTA is finished there; else each CTA
 // writes an unnormalised partial to the workspace (two slots a CTA: the job
 // that it continues, the job that it leaves) and a second kernel joins them in
-// order.  A producer warp copies units into a ring with bulk copies (a unit of
-// a page is contiguous), eight consumer warps take 16 tokens of each.
+// order.  Units come through a ring by bulk copies (a unit of a page is
+// contiguous); four warps take 16 tokens at a time.  One thread of them issues the
+// copies: a warp of its own for that would hold a fifth of the registers.
 //
 // Arithmetic, per 16 tokens and warp, on mma.sync:
 //   S^T [16 tokens x 8 heads], m16n8k16 in BF16: A = K codes as 128 + u (the nibble
@@ -345,7 +346,7 @@ int launch_qk_norm_rope_store_kv4(const void* qkv, const void* q_weight, const v
 // p reaches its B fragment with movmatrix.  The running maximum is moved only
 // when a score exceeds it by 2^8 (p and its sum are at most 2^8 larger then).
 constexpr int kKv4Warps = 4;
-constexpr int kKv4Threads = (kKv4Warps + 1) * 32;
+constexpr int kKv4Threads = kKv4Warps * 32;
 constexpr int kKv4Tiles = 2;                          // 16-token tiles a warp takes of a unit
 constexpr int kKv4Unit = kKv4Warps * kKv4Tiles * 16;  // tokens of a unit; divides the page
 constexpr int kKv4Stages = 2;  // what four CTAs an SM leave room for
@@ -386,6 +387,19 @@ struct Kv4Meta {  // of a unit in the ring
   int tokens;  // valid tokens, 0 for an absent page
   int first;   // first unit of the job in this CTA
   int last;    // 0, or 1 + where the result goes: 1 the output, 2 / 3 partial slot 0 / 1
+};
+
+// What the thread that feeds the ring keeps between units, in shared memory so that
+// it takes no registers meanwhile.
+struct Kv4Feed {
+  int64_t left;      // units to copy
+  int64_t row;       // cache row of the next unit
+  int b, h, k;       // its sequence, KV head and place among the job's n units
+  int n, ctx;
+  int next;          // the page of the next unit that begins one
+  int first, begun;  // the unit is the job's first in this CTA; the job began in this CTA
+  int there;         // its page exists
+  int issued;        // units copied
 };
 
 __device__ __forceinline__ int kv4_context(const Kv4AttnArgs& p, int b) {
@@ -449,6 +463,7 @@ __global__ void __launch_bounds__(kKv4Threads, kKv4CtasPerSm) paged_decode_atten
   extern __shared__ __align__(128) uint8_t smem_kv4[];
   __shared__ uint64_t full[kKv4Stages], empty[kKv4Stages], red_full, red_free;
   __shared__ Kv4Meta meta[kKv4Stages];
+  __shared__ Kv4Feed feed;
   __shared__ int64_t sums[kKv4Threads / 32];
   __shared__ int64_t start_of_b;
   __shared__ int start_b;
@@ -505,87 +520,91 @@ __global__ void __launch_bounds__(kKv4Threads, kKv4CtasPerSm) paged_decode_atten
   grid_dependents_launch();
   if (!working) return;
 
-  if (warp == kKv4Warps) {  // ---- producer: one thread
-    if (lane != 0) return;
+  // The copies of the next unit, by one thread once its stage is free.
+  const auto feed_unit = [&]() {
     constexpr int kPerPage = kKv4Page / kKv4Unit;
-    int b = start_b;
-    const int64_t rest = u0 - start_of_b * p.Hkv;  // units into this sequence
-    int ctx = kv4_context(p, b), n = kv4_units(ctx);
-    int h = static_cast<int>(rest / n), k = static_cast<int>(rest - static_cast<int64_t>(h) * n);
-    const int* table = p.block_tables + static_cast<int64_t>(b) * p.max_pages;
-    int next = table[k / kPerPage];  // the page of the next unit that begins one
-    bool first = true;         // of the job in this CTA
-    bool begun = k == 0;       // the job began in this CTA
-    bool there = true;         // the page exists
-    bool ok = true;
-    int st = 0, filled = 0;    // ring position; stages filled so far, at most kKv4Stages
-    uint32_t round = 0;        // parity of the ring's current round
-    const uint8_t *kc = nullptr, *vc = nullptr, *ks = nullptr, *vs = nullptr;
-    for (int64_t left = u1 - u0; left > 0; --left) {
-      if (first || k % kPerPage == 0) {
-        const int page = next;
-        there = page >= 0 && page < p.num_pages;
-        if (!there) record_error(kErrBadPage);
-        const int64_t row = (static_cast<int64_t>(page) * p.Hkv + h) * kKv4Page + (k % kPerPage) * kKv4Unit;
-        kc = p.k_codes + row * kKv4RowBytes;
-        vc = p.v_codes + row * kKv4RowBytes;
-        ks = reinterpret_cast<const uint8_t*>(p.k_scales + row * kKv4Groups);
-        vs = reinterpret_cast<const uint8_t*>(p.v_scales + row * kKv4Groups);
-        // the page after it, of this job or the first of the next head's
-        const int pi = k / kPerPage + 1;
-        next = table[pi * kPerPage < n ? pi : 0];
-      }
-      if (filled == kKv4Stages) {
-        ok = mbar_wait(&empty[st], round ^ 1, kErrTimeoutEmpty);
-        if (!ok) break;
-      } else {
-        ++filled;
-      }
-      const int tokens = there ? min(kKv4Unit, ctx - k * kKv4Unit) : 0;
-      const bool ends = k + 1 == n, last = left == 1 || ends;
-      Kv4Meta mt;
-      mt.job = b * p.Hkv + h;
-      mt.tokens = tokens;
-      mt.first = first;
-      // the slot of a job that goes on from the CTA before is 0, as is that of one that begins with the CTA
-      mt.last = !last ? 0 : begun && ends ? 1 : begun && u1 - left - k > u0 ? 3 : 2;
-      meta[st] = mt;
-      const uint32_t rows = (tokens + 15) & ~15;
-      const uint32_t q_bytes = first ? G * kKv4D * 2 : 0;
-      mbar_arrive_expect_tx(&full[st], rows * (2 * kKv4RowBytes + 4 * kKv4Groups) + q_bytes);
-      uint8_t* dst = smem_kv4 + st * kKv4StageBytes;
-      if (first) bulk_load(dst + kKv4QAt, p.q + (static_cast<int64_t>(b) * p.Hq + h * G) * kKv4D, q_bytes, &full[st]);
-      if (rows) {
-        bulk_load(dst, kc, rows * kKv4RowBytes, &full[st]);
-        bulk_load(dst + 2 * kKv4CodeBytes, ks, rows * kKv4Groups * 2, &full[st]);
-        bulk_load(dst + kKv4CodeBytes, vc, rows * kKv4RowBytes, &full[st]);
-        bulk_load(dst + 2 * kKv4CodeBytes + kKv4ScaleBytes, vs, rows * kKv4Groups * 2, &full[st]);
-      }
-      kc += kKv4CodeBytes, vc += kKv4CodeBytes, ks += kKv4ScaleBytes, vs += kKv4ScaleBytes;
-      if (++st == kKv4Stages) st = 0, round ^= 1;
-      first = false;
-      if (++k == n) {
-        k = 0, first = begun = true;
-        if (++h == p.Hkv) {
-          h = 0;
-          if (left > 1) {
-            do {
-              ctx = kv4_context(p, ++b);
-              n = kv4_units(ctx);
-            } while (n == 0);
-            table = p.block_tables + static_cast<int64_t>(b) * p.max_pages;
-            next = table[0];
-          }
+    Kv4Feed f = feed;
+    if (f.left == 0) return;
+    const int st = f.issued % kKv4Stages;
+    if (f.first || f.k % kPerPage == 0) {
+      const int page = f.next;
+      f.there = page >= 0 && page < p.num_pages;
+      if (!f.there) record_error(kErrBadPage);
+      f.row = (static_cast<int64_t>(page) * p.Hkv + f.h) * kKv4Page + (f.k % kPerPage) * kKv4Unit;
+      // the page after it, of this job or the first of the next head's
+      const int pi = f.k / kPerPage + 1;
+      f.next = p.block_tables[static_cast<int64_t>(f.b) * p.max_pages + (pi * kPerPage < f.n ? pi : 0)];
+    }
+    const int tokens = f.there ? min(kKv4Unit, f.ctx - f.k * kKv4Unit) : 0;
+    const bool ends = f.k + 1 == f.n;
+    Kv4Meta mt;
+    mt.job = f.b * p.Hkv + f.h;
+    mt.tokens = tokens;
+    mt.first = f.first;
+    // the slot of a job that goes on from the CTA before is 0, as is that of one that begins with the CTA
+    mt.last = f.left > 1 && !ends ? 0 : f.begun && ends ? 1 : f.begun && u1 - f.left - f.k > u0 ? 3 : 2;
+    meta[st] = mt;
+    const uint32_t rows = (tokens + 15) & ~15;
+    const uint32_t q_bytes = f.first ? G * kKv4D * 2 : 0;
+    mbar_arrive_expect_tx(&full[st], rows * (2 * kKv4RowBytes + 4 * kKv4Groups) + q_bytes);
+    uint8_t* dst = smem_kv4 + st * kKv4StageBytes;
+    if (f.first)
+      bulk_load(dst + kKv4QAt, p.q + (static_cast<int64_t>(f.b) * p.Hq + f.h * G) * kKv4D, q_bytes, &full[st]);
+    if (rows) {
+      bulk_load(dst, p.k_codes + f.row * kKv4RowBytes, rows * kKv4RowBytes, &full[st]);
+      bulk_load(dst + 2 * kKv4CodeBytes, p.k_scales + f.row * kKv4Groups, rows * kKv4Groups * 2, &full[st]);
+      bulk_load(dst + kKv4CodeBytes, p.v_codes + f.row * kKv4RowBytes, rows * kKv4RowBytes, &full[st]);
+      bulk_load(dst + 2 * kKv4CodeBytes + kKv4ScaleBytes, p.v_scales + f.row * kKv4Groups, rows * kKv4Groups * 2,
+                &full[st]);
+    }
+    f.row += kKv4Unit;
+    ++f.issued;
+    --f.left;
+    f.first = 0;
+    if (ends) {
+      f.k = 0, f.first = f.begun = 1;
+      if (++f.h == p.Hkv) {
+        f.h = 0;
+        if (f.left > 0) {
+          do {
+            f.ctx = kv4_context(p, ++f.b);
+            f.n = kv4_units(f.ctx);
+          } while (f.n == 0);
+          f.next = p.block_tables[static_cast<int64_t>(f.b) * p.max_pages];
         }
       }
+    } else {
+      ++f.k;
     }
-    // The CTA's shared memory must outlive its copies.
-    if (!ok)  // stages at and behind st were last filled in the round before
-      for (int i = 0; i < filled; ++i) mbar_wait(&full[i], i < st ? round : round ^ 1, kErrTimeoutDrain);
-    return;
+    feed = f;
+  };
+  // The CTA's shared memory must outlive its copies: before leaving early, the
+  // feeding thread waits for those on their way.
+  const auto drain = [&]() {
+    if (tid != 0) return;
+    for (int i = max(feed.issued - kKv4Stages, 0); i < feed.issued; ++i)
+      mbar_wait_drain(&full[i % kKv4Stages], (i / kKv4Stages) & 1);
+  };
+  if (tid == 0) {
+    const int64_t rest = u0 - start_of_b * p.Hkv;  // units into the sequence
+    Kv4Feed f;
+    f.left = u1 - u0;
+    f.row = 0;
+    f.b = start_b;
+    f.ctx = kv4_context(p, f.b);
+    f.n = kv4_units(f.ctx);
+    f.h = static_cast<int>(rest / f.n);
+    f.k = static_cast<int>(rest - static_cast<int64_t>(f.h) * f.n);
+    f.next = p.block_tables[static_cast<int64_t>(f.b) * p.max_pages + f.k / (kKv4Page / kKv4Unit)];
+    f.first = 1;
+    f.begun = f.k == 0;
+    f.there = 1;
+    f.issued = 0;
+    feed = f;
+    for (int i = 0; i < kKv4Stages; ++i) feed_unit();
   }
+  __syncwarp();
 
-  // ---- consumers
   uint32_t magic;
   asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(magic) : "r"(smem_u32(&magic_word)));
   const int gid = lane >> 2, tig = lane & 3;
@@ -597,7 +616,7 @@ __global__ void __launch_bounds__(kKv4Threads, kKv4CtasPerSm) paged_decode_atten
   int st = 0;
   uint32_t round = 0;
   for (int64_t left = u1 - u0; left > 0; --left) {
-    if (!mbar_wait(&full[st], round, kErrTimeoutFull)) return;
+    if (!mbar_wait(&full[st], round, kErrTimeoutFull)) return drain();
     const uint8_t* buf = smem_kv4 + st * kKv4StageBytes;
     const Kv4Meta mt = meta[st];
     if (mt.first) {
@@ -693,6 +712,12 @@ __global__ void __launch_bounds__(kKv4Threads, kKv4CtasPerSm) paged_decode_atten
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(&empty[st]);
+    bool fed = true;
+    if (tid == 0 && left > kKv4Stages) {
+      fed = mbar_wait(&empty[st], round, kErrTimeoutEmpty);
+      if (fed) feed_unit();
+    }
+    if (!__all_sync(0xffffffffu, fed)) return drain();
     if (++st == kKv4Stages) st = 0, round ^= 1;
 
     if (mt.last) {  // join the warps
@@ -703,7 +728,7 @@ __global__ void __launch_bounds__(kKv4Threads, kKv4CtasPerSm) paged_decode_atten
       const int b = mt.job / p.Hkv, h0 = (mt.job - b * p.Hkv) * G;
       float* slot = p.partials + (2 * static_cast<int64_t>(blockIdx.x) + (mt.last == 3)) * kKv4SlotFloats;
       for (int g0 = 0; g0 < G; g0 += 4, ++merges) {  // four heads at a time
-        if (merges > 0 && !mbar_wait(&red_free, (merges - 1) & 1, kErrTimeoutEmpty)) return;
+        if (merges > 0 && !mbar_wait(&red_free, (merges - 1) & 1, kErrTimeoutEmpty)) return drain();
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int head = 2 * tig + e;
@@ -718,7 +743,7 @@ __global__ void __launch_bounds__(kKv4Threads, kKv4CtasPerSm) paged_decode_atten
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&red_full);
-        if (!mbar_wait(&red_full, merges & 1, kErrTimeoutFull)) return;
+        if (!mbar_wait(&red_full, merges & 1, kErrTimeoutFull)) return drain();
         const int d = tid;  // a channel a thread: kKv4Warps * 32 == kKv4D
         for (int head = g0; head < min(G, g0 + 4); ++head) {
           float M = kKv4NoMax, S = 0.0f, acc = 0.0f;
