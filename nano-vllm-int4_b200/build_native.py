@@ -1,4 +1,4 @@
-"""Build libnv4.so, the sm_100a kernel library, in-tree.
+"""Build libnv4.so, the sm_100a kernel library, and its torch binding in-tree.
 
     python nano-vllm-int4_b200/build_native.py [--force] [--ptxas-verbose]
 
@@ -7,6 +7,10 @@ compiled as one translation unit (csrc/nv4_unity.cu) so the device-side error
 word is a single symbol without relocatable device code.  The CUDA runtime is
 linked statically and the driver's tensor-map encoder is resolved at run time,
 so the library depends on nothing but the driver.
+
+_nv4_serving.so (csrc/serving_binding.cpp, a host compiler only) is a Python
+module for the short calls of the serving operators: it checks and allocates
+torch tensors and calls libnv4.so beside it.
 """
 from __future__ import annotations
 
@@ -22,6 +26,7 @@ INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 OUT_DIR = os.path.join(HERE, "nanovllm", "_lib")
 OUT = os.path.join(OUT_DIR, "libnv4.so")
 STAMP = OUT + ".srchash"
+BINDING = os.path.join(OUT_DIR, "_nv4_serving.so")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
@@ -30,16 +35,40 @@ def source_hash() -> str:
     h = hashlib.sha256()
     for d in (CSRC, INCLUDE):
         for name in sorted(os.listdir(d)):
-            if name.endswith((".cu", ".cuh", ".h")):
+            if name.endswith((".cu", ".cuh", ".h", ".cpp")):
                 with open(os.path.join(d, name), "rb") as f:
                     h.update(name.encode() + b"\0" + f.read())
     h.update(" ".join(ARCH).encode())
     return h.hexdigest()
 
 
+def _run(cmd: list[str], failure: str) -> str:
+    proc = subprocess.run(cmd, capture_output=True, text=True)
+    if proc.returncode != 0:
+        sys.stderr.write(proc.stdout + proc.stderr)
+        raise RuntimeError(failure)
+    return proc.stderr
+
+
+def _binding_command() -> list[str]:
+    import sysconfig
+
+    import torch
+    base = os.path.join(os.path.dirname(torch.__file__))
+    lib = os.path.join(base, "lib")
+    cuda = os.path.dirname(os.path.dirname(NVCC))
+    return [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+            "-isystem", os.path.join(base, "include"),
+            "-isystem", os.path.join(base, "include", "torch", "csrc", "api", "include"),
+            "-isystem", sysconfig.get_paths()["include"], "-isystem", os.path.join(cuda, "include"),
+            "-o", BINDING + ".tmp", os.path.join(CSRC, "serving_binding.cpp"), "-L", OUT_DIR, "-lnv4", "-L", lib,
+            "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"]
+
+
 def build(force: bool = False, verbose_ptxas: bool = False) -> str:
     digest = source_hash()
-    if not force and os.path.exists(OUT) and os.path.exists(STAMP):
+    if not force and os.path.exists(OUT) and os.path.exists(BINDING) and os.path.exists(STAMP):
         with open(STAMP) as f:
             if f.read().strip() == digest:
                 return OUT
@@ -49,13 +78,14 @@ def build(force: bool = False, verbose_ptxas: bool = False) -> str:
            "-o", OUT + ".tmp", os.path.join(CSRC, "nv4_unity.cu")]
     if verbose_ptxas:
         cmd[1:1] = ["-Xptxas", "-v"]
-    proc = subprocess.run(cmd, capture_output=True, text=True)
-    if proc.returncode != 0:
-        sys.stderr.write(proc.stdout + proc.stderr)
-        raise RuntimeError("nvcc failed building libnv4.so")
+    if os.path.exists(STAMP):
+        os.remove(STAMP)
+    log = _run(cmd, "nvcc failed building libnv4.so")
     if verbose_ptxas:
-        sys.stderr.write(proc.stderr)
+        sys.stderr.write(log)
     os.replace(OUT + ".tmp", OUT)
+    _run(_binding_command(), "the host compiler failed building _nv4_serving.so")
+    os.replace(BINDING + ".tmp", BINDING)
     with open(STAMP, "w") as f:
         f.write(digest + "\n")
     return OUT

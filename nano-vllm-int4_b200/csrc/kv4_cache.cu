@@ -744,8 +744,8 @@ __global__ void __launch_bounds__(kKv4Threads, kKv4CtasPerSm) paged_decode_atten
         __syncwarp();
         if (lane == 0) mbar_arrive(&red_full);
         if (!mbar_wait(&red_full, merges & 1, kErrTimeoutFull)) return drain();
-        const int d = tid;  // a channel a thread: kKv4Warps * 32 == kKv4D
-        for (int head = g0; head < min(G, g0 + 4); ++head) {
+        const int d = tid % kKv4D;
+        for (int head = g0 + tid / kKv4D; head < min(G, g0 + 4); head += kKv4Threads / kKv4D) {
           float M = kKv4NoMax, S = 0.0f, acc = 0.0f;
 #pragma unroll
           for (int w = 0; w < kKv4Warps; ++w) M = fmaxf(M, red_ml[w][head][0]);
@@ -769,7 +769,7 @@ __global__ void __launch_bounds__(kKv4Threads, kKv4CtasPerSm) paged_decode_atten
     }
   }
 }
-static_assert(kKv4Warps * 32 == kKv4D, "the join takes a channel a thread");
+static_assert(kKv4Threads % kKv4D == 0, "the join takes a channel a thread");
 
 // Joins the partials of the jobs that several CTAs hold, in CTA order, and
 // writes the zeros of empty sequences.  One CTA per (sequence, query head), a

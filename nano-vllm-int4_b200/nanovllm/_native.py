@@ -1,7 +1,8 @@
 """ctypes binding of libnv4.so, the sm_100a kernel library (C ABI in include/nv4.h).
 
-This is the only route from Python to the kernels.  There is no fallback: if
-the library is missing, or the current device is not an sm_100 GPU, every
+This, and for the short serving calls the torch binding beside it (``serving``),
+is the only route from Python to the kernels.  There is no fallback: if the
+library is missing, or the current device is not an sm_100 GPU, every
 entry point raises.  Tensors are passed as raw device pointers and the work is
 enqueued on torch's current stream of the tensors' device, so calls compose
 with torch's stream semantics and CUDA-graph capture.
@@ -401,76 +402,30 @@ def qk_norm_rope_store(qkv, q_weight, k_weight, cos_sin, positions, slot_mapping
 
 
 # ---------------------------------------------------------------- 4-bit KV cache, step tables, log-probabilities
-# These calls are short, so the host's share counts: the device is switched only
-# when another one is current (1.5 us otherwise), and the stream's handle is
-# taken without building a torch.cuda.Stream (0.1 us instead of 2.4).
-def _call(fn, what: str, device: int, *args) -> None:
-    """fn(*args, the current stream of `device`), with `device` current."""
-    if torch.cuda.current_device() == device:
-        status = fn(*args, torch._C._cuda_getCurrentRawStream(device))
-    else:
-        with torch.cuda.device(device):
-            status = fn(*args, torch._C._cuda_getCurrentRawStream(device))
-    if status != OK:
-        check(status, what)
+_serving = None
 
 
-def on_one_device(device: int, *tensors) -> bool:
-    """Whether all tensors (None: left out) are contiguous on the CUDA device of that index."""
-    for t in tensors:
-        if t is not None and (t.get_device() != device or not t.is_contiguous()):
-            return False
-    return device >= 0
-
-
-def _addr(t) -> int:
-    return 0 if t is None else t.data_ptr()
+def serving():
+    """The torch binding of the short serving calls (csrc/serving_binding.cpp), whose
+    kernels are libnv4's; loaded once."""
+    global _serving
+    if _serving is None:
+        load()
+        with _lock:
+            if _serving is None:
+                import importlib.machinery
+                import importlib.util
+                path = os.path.join(os.path.dirname(LIB_PATH), "_nv4_serving.so")
+                if not os.path.exists(path):
+                    raise NativeLibraryError(
+                        f"{path} not found; build it with `python nano-vllm-int4_b200/build_native.py`")
+                loader = importlib.machinery.ExtensionFileLoader("_nv4_serving", path)
+                spec = importlib.util.spec_from_file_location("_nv4_serving", path, loader=loader)
+                module = importlib.util.module_from_spec(spec)
+                loader.exec_module(module)
+                _serving = module
+    return _serving
 
 
 def paged_attention_kv4_workspace_bytes(batch: int, num_heads: int, max_pages: int) -> int:
     return int(load().nv4_paged_attention_kv4_workspace_bytes(batch, num_heads, max_pages))
-
-
-def paged_decode_attention_kv4(q, k_codes, k_scales, v_codes, v_scales, block_tables, context_lens, out, workspace,
-                               scale: float) -> None:
-    """nv4_paged_decode_attention_kv4: q, out [B, Hq, 128], codes [pages, Hkv, 256, 64], scales [pages, Hkv, 256, 4]."""
-    b, hq, d = q.shape
-    pages, hkv, page_size = k_codes.shape[:3]
-    _call(load().nv4_paged_decode_attention_kv4, "nv4_paged_decode_attention_kv4", q.get_device(),
-          q.data_ptr(), k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr(),
-          block_tables.data_ptr(), context_lens.data_ptr(), out.data_ptr(), workspace.data_ptr(),
-          workspace.nbytes, b, hq, hkv, d, page_size, pages, block_tables.shape[1], scale)
-
-
-def qk_norm_rope_store_kv4(qkv, q_weight, k_weight, cos_sin, positions, slot_mapping, q_out, k_out, v_out, k_codes,
-                           k_scales, v_codes, v_scales, num_heads: int, num_kv_heads: int, eps: float) -> None:
-    """nv4_qk_norm_rope_store_kv4 (k_out with v_out, and slot_mapping with the four cache tensors, may be None)."""
-    pages, page_size = (k_codes.shape[0], k_codes.shape[2]) if k_codes is not None else (0, 256)
-    _call(load().nv4_qk_norm_rope_store_kv4, "nv4_qk_norm_rope_store_kv4", qkv.get_device(),
-          qkv.data_ptr(), q_weight.data_ptr(), k_weight.data_ptr(), cos_sin.data_ptr(), positions.data_ptr(),
-          _addr(slot_mapping), q_out.data_ptr(), _addr(k_out), _addr(v_out), _addr(k_codes), _addr(k_scales),
-          _addr(v_codes), _addr(v_scales), qkv.shape[0], num_heads, num_kv_heads, q_out.shape[-1], page_size, pages,
-          cos_sin.shape[0], eps)
-
-
-def step_tables(cached_lens, new_lens, pages, block_tables, context_lens, query_starts, slot_mapping, positions,
-                page_size: int) -> None:
-    """nv4_step_tables; the outputs' shapes give rows, max_pages and tokens."""
-    rows, max_pages = block_tables.shape
-    _call(load().nv4_step_tables, "nv4_step_tables", cached_lens.get_device(),
-          cached_lens.data_ptr(), new_lens.data_ptr(), pages.data_ptr(), block_tables.data_ptr(),
-          context_lens.data_ptr(), query_starts.data_ptr(), slot_mapping.data_ptr(), positions.data_ptr(),
-          cached_lens.shape[0], rows, pages.shape[0], slot_mapping.shape[0], max_pages, page_size)
-
-
-def token_logprobs(logits, targets, logprobs, ranks, entropy, top_logprobs, top_ids) -> None:
-    """nv4_token_logprobs (top_logprobs and top_ids None: no alternatives); the
-    workspace comes from torch's allocator."""
-    rows, vocab = logits.shape
-    top_k = 0 if top_ids is None else top_ids.shape[1]
-    nbytes = load().nv4_token_logprobs_workspace_bytes(rows, vocab, top_k)
-    workspace = logits.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
-    _call(load().nv4_token_logprobs, "nv4_token_logprobs", logits.get_device(),
-          logits.data_ptr(), 1 if logits.dtype == torch.float32 else 0, targets.data_ptr(), logprobs.data_ptr(),
-          ranks.data_ptr(), entropy.data_ptr(), _addr(top_logprobs), _addr(top_ids), _addr(workspace), nbytes, rows,
-          vocab, logits.stride(0), top_k)

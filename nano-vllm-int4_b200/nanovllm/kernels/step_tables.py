@@ -10,8 +10,6 @@ import torch
 
 from nanovllm import _native
 
-MAX_BATCH = 28672
-
 
 class StepTables(NamedTuple):
     block_tables: torch.Tensor   # INT32 [rows, max_pages]: the request's pages, then 0
@@ -25,12 +23,9 @@ def alloc_step_tables(rows: int, tokens: int, max_pages: int, device) -> StepTab
     """Output buffers, for instance a captured graph's static ones."""
     if rows < 1 or tokens < 0 or max_pages < 1:
         raise ValueError("Expected rows>0, tokens>=0, max_pages>0")
-    return _like(torch.empty(0, dtype=torch.int32, device=device), rows, tokens, max_pages)
-
-
-def _like(x, rows: int, tokens: int, max_pages: int) -> StepTables:
-    return StepTables(x.new_empty((rows, max_pages)), x.new_empty(rows), x.new_empty(tokens),
-                      x.new_empty(tokens, dtype=torch.int64), x.new_empty(rows + 1))
+    def new(*shape, dtype=torch.int32):
+        return torch.empty(shape, dtype=dtype, device=device)
+    return StepTables(new(rows, max_pages), new(rows), new(tokens), new(tokens, dtype=torch.int64), new(rows + 1))
 
 
 def build_step_tables(cached_lens, new_lens, pages, *, num_tokens: int, max_pages: int, page_size: int = 256,
@@ -47,31 +42,5 @@ def build_step_tables(cached_lens, new_lens, pages, *, num_tokens: int, max_page
     A token whose page is not listed, is negative or lies beyond ``max_pages``
     gets slot -1 and records device error 6 (``_native.device_error``).
     """
-    if cached_lens.ndim != 1 or cached_lens.shape[0] < 1 or cached_lens.dtype != torch.int32 \
-            or new_lens.shape != cached_lens.shape or new_lens.dtype != torch.int32:
-        raise ValueError("Expected INT32 cached_lens[B] and new_lens[B], B>0")
-    b = cached_lens.shape[0]
-    if b > MAX_BATCH:
-        raise ValueError(f"Expected at most {MAX_BATCH} requests")
-    if pages.ndim != 1 or pages.dtype != torch.int32:
-        raise ValueError("Expected INT32 pages[P]")
-    if num_tokens < 0 or max_pages < 1 or page_size < 1:
-        raise ValueError("Expected num_tokens>=0, max_pages>0, page_size>0")
-    if out is None:
-        out = _like(cached_lens, b, num_tokens, max_pages)
-    else:
-        rows = out.block_tables.shape[0]
-        if out.block_tables.shape != (rows, max_pages) or rows < b or out.context_lens.shape != (rows,) \
-                or out.query_starts.shape != (rows + 1,) or out.slot_mapping.ndim != 1 \
-                or out.slot_mapping.shape[0] < num_tokens or out.positions.shape != out.slot_mapping.shape:
-            raise ValueError("Expected out with block_tables[rows>=B,max_pages], context_lens[rows], "
-                             "query_starts[rows+1], slot_mapping and positions[tokens>=num_tokens]")
-        if out.positions.dtype != torch.int64 or any(
-                x.dtype != torch.int32 for x in (out.block_tables, out.context_lens, out.slot_mapping,
-                                                 out.query_starts)):
-            raise TypeError("Expected INT64 positions and INT32 other outputs")
-    if not _native.on_one_device(cached_lens.get_device(), cached_lens, new_lens, pages, *out):
-        raise ValueError("All tensors must be contiguous on one CUDA device")
-    _native.step_tables(cached_lens, new_lens, pages, out.block_tables, out.context_lens, out.query_starts,
-                        out.slot_mapping, out.positions, page_size)
-    return out
+    return StepTables._make(_native.serving().step_tables(cached_lens, new_lens, pages, num_tokens, max_pages,
+                                                          page_size, *(out or ())))

@@ -150,14 +150,14 @@ def test_python_refusals():
 
 
 def test_cache_checks():
-    from nanovllm.kernels.kv4_cache import _check_cache
+    check = _native.serving().check_cache
     c = alloc_kv4_cache(2, 3, "cpu")
-    assert _check_cache(c) == 3
+    assert check(*c) == 3
     for bad, err in ((c._replace(k_codes=c.k_codes[:, :, :128]), ValueError), (c._replace(v_codes=c.v_codes[:1]), ValueError),
                      (c._replace(k_scales=c.k_scales[..., :2]), ValueError), (c._replace(v_scales=c.v_scales.half()), TypeError),
                      (c._replace(k_codes=c.k_codes.to(torch.int8)), TypeError)):
         with pytest.raises(err):
-            _check_cache(bad)
+            check(*bad)
 
 
 def test_reference_packing_round_trip():

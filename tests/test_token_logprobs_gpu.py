@@ -163,7 +163,12 @@ def test_outputs_stay_in_their_bounds(cuda_device):
     x, targets = logits(t, v, torch.bfloat16, seed=7)
     outs = [Guarded(s, d, cuda_device, canary=9, fill=-5) for s, d in (
         ((t,), torch.float32), ((t,), torch.int64), ((t,), torch.float32), ((t, k), torch.float32), ((t, k), torch.int64))]
-    _native.token_logprobs(x.to(cuda_device), targets.to(cuda_device), *(o.view for o in outs))
+    xd, td = x.to(cuda_device), targets.to(cuda_device)
+    lib = _native.load()
+    ws = torch.empty(lib.nv4_token_logprobs_workspace_bytes(t, v, k), dtype=torch.uint8, device=cuda_device)
+    _native.check(lib.nv4_token_logprobs(xd.data_ptr(), 0, td.data_ptr(), *(o.view.data_ptr() for o in outs[:3]),
+                                         outs[3].view.data_ptr(), outs[4].view.data_ptr(), ws.data_ptr(), ws.numel(), t,
+                                         v, v, k, torch.cuda.current_stream().cuda_stream), "nv4_token_logprobs")
     check(TokenLogprobs(*(o.view for o in outs)), x, targets, k)
     assert all(o.intact() for o in outs)
     empty = token_logprobs(x[:0].to(cuda_device), targets[:0].to(cuda_device), top_k=k)
