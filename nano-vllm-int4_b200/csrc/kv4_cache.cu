@@ -356,6 +356,11 @@ constexpr int kKv4RedStride = kKv4D + 4;  // floats; conflict-free stores of the
 constexpr int kKv4CtasPerSm = 4;
 constexpr int kKv4MaxCtas = kKv4CtasPerSm * 160;
 constexpr int kKv4SlotFloats = kKv4MaxGroup * (kKv4D + 2);  // a partial: outputs, then (max, sum) per head
+// Up to so many output rows the probabilities are taken in two BF16 terms: few
+// values show the rounding's noise (1.41 times the output's own rounding), and
+// one or two short sequences are bound by latency (a 700-token sequence 8.3 and
+// 8.5 us).  Above, one term: 64 ragged sequences 102 us instead of 114.
+constexpr int kKv4TwoTermRows = 32;
 constexpr float kKv4NoMax = -1e30f;
 constexpr float kKv4Slack = 8.0f;  // log2 units by which a score may pass the running maximum
 
@@ -459,6 +464,7 @@ __device__ __forceinline__ uint32_t nibbles_code(uint32_t w, uint32_t magic) {
 // First unit of CTA i of n over `total` units.
 __device__ __forceinline__ int64_t kv4_cut(int64_t total, int i, int n) { return total * i / n; }
 
+template <bool kTwoTerms>
 __global__ void __launch_bounds__(kKv4Threads, kKv4CtasPerSm) paged_decode_attention_kv4_kernel(const Kv4AttnArgs p) {
   extern __shared__ __align__(128) uint8_t smem_kv4[];
   __shared__ uint64_t full[kKv4Stages], empty[kKv4Stages], red_full, red_free;
@@ -702,12 +708,21 @@ __global__ void __launch_bounds__(kKv4Threads, kKv4CtasPerSm) paged_decode_atten
       const uint32_t xa[4] = {va.x, va.y, va.z, va.w}, xb[4] = {vb.x, vb.y, vb.z, vb.w};
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const uint32_t b0 = movmatrix_trans(pack_bf16x2(pr[0] * ga[j], pr[1] * ga[j]));
-        const uint32_t b1 = movmatrix_trans(pack_bf16x2(pr[2] * gb[j], pr[3] * gb[j]));
-        mma_bf16_acc(o[2 * j], nibbles_code<0>(xa[j], magic), nibbles_code<1>(xa[j], magic),
-                     nibbles_code<0>(xb[j], magic), nibbles_code<1>(xb[j], magic), b0, b1);
-        mma_bf16_acc(o[2 * j + 1], nibbles_code<2>(xa[j], magic), nibbles_code<3>(xa[j], magic),
-                     nibbles_code<2>(xb[j], magic), nibbles_code<3>(xb[j], magic), b0, b1);
+        const float x0 = pr[0] * ga[j], x1 = pr[1] * ga[j], x2 = pr[2] * gb[j], x3 = pr[3] * gb[j];
+        const uint32_t p0 = pack_bf16x2(x0, x1), p1 = pack_bf16x2(x2, x3);
+        const uint32_t b0 = movmatrix_trans(p0), b1 = movmatrix_trans(p1);
+        const uint32_t v0 = nibbles_code<0>(xa[j], magic), v1 = nibbles_code<1>(xa[j], magic);
+        const uint32_t v2 = nibbles_code<0>(xb[j], magic), v3 = nibbles_code<1>(xb[j], magic);
+        const uint32_t v4 = nibbles_code<2>(xa[j], magic), v5 = nibbles_code<3>(xa[j], magic);
+        const uint32_t v6 = nibbles_code<2>(xb[j], magic), v7 = nibbles_code<3>(xb[j], magic);
+        mma_bf16_acc(o[2 * j], v0, v1, v2, v3, b0, b1);
+        mma_bf16_acc(o[2 * j + 1], v4, v5, v6, v7, b0, b1);
+        if constexpr (kTwoTerms) {
+          const uint32_t r0 = movmatrix_trans(pack_bf16x2(x0 - bf16lo_to_f32(p0), x1 - bf16hi_to_f32(p0)));
+          const uint32_t r1 = movmatrix_trans(pack_bf16x2(x2 - bf16lo_to_f32(p1), x3 - bf16hi_to_f32(p1)));
+          mma_bf16_acc(o[2 * j], v0, v1, v2, v3, r0, r1);
+          mma_bf16_acc(o[2 * j + 1], v4, v5, v6, v7, r0, r1);
+        }
       }
     }
     __syncwarp();
@@ -771,18 +786,23 @@ __global__ void __launch_bounds__(kKv4Threads, kKv4CtasPerSm) paged_decode_atten
 }
 static_assert(kKv4Threads % kKv4D == 0, "the join takes a channel a thread");
 
-// Joins the partials of the jobs that several CTAs hold, in CTA order, and
-// writes the zeros of empty sequences.  One CTA per (sequence, query head), a
-// thread per channel.  Latency bound, so three rounds of loads: the cuts, the
-// maxima and sums (one part a lane), the outputs (eight in flight).
-__global__ void __launch_bounds__(kKv4D) kv4_merge_kernel(const Kv4AttnArgs p, int grid) {
+// Joins the partials of the jobs that several CTAs hold, and writes the zeros of
+// empty sequences.  One CTA per (sequence, query head), a thread per channel, or
+// four that take every fourth part where a job is spread over many CTAs (a single
+// 32k sequence: 74 parts).  Latency bound, so two rounds of loads: the cuts; the
+// maxima and sums, one part a thread, with the first eight outputs of each thread.
+constexpr int kKv4MergeGroups = 4;
+__global__ void __launch_bounds__(kKv4MergeGroups * kKv4D) kv4_merge_kernel(const Kv4AttnArgs p, int grid) {
+  __shared__ float weight[kKv4MaxCtas], most[kKv4MergeGroups * 4], sums[kKv4MergeGroups * 4];
+  __shared__ float part_acc[kKv4MergeGroups][kKv4D];
   const int b = blockIdx.x / p.Hq, hq = blockIdx.x - b * p.Hq, G = p.Hq / p.Hkv, h = hq / G, g = hq - h * G;
-  const int d = threadIdx.x, lane = d & 31;
+  const int tid = threadIdx.x, d = tid % kKv4D, group = tid / kKv4D, groups = blockDim.x / kKv4D;
+  const int lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
   grid_dependency_wait();
   const int64_t first = p.starts[b], n = p.starts[b + 1] - first, total = p.starts[p.B] * p.Hkv;
   uint16_t* out = p.out + static_cast<int64_t>(blockIdx.x) * kKv4D + d;
   if (n == 0) {
-    *out = 0;
+    if (group == 0) *out = 0;
     return;
   }
   const int ctas = static_cast<int>(min(total, static_cast<int64_t>(grid)));
@@ -792,34 +812,51 @@ __global__ void __launch_bounds__(kKv4D) kv4_merge_kernel(const Kv4AttnArgs p, i
   const int c1 = static_cast<int>((e * ctas + total - 1) / total) - 1;
   if (c0 == c1) return;
   // c0 holds its part in slot 0 when the job is the first of its units, the others always do
-  const int slot0 = kv4_cut(total, c0, ctas) < a ? 1 : 0;
-  float M = kKv4NoMax, S = 0.0f, acc = 0.0f;
-  for (int c = c0; c <= c1; c += 32) {
-    const int parts = min(32, c1 - c + 1);
-    const float* at = p.partials + static_cast<int64_t>(c) * 2 * kKv4SlotFloats;  // part i at 2 i slots, but for slot0
-    float2 ml = make_float2(kKv4NoMax, 0.0f);
-    const int skew = c == c0 ? slot0 : 0;
-    if (lane < parts)
-      ml = *reinterpret_cast<const float2*>(at + (2 * lane + (lane == 0 ? skew : 0)) * kKv4SlotFloats +
-                                            kKv4MaxGroup * kKv4D + 2 * g);
-    float mx = fmaxf(ml.x, M);
+  const int parts = c1 - c0 + 1;
+  const float* at = p.partials + (2 * static_cast<int64_t>(c0)) * kKv4SlotFloats;
+  const int64_t skew = kv4_cut(total, c0, ctas) < a ? kKv4SlotFloats : 0;  // of part 0
+  const auto part = [&](int i) { return at + i * (2 * kKv4SlotFloats) + (i == 0 ? skew : 0); };
+  float v[8];
+  const auto load = [&](int i0) {
 #pragma unroll
-    for (int x = 16; x >= 1; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-    const float keep = ex2(M - mx), f = ex2(ml.x - mx);
-    M = mx;
-    float fs = f * ml.y;
-#pragma unroll
-    for (int x = 16; x >= 1; x >>= 1) fs += __shfl_xor_sync(0xffffffffu, fs, x);
-    S = fmaf(S, keep, fs);
-    acc *= keep;
-    for (int i = 0; i < parts; i += 8) {
-      float v[8];
-#pragma unroll
-      for (int x = 0; x < 8; ++x)
-        v[x] = i + x < parts ? at[(2 * (i + x) + (i + x == 0 ? skew : 0)) * kKv4SlotFloats + g * kKv4D + d] : 0.0f;
-#pragma unroll
-      for (int x = 0; x < 8; ++x) acc = fmaf(__shfl_sync(0xffffffffu, f, (i + x) & 31), v[x], acc);
+    for (int x = 0; x < 8; ++x) {
+      const int i = i0 + x * groups;
+      v[x] = i < parts ? part(i)[g * kKv4D + d] : 0.0f;
     }
+  };
+  load(group);
+  const int kMl = kKv4MaxGroup * kKv4D + 2 * g;
+  float mx = kKv4NoMax;
+  for (int i = tid; i < parts; i += blockDim.x) mx = fmaxf(mx, part(i)[kMl]);
+#pragma unroll
+  for (int x = 16; x >= 1; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+  if (lane == 0) most[warp] = mx;
+  __syncthreads();
+  for (int w = 0; w < warps; ++w) mx = fmaxf(mx, most[w]);
+  float fs = 0.0f;
+  for (int i = tid; i < parts; i += blockDim.x) {
+    const float2 ml = *reinterpret_cast<const float2*>(part(i) + kMl);
+    const float f = ex2(ml.x - mx);
+    weight[i] = f;
+    fs = fmaf(f, ml.y, fs);
+  }
+#pragma unroll
+  for (int x = 16; x >= 1; x >>= 1) fs += __shfl_xor_sync(0xffffffffu, fs, x);
+  if (lane == 0) sums[warp] = fs;
+  __syncthreads();
+  float S = 0.0f, acc = 0.0f;
+  for (int w = 0; w < warps; ++w) S += sums[w];
+  for (int i0 = group; i0 < parts; i0 += 8 * groups) {
+    if (i0 != group) load(i0);
+#pragma unroll
+    for (int x = 0; x < 8; ++x)
+      if (i0 + x * groups < parts) acc = fmaf(weight[i0 + x * groups], v[x], acc);
+  }
+  if (groups > 1) {
+    part_acc[group][d] = acc;
+    __syncthreads();
+    if (group != 0) return;
+    for (int i = 1; i < groups; ++i) acc += part_acc[i][d];
   }
   *out = __bfloat16_as_ushort(__float2bfloat16_rn(S == 0.0f ? 0.0f : acc / S));
 }
@@ -837,8 +874,10 @@ int launch_paged_decode_attention_kv4(const void* q, const void* k_codes, const 
                                       void* out, void* workspace, int64_t batch, int64_t num_heads,
                                       int64_t num_kv_heads, int64_t num_pages, int64_t max_pages, float scale,
                                       cudaStream_t stream) {
-  static int done[64] = {};
-  int rc = ensure_smem_attr(reinterpret_cast<const void*>(&paged_decode_attention_kv4_kernel), kKv4Smem, done);
+  static int done[2][64] = {};
+  const bool two_terms = batch * num_heads <= kKv4TwoTermRows;
+  const auto kernel = two_terms ? paged_decode_attention_kv4_kernel<true> : paged_decode_attention_kv4_kernel<false>;
+  int rc = ensure_smem_attr(reinterpret_cast<const void*>(kernel), kKv4Smem, done[two_terms]);
   if (rc != NV4_OK) return rc;
   Kv4AttnArgs a;
   a.q = static_cast<const uint16_t*>(q);
@@ -860,9 +899,11 @@ int launch_paged_decode_attention_kv4(const void* q, const void* k_codes, const 
   // no more CTAs than there can be units
   const int ctas = static_cast<int>(std::min<int64_t>(
       kv4_max_ctas(batch, num_kv_heads, max_pages), kKv4CtasPerSm * static_cast<int64_t>(device_sm_count())));
-  rc = launch_kernel(paged_decode_attention_kv4_kernel, dim3(ctas), dim3(kKv4Threads), kKv4Smem, stream, false, a);
+  rc = launch_kernel(kernel, dim3(ctas), dim3(kKv4Threads), kKv4Smem, stream, false, a);
   if (rc != NV4_OK) return rc;
-  return launch_kernel(kv4_merge_kernel, dim3(static_cast<unsigned>(batch * num_heads)), dim3(kKv4D), 0, stream,
+  // more than eight parts a job at the most: four threads a channel
+  const int groups = ctas > 8 * batch * num_kv_heads ? kKv4MergeGroups : 1;
+  return launch_kernel(kv4_merge_kernel, dim3(static_cast<unsigned>(batch * num_heads)), dim3(groups * kKv4D), 0, stream,
                        true, a, ctas);
 }
 
