@@ -428,9 +428,10 @@ int nv4_token_logprobs(const void* logits, int fp32, const int64_t* targets, flo
 int nv4_version(void);                      /* major*10000 + minor*100 + patch */
 const char* nv4_status_string(int status);  /* static string for a status code */
 int nv4_last_cuda_error(void);              /* cudaError_t of the last NV4_ERR_CUDA in this thread */
-/* Reads and clears the error word that bounded device-side waits set when they
- * give up (1-5), and that the bounds checks on device-side indices set: 6 a page,
- * 7 a cache slot, 8 a position (0 = none).  Synchronises the current device. */
+/* Reads and clears the errors recorded on the device: of bounded waits that gave
+ * up (1-5; until it is read, other waits give up early as well), else of the
+ * bounds checks on device-side indices: 6 a page, 7 a cache slot, 8 a position
+ * (0 = none; later calls are not affected).  Synchronises the current device. */
 int nv4_device_error(int* code);
 
 #ifdef __cplusplus

@@ -45,6 +45,12 @@ constexpr int kKv4MaxGroup = 8;     // query heads per KV head
 // exact; about 2^-46 off before the rounding).  That is 18 FP32 operations a
 // value; in FP64 the conversions alone took twice the time.  q needs no such
 // care: FP32, rounded once to BF16.
+//
+// Measured (32 / 8 heads, with the values): 16384 tokens 103 us = 4.1 TB/s (0.63 of
+// the measured copy rate), 301 tokens of 40 / 8 heads 4.7 us, 32 tokens 3.3 us.
+// Next bound: issue (the K and V rows' arithmetic) and the latency of cos, sin and
+// the weights.  Tried and not better: a ring of four rows in shared memory, cos
+// and sin before the row, 64-thread CTAs, five, seven or eight CTAs an SM.
 struct Kv4StoreArgs {
   const uint16_t* qkv;
   const uint16_t* q_weight;
@@ -233,7 +239,7 @@ __global__ void __launch_bounds__(kKv4StoreThreads, kKv4StoreCtas)
       } else {  // beyond the table: NaN, and an error
 #pragma unroll
         for (int i = 0; i < 4; ++i) c[i] = s[i] = pair(NAN, NAN);
-        if (lane == 0) record_error(kErrBadPosition);
+        if (lane == 0) record_index_error(kErrBadPosition);
       }
       if (is_q) norm_rope_q(x, w, c, s, static_cast<float>(p.eps), mask);
       else norm_rope_k(x, w, c, s, p.eps, mask);
@@ -272,7 +278,7 @@ __global__ void __launch_bounds__(kKv4StoreThreads, kKv4StoreCtas)
           scales[2] = static_cast<uint16_t>(__float_as_uint(scale[1]) >> 16);
         }
       } else if (slot >= 0 && lane == 0) {
-        record_error(kErrBadSlot);
+        record_index_error(kErrBadSlot);
       }
     }
     if (!more) return;
@@ -345,6 +351,15 @@ int launch_qk_norm_rope_store_kv4(const void* qkv, const void* q_weight, const v
 //     rounded to BF16: the probability's only rounding.
 // p reaches its B fragment with movmatrix.  The running maximum is moved only
 // when a score exceeds it by 2^8 (p and its sum are at most 2^8 larger then).
+//
+// Measured (32 / 8 heads, with the merge): 32 x 4.2k tokens 50 us = 3.1 TB/s, 64
+// ragged up to 16k 101 us = 3.5 TB/s (0.54 of the measured copy rate), one of 700
+// tokens 7.8 us.  Bound by issue: 303 instructions per 16 tokens, half of them ALU
+// work of the widening at one in two cycles, with four warps a scheduler; without
+// the products the same copies take 65 of the 101 us.  Tried and slower: K as 8-bit
+// integers against q in 16-bit fixed point (exact products, but large scores lost
+// precision with q's outliers), units of 64 tokens, eight-warp CTAs, a producer
+// warp, two tiles of a warp interleaved.
 constexpr int kKv4Warps = 4;
 constexpr int kKv4Threads = kKv4Warps * 32;
 constexpr int kKv4Tiles = 2;                          // 16-token tiles a warp takes of a unit
@@ -535,7 +550,7 @@ __global__ void __launch_bounds__(kKv4Threads, kKv4CtasPerSm) paged_decode_atten
     if (f.first || f.k % kPerPage == 0) {
       const int page = next;
       f.there = page >= 0 && page < p.num_pages;
-      if (!f.there) record_error(kErrBadPage);
+      if (!f.there) record_index_error(kErrBadPage);
       f.row = (static_cast<int64_t>(page) * p.Hkv + f.h) * kKv4Page + (f.k % kPerPage) * kKv4Unit;
       // the page after it, of this job or the first of the next head's
       const int pi = f.k / kPerPage + 1;

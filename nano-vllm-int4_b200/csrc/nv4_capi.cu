@@ -160,15 +160,17 @@ int nv4_last_cuda_error(void) { return t_last_cuda_error; }
 int nv4_device_error(int* code) {
   if (!code) return NV4_ERR_INVALID_ARGUMENT;
   cudaError_t e = cudaDeviceSynchronize();
-  int v = 0;
+  int v = 0, index = 0;
   if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&v, g_device_error, sizeof(int));
+  if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&index, g_index_error, sizeof(int));
   const int zero = 0;
   if (e == cudaSuccess) e = cudaMemcpyToSymbol(g_device_error, &zero, sizeof(int));
+  if (e == cudaSuccess) e = cudaMemcpyToSymbol(g_index_error, &zero, sizeof(int));
   if (e != cudaSuccess) {
     set_last_cuda_error(e);
     return NV4_ERR_CUDA;
   }
-  *code = v;
+  *code = v != 0 ? v : index;
   return NV4_OK;
 }
 

@@ -50,6 +50,14 @@ __device__ __forceinline__ void record_error(int code) {
   atomicCAS(&g_device_error, 0, code);
 }
 
+// Bad indices (6 and up) have a word of their own: the kernel goes on without
+// them, while an error in the first word makes every wait give up.
+__device__ int g_index_error = 0;
+
+__device__ __forceinline__ void record_index_error(int code) {
+  atomicCAS(&g_index_error, 0, code);
+}
+
 __device__ __forceinline__ uint64_t global_timer_ns() {
   uint64_t t;
   asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));

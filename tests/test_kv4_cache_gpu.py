@@ -141,6 +141,26 @@ def test_attention_bad_pages_count_as_absent(cuda_device):
     ref.assert_attention_close(out, want, size)
 
 
+def test_bad_indices_leave_the_rest_and_later_calls_alone(cuda_device):
+    """One sequence's pages are all bad; the other sequences' outputs, and a later call's before the error is
+    read, are those of a batch without it."""
+    cache, _, _ = random_cache(64, 4, cuda_device, seed=20)
+    gen = torch.Generator().manual_seed(21)
+    lens = torch.randint(4000, 16384, (24,), generator=gen, dtype=torch.int32).to(cuda_device)
+    tables = torch.randint(0, 64, (24, 64), generator=gen, dtype=torch.int32).to(cuda_device)
+    q = torch.randn(24, 16, D, generator=gen).bfloat16().to(cuda_device)
+    want = paged_decode_attention_kv4(q, cache, tables, lens, scale=0.1)
+    assert _native.device_error() == 0
+    bad = tables.clone()
+    bad[0] = 64
+    for _ in range(5):
+        out = paged_decode_attention_kv4(q, cache, bad, lens, scale=0.1)
+        assert torch.equal(out[1:], want[1:]) and not out[0].any()
+        assert torch.equal(paged_decode_attention_kv4(q, cache, tables, lens, scale=0.1), want)
+    assert _native.device_error() == 6
+    assert _native.device_error() == 0
+
+
 def test_attention_lengths_beyond_the_table_and_below_zero(cuda_device):
     cache, k, v = random_cache(4, 2, cuda_device, seed=9)
     q = torch.randn(2, 4, D, generator=torch.Generator().manual_seed(2)).bfloat16()
