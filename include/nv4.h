@@ -343,7 +343,8 @@ int nv4_qk_norm_rope_store(const void* qkv, const void* q_weight, const void* k_
  *   k_out/v_out bf16 [tokens, num_kv_heads, 128] or NULL: the values that the
  *              cache holds for the token (what a later read gives), for the
  *              prefill's own attention
- * All pointers 16-byte aligned (positions 8, slot_mapping 4).  head_dim == 128, page_size == 256.
+ * All pointers 16-byte aligned (positions 8, slot_mapping 4).  head_dim == 128, page_size == 256;
+ * up to 2^30 tokens and 2^33 rows (a row: one head of one token).
  */
 int nv4_qk_norm_rope_store_kv4(const void* qkv, const void* q_weight, const void* k_weight, const float* cos_sin,
                                const int64_t* positions, const int32_t* slot_mapping, void* q_out, void* k_out,
@@ -363,8 +364,8 @@ int nv4_qk_norm_rope_store_kv4(const void* qkv, const void* q_weight, const void
  *   workspace     nv4_paged_attention_kv4_workspace_bytes(...) bytes of scratch;
  *                 calls that may overlap need one each
  * Grouped-query attention as nv4_paged_decode_attention (at most 8 query heads
- * per KV head), scale > 0.  Statistics and sums in FP32, the products' operands
- * in 16 bits.  All pointers 16-byte aligned (block_tables, context_lens 4).
+ * per KV head), scale > 0, batch and max_pages up to 65535, batch * num_heads
+ * below 2^31.  Statistics and sums in FP32, the products' operands in 16 bits.  All pointers 16-byte aligned (block_tables, context_lens 4).
  */
 int64_t nv4_paged_attention_kv4_workspace_bytes(int64_t batch, int64_t num_heads, int64_t max_pages);
 int nv4_paged_decode_attention_kv4(const void* q, const void* k_codes, const void* k_scales, const void* v_codes,

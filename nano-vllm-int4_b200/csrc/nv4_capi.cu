@@ -464,7 +464,7 @@ int nv4_paged_decode_attention_kv4(const void* q, const void* k_codes, const voi
     return NV4_ERR_INVALID_ARGUMENT;
   if (batch < 1 || batch > 65535 || num_kv_heads < 1 || num_kv_heads > 65535 || num_heads < num_kv_heads ||
       num_heads % num_kv_heads || num_pages < 1 || num_pages > (int64_t(1) << 23) - 1 || max_pages < 1 ||
-      max_pages > 65535 || !(scale > 0.0f) || !(scale < 1e30f))
+      max_pages > 65535 || batch * num_heads > (int64_t(1) << 31) - 1 || !(scale > 0.0f) || !(scale < 1e30f))
     return NV4_ERR_INVALID_ARGUMENT;
   if (head_dim != 128 || page_size != 256 || num_heads / num_kv_heads > 8) return NV4_ERR_UNSUPPORTED;
   if (workspace_bytes < paged_attention_kv4_workspace_bytes(batch, num_heads, max_pages))

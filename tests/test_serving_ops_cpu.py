@@ -32,7 +32,8 @@ def attention(ptrs=(), **over):
     (dict(hq=1), INVALID), (dict(pages=0), INVALID), (dict(pages=1 << 23), INVALID), (dict(max_pages=0), INVALID),
     (dict(max_pages=1 << 16), INVALID), (dict(scale=0.0), INVALID), (dict(scale=float("nan")), INVALID),
     (dict(scale=float("inf")), INVALID), (dict(ws=16), INVALID), (dict(d=64), UNSUPPORTED), (dict(page=128), UNSUPPORTED),
-    (dict(hq=18), UNSUPPORTED)])
+    (dict(hq=18), UNSUPPORTED),
+    (dict(batch=65535, hq=65535, hkv=65535, ws=1 << 62), INVALID)])
 def test_attention_refusals(over, status):
     assert attention(**over) == status
 
