@@ -180,7 +180,8 @@ PyObject* py_store(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int64_t hq = integer(a[10]), hkv = integer(a[11]);
     const double eps = real(a[12]);
     const at::Tensor* q_in = optional(a[13], "q_out");
-    const bool values = PyObject_IsTrue(a[14]) == 1;
+    const int values = PyObject_IsTrue(a[14]);
+    if (values < 0) throw Raised{};
     if (hq < 1 || hkv < 1) refuse("Expected at least one query head and one KV head");
     if (qkv.dim() != 2 || qkv.scalar_type() != at::kBFloat16 || qkv.size(0) < 1 || qkv.size(1) != (hq + 2 * hkv) * kD)
       refuse("Expected BF16 qkv[T,(Hq+2Hkv)*128], T>0");
@@ -190,7 +191,8 @@ PyObject* py_store(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (cos_sin.dim() != 2 || cos_sin.size(0) < 1 || cos_sin.size(1) != kD || cos_sin.scalar_type() != at::kFloat)
       refuse("Expected FP32 cos_sin[max_position,128]");
     if (!shaped(positions, at::kLong, {t})) refuse("Expected INT64 positions[T]");
-    if (!slots != !cache[0]) refuse("slot_mapping and cache go together");
+    for (const at::Tensor* x : cache)
+      if (!slots != !x) refuse("slot_mapping and cache go together");
     if (slots && !shaped(*slots, at::kInt, {t})) refuse("Expected INT32 slot_mapping[T]");
     if (cache[0] && check_cache(cache) != hkv) refuse("The cache has another number of KV heads");
     if (q_in && !shaped(*q_in, at::kBFloat16, {t, hq, kD})) refuse("Expected BF16 q_out[T,Hq,128]");

@@ -133,9 +133,15 @@ def test_python_refusals():
     for bad, match in (((qkv[:, :-1], w, w, cs, pos, slots, cache), "qkv"), ((qkv, w[:64], w, cs, pos, slots, cache), "weight"),
                        ((qkv, w, w, cs.double(), pos, slots, cache), "cos_sin"), ((qkv, w, w, cs, pos.int(), slots, cache), "positions"),
                        ((qkv, w, w, cs, pos, slots.long(), cache), "slot"), ((qkv, w, w, cs, pos, None, cache), "together"),
+                       ((qkv, w, w, cs, pos, slots, cache._replace(k_scales=None)), "together"),
+                       ((qkv, w, w, cs, pos, None, cache._replace(k_codes=None)), "together"),
                        ((qkv, w, w, cs, pos, slots, cache), "CUDA")):
         with pytest.raises(ValueError, match=match):
             qk_norm_rope_store_kv4(*bad, **kw)
+    with pytest.raises(RuntimeError, match="ambiguous"):
+        qk_norm_rope_store_kv4(qkv, w, w, cs, pos, slots, cache, return_values=torch.ones(2), **kw)
+    with pytest.raises(TypeError, match="tensor"):
+        paged_decode_attention_kv4(q, cache._replace(v_codes=None), tab, lens, scale=0.1)
     one = torch.ones(2, dtype=torch.int32)
     for bad, over, match in (((one.long(), one, one), {}, "cached"), ((one, one[:1], one), {}, "cached"), ((one, one, one[None]), {}, "pages"),
                              ((one, one, one), dict(num_tokens=-1), "num_tokens"), ((one, one, one), dict(max_pages=0), "max_pages"),
