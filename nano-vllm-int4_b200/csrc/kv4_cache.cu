@@ -332,7 +332,7 @@ int launch_qk_norm_rope_store_kv4(const void* qkv, const void* q_weight, const v
 // work per code is what the kernel is arranged around.
 //
 // Split: the tokens of all (sequence, KV head) jobs form one line of 128-token
-// units, cut evenly over a fixed grid (two CTAs an SM), so ragged lengths cost
+// units, cut evenly over a fixed grid (four CTAs an SM), so ragged lengths cost
 // nothing.  The lengths live on the device: every CTA makes the prefix sum
 // itself.  A job that lies within one CTA is finished there; else each CTA
 // writes an unnormalised partial to the workspace (two slots a CTA: the job
@@ -376,7 +376,7 @@ constexpr int kKv4SlotFloats = kKv4MaxGroup * (kKv4D + 2);  // a partial: output
 // one or two short sequences are bound by latency (a 700-token sequence 8.3 and
 // 8.5 us).  Above, one term: 64 ragged sequences 102 us instead of 114.
 constexpr int kKv4TwoTermRows = 32;
-constexpr float kKv4NoMax = -1e30f;
+constexpr float kKv4NoMax = -3.4028234e38f;  // the lowest FP32: any finite score is above it or equal
 constexpr float kKv4Slack = 8.0f;  // log2 units by which a score may pass the running maximum
 
 // Shared memory: the stages (K, V, K scales, V scales, q), then the warps' outputs

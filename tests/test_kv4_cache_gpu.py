@@ -141,6 +141,21 @@ def test_attention_bad_pages_count_as_absent(cuda_device):
     ref.assert_attention_close(out, want, size)
 
 
+def test_attention_scores_far_below_zero(cuda_device):
+    """All scores equal and about -1e33: the mean of the values."""
+    cache, _, _ = random_cache(4, 1, cuda_device, seed=22)
+    cache.k_codes.copy_(cache.k_codes[0, 0, 0].clone().expand_as(cache.k_codes))
+    cache.k_scales.copy_(cache.k_scales[0, 0, 0].clone().expand_as(cache.k_scales))
+    k, v = ref.read_k(cache), ref.read_v(cache)
+    q = (-1e32 * k[0, 0, 0].sign()).bfloat16().view(1, 1, D).expand(3, 4, D).contiguous()
+    tables = torch.tensor([[2, 0], [1, 3], [0, 1]], dtype=torch.int32)
+    lens = [300, 17, 512]
+    out = paged_decode_attention_kv4(q.to(cuda_device), cache, tables.to(cuda_device),
+                                     torch.tensor(lens, dtype=torch.int32, device=cuda_device), scale=0.1)
+    want, size = ref.attention(torch.zeros_like(q), k, v, tables, lens, 0.1)  # equal scores
+    ref.assert_attention_close(out, want, size)
+
+
 def test_bad_indices_leave_the_rest_and_later_calls_alone(cuda_device):
     """One sequence's pages are all bad; the other sequences' outputs, and a later call's before the error is
     read, are those of a batch without it."""
