@@ -416,6 +416,7 @@ struct Kv4Feed {
   int64_t row;       // cache row of the next unit
   int b, h, k;       // its sequence, KV head and place among the job's n units
   int n, ctx;
+  int next;          // the page of the next unit that begins one
   int first, begun;  // the unit is the job's first in this CTA; the job began in this CTA
   int there;         // its page exists
   int issued;        // units copied
@@ -541,20 +542,19 @@ __global__ void __launch_bounds__(kKv4Threads, kKv4CtasPerSm) paged_decode_atten
   if (!working) return;
 
   // The copies of the next unit, by one thread once its stage is free.
-  int next = 0;  // the page of the next unit that begins one: in a register, so that its load is not waited for
   const auto feed_unit = [&]() {
     constexpr int kPerPage = kKv4Page / kKv4Unit;
     Kv4Feed f = feed;
     if (f.left == 0) return;
     const int st = f.issued % kKv4Stages;
     if (f.first || f.k % kPerPage == 0) {
-      const int page = next;
+      const int page = f.next;
       f.there = page >= 0 && page < p.num_pages;
       if (!f.there) record_index_error(kErrBadPage);
       f.row = (static_cast<int64_t>(page) * p.Hkv + f.h) * kKv4Page + (f.k % kPerPage) * kKv4Unit;
       // the page after it, of this job or the first of the next head's
       const int pi = f.k / kPerPage + 1;
-      next = p.block_tables[static_cast<int64_t>(f.b) * p.max_pages + (pi * kPerPage < f.n ? pi : 0)];
+      f.next = p.block_tables[static_cast<int64_t>(f.b) * p.max_pages + (pi * kPerPage < f.n ? pi : 0)];
     }
     const int tokens = f.there ? min(kKv4Unit, f.ctx - f.k * kKv4Unit) : 0;
     const bool ends = f.k + 1 == f.n;
@@ -591,7 +591,7 @@ __global__ void __launch_bounds__(kKv4Threads, kKv4CtasPerSm) paged_decode_atten
             f.ctx = kv4_context(p, ++f.b);
             f.n = kv4_units(f.ctx);
           } while (f.n == 0);
-          next = p.block_tables[static_cast<int64_t>(f.b) * p.max_pages];
+          f.next = p.block_tables[static_cast<int64_t>(f.b) * p.max_pages];
         }
       }
     } else {
@@ -616,7 +616,7 @@ __global__ void __launch_bounds__(kKv4Threads, kKv4CtasPerSm) paged_decode_atten
     f.n = kv4_units(f.ctx);
     f.h = static_cast<int>(rest / f.n);
     f.k = static_cast<int>(rest - static_cast<int64_t>(f.h) * f.n);
-    next = p.block_tables[static_cast<int64_t>(f.b) * p.max_pages + f.k / (kKv4Page / kKv4Unit)];
+    f.next = p.block_tables[static_cast<int64_t>(f.b) * p.max_pages + f.k / (kKv4Page / kKv4Unit)];
     f.first = 1;
     f.begun = f.k == 0;
     f.there = 1;
