@@ -47,7 +47,7 @@ constexpr int kKv4MaxGroup = 8;     // query heads per KV head
 // care: FP32, rounded once to BF16.
 //
 // Measured (32 / 8 heads, with the values): 16384 tokens 103 us = 4.1 TB/s (0.63 of
-// the measured copy rate), 301 tokens of 40 / 8 heads 4.7 us, 32 tokens 3.3 us.
+// the measured copy rate), 301 tokens of 40 / 8 heads 4.5 us, 32 tokens 3.1 us.
 // Next bound: issue (the K and V rows' arithmetic) and the latency of cos, sin and
 // the weights.  Tried and not better: a ring of four rows in shared memory, cos
 // and sin before the row, 64-thread CTAs, five, seven or eight CTAs an SM.
@@ -354,12 +354,13 @@ int launch_qk_norm_rope_store_kv4(const void* qkv, const void* q_weight, const v
 //
 // Measured (32 / 8 heads, with the merge): 32 x 4.2k tokens 50 us = 3.1 TB/s, 64
 // ragged up to 16k 101 us = 3.5 TB/s (0.54 of the measured copy rate), one of 700
-// tokens 7.8 us.  Bound by issue: 303 instructions per 16 tokens, half of them ALU
-// work of the widening at one in two cycles, with four warps a scheduler; without
-// the products the same copies take 65 of the 101 us.  Tried and slower: K as 8-bit
-// integers against q in 16-bit fixed point (exact products, but large scores lost
-// precision with q's outliers), units of 64 tokens, eight-warp CTAs, a producer
-// warp, two tiles of a warp interleaved.
+// tokens 7.8 us.  Bound by issue: about 303 instructions per 16 tokens, half of them
+// ALU work of the widening at one in two cycles; without the products the same
+// copies take 65 of the 101 us, without the copies the products 99.  Tried and
+// slower (64 ragged): units of 64 tokens, five CTAs an SM at 96 registers (110 us),
+// a warp of its own for the copies (105), two tiles of a warp at once, eight-warp
+// CTAs; K as 8-bit integers against q in 16-bit fixed point lost precision at large
+// scores.
 constexpr int kKv4Warps = 4;
 constexpr int kKv4Threads = kKv4Warps * 32;
 constexpr int kKv4Tiles = 2;                          // 16-token tiles a warp takes of a unit

@@ -25,6 +25,10 @@
 //
 // With few rows a row is split over several CTAs, whose results a second kernel
 // joins.
+//
+// Measured: 1024 BF16 rows of 151936 56 us = 5.6 TB/s (0.86 of the measured copy
+// rate; 65 us with 5 alternatives, 72 us with 20), 48 FP32 rows of 100003 with 20
+// alternatives 15 us, one row with 5 alternatives 10 us (two launches' latency).
 #include <cfloat>
 
 #include "nv4_device.cuh"

@@ -9,6 +9,10 @@ Drop-in module paths of the reference:
   nanovllm.utils.loader_w4a4            load_w4a4_model
   nanovllm.LLM, nanovllm.SamplingParams  the engine (Qwen3; W4A4, W4A16 or BF16 linears;
                                         tensor parallelism one process per GPU)
+Beside them:
+  nanovllm.kernels.kv4_cache            4-bit KV cache: store and decode attention
+  nanovllm.kernels.step_tables          block tables, slots, positions from request lengths
+  nanovllm.kernels.token_logprobs       log-probabilities, ranks, entropy, alternatives
 All kernels live in the C-ABI library _lib/libnv4.so (see include/nv4.h).
 """
 __version__ = "0.1.0"

@@ -23,6 +23,7 @@ def alloc_step_tables(rows: int, tokens: int, max_pages: int, device) -> StepTab
     """Output buffers, for instance a captured graph's static ones."""
     if rows < 1 or tokens < 0 or max_pages < 1:
         raise ValueError("Expected rows>0, tokens>=0, max_pages>0")
+
     def new(*shape, dtype=torch.int32):
         return torch.empty(shape, dtype=dtype, device=device)
     return StepTables(new(rows, max_pages), new(rows), new(tokens), new(tokens, dtype=torch.int64), new(rows + 1))
