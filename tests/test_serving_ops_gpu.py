@@ -119,3 +119,48 @@ def test_two_streams_at_once(cuda_device):
         for got, wanted in zip(run, want):
             assert all(torch.equal(x, y) for x, y in zip(got, wanted))
     assert _native.device_error() == 0
+
+
+@pytest.mark.parametrize("inference", [False, True])
+def test_outputs_are_ordinary_tensors(cuda_device, inference):
+    """Contiguous, aligned, apart from one another, alive after the others are gone; writable and copyable."""
+    with torch.inference_mode(inference):
+        _, table = calls(cuda_device)
+        for which, types in ((2, [torch.int32, torch.int32, torch.int32, torch.int64, torch.int32]),
+                             (3, [torch.float32, torch.int64, torch.float32, torch.float32, torch.int64])):
+            call, args = table[which]
+            want = [x.clone() for x in call(**args)]
+            got = list(call(**args))
+            spans = sorted((x.data_ptr(), x.data_ptr() + x.numel() * x.element_size()) for x in got)
+            assert all(a[1] <= b[0] for a, b in zip(spans, spans[1:]))
+            for x, t in zip(got, types):
+                assert x.dtype == t and x.is_contiguous() and x.data_ptr() % 16 == 0 and x.device == cuda_device
+                assert not x.requires_grad and x.is_inference() == inference
+            first = got[0]
+            first.fill_(7)
+            assert all(torch.equal(x, y) for x, y in zip(got[1:], want[1:]))
+            last = got[-1]
+            del got
+            other = [torch.full((1 << 12,), -1, dtype=torch.int32, device=cuda_device) for _ in range(8)]
+            assert torch.equal(last, want[-1]) and (first == 7).all() and len(other) == 8
+            assert torch.equal(last.reshape(-1).cpu(), want[-1].reshape(-1).cpu())
+            assert (last[1:].contiguous() == want[-1][1:]).all()
+    none = token_logprobs(torch.empty(0, 10, device=cuda_device), torch.empty(0, dtype=torch.int64, device=cuda_device), top_k=2)
+    assert [tuple(x.shape) for x in none] == [(0,), (0,), (0,), (0, 2), (0, 2)]
+    for over in (dict(max_pages=(1 << 24) + 1), dict(num_tokens=(1 << 30) + 1)):
+        with pytest.raises(ValueError):
+            build_step_tables(**table[2][1], **(dict(num_tokens=3, max_pages=2) | over))
+
+
+def test_outputs_in_a_captured_graph(cuda_device):
+    _, table = calls(cuda_device)
+    args, probs = table[2][1], table[3][1]
+    table[2][0](**args), table[3][0](**probs)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        tables, found = table[2][0](**args), table[3][0](**probs)
+    args["cached_lens"].copy_(torch.tensor([7, 400], dtype=torch.int32))
+    probs["logits"].copy_(torch.randn(4, 100, device=cuda_device))
+    graph.replay()
+    for got, want in ((tables, table[2][0](**args)), (found, table[3][0](**probs))):
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
