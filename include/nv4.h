@@ -365,7 +365,10 @@ int nv4_qk_norm_rope_store_kv4(const void* qkv, const void* q_weight, const void
  *                 calls that may overlap need one each
  * Grouped-query attention as nv4_paged_decode_attention (at most 8 query heads
  * per KV head), scale > 0, batch and max_pages up to 65535, batch * num_heads
- * below 2^31.  Statistics and sums in FP32, the products' operands in 16 bits.  All pointers 16-byte aligned (block_tables, context_lens 4).
+ * below 2^31.  Statistics and sums in FP32; the probabilities are multiplied in
+ * two BF16 terms whatever the batch, so a sequence's output does not change with
+ * the sequences beside it but for the order of its sums.  All pointers 16-byte
+ * aligned (block_tables, context_lens 4).
  */
 int64_t nv4_paged_attention_kv4_workspace_bytes(int64_t batch, int64_t num_heads, int64_t max_pages);
 int nv4_paged_decode_attention_kv4(const void* q, const void* k_codes, const void* k_scales, const void* v_codes,

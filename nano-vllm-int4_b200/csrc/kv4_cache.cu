@@ -347,16 +347,20 @@ int launch_qk_norm_rope_store_kv4(const void* qkv, const void* q_weight, const v
 //     excess of 136 leaves through the accumulator's start, -136 sum(q), so K needs no
 //     subtraction. The scale is one per token and 32 channels: two MMAs, one FMA.
 //   O^T [128 channels x 8 heads], likewise: A = V codes, exactly (accumulated over
-//     the whole context, so the excess is subtracted first), B = p * scale,
-//     rounded to BF16: the probability's only rounding.
+//     the whole context, so the excess is subtracted first), B = p * scale in two
+//     BF16 terms, whose products go into the same accumulators: the output's own
+//     rounding is then the only one that shows (0.0017 of the norm; 0.0023 with one
+//     term, which takes 102 us instead of 114 for 64 ragged sequences, and nothing less
+//     for a single short one).
 // p reaches its B fragment with movmatrix.  The running maximum is moved only
 // when a score exceeds it by 2^8 (p and its sum are at most 2^8 larger then).
 //
-// Measured (32 / 8 heads, with the merge): 32 x 4.2k tokens 50 us = 3.1 TB/s, 64
-// ragged up to 16k 101 us = 3.5 TB/s (0.54 of the measured copy rate), one of 700
-// tokens 7.8 us.  Bound by issue: about 303 instructions per 16 tokens, half of them
+// Measured (32 / 8 heads, with the merge): 32 x 4.2k tokens 56 us = 2.8 TB/s, 64
+// ragged up to 16k 114 us = 3.1 TB/s (0.48 of the measured copy rate), one of 700
+// tokens 7.9 us.  Before the second term of the probabilities (101 us for the
+// ragged case): bound by issue, about 303 instructions per 16 tokens, half of them
 // ALU work of the widening at one in two cycles; without the products the same
-// copies take 65 of the 101 us, without the copies the products 99.  Tried and
+// copies take 65 of the 101 us, without the copies the products 99.  Tried then and
 // slower (64 ragged): units of 64 tokens, five CTAs an SM at 96 registers (110 us),
 // a warp of its own for the copies (105), two tiles of a warp at once, eight-warp
 // CTAs; K as 8-bit integers against q in 16-bit fixed point lost precision at large
@@ -372,11 +376,6 @@ constexpr int kKv4RedStride = kKv4D + 4;  // floats; conflict-free stores of the
 constexpr int kKv4CtasPerSm = 4;
 constexpr int kKv4MaxCtas = kKv4CtasPerSm * 160;
 constexpr int kKv4SlotFloats = kKv4MaxGroup * (kKv4D + 2);  // a partial: outputs, then (max, sum) per head
-// Up to so many output rows the probabilities are taken in two BF16 terms: few
-// values show the rounding's noise (1.41 times the output's own rounding), and
-// one or two short sequences are bound by latency (a 700-token sequence 8.3 and
-// 8.5 us).  Above, one term: 64 ragged sequences 102 us instead of 114.
-constexpr int kKv4TwoTermRows = 32;
 constexpr float kKv4NoMax = -3.4028234e38f;  // the lowest FP32: any finite score is above it or equal
 constexpr float kKv4Slack = 8.0f;  // log2 units by which a score may pass the running maximum
 
@@ -480,7 +479,6 @@ __device__ __forceinline__ uint32_t nibbles_code(uint32_t w, uint32_t magic) {
 // First unit of CTA i of n over `total` units.
 __device__ __forceinline__ int64_t kv4_cut(int64_t total, int i, int n) { return total * i / n; }
 
-template <bool kTwoTerms>
 __global__ void __launch_bounds__(kKv4Threads, kKv4CtasPerSm) paged_decode_attention_kv4_kernel(const Kv4AttnArgs p) {
   extern __shared__ __align__(128) uint8_t smem_kv4[];
   __shared__ uint64_t full[kKv4Stages], empty[kKv4Stages], red_full, red_free;
@@ -733,12 +731,10 @@ __global__ void __launch_bounds__(kKv4Threads, kKv4CtasPerSm) paged_decode_atten
         const uint32_t v6 = nibbles_code<2>(xb[j], magic), v7 = nibbles_code<3>(xb[j], magic);
         mma_bf16_acc(o[2 * j], v0, v1, v2, v3, b0, b1);
         mma_bf16_acc(o[2 * j + 1], v4, v5, v6, v7, b0, b1);
-        if constexpr (kTwoTerms) {
-          const uint32_t r0 = movmatrix_trans(pack_bf16x2(x0 - bf16lo_to_f32(p0), x1 - bf16hi_to_f32(p0)));
-          const uint32_t r1 = movmatrix_trans(pack_bf16x2(x2 - bf16lo_to_f32(p1), x3 - bf16hi_to_f32(p1)));
-          mma_bf16_acc(o[2 * j], v0, v1, v2, v3, r0, r1);
-          mma_bf16_acc(o[2 * j + 1], v4, v5, v6, v7, r0, r1);
-        }
+        const uint32_t r0 = movmatrix_trans(pack_bf16x2(x0 - bf16lo_to_f32(p0), x1 - bf16hi_to_f32(p0)));
+        const uint32_t r1 = movmatrix_trans(pack_bf16x2(x2 - bf16lo_to_f32(p1), x3 - bf16hi_to_f32(p1)));
+        mma_bf16_acc(o[2 * j], v0, v1, v2, v3, r0, r1);
+        mma_bf16_acc(o[2 * j + 1], v4, v5, v6, v7, r0, r1);
       }
     }
     __syncwarp();
@@ -890,10 +886,9 @@ int launch_paged_decode_attention_kv4(const void* q, const void* k_codes, const 
                                       void* out, void* workspace, int64_t batch, int64_t num_heads,
                                       int64_t num_kv_heads, int64_t num_pages, int64_t max_pages, float scale,
                                       cudaStream_t stream) {
-  static int done[2][64] = {};
-  const bool two_terms = batch * num_heads <= kKv4TwoTermRows;
-  const auto kernel = two_terms ? paged_decode_attention_kv4_kernel<true> : paged_decode_attention_kv4_kernel<false>;
-  int rc = ensure_smem_attr(reinterpret_cast<const void*>(kernel), kKv4Smem, done[two_terms]);
+  static int done[64] = {};
+  const auto kernel = paged_decode_attention_kv4_kernel;
+  int rc = ensure_smem_attr(reinterpret_cast<const void*>(kernel), kKv4Smem, done);
   if (rc != NV4_OK) return rc;
   Kv4AttnArgs a;
   a.q = static_cast<const uint16_t*>(q);

@@ -416,3 +416,28 @@ def test_store_then_attend_in_a_graph(cuda_device):
         want, size = ref.attention(q, ref.read_k(cache), ref.read_v(cache), tables, [a + 1 for a in at], D ** -0.5)
         ref.assert_attention_close(out, want, size)
     assert _native.device_error() == 0
+
+
+@pytest.mark.parametrize("hq,hkv", [(8, 2), (32, 8), (5, 1)])
+def test_attention_rounds_its_result_once(cuda_device, hq, hkv):
+    """The output's rounding to BF16 is the only one that shows, in a batch of any size, and a sequence's
+    output does not depend on the sequences beside it."""
+    lens = [2, 3, 4, 5, 7, 19, 33, 128] * 8
+    scale = 0.1
+    cache, k, v = random_cache(16, hkv, cuda_device, seed=30)
+    tables = spread_tables(lens, 16, 1, seed=31)
+    q = (0.02 * torch.randn(len(lens), hq, D, generator=torch.Generator().manual_seed(32))).bfloat16()
+    td, ld = tables.to(cuda_device), torch.tensor(lens, dtype=torch.int32, device=cuda_device)
+    out = paged_decode_attention_kv4(q.to(cuda_device), cache, td, ld, scale=scale)
+    want, size = ref.attention(q, k, v, tables, lens, scale)
+    # Scores: a group's 32 products with 128 + u <= 143 and their excess 136 sum(q) are summed in FP32, in at most
+    # four roundings (or truncations: 2^-23) of a partial sum of at most 143 sum |q|; group scales are below 1.1.
+    # A probability moves by twice a score's error, and is held in two BF16 terms (2^-16) and FP32 (2^-18 for the
+    # exponential and the sums).
+    moved = 2 * 4 * 2.0 ** -23 * 143 * 1.1 * scale * q.double().abs().sum(-1, keepdim=True)
+    bound = 2.0 ** -8 * want.abs() + (2.0 ** -16 + 2.0 ** -18 + moved) * size
+    assert moved.max() < 2.0 ** -11  # well below a BF16 rounding
+    assert ((out.double().cpu() - want).abs() <= bound).all()
+    for i in (0, 5, 63):
+        alone = paged_decode_attention_kv4(q[i:i + 1].to(cuda_device), cache, td[i:i + 1], ld[i:i + 1], scale=scale)
+        assert torch.equal(alone[0], out[i])
