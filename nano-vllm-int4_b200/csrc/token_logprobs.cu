@@ -64,8 +64,9 @@ struct LogprobArgs {
 };
 
 // Statistics of a set of logits relative to m; m = -inf and S = W = 0 for none
-// above -inf.  From |m| = 2^40 on, neighbouring numbers differ by more than any
-// exponential shows: S is then the number of logits equal to the maximum m, W 0.
+// above -inf.  From |m| = 2^31 on, the next lower FP32 number is 128 or more away
+// (256 but for 2^31 itself) and its exponential is 0: S is then the number of logits
+// equal to the maximum m, W 0.  Below, m - 110 rounds to a number under m.
 struct LogprobStat {
   float m, s, w;
   int above;
@@ -147,7 +148,7 @@ __device__ __forceinline__ void unpack_chunk(const uint4 (&raw)[LaneOf<T>::kVecs
   }
 }
 
-__device__ __forceinline__ bool is_big(float m) { return fabsf(m) >= 0x1p40f; }
+__device__ __forceinline__ bool is_big(float m) { return fabsf(m) >= 0x1p31f; }
 
 // Moves statistics from their reference to the larger m.
 __device__ __forceinline__ void move_stat(float& s, float& w, float from, float m) {
@@ -242,7 +243,7 @@ __device__ __forceinline__ void finish_row(const LogprobArgs& p, int64_t row, fl
 // count are the lanes'.
 template <typename T>
 struct WarpStat {
-  float m, limit, floor;  // reference, m + 1; m - 110 or less, whose exponential is 0
+  float m, limit, floor;  // reference, m + 1; m - 110 or less, whose exponential is 0 (m itself for a big one)
   uint64_t s = 0, w = 0;  // pairs of FP32: even and odd elements
   float above = 0.0f;  // whole numbers below 2^24
   bool nan = false;

@@ -212,3 +212,33 @@ def test_in_a_graph_and_on_streams(cuda_device):
     torch.cuda.synchronize()
     for o in outs:
         check(o, x, targets, 5)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("v", [5003, 40003], ids=["one CTA a row", "split rows"])
+@pytest.mark.parametrize("power", [24, 25, 30, 31, 32, 33, 36, 39, 40, 60])
+def test_maxima_of_any_size(cuda_device, dtype, v, power):
+    """Maxima around and beyond where m - 1 and m - 110 round to m, of either sign, beside zeros, -inf, the type's
+    lowest value and the next number below."""
+    rows = []
+    for m in (2.0 ** power, 1.4 * 2.0 ** power, -(2.0 ** power), -1.4 * 2.0 ** power):
+        m = torch.tensor(m, dtype=dtype)
+        below = torch.nextafter(m, torch.tensor(-INF, dtype=dtype))
+        for other in ([0.0] if m > 0 else []) + [-INF, torch.finfo(dtype).min, below.item(), 2 * m.item() if m < 0 else -m.item()]:
+            row = torch.full((v,), other, dtype=dtype)
+            row[[3, v // 2, v - 1][:1 + len(rows) % 3]] = m
+            rows.append(row)
+    x = torch.stack(rows)
+    targets = torch.arange(len(rows)) % 2 * 7 + 3  # the maximum, another
+    check(token_logprobs(x.to(cuda_device), targets.to(cuda_device), top_k=5), x, targets, 5)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_a_large_maximum_among_ordinary_logits(cuda_device, dtype):
+    """A forced token, wherever it stands: logprob 0, entropy 0."""
+    x, _ = logits(9, 20000, dtype, seed=12)
+    at = torch.tensor([0, 511, 512, 7777, 19999, 8191, 4096, 100, 15000])
+    x[torch.arange(9), at] = torch.tensor([2e9, 3e9, 1e10, 1e11, 1e12, 5e9, 2.5e9, 4.3e9, 1e30]).to(dtype)
+    got = token_logprobs(x.to(cuda_device), at.to(cuda_device), top_k=3)
+    check(got, x, at, 3)
+    assert not got.logprobs.any() and not got.entropy.any()
