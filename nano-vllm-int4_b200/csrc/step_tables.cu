@@ -131,12 +131,11 @@ int launch_step_tables(const int* cached, const int* fresh, const int* pages, in
   const int64_t items = std::max(std::max(rows * max_pages, tokens), rows + 1);
   const int64_t ctas = std::min<int64_t>((items + kStepThreads - 1) / kStepThreads, 2 * device_sm_count());
   static int done[64] = {};
+  // For every batch: without it the static shared memory takes its part of the 48 KB.
+  const int rc = ensure_smem_attr(reinterpret_cast<const void*>(&step_tables_kernel),
+                                  2 * (NV4_STEP_MAX_BATCH + 1) * sizeof(int), done);
+  if (rc != NV4_OK) return rc;
   const int smem = 2 * (a.batch + 1) * static_cast<int>(sizeof(int));
-  if (smem > 48 * 1024) {
-    const int rc = ensure_smem_attr(reinterpret_cast<const void*>(&step_tables_kernel),
-                                    2 * (NV4_STEP_MAX_BATCH + 1) * sizeof(int), done);
-    if (rc != NV4_OK) return rc;
-  }
   return launch_kernel(step_tables_kernel, dim3(static_cast<unsigned>(ctas)), dim3(kStepThreads),
                        smem, stream, false, a);
 }

@@ -1,5 +1,9 @@
 """Step tables built on the GPU against the engine's own lists (Sequence.slot and
 the padded page lists)."""
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -105,3 +109,22 @@ def test_in_a_graph(cuda_device):
         graph.replay()
         for o, want in zip(out, expected(lens, ones, pages.tolist(), max_pages, 256, b, b)):
             assert torch.equal(o.cpu(), want)
+
+
+def test_batches_around_48_kb_of_shared_memory(cuda_device):
+    """In a process of its own, so that no larger batch came before."""
+    program = """
+import sys, torch
+sys.path[:0] = sys.argv[1:]
+from nanovllm.kernels.step_tables import build_step_tables
+for b in (6128, 6143, 6127, 6142, 6144, 28672, 1):
+    one = torch.ones(b, dtype=torch.int32, device="cuda")
+    pages = torch.arange(b, dtype=torch.int32, device="cuda")
+    t = build_step_tables(one, one, pages, num_tokens=b, max_pages=1)
+    assert torch.equal(t.block_tables[:, 0], pages) and (t.context_lens == 2).all() and (t.positions == 1).all(), b
+    assert torch.equal(t.slot_mapping, pages * 256 + 1), b
+    assert torch.equal(t.query_starts, torch.arange(b + 1, dtype=torch.int32, device="cuda")), b
+"""
+    package = os.path.dirname(os.path.dirname(os.path.abspath(_native.__file__)))
+    done = subprocess.run([sys.executable, "-c", program, package], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
