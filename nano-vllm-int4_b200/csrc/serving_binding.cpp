@@ -4,6 +4,8 @@
 // call itself.  The same through Python and ctypes took 17 to 22 us of host time
 // a call, most of it in new tensors (2.5 us each there, 0.9 us here) and checks;
 // here it is 4 to 8 us in a loop of one call (x.add_(1) takes 4.4), 6 to 12 among others.
+// Every output has storage of its own: parts of one allocation would save 3 us of
+// the step tables' 9, but could not be saved together and would keep one another alive.
 // The calls go to the C ABI of include/nv4.h.
 #include <Python.h>
 
@@ -81,29 +83,6 @@ void launch(int device, const char* name, const Call& call) {
 
 at::Tensor fresh(const at::Tensor& like, at::IntArrayRef sizes, at::ScalarType type) {
   return at::empty(sizes, like.options().dtype(type).memory_format(c10::nullopt));
-}
-
-// Several small outputs of a call in one allocation, which lives as long as any of
-// them: a tensor of its own costs 0.8 us more than a part.
-struct Part {
-  at::IntArrayRef sizes;
-  at::ScalarType type;
-};
-template <size_t N>
-void fresh_parts(const at::Tensor& like, const Part (&parts)[N], at::Tensor* out) {
-  int64_t at[N], bytes = 0;
-  for (size_t i = 0; i < N; ++i) {
-    at[i] = bytes;
-    bytes += (c10::multiply_integers(parts[i].sizes) * static_cast<int64_t>(c10::elementSize(parts[i].type)) + 255) / 256 * 256;
-  }
-  const at::Tensor whole = fresh(like, {bytes}, at::kByte);
-  for (size_t i = 0; i < N; ++i) {
-    out[i] = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(whole.storage()), whole.key_set(),
-                                                      c10::scalarTypeToTypeMeta(parts[i].type));
-    c10::TensorImpl* impl = out[i].unsafeGetTensorImpl();
-    impl->set_sizes_contiguous(parts[i].sizes);
-    impl->set_storage_offset(at[i] / static_cast<int64_t>(c10::elementSize(parts[i].type)));
-  }
 }
 
 // KV heads of a well-formed cache (k_codes, k_scales, v_codes, v_scales).
@@ -280,9 +259,11 @@ PyObject* py_step_tables(PyObject*, PyObject* const* a, Py_ssize_t n) {
       device.check();
       if (max_pages > int64_t(1) << 24 || tokens > int64_t(1) << 30)
         refuse("Expected num_tokens<=2^30 and max_pages<=2^24");
-      const int64_t table[2] = {b, max_pages}, starts = b + 1;
-      fresh_parts(cached, {{table, at::kInt}, {b, at::kInt}, {tokens, at::kInt}, {tokens, at::kLong}, {starts, at::kInt}},
-                  out);
+      out[0] = fresh(cached, {b, max_pages}, at::kInt);
+      out[1] = fresh(cached, {b}, at::kInt);
+      out[2] = fresh(cached, {tokens}, at::kInt);
+      out[3] = fresh(cached, {tokens}, at::kLong);
+      out[4] = fresh(cached, {b + 1}, at::kInt);
     }
     const auto i32 = [](const at::Tensor& t) { return static_cast<int32_t*>(t.data_ptr()); };
     launch(device.index(), "nv4_step_tables", [&](void* stream) {
@@ -319,12 +300,8 @@ PyObject* py_logprobs(PyObject*, PyObject* const* a, Py_ssize_t n) {
       refuse("All tensors must be on one CUDA device, targets contiguous");
     if ((v > 1 && logits.stride(1) != 1) || (t > 1 && logits.stride(0) < v))
       refuse("The logits of a row must be contiguous, and rows must not overlap");
-    at::Tensor out[5];
-    const int64_t tops[2] = {t, k};
-    if (k)
-      fresh_parts(logits, {{t, at::kFloat}, {t, at::kLong}, {t, at::kFloat}, {tops, at::kFloat}, {tops, at::kLong}}, out);
-    else
-      fresh_parts(logits, {{t, at::kFloat}, {t, at::kLong}, {t, at::kFloat}}, out);
+    at::Tensor out[5] = {fresh(logits, {t}, at::kFloat), fresh(logits, {t}, at::kLong), fresh(logits, {t}, at::kFloat)};
+    if (k) out[3] = fresh(logits, {t, k}, at::kFloat), out[4] = fresh(logits, {t, k}, at::kLong);
     if (t) {
       const int64_t nbytes = nv4_token_logprobs_workspace_bytes(t, v, k);
       at::Tensor ws;

@@ -1,6 +1,8 @@
 """What the Python entry points of the 4-bit cache, the step tables and the
 log-probabilities refuse on a GPU, before any launch: tensors of another device,
 not contiguous or not aligned; and their use on other streams."""
+import io
+
 import pytest
 import torch
 
@@ -164,3 +166,18 @@ def test_outputs_in_a_captured_graph(cuda_device):
     graph.replay()
     for got, want in ((tables, table[2][0](**args)), (found, table[3][0](**probs))):
         assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+def test_outputs_have_storage_of_their_own(cuda_device):
+    """They can be saved together, and one that is kept keeps no other alive."""
+    _, table = calls(cuda_device)
+    for which in (2, 3):
+        call, args = table[which]
+        got = list(call(**args))
+        for x in got:
+            assert x.untyped_storage().nbytes() == x.numel() * x.element_size() and x.storage_offset() == 0
+        assert len({x.untyped_storage().data_ptr() for x in got}) == len(got)
+        file = io.BytesIO()
+        torch.save(got, file)
+        file.seek(0)
+        assert all(torch.equal(a, b) for a, b in zip(torch.load(file), got))
