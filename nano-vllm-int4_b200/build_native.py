@@ -1,6 +1,6 @@
 """Build libnv4.so, the sm_100a kernel library, and its torch binding in-tree.
 
-    python nano-vllm-int4_b200/build_native.py [--force] [--ptxas-verbose]
+    python nano-vllm-int4_b200/build_native.py [--force] [--ptxas-verbose] [--no-binding]
 
 nvcc cross-compiles for sm_100a without a GPU.  All kernel sources are
 compiled as one translation unit (csrc/nv4_unity.cu) so the device-side error
@@ -10,7 +10,9 @@ so the library depends on nothing but the driver.
 
 _nv4_serving.so (csrc/serving_binding.cpp, a host compiler only) is a Python
 module for the short calls of the serving operators: it checks and allocates
-torch tensors and calls libnv4.so beside it.
+torch tensors and calls libnv4.so beside it.  It holds to the torch and Python
+that it was compiled against, so these belong to its stamp; a user of the C ABI
+alone, without torch, leaves it out with --no-binding.
 """
 from __future__ import annotations
 
@@ -25,21 +27,55 @@ CSRC = os.path.join(HERE, "csrc")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 OUT_DIR = os.path.join(HERE, "nanovllm", "_lib")
 OUT = os.path.join(OUT_DIR, "libnv4.so")
-STAMP = OUT + ".srchash"
 BINDING = os.path.join(OUT_DIR, "_nv4_serving.so")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
-def source_hash() -> str:
+def _digest(names: list[tuple[str, str]], rest: str) -> str:
     h = hashlib.sha256()
-    for d in (CSRC, INCLUDE):
-        for name in sorted(os.listdir(d)):
-            if name.endswith((".cu", ".cuh", ".h", ".cpp")):
-                with open(os.path.join(d, name), "rb") as f:
-                    h.update(name.encode() + b"\0" + f.read())
-    h.update(" ".join(ARCH).encode())
+    for d, name in names:
+        with open(os.path.join(d, name), "rb") as f:
+            h.update(name.encode() + b"\0" + f.read())
+    h.update(rest.encode())
     return h.hexdigest()
+
+
+def source_hash() -> str:
+    """Of what libnv4.so is built from."""
+    return _digest([(d, n) for d in (CSRC, INCLUDE) for n in sorted(os.listdir(d)) if n.endswith((".cu", ".cuh", ".h"))],
+                   " ".join(ARCH))
+
+
+def binding_hash() -> str:
+    """Of what _nv4_serving.so is built from and against: a module of another torch
+    or Python may load and then misread their objects."""
+    import sysconfig
+
+    import torch
+    return _digest([(CSRC, "serving_binding.cpp"), (INCLUDE, "nv4.h")],
+                   " ".join((torch.__version__, str(torch.compiled_with_cxx11_abi()),
+                             sysconfig.get_config_var("EXT_SUFFIX") or sys.version)))
+
+
+def _fresh(built: str, digest: str) -> bool:
+    stamp = built + ".srchash"
+    if not os.path.exists(built) or not os.path.exists(stamp):
+        return False
+    with open(stamp) as f:
+        return f.read().strip() == digest
+
+
+def _replace(built: str, cmd: list[str], digest: str, failure: str) -> str:
+    """Runs cmd, which writes built + ".tmp", and puts that and its stamp in place."""
+    stamp = built + ".srchash"
+    if os.path.exists(stamp):
+        os.remove(stamp)
+    log = _run(cmd, failure)
+    os.replace(built + ".tmp", built)
+    with open(stamp, "w") as f:
+        f.write(digest + "\n")
+    return log
 
 
 def _run(cmd: list[str], failure: str) -> str:
@@ -66,28 +102,23 @@ def _binding_command() -> list[str]:
             "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"]
 
 
-def build(force: bool = False, verbose_ptxas: bool = False) -> str:
-    digest = source_hash()
-    if not force and os.path.exists(OUT) and os.path.exists(BINDING) and os.path.exists(STAMP):
-        with open(STAMP) as f:
-            if f.read().strip() == digest:
-                return OUT
+def build(force: bool = False, verbose_ptxas: bool = False, binding: bool = True) -> str:
+    """Builds what is not current; `binding` false leaves _nv4_serving.so (and torch) aside."""
     os.makedirs(OUT_DIR, exist_ok=True)
-    cmd = [NVCC, *ARCH, "-O3", "-lineinfo", "-std=c++17", "-shared", "-Xcompiler", "-fPIC",
-           "-Xcompiler", "-fvisibility=hidden", "--cudart", "static", "-I", INCLUDE,
-           "-o", OUT + ".tmp", os.path.join(CSRC, "nv4_unity.cu")]
-    if verbose_ptxas:
-        cmd[1:1] = ["-Xptxas", "-v"]
-    if os.path.exists(STAMP):
-        os.remove(STAMP)
-    log = _run(cmd, "nvcc failed building libnv4.so")
-    if verbose_ptxas:
-        sys.stderr.write(log)
-    os.replace(OUT + ".tmp", OUT)
-    _run(_binding_command(), "the host compiler failed building _nv4_serving.so")
-    os.replace(BINDING + ".tmp", BINDING)
-    with open(STAMP, "w") as f:
-        f.write(digest + "\n")
+    digest = source_hash()
+    if force or not _fresh(OUT, digest):
+        cmd = [NVCC, *ARCH, "-O3", "-lineinfo", "-std=c++17", "-shared", "-Xcompiler", "-fPIC",
+               "-Xcompiler", "-fvisibility=hidden", "--cudart", "static", "-I", INCLUDE,
+               "-o", OUT + ".tmp", os.path.join(CSRC, "nv4_unity.cu")]
+        if verbose_ptxas:
+            cmd[1:1] = ["-Xptxas", "-v"]
+        log = _replace(OUT, cmd, digest, "nvcc failed building libnv4.so")
+        if verbose_ptxas:
+            sys.stderr.write(log)
+    if binding:
+        digest = binding_hash()
+        if force or not _fresh(BINDING, digest):
+            _replace(BINDING, _binding_command(), digest, "the host compiler failed building _nv4_serving.so")
     return OUT
 
 
@@ -95,5 +126,6 @@ if __name__ == "__main__":
     ap = argparse.ArgumentParser(description=__doc__)
     ap.add_argument("--force", action="store_true")
     ap.add_argument("--ptxas-verbose", action="store_true")
+    ap.add_argument("--no-binding", action="store_true")
     args = ap.parse_args()
-    print(build(args.force, args.ptxas_verbose))
+    print(build(args.force, args.ptxas_verbose, not args.no_binding))

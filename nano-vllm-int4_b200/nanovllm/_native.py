@@ -62,9 +62,10 @@ _lock = threading.Lock()
 _vp, _i64, _int = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int
 
 
-def _check_fresh(path: str) -> None:
+def _check_fresh(path: str, digest: str = "source_hash") -> None:
     """Refuse a library built from other sources than the ones beside it (when
-    the sources are present): a stale binary would silently run old kernels."""
+    the sources are present): a stale binary would silently run old kernels.
+    ``digest`` names the build script's function for what it is built from."""
     pkg = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     builder = os.path.join(pkg, "build_native.py")
     stamp = path + ".srchash"
@@ -75,9 +76,10 @@ def _check_fresh(path: str) -> None:
     mod = importlib.util.module_from_spec(spec)
     spec.loader.exec_module(mod)
     recorded = open(stamp).read().strip() if os.path.exists(stamp) else ""
-    if recorded != mod.source_hash():
+    if recorded != getattr(mod, digest)():
+        what = "sources" if digest == "source_hash" else "sources, for this torch and Python"
         raise NativeLibraryError(
-            f"{path} was not built from the current sources; rebuild with "
+            f"{path} was not built from the current {what}; rebuild with "
             f"`python nano-vllm-int4_b200/build_native.py`")
 
 
@@ -419,6 +421,7 @@ def serving():
                 if not os.path.exists(path):
                     raise NativeLibraryError(
                         f"{path} not found; build it with `python nano-vllm-int4_b200/build_native.py`")
+                _check_fresh(path, "binding_hash")
                 loader = importlib.machinery.ExtensionFileLoader("_nv4_serving", path)
                 spec = importlib.util.spec_from_file_location("_nv4_serving", path, loader=loader)
                 module = importlib.util.module_from_spec(spec)
