@@ -58,8 +58,9 @@ class ModelRunner:
         torch.set_default_dtype(torch.bfloat16)
         try:
             with torch.device(self.device):
+                # a request may grow to the end of its last page
                 self.model = Qwen3ForCausalLM(cfg, mode, rank, world, layout, clamp_lo,
-                                              max_position=max(config.max_model_len, 1) + 1)
+                                              max_position=self.max_pages * PAGE_TOKENS)
         finally:
             torch.set_default_dtype(dtype)
         self._load_weights()

@@ -202,3 +202,12 @@ def test_a_step_of_operators_against_64_bits(cuda_device):
         assert abs(got.logprobs[i].item() - logp[targets[i]].item()) <= 2 * off + 1e-5
         assert abs(got.top_logprobs[i, 0].item() - logp.max().item()) <= 2 * off + 1e-5
     assert _native.device_error() == 0
+
+
+@pytest.mark.parametrize("cache", ["int4", "bf16"])
+def test_tokens_up_to_the_end_of_the_last_page(cuda_device, model_dir, cache):
+    """max_model_len within a page: requests may grow to the page's end, as with the next multiple of 256."""
+    texts = prompts((990, 1))
+    short, _ = generate(model_dir, kv_cache_dtype=cache, max_model_len=1000, texts=texts)
+    whole, _ = generate(model_dir, kv_cache_dtype=cache, max_model_len=1024, texts=texts)
+    assert [o["token_ids"] for o in short] == [o["token_ids"] for o in whole]
