@@ -66,6 +66,8 @@ class LLMEngine:
                 raise ValueError("text prompts need a tokenizer in the model directory")
             prompt = self.tokenizer.encode(prompt)
         seq = Sequence(prompt, params)
+        if seq.pages_needed() > self.runner.max_pages:
+            raise ValueError("prompt longer than max_model_len")
         self.scheduler.add(seq)
         return seq
 

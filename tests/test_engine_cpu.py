@@ -194,3 +194,18 @@ def test_bf16_loader_fills_fused_and_sharded_parameters(model_dir, tmp_path):
     sq = src.model.layers[0].self_attn.qkv_proj.weight
     assert torch.equal(qkv[:512], sq[512:1024]) and torch.equal(qkv[512:640], sq[1024 + 128:1280])
     assert torch.equal(dst.model.embed_tokens.weight, src.model.embed_tokens.weight[2048:])
+
+
+def test_prompts_longer_than_the_tables_are_refused_at_the_door():
+    """Before a step would raise with the request, and those beside it, already scheduled."""
+    from types import SimpleNamespace
+
+    from nanovllm.engine.llm_engine import LLMEngine
+    engine = object.__new__(LLMEngine)
+    engine.tokenizer, engine.runner = None, SimpleNamespace(max_pages=2)
+    engine.scheduler = Scheduler(max_num_seqs=4, max_num_batched_tokens=4096, num_pages=10, eos=-1)
+    greedy = SamplingParams(temperature=0.0)
+    kept = engine.add_request(list(range(2 * PAGE_TOKENS)), greedy)
+    with pytest.raises(ValueError, match="max_model_len"):
+        engine.add_request(list(range(2 * PAGE_TOKENS + 1)), greedy)
+    assert list(engine.scheduler.waiting) == [kept]
