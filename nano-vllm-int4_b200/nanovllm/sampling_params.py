@@ -8,6 +8,7 @@ likely alternatives; ``prompt_logprobs = k`` for the same of the prompt's tokens
 after the first.  The reference returns neither.
 """
 from dataclasses import dataclass
+from operator import index
 
 from nanovllm.kernels.token_logprobs import MAX_TOP_K
 
@@ -25,6 +26,14 @@ class SamplingParams:
             raise ValueError("temperature must be >= 0 (0 is greedy)")
         if self.max_tokens < 1:
             raise ValueError("max_tokens must be >= 1")
-        for k in (self.logprobs, self.prompt_logprobs):
-            if k is not None and not 0 <= k <= MAX_TOP_K:
-                raise ValueError(f"logprobs and prompt_logprobs must be None or in 0..{MAX_TOP_K}")
+        for name in ("logprobs", "prompt_logprobs"):
+            k = getattr(self, name)
+            if k is None:
+                continue
+            try:
+                k = index(k)
+            except TypeError:
+                k = -1
+            if not 0 <= k <= MAX_TOP_K:
+                raise ValueError(f"logprobs and prompt_logprobs must be None or an integer in 0..{MAX_TOP_K}")
+            setattr(self, name, k)

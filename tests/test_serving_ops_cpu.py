@@ -202,3 +202,13 @@ def test_engine_parameters(tmp_path):
     s = Sequence([1, 2], SamplingParams(logprobs=0, prompt_logprobs=4))
     assert s.top_logprobs == 0 and s.top_prompt_logprobs == 4 and s.logprobs == [] and s.prompt_logprobs is None
     assert Sequence([1]).top_logprobs is None
+
+
+@pytest.mark.parametrize("bad", [2.5, 1.0, "3", float("nan"), [1], -1, 33])
+def test_logprob_counts_are_whole_numbers(bad):
+    """A step would refuse the rest, with its requests already scheduled."""
+    from nanovllm.sampling_params import SamplingParams
+    for name in ("logprobs", "prompt_logprobs"):
+        with pytest.raises(ValueError, match="logprobs"):
+            SamplingParams(**{name: bad})
+        assert getattr(SamplingParams(**{name: torch.tensor(3)}), name) == 3
