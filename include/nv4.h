@@ -393,7 +393,8 @@ int nv4_paged_decode_attention_kv4(const void* q, const void* k_codes, const voi
  * rows >= batch; rows behind the last request get context 0, pages 0.  Lengths
  * below 0 count as 0.  A token whose page lies beyond `pages` or beyond
  * max_pages, or is negative, gets slot -1, a table entry without a page 0, and
- * error 6 is recorded; tokens beyond `tokens` are dropped.
+ * error 6 is recorded; tokens beyond `tokens` are dropped.  No output may overlap
+ * an input or another output.
  * batch <= NV4_STEP_MAX_BATCH.  One launch, no workspace.
  */
 #define NV4_STEP_MAX_BATCH 28672

@@ -522,6 +522,19 @@ int nv4_step_tables(const int32_t* cached_lens, const int32_t* new_lens, const i
   if (!aligned(cached_lens, 4) || !aligned(new_lens, 4) || !aligned(pages, 4) || !aligned(block_tables, 4) ||
       !aligned(context_lens, 4) || !aligned(query_starts, 4) || !aligned(slot_mapping, 4) || !aligned(positions, 8))
     return NV4_ERR_ALIGNMENT;
+  // Every CTA reads all lengths and pages while others write: no output over an input.
+  const struct {
+    const void* at;
+    int64_t bytes;
+  } spans[8] = {{block_tables, rows * max_pages * 4}, {context_lens, rows * 4}, {query_starts, (rows + 1) * 4},
+                {slot_mapping, tokens * 4}, {positions, tokens * 8}, {cached_lens, batch * 4}, {new_lens, batch * 4},
+                {pages, num_listed * 4}};
+  for (int i = 0; i < 5; ++i)
+    for (int j = i + 1; j < 8; ++j) {
+      const char *a = static_cast<const char*>(spans[i].at), *b = static_cast<const char*>(spans[j].at);
+      if (spans[i].bytes > 0 && spans[j].bytes > 0 && a < b + spans[j].bytes && b < a + spans[i].bytes)
+        return NV4_ERR_INVALID_ARGUMENT;
+    }
   if (!device_is_sm100()) return NV4_ERR_DEVICE;
   return launch_step_tables(cached_lens, new_lens, pages, block_tables, context_lens, query_starts, slot_mapping,
                             positions, batch, rows, num_listed, tokens, max_pages, page_size,

@@ -38,7 +38,8 @@ def build_step_tables(cached_lens, new_lens, pages, *, num_tokens: int, max_page
     page_size) entries of the flat list ``pages`` (INT32).  ``num_tokens`` is the
     number of new tokens.  ``out`` may have more rows and tokens than the step
     (the padding of a captured batch): rows behind the last request get context
-    0 and pages 0, tokens behind the last slot -1 and position 0.
+    0 and pages 0, tokens behind the last slot -1 and position 0.  Its tensors may
+    overlap neither the inputs nor one another.
 
     A token whose page is not listed, is negative or lies beyond ``max_pages``
     gets slot -1 and records device error 6 (``_native.device_error``).

@@ -212,3 +212,24 @@ def test_logprob_counts_are_whole_numbers(bad):
         with pytest.raises(ValueError, match="logprobs"):
             SamplingParams(**{name: bad})
         assert getattr(SamplingParams(**{name: torch.tensor(3)}), name) == 3
+
+
+def spread_pointers():
+    """Addresses of the step tables' arguments, far from one another."""
+    return {i: V(4096 * (i + 1)) for i in range(8)}
+
+
+def test_step_tables_refuse_outputs_over_inputs_or_one_another():
+    """Every CTA reads the lengths and pages while others write."""
+    far = spread_pointers()
+    without_gpu = _native.ERR_DEVICE if not torch.cuda.is_available() else None
+    if without_gpu is not None:  # the arguments pass, the device does not
+        assert tables(ptrs=far) == without_gpu
+        # side by side: 3 lengths, 10 pages; 4 x 4 table, 4 lengths, 5 starts, 9 slots, 9 positions
+        assert tables(ptrs={0: V(256), 1: V(268), 2: V(280), 3: V(320), 4: V(384), 5: V(400), 6: V(420), 7: V(456)}) == without_gpu
+    for out in range(3, 8):
+        for other in range(8):
+            if other != out:
+                assert tables(ptrs=far | {out: far[other]}) == INVALID
+    assert tables(ptrs=far | {3: V(far[0].value - 4 * 4 * 4 + 4)}) == INVALID   # the table's last element
+    assert tables(ptrs=far | {7: V(far[2].value + 9 * 4 + 4 - 8)}) == INVALID   # the last page

@@ -181,3 +181,16 @@ def test_outputs_have_storage_of_their_own(cuda_device):
         torch.save(got, file)
         file.seek(0)
         assert all(torch.equal(a, b) for a, b in zip(torch.load(file), got))
+
+
+def test_step_tables_in_place_are_refused(cuda_device):
+    """Advancing a batch in place: the lengths may not be both input and output."""
+    _, table = calls(cuda_device)
+    call, args = table[2]
+    good = alloc_step_tables(2, 3, 2, cuda_device)
+    for out in (good._replace(context_lens=args["cached_lens"]), good._replace(context_lens=args["new_lens"]),
+                good._replace(query_starts=args["pages"]), good._replace(slot_mapping=good.query_starts)):
+        with pytest.raises(ValueError):
+            call(**args, out=out)
+    want = call(**args)
+    assert all(torch.equal(a, b) for a, b in zip(call(**args, out=good), want))
