@@ -23,6 +23,8 @@ from dataclasses import dataclass
 
 from transformers import AutoConfig
 
+from nanovllm.kernels.kv4_cache import HEAD_DIM
+
 RANDOM_W4A4 = "random"
 
 
@@ -56,6 +58,10 @@ class Config:
         if self.load_format not in ("auto", "dummy"):
             raise ValueError("load_format must be 'auto' or 'dummy'")
         self.hf_config = AutoConfig.from_pretrained(self.model)
+        head_dim = getattr(self.hf_config, "head_dim", None) or \
+            self.hf_config.hidden_size // self.hf_config.num_attention_heads
+        if self.kv_cache_dtype == "int4" and head_dim != HEAD_DIM:
+            raise ValueError(f"the 4-bit KV cache needs head_dim {HEAD_DIM}")
         self.max_model_len = min(self.max_model_len, self.hf_config.max_position_embeddings)
         if self.max_num_batched_tokens < self.max_model_len:
             raise ValueError("max_num_batched_tokens must hold one whole prompt (no chunked prefill)")

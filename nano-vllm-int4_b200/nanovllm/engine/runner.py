@@ -110,8 +110,6 @@ class ModelRunner:
     def _allocate_kv_cache(self):
         c, cfg = self.config, self.config.hf_config
         attn0 = self.attn_layers[0]
-        if self.kv_int4 and attn0.head_dim != kv4_cache.HEAD_DIM:
-            raise ValueError(f"the 4-bit KV cache needs head_dim {kv4_cache.HEAD_DIM}")
         page_bytes = kv4_cache.page_bytes(attn0.num_kv_heads) if self.kv_int4 \
             else 2 * PAGE_TOKENS * attn0.num_kv_heads * attn0.head_dim * 2
         page_bytes *= len(self.attn_layers)

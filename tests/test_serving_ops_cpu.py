@@ -233,3 +233,13 @@ def test_step_tables_refuse_outputs_over_inputs_or_one_another():
                 assert tables(ptrs=far | {out: far[other]}) == INVALID
     assert tables(ptrs=far | {3: V(far[0].value - 4 * 4 * 4 + 4)}) == INVALID   # the table's last element
     assert tables(ptrs=far | {7: V(far[2].value + 9 * 4 + 4 - 8)}) == INVALID   # the last page
+
+
+def test_the_4_bit_cache_needs_its_head_dim(tmp_path):
+    """Said before a model is built."""
+    from nanovllm.config import Config
+    from nanovllm.utils import synthetic
+    model = synthetic.write_qwen3_config(str(tmp_path), num_hidden_layers=1, head_dim=64)
+    with pytest.raises(ValueError, match="head_dim 128"):
+        Config(model, kv_cache_dtype="int4")
+    assert Config(model).kv_cache_dtype == "bf16"
