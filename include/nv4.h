@@ -341,8 +341,9 @@ int nv4_qk_norm_rope_store(const void* qkv, const void* q_weight, const void* k_
  *              slot beyond the cache stores nothing and records error 7; no slot may occur twice
  *   q_out      bf16 [tokens, num_heads, 128]
  *   k_out/v_out bf16 [tokens, num_kv_heads, 128] or NULL: the values that the
- *              cache holds for the token (what a later read gives), for the
- *              prefill's own attention
+ *              cache holds for the token, rounded to BF16 (code * scale has up to
+ *              11 significant bits, BF16 eight; nv4_paged_decode_attention_kv4
+ *              reads it unrounded), for the prefill's own attention
  * All pointers 16-byte aligned (positions 8, slot_mapping 4).  head_dim == 128, page_size == 256;
  * up to 2^30 tokens and 2^33 rows (a row: one head of one token).
  */

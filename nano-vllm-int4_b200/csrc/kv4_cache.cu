@@ -59,7 +59,7 @@ struct Kv4StoreArgs {
   const int64_t* positions;
   const int* slot_mapping;
   uint16_t* q_out;
-  uint16_t* k_out;  // values held by the cache, or nullptr
+  uint16_t* k_out;  // values held by the cache, rounded to BF16, or nullptr
   uint16_t* v_out;
   uint8_t* k_codes;
   uint16_t* k_scales;

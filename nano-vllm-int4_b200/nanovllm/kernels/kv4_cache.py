@@ -60,7 +60,8 @@ def qk_norm_rope_store_kv4(qkv, q_weight, k_weight, cos_sin, positions, slot_map
     (cos, then sin), ``positions`` INT64 [T], ``slot_mapping`` INT32 [T].  Returns
     q [T, num_heads, 128] in BF16, with ``return_values`` (q, k, v) where k and v
     [T, num_kv_heads, 128] are the values that the cache holds for the tokens,
-    in BF16: attention over them gives what a later read of the cache gives.
+    rounded to BF16 (each by up to 2^-8 of itself; the decode attention reads them
+    unrounded).
     ``slot_mapping`` and ``cache`` may both be None: nothing is stored then.
     """
     return _native.serving().store(qkv, q_weight, k_weight, cos_sin, positions, slot_mapping, *(cache or _NO_CACHE),

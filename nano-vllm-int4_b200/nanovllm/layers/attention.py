@@ -14,8 +14,9 @@ Triton store kernel) and the q/k norm + rotary steps of
 
 With a 4-bit cache (``kv_int4``) the store and the decode attention are those of
 ``nanovllm/kernels/kv4_cache.py``.  A prompt then attends to the values that the
-cache holds for it, so that its tokens' states do not depend on whether they came
-from a prefill or from decode steps (a preempted request is prefilled again).
+cache holds for it, rounded to BF16, so that its tokens' states agree up to that
+rounding whether they came from a prefill or from decode steps (a preempted
+request is prefilled again).
 
 The step's metadata lives in a module-level ``StepContext`` that the model
 runner sets before each forward (and that CUDA-graph capture binds to static

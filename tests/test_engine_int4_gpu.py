@@ -211,3 +211,24 @@ def test_tokens_up_to_the_end_of_the_last_page(cuda_device, model_dir, cache):
     short, _ = generate(model_dir, kv_cache_dtype=cache, max_model_len=1000, texts=texts)
     whole, _ = generate(model_dir, kv_cache_dtype=cache, max_model_len=1024, texts=texts)
     assert [o["token_ids"] for o in short] == [o["token_ids"] for o in whole]
+
+
+def test_preemption_happens_and_keeps_what_was_generated(cuda_device, model_dir, monkeypatch):
+    from nanovllm.engine.scheduler import Scheduler
+    preempted, inner = [], Scheduler._preempt
+
+    def preempt(self, seq):
+        preempted.append(seq.num_completion_tokens)
+        inner(self, seq)
+    monkeypatch.setattr(Scheduler, "_preempt", preempt)
+    texts, params = prompts((250, 250, 250, 250)), dict(logprobs=1)
+    plain, _ = generate(model_dir, kv_cache_dtype="int4", texts=texts, params=params)
+    assert not preempted
+    out, _ = generate(model_dir, kv_cache_dtype="int4", num_kvcache_blocks=5, texts=texts, params=params)
+    # the 257th token needs a second page for each of the four, and one page is free: the last is preempted for the
+    # second's, the third for want of one
+    assert preempted == [7, 7]
+    for o, p in zip(out, plain):
+        assert len(o["logprobs"]) == len(o["token_ids"]) == 24
+        assert [d["token_id"] for d in o["logprobs"]] == o["token_ids"]
+        assert o["token_ids"][:7] == p["token_ids"][:7] and o["logprobs"][:7] == p["logprobs"][:7]

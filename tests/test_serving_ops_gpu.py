@@ -194,3 +194,16 @@ def test_step_tables_in_place_are_refused(cuda_device):
             call(**args, out=out)
     want = call(**args)
     assert all(torch.equal(a, b) for a, b in zip(call(**args, out=good), want))
+
+
+def test_returned_values_are_the_caches_rounded_to_bf16(cuda_device):
+    """The decode attention reads code * scale unrounded, up to 11 significant bits."""
+    import kv4_reference as ref
+    cache, table = calls(cuda_device)
+    call, args = table[0]
+    _, k, v = call(**args, return_values=True)
+    for got, held in ((k, ref.read_k(cache)), (v, ref.read_v(cache))):
+        held = held[0, :, :3].transpose(0, 1)
+        got = got.cpu()
+        assert torch.equal(got, held.bfloat16()) and not torch.equal(got.double(), held)
+        assert ((got.double() - held).abs() <= 2.0 ** -8 * held.abs()).all()
