@@ -27,6 +27,7 @@ def token_logprobs(logits, targets, *, top_k: int = 0) -> TokenLogprobs:
     A target outside [0, V) is no token: logprob 0, rank 0.  Logits of -inf are
     no alternatives: where fewer than ``top_k`` (at most 32) are left, id -1 and
     -inf.  A row of nothing but -inf gives logprob -inf and entropy 0; a row that
-    holds a NaN or +inf gives NaN.  With no rows the outputs are empty.
+    holds a NaN or +inf gives NaN.  With no rows the outputs are empty.  They
+    carry no gradient, also for logits that require one.
     """
     return TokenLogprobs._make(_native.serving().logprobs(logits, targets, top_k))

@@ -207,3 +207,10 @@ def test_returned_values_are_the_caches_rounded_to_bf16(cuda_device):
         got = got.cpu()
         assert torch.equal(got, held.bfloat16()) and not torch.equal(got.double(), held)
         assert ((got.double() - held).abs() <= 2.0 ** -8 * held.abs()).all()
+
+
+def test_logprobs_of_logits_that_require_a_gradient(cuda_device):
+    _, table = calls(cuda_device)
+    call, args = table[3]
+    got = call(**(args | dict(logits=args["logits"].clone().requires_grad_())))
+    assert all(torch.equal(a, b) and not a.requires_grad for a, b in zip(got, call(**args)))
