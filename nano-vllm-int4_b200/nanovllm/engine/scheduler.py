@@ -15,6 +15,7 @@ from __future__ import annotations
 from collections import deque
 
 from nanovllm.engine.sequence import Sequence, Status
+from nanovllm.kernels.step_tables import MAX_REQUESTS
 
 
 class PagePool:
@@ -35,7 +36,7 @@ class PagePool:
 
 class Scheduler:
     def __init__(self, max_num_seqs: int, max_num_batched_tokens: int, num_pages: int, eos: int):
-        self.max_num_seqs = max_num_seqs
+        self.max_num_seqs = min(max_num_seqs, MAX_REQUESTS)  # of a step: its tables hold no more
         self.max_num_batched_tokens = max_num_batched_tokens
         self.eos = eos
         self.pool = PagePool(num_pages)

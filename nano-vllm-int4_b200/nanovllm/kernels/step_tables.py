@@ -10,6 +10,8 @@ import torch
 
 from nanovllm import _native
 
+MAX_REQUESTS = 28672  # of a batch
+
 
 class StepTables(NamedTuple):
     block_tables: torch.Tensor   # INT32 [rows, max_pages]: the request's pages, then 0

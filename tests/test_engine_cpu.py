@@ -209,3 +209,18 @@ def test_prompts_longer_than_the_tables_are_refused_at_the_door():
     with pytest.raises(ValueError, match="max_model_len"):
         engine.add_request(list(range(2 * PAGE_TOKENS + 1)), greedy)
     assert list(engine.scheduler.waiting) == [kept]
+
+
+def test_a_step_takes_no_more_requests_than_its_tables():
+    """The step tables hold 28672 requests; more wait for the next step."""
+    sch = Scheduler(max_num_seqs=40000, max_num_batched_tokens=40000, num_pages=30000, eos=-1)
+    for _ in range(30000):
+        sch.add(Sequence([1], SamplingParams(temperature=0.0, max_tokens=2, ignore_eos=True)))
+    first, prefill = sch.schedule()
+    assert prefill and len(first) == 28672
+    sch.postprocess(first, [0] * len(first))
+    rest, prefill = sch.schedule()
+    assert prefill and len(rest) == 30000 - 28672
+    sch.postprocess(rest, [0] * len(rest))
+    batch, prefill = sch.schedule()
+    assert not prefill and len(batch) == 28672
