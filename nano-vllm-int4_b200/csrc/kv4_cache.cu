@@ -47,9 +47,10 @@ constexpr int kKv4MaxGroup = 8;     // query heads per KV head
 // care: FP32, rounded once to BF16.
 //
 // Measured (32 / 8 heads, with the values): 16384 tokens 103 us = 4.1 TB/s (0.63 of
-// the measured copy rate), 301 tokens of 40 / 8 heads 4.5 us, 32 tokens 3.1 us.
-// Next bound: issue (the K and V rows' arithmetic) and the latency of cos, sin and
-// the weights.  Tried and not better: a ring of four rows in shared memory, cos
+// the measured copy rate), 301 tokens of 40 / 8 heads 4.8 us, 32 tokens 3.5 us.
+// Next: the latency of cos, sin and the weights, which every row loads again, and the
+// two-term arithmetic, which every K value takes though only those next to a border
+// need it; no pipe is full (0.60 instructions a cycle and scheduler).  Tried and not better: a ring of four rows in shared memory, cos
 // and sin before the row, 64-thread CTAs, five, seven or eight CTAs an SM.
 struct Kv4StoreArgs {
   const uint16_t* qkv;
@@ -357,14 +358,16 @@ int launch_qk_norm_rope_store_kv4(const void* qkv, const void* q_weight, const v
 //
 // Measured (32 / 8 heads, with the merge): 32 x 4.2k tokens 56 us = 2.8 TB/s, 64
 // ragged up to 16k 114 us = 3.1 TB/s (0.48 of the measured copy rate), one of 700
-// tokens 7.9 us.  Before the second term of the probabilities (101 us for the
-// ragged case): bound by issue, about 303 instructions per 16 tokens, half of them
-// ALU work of the widening at one in two cycles; without the products the same
-// copies take 65 of the 101 us, without the copies the products 99.  Tried then and
-// slower (64 ragged): units of 64 tokens, five CTAs an SM at 96 registers (110 us),
-// a warp of its own for the copies (105), two tiles of a warp at once, eight-warp
-// CTAs; K as 8-bit integers against q in 16-bit fixed point lost precision at large
-// scores.
+// tokens 7.9 us.  Bound by the latency of a warp's own chain (load, widen, two MMAs
+// a group, FMAs, vote, exponential, pack, movmatrix, MMA) with four warps a
+// scheduler: 0.57 instructions a cycle and scheduler, the ALU at half of its rate, the
+// tensor pipe at 25%, HBM at 0.43, none of them full.  With one term of the
+// probabilities (101 us for the ragged case) the copies took 65 us without the
+// products and the products 99 without the copies; 64 mask-and-or instructions fewer
+// of about 303 per 16 tokens gave 15%.  Tried then and slower (64 ragged): units of 64
+// tokens, five CTAs an SM at 96 registers (110 us), a warp of its own for the copies
+// (105), two tiles of a warp at once, eight-warp CTAs; K as 8-bit integers against q
+// in 16-bit fixed point lost precision at large scores.
 constexpr int kKv4Warps = 4;
 constexpr int kKv4Threads = kKv4Warps * 32;
 constexpr int kKv4Tiles = 2;                          // 16-token tiles a warp takes of a unit

@@ -7,8 +7,8 @@
 // the first page of a request and its first token are two prefix sums over the
 // batch, and each output element follows from them by itself.  One launch:
 // every CTA makes both sums in shared memory (eight bytes a request, which limits
-// the batch) and takes its share of the outputs.  3.4 us for 32 or 40
-// requests, 4.5 us for 512.  Bound by latency: two loads in a row, the scan, a
+// the batch) and takes its share of the outputs.  3.5 us for 32 or 40
+// requests, 4.6 us for 512.  Bound by latency: two loads in a row, the scan, a
 // binary search.
 #include "nv4_device.cuh"
 #include "nv4_launch.h"

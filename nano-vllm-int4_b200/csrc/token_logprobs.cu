@@ -28,7 +28,7 @@
 //
 // Measured: 1024 BF16 rows of 151936 56 us = 5.6 TB/s (0.86 of the measured copy
 // rate; 65 us with 5 alternatives, 72 us with 20), 48 FP32 rows of 100003 with 20
-// alternatives 15 us, one row with 5 alternatives 10 us (two launches' latency).
+// alternatives 15 us, one row with 5 alternatives 11 us (two launches' latency).
 #include <cfloat>
 
 #include "nv4_device.cuh"
@@ -590,7 +590,8 @@ __global__ void __launch_bounds__(kLpThreads) token_logprobs_join_kernel(const L
 }
 
 // CTAs of a row: one where the rows alone fill the SMs, else so many that all do,
-// with a chunk for every warp at least.
+// with a chunk for every warp at least.  148 are a B200's SMs: the workspace's size
+// follows from it, which a caller asks for without a current device.
 static int64_t logprob_splits(int64_t rows, int64_t vocab) {
   const int64_t chunks = (vocab + kLpChunk - 1) / kLpChunk;
   const int64_t wanted = std::min<int64_t>(kLpCtasPerSm * 148 / rows, std::min<int64_t>(chunks / kLpWarps, kLpMaxSplits));
