@@ -50,8 +50,9 @@ constexpr int kKv4MaxGroup = 8;     // query heads per KV head
 // the measured copy rate), 301 tokens of 40 / 8 heads 4.8 us, 32 tokens 3.5 us.
 // Next: the latency of cos, sin and the weights, which every row loads again, and the
 // two-term arithmetic, which every K value takes though only those next to a border
-// need it; no pipe is full (0.60 instructions a cycle and scheduler).  Tried and not better: a ring of four rows in shared memory, cos
-// and sin before the row, 64-thread CTAs, five, seven or eight CTAs an SM.
+// need it; no pipe is full (0.60 instructions a cycle and scheduler).  Tried and not
+// better: a ring of four rows in shared memory, cos and sin before the row, 64-thread
+// CTAs, five, seven or eight CTAs an SM.
 struct Kv4StoreArgs {
   const uint16_t* qkv;
   const uint16_t* q_weight;
