@@ -379,6 +379,87 @@ int nv4_paged_decode_attention_kv4(const void* q, const void* k_codes, const voi
                                    int64_t num_pages, int64_t max_pages, float scale, void* stream);
 
 /*
+ * Requests that share cached tokens, over the paged BF16 cache of
+ * nv4_paged_decode_attention (head_dim 128, page_size 256; the reference calls
+ * flash-attn over its block tables, nanovllm/layers/attention.py:59-75, which
+ * reads a shared prefix once per request).
+ *
+ * Append: keys and values written to the cache rows slot_mapping[t], the rotation
+ * (and, with weights, the RMSNorm) applied on the way; q likewise to q_out.  As
+ * nv4_qk_norm_rope_store, with q, k and v of their own, an optional norm, partial
+ * rotation, and one rounding instead of three.
+ *   q, k, v    bf16 [tokens, heads, 128], a token's heads contiguous, tokens
+ *              *_stride elements apart (a multiple of 8); q NULL with q_out NULL
+ *   q_weight, k_weight  bf16 [128] or NULL (no norm of that side)
+ *   cos_sin    float32 [max_position, rotary_dim]: cos in the first half, sin in
+ *              the second; channels c and c + rotary_dim / 2 of the first
+ *              rotary_dim (a multiple of 16 up to 128) are rotated
+ *   positions  int64 [tokens]; one outside [0, max_position) makes q and k NaN and
+ *              records error 8 (nv4_device_error)
+ *   slot_mapping int32 [tokens]: cache row (page * 256 + offset), none twice; < 0
+ *              stores nothing, one beyond the cache too and records error 7
+ *   q_out      bf16 [tokens, num_heads, 128]; may be q itself (contiguous), no
+ *              other output may overlap an input or another output
+ */
+int nv4_append_kv(const void* q, const void* k, const void* v, const void* q_weight, const void* k_weight,
+                  const void* cos_sin, const int64_t* positions, const int32_t* slot_mapping, void* q_out,
+                  void* k_cache, void* v_cache, int64_t tokens, int64_t num_heads, int64_t num_kv_heads,
+                  int64_t head_dim, int64_t q_stride, int64_t k_stride, int64_t v_stride, int64_t rotary_dim,
+                  int64_t page_size, int64_t num_pages, int64_t max_position, float eps, void* stream);
+
+/*
+ * Attention of the new tokens of several requests, each over what its request has
+ * in the cache, the new tokens included (causal).
+ *   q, out        bf16 [tokens, num_heads, 128]
+ *   block_tables  int32 [batch, max_pages]; a page outside [0, num_pages) counts as
+ *                 absent and records error 6
+ *   context_lens  int32 [batch]: tokens of each request, the new ones included
+ *   query_starts  int32 [batch + 1], not falling: request b's new tokens are rows
+ *                 query_starts[b] .. query_starts[b + 1] - 1 (none is allowed); row
+ *                 i of its n sees the first context_lens[b] - n + i + 1 tokens, at
+ *                 most max_pages * 256; a row that sees none gets 0
+ *   workspace     nv4_paged_prefill_attention_workspace_bytes(...) bytes of
+ *                 scratch; calls that may overlap need one each
+ * Rows of no request are left as they are.  out and workspace overlap no input nor
+ * one another.  Values of the request's own later
+ * tokens (masked, but in the cache) must be finite; what lies behind its last
+ * token may be anything.  At most NV4_PAGED_MAX_GROUP query heads per KV head.
+ * Statistics and sums in FP32, the probabilities multiplied in two BF16 terms.
+ * All pointers 16-byte aligned (the int32 ones 4).
+ */
+#define NV4_PAGED_MAX_GROUP 16
+#define NV4_PAGED_MAX_TOKENS (1 << 22)
+int64_t nv4_paged_prefill_attention_workspace_bytes(int64_t tokens, int64_t batch, int64_t num_heads,
+                                                    int64_t num_kv_heads);
+int nv4_paged_prefill_attention(const void* q, const void* k_cache, const void* v_cache, const int32_t* block_tables,
+                                const int32_t* context_lens, const int32_t* query_starts, void* out, void* workspace,
+                                int64_t workspace_bytes, int64_t tokens, int64_t batch, int64_t num_heads,
+                                int64_t num_kv_heads, int64_t head_dim, int64_t page_size, int64_t num_pages,
+                                int64_t max_pages, float scale, void* stream);
+
+/*
+ * Decode attention (one query token per request) of a batch in which groups of
+ * consecutive requests share the pages of a prefix, whose tokens are read once
+ * for the group.  The result is that of each request over its whole context.
+ *   group_starts  int32 [groups + 1], not falling: requests group_starts[g] ..
+ *                 group_starts[g + 1] - 1 are a group; requests of none share nothing
+ *   prefix_lens   int32 [groups]: tokens that the group has in common.  The whole
+ *                 pages of it are read through the first request's block table
+ *                 (the others' must name the same pages), the rest, as all other
+ *                 tokens, through each request's own
+ *   context_lens  int32 [batch]; 0 (or less) marks a padding row, whose output is zero
+ * Everything else as nv4_paged_prefill_attention; groups may be 0 (then
+ * group_starts and prefix_lens may be NULL).
+ */
+int64_t nv4_shared_prefix_attention_workspace_bytes(int64_t batch, int64_t groups, int64_t num_heads,
+                                                    int64_t num_kv_heads);
+int nv4_shared_prefix_attention(const void* q, const void* k_cache, const void* v_cache, const int32_t* block_tables,
+                                const int32_t* context_lens, const int32_t* group_starts, const int32_t* prefix_lens,
+                                void* out, void* workspace, int64_t workspace_bytes, int64_t batch, int64_t groups,
+                                int64_t num_heads, int64_t num_kv_heads, int64_t head_dim, int64_t page_size,
+                                int64_t num_pages, int64_t max_pages, float scale, void* stream);
+
+/*
  * Step metadata of a batch from request lengths (the reference builds these
  * lists on the host: nanovllm/engine/model_runner.py prepare_prefill /
  * prepare_decode).  Request b has cached_lens[b] tokens in the cache and

@@ -507,6 +507,146 @@ int nv4_qk_norm_rope_store_kv4(const void* qkv, const void* q_weight, const void
                                        num_pages, max_position, eps, static_cast<cudaStream_t>(stream));
 }
 
+// ---- requests that share cached tokens
+namespace {
+struct Span {
+  const void* at;
+  int64_t bytes;
+};
+bool overlap(const Span& a, const Span& b) {
+  const char *x = static_cast<const char*>(a.at), *y = static_cast<const char*>(b.at);
+  return a.bytes > 0 && b.bytes > 0 && x < y + b.bytes && y < x + a.bytes;
+}
+}  // namespace
+
+int nv4_append_kv(const void* q, const void* k, const void* v, const void* q_weight, const void* k_weight,
+                  const void* cos_sin, const int64_t* positions, const int32_t* slot_mapping, void* q_out,
+                  void* k_cache, void* v_cache, int64_t tokens, int64_t num_heads, int64_t num_kv_heads,
+                  int64_t head_dim, int64_t q_stride, int64_t k_stride, int64_t v_stride, int64_t rotary_dim,
+                  int64_t page_size, int64_t num_pages, int64_t max_position, float eps, void* stream) {
+  if (!k || !v || !cos_sin || !positions || !slot_mapping || !k_cache || !v_cache || (q != nullptr) != (q_out != nullptr))
+    return NV4_ERR_INVALID_ARGUMENT;
+  if (tokens < 1 || tokens > (int64_t(1) << 30) || num_heads < 1 || num_heads > 65535 || num_kv_heads < 1 ||
+      num_kv_heads > 65535 || num_pages < 1 || num_pages > (int64_t(1) << 23) - 1 || max_position < 1 ||
+      !(eps >= 0.0f) || !(eps < 1.0f))
+    return NV4_ERR_INVALID_ARGUMENT;
+  if (head_dim != 128 || page_size != 256 || rotary_dim < 16 || rotary_dim > 128 || rotary_dim % 16)
+    return NV4_ERR_UNSUPPORTED;
+  const int64_t most = int64_t(1) << 32;
+  if (k_stride < num_kv_heads * 128 || v_stride < num_kv_heads * 128 || (q && q_stride < num_heads * 128) ||
+      k_stride > most || v_stride > most || (q && q_stride > most))
+    return NV4_ERR_INVALID_ARGUMENT;
+  if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(q_weight, 16) || !aligned(k_weight, 16) ||
+      !aligned(cos_sin, 16) || !aligned(positions, 8) || !aligned(slot_mapping, 4) || !aligned(q_out, 16) ||
+      !aligned(k_cache, 16) || !aligned(v_cache, 16) || k_stride % 8 || v_stride % 8 || (q && q_stride % 8))
+    return NV4_ERR_ALIGNMENT;
+  // Rows are written while others are read: no output over an input or another output (q_out may be q itself).
+  const int64_t cache = num_pages * 256 * num_kv_heads * 256, q_row = num_heads * 256;
+  const Span outs[3] = {{q_out, q ? tokens * q_row : 0}, {k_cache, cache}, {v_cache, cache}};
+  const Span ins[8] = {{q, q && (q != q_out || q_stride != num_heads * 128) ? (tokens - 1) * q_stride * 2 + q_row : 0},
+                       {k, (tokens - 1) * k_stride * 2 + num_kv_heads * 256},
+                       {v, (tokens - 1) * v_stride * 2 + num_kv_heads * 256},
+                       {cos_sin, max_position * rotary_dim * 4},
+                       {positions, tokens * 8},
+                       {slot_mapping, tokens * 4},
+                       {q_weight, q_weight ? 256 : 0},
+                       {k_weight, k_weight ? 256 : 0}};
+  for (int i = 0; i < 3; ++i) {
+    for (const Span& in : ins)
+      if (overlap(outs[i], in)) return NV4_ERR_INVALID_ARGUMENT;
+    for (int j = i + 1; j < 3; ++j)
+      if (overlap(outs[i], outs[j])) return NV4_ERR_INVALID_ARGUMENT;
+  }
+  if (!device_is_sm100()) return NV4_ERR_DEVICE;
+  return launch_append_kv(q, k, v, q_weight, k_weight, static_cast<const float*>(cos_sin), positions, slot_mapping,
+                          q_out, k_cache, v_cache, tokens, num_heads, num_kv_heads, q_stride, k_stride, v_stride,
+                          rotary_dim, num_pages, max_position, eps, static_cast<cudaStream_t>(stream));
+}
+
+namespace {
+// The checks that the two attentions over shared cached tokens have in common.
+int check_paged_attention(const void* q, const void* k_cache, const void* v_cache, const void* block_tables,
+                          const void* context_lens, const void* out, const void* workspace, int64_t workspace_bytes,
+                          int64_t wanted, int64_t rows, int64_t batch, int64_t num_heads, int64_t num_kv_heads,
+                          int64_t head_dim, int64_t page_size, int64_t num_pages, int64_t max_pages, float scale) {
+  if (!q || !k_cache || !v_cache || !block_tables || !context_lens || !out || !workspace)
+    return NV4_ERR_INVALID_ARGUMENT;
+  if (rows < 1 || rows > NV4_PAGED_MAX_TOKENS || batch < 1 || batch > 65535 || num_kv_heads < 1 ||
+      num_kv_heads > 1024 || num_heads < num_kv_heads || num_heads > 65535 || num_heads % num_kv_heads ||
+      num_pages < 1 || num_pages > (int64_t(1) << 23) - 1 || max_pages < 1 || max_pages > 65535 || !(scale > 0.0f) ||
+      !(scale < 1e30f))
+    return NV4_ERR_INVALID_ARGUMENT;
+  if (head_dim != 128 || page_size != 256 || num_heads / num_kv_heads > NV4_PAGED_MAX_GROUP)
+    return NV4_ERR_UNSUPPORTED;
+  if (workspace_bytes < wanted) return NV4_ERR_INVALID_ARGUMENT;
+  if (!aligned(q, 16) || !aligned(k_cache, 16) || !aligned(v_cache, 16) || !aligned(out, 16) ||
+      !aligned(workspace, 16) || !aligned(block_tables, 4) || !aligned(context_lens, 4))
+    return NV4_ERR_ALIGNMENT;
+  // q and the cache are read again after other rows were written
+  const int64_t cache = num_pages * 256 * num_kv_heads * 256, row_bytes = rows * num_heads * 256;
+  const Span spans[7] = {{out, row_bytes}, {workspace, wanted}, {q, row_bytes}, {k_cache, cache}, {v_cache, cache},
+                         {block_tables, batch * max_pages * 4}, {context_lens, batch * 4}};
+  for (int i = 0; i < 2; ++i)
+    for (int j = i + 1; j < 7; ++j)
+      if (overlap(spans[i], spans[j])) return NV4_ERR_INVALID_ARGUMENT;
+  return NV4_OK;
+}
+}  // namespace
+
+int64_t nv4_paged_prefill_attention_workspace_bytes(int64_t tokens, int64_t batch, int64_t num_heads,
+                                                    int64_t num_kv_heads) {
+  if (tokens < 1 || tokens > NV4_PAGED_MAX_TOKENS || batch < 1 || batch > 65535 || num_kv_heads < 1 ||
+      num_kv_heads > 1024 || num_heads < num_kv_heads || num_heads > 65535 || num_heads % num_kv_heads ||
+      num_heads / num_kv_heads > NV4_PAGED_MAX_GROUP)
+    return 0;
+  return paged_prefill_attention_workspace_bytes(tokens, batch, num_heads, num_kv_heads);
+}
+
+int nv4_paged_prefill_attention(const void* q, const void* k_cache, const void* v_cache, const int32_t* block_tables,
+                                const int32_t* context_lens, const int32_t* query_starts, void* out, void* workspace,
+                                int64_t workspace_bytes, int64_t tokens, int64_t batch, int64_t num_heads,
+                                int64_t num_kv_heads, int64_t head_dim, int64_t page_size, int64_t num_pages,
+                                int64_t max_pages, float scale, void* stream) {
+  if (!query_starts) return NV4_ERR_INVALID_ARGUMENT;
+  const int rc = check_paged_attention(
+      q, k_cache, v_cache, block_tables, context_lens, out, workspace, workspace_bytes,
+      nv4_paged_prefill_attention_workspace_bytes(tokens, batch, num_heads, num_kv_heads), tokens, batch, num_heads,
+      num_kv_heads, head_dim, page_size, num_pages, max_pages, scale);
+  if (rc != NV4_OK) return rc;
+  if (!aligned(query_starts, 4)) return NV4_ERR_ALIGNMENT;
+  if (!device_is_sm100()) return NV4_ERR_DEVICE;
+  return launch_paged_prefill_attention(q, k_cache, v_cache, block_tables, context_lens, query_starts, out, workspace,
+                                        tokens, batch, num_heads, num_kv_heads, num_pages, max_pages, scale,
+                                        static_cast<cudaStream_t>(stream));
+}
+
+int64_t nv4_shared_prefix_attention_workspace_bytes(int64_t batch, int64_t groups, int64_t num_heads,
+                                                    int64_t num_kv_heads) {
+  if (batch < 1 || batch > 65535 || groups < 0 || groups > 65535 || num_kv_heads < 1 || num_kv_heads > 1024 ||
+      num_heads < num_kv_heads || num_heads > 65535 || num_heads % num_kv_heads ||
+      num_heads / num_kv_heads > NV4_PAGED_MAX_GROUP)
+    return 0;
+  return shared_prefix_attention_workspace_bytes(batch, groups, num_heads, num_kv_heads);
+}
+
+int nv4_shared_prefix_attention(const void* q, const void* k_cache, const void* v_cache, const int32_t* block_tables,
+                                const int32_t* context_lens, const int32_t* group_starts, const int32_t* prefix_lens,
+                                void* out, void* workspace, int64_t workspace_bytes, int64_t batch, int64_t groups,
+                                int64_t num_heads, int64_t num_kv_heads, int64_t head_dim, int64_t page_size,
+                                int64_t num_pages, int64_t max_pages, float scale, void* stream) {
+  if (groups < 0 || groups > 65535 || (groups > 0 && (!group_starts || !prefix_lens))) return NV4_ERR_INVALID_ARGUMENT;
+  const int rc = check_paged_attention(
+      q, k_cache, v_cache, block_tables, context_lens, out, workspace, workspace_bytes,
+      nv4_shared_prefix_attention_workspace_bytes(batch, groups, num_heads, num_kv_heads), batch, batch, num_heads,
+      num_kv_heads, head_dim, page_size, num_pages, max_pages, scale);
+  if (rc != NV4_OK) return rc;
+  if (!aligned(group_starts, 4) || !aligned(prefix_lens, 4)) return NV4_ERR_ALIGNMENT;
+  if (!device_is_sm100()) return NV4_ERR_DEVICE;
+  return launch_shared_prefix_attention(q, k_cache, v_cache, block_tables, context_lens, group_starts, prefix_lens,
+                                        out, workspace, batch, groups, num_heads, num_kv_heads, num_pages, max_pages,
+                                        scale, static_cast<cudaStream_t>(stream));
+}
+
 int nv4_step_tables(const int32_t* cached_lens, const int32_t* new_lens, const int32_t* pages,
                     int32_t* block_tables, int32_t* context_lens, int32_t* query_starts, int32_t* slot_mapping,
                     int64_t* positions, int64_t batch, int64_t rows, int64_t num_listed, int64_t tokens,

@@ -108,6 +108,25 @@ int launch_qk_norm_rope_store_kv4(const void* qkv, const void* q_weight, const v
                                   void* v_out, void* k_codes, void* k_scales, void* v_codes, void* v_scales,
                                   int64_t tokens, int64_t num_heads, int64_t num_kv_heads, int64_t num_pages,
                                   int64_t max_position, double eps, cudaStream_t stream);
+// Requests that share cached tokens, over the paged BF16 cache (paged_attention.cu).
+int launch_append_kv(const void* q, const void* k, const void* v, const void* q_weight, const void* k_weight,
+                     const float* cos_sin, const int64_t* positions, const int* slot_mapping, void* q_out,
+                     void* k_cache, void* v_cache, int64_t tokens, int64_t num_heads, int64_t num_kv_heads,
+                     int64_t q_stride, int64_t k_stride, int64_t v_stride, int64_t rotary_dim, int64_t num_pages,
+                     int64_t max_position, float eps, cudaStream_t stream);
+int64_t paged_prefill_attention_workspace_bytes(int64_t tokens, int64_t batch, int64_t num_heads,
+                                                int64_t num_kv_heads);
+int launch_paged_prefill_attention(const void* q, const void* k_cache, const void* v_cache, const int* block_tables,
+                                   const int* context_lens, const int* query_starts, void* out, void* workspace,
+                                   int64_t tokens, int64_t batch, int64_t num_heads, int64_t num_kv_heads,
+                                   int64_t num_pages, int64_t max_pages, float scale, cudaStream_t stream);
+int64_t shared_prefix_attention_workspace_bytes(int64_t batch, int64_t groups, int64_t num_heads,
+                                                int64_t num_kv_heads);
+int launch_shared_prefix_attention(const void* q, const void* k_cache, const void* v_cache, const int* block_tables,
+                                   const int* context_lens, const int* group_starts, const int* prefix_lens, void* out,
+                                   void* workspace, int64_t batch, int64_t groups, int64_t num_heads,
+                                   int64_t num_kv_heads, int64_t num_pages, int64_t max_pages, float scale,
+                                   cudaStream_t stream);
 // Step metadata from request lengths (step_tables.cu).
 int launch_step_tables(const int* cached, const int* fresh, const int* pages, int* block_tables, int* context_lens,
                        int* query_starts, int* slot_mapping, int64_t* positions, int64_t batch, int64_t rows,

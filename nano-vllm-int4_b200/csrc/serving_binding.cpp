@@ -1,6 +1,6 @@
-// Python binding of the 4-bit cache, step table and log-probability entry points
-// (nanovllm/kernels/{kv4_cache,step_tables,token_logprobs}.py), whose kernels
-// take 3 to 15 us: the checks of the arguments, the outputs' allocation and the
+// Python binding of the 4-bit cache, step table, log-probability and shared-token
+// entry points (nanovllm/kernels/{kv4_cache,step_tables,token_logprobs,
+// paged_attention}.py), whose kernels take 3 to 15 us when short: the checks of the arguments, the outputs' allocation and the
 // call itself.  The same through Python and ctypes took 17 to 22 us of host time
 // a call, most of it in new tensors (2.5 us each there, 0.9 us here) and checks;
 // here it is 4 to 8 us in a loop of one call (x.add_(1) takes 4.4), 6 to 12 among others.
@@ -321,6 +321,156 @@ PyObject* py_logprobs(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// Rows of a [T, heads, 128] operand whose tokens may be any distance apart: that distance.
+int64_t token_stride(const at::Tensor& x) {
+  const int64_t heads = x.size(1), t = x.size(0);
+  if (x.stride(2) != 1 || (heads > 1 && x.stride(1) != kD) || (t > 1 && x.stride(0) < heads * kD))
+    refuse("The heads of a token must be contiguous, and tokens must not overlap");
+  return t > 1 ? x.stride(0) : heads * kD;
+}
+
+// KV heads of a well-formed BF16 cache.
+int64_t check_bf16_cache(const at::Tensor& k, const at::Tensor& v) {
+  if (k.dim() != 4 || k.size(0) < 1 || k.size(1) != kPage || k.size(2) < 1 || k.size(3) != kD ||
+      v.sizes() != k.sizes() || k.scalar_type() != at::kBFloat16 || v.scalar_type() != at::kBFloat16)
+    refuse("Expected BF16 k_cache and v_cache[pages,256,Hkv,128]");
+  return k.size(2);
+}
+
+// append_kv(q, k, v, cos_sin, positions, slot_mapping, k_cache, v_cache, q_weight, k_weight, eps, q_out) -> q_out,
+// or None without q
+PyObject* py_append_kv(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    expect_args(n, 12);
+    const at::Tensor* q = optional(a[0], "q");
+    const at::Tensor &k = tensor(a[1], "k"), &v = tensor(a[2], "v"), &cos_sin = tensor(a[3], "cos_sin");
+    const at::Tensor &positions = tensor(a[4], "positions"), &slots = tensor(a[5], "slot_mapping");
+    const at::Tensor &kc = tensor(a[6], "k_cache"), &vc = tensor(a[7], "v_cache");
+    const at::Tensor *qw = optional(a[8], "q_weight"), *kw = optional(a[9], "k_weight");
+    const double eps = real(a[10]);
+    const at::Tensor* q_in = optional(a[11], "q_out");
+    const int64_t hkv = check_bf16_cache(kc, vc);
+    if (k.dim() != 3 || k.size(1) != hkv || k.size(2) != kD || v.sizes() != k.sizes() ||
+        k.scalar_type() != at::kBFloat16 || v.scalar_type() != at::kBFloat16)
+      refuse("Expected BF16 k and v[T,Hkv,128] with the cache's KV heads");
+    const int64_t t = k.size(0);
+    if (q && (q->dim() != 3 || q->size(0) != t || q->size(1) < 1 || q->size(2) != kD || q->scalar_type() != at::kBFloat16))
+      refuse("Expected BF16 q[T,Hq,128]");
+    const int64_t hq = q ? q->size(1) : 1;
+    for (const at::Tensor* w : {qw, kw})
+      if (w && !shaped(*w, at::kBFloat16, {kD})) refuse("Expected BF16 q_weight[128] and k_weight[128]");
+    if (cos_sin.dim() != 2 || cos_sin.size(0) < 1 || cos_sin.size(1) < 16 || cos_sin.size(1) > kD ||
+        cos_sin.size(1) % 16 || cos_sin.scalar_type() != at::kFloat)
+      refuse("Expected FP32 cos_sin[max_position,rotary_dim], rotary_dim a multiple of 16 up to 128");
+    if (!shaped(positions, at::kLong, {t})) refuse("Expected INT64 positions[T]");
+    if (!shaped(slots, at::kInt, {t})) refuse("Expected INT32 slot_mapping[T]");
+    if (!(eps >= 0) || !(eps < 1)) refuse("eps must be in [0, 1)");
+    if (q_in && !q) refuse("q_out goes with q");
+    if (q_in && !shaped(*q_in, at::kBFloat16, {t, hq, kD})) refuse("Expected BF16 q_out[T,Hq,128]");
+    Device device(positions);
+    for (const at::Tensor* x : {&cos_sin, &slots, &kc, &vc, qw, kw, q_in}) device.add(x);
+    device.check();
+    for (const at::Tensor* x : {q, &k, &v})
+      if (x && (!x->is_cuda() || x->get_device() != device.index())) refuse("All tensors must be on one CUDA device");
+    at::Tensor out;
+    if (q) out = q_in ? *q_in : fresh(*q, {t, hq, kD}, at::kBFloat16);
+    if (t) {
+      const int64_t qs = q ? token_stride(*q) : 0, ks = token_stride(k), vs = token_stride(v);
+      launch(device.index(), "nv4_append_kv", [&](void* stream) {
+        return nv4_append_kv(address(q), k.data_ptr(), v.data_ptr(), address(qw), address(kw), cos_sin.data_ptr(),
+                             static_cast<const int64_t*>(positions.data_ptr()),
+                             static_cast<const int32_t*>(slots.data_ptr()), q ? out.data_ptr() : nullptr,
+                             kc.data_ptr(), vc.data_ptr(), t, hq, hkv, kD, qs, ks, vs, cos_sin.size(1), kPage,
+                             kc.size(0), cos_sin.size(0), static_cast<float>(eps), stream);
+      });
+    }
+    if (!q) Py_RETURN_NONE;
+    return THPVariable_Wrap(out);
+  });
+}
+
+// What the two attentions over shared cached tokens have in common: their checks, output and workspace.
+struct PagedCall {
+  const at::Tensor &q, &kc, &vc, &tables, &lens;
+  int64_t rows, hq, hkv, batch;
+  double scale;
+  at::Tensor out, ws;
+
+  PagedCall(PyObject* const* a, PyObject* scale_o) : q(tensor(a[0], "q")), kc(tensor(a[1], "k_cache")),
+      vc(tensor(a[2], "v_cache")), tables(tensor(a[3], "block_tables")), lens(tensor(a[4], "context_lens")),
+      scale(real(scale_o)) {
+    hkv = check_bf16_cache(kc, vc);
+    if (q.dim() != 3 || q.scalar_type() != at::kBFloat16 || q.size(2) != kD) refuse("Expected BF16 q[T,Hq,128]");
+    rows = q.size(0), hq = q.size(1);
+    if (hq < hkv || hq % hkv || hq / hkv > NV4_PAGED_MAX_GROUP)
+      refuse("Expected query heads to be 1 to 16 times the KV heads");
+    if (tables.dim() != 2 || tables.size(0) < 1 || tables.size(1) < 1 || tables.scalar_type() != at::kInt)
+      refuse("Expected INT32 block_tables[B,max_pages], B>0");
+    batch = tables.size(0);
+    if (!shaped(lens, at::kInt, {batch})) refuse("Expected INT32 context_lens[B]");
+    if (!(scale > 0)) refuse("scale must be positive");
+  }
+
+  int finish(PyObject* out_o, PyObject* ws_o, std::initializer_list<const at::Tensor*> more, int64_t nbytes) {
+    const at::Tensor *out_in = optional(out_o, "out"), *ws_in = optional(ws_o, "workspace");
+    if (out_in && (out_in->scalar_type() != at::kBFloat16 || out_in->sizes() != q.sizes()))
+      refuse("Expected BF16 out[T,Hq,128]");
+    Device device(q);
+    for (const at::Tensor* t : {&kc, &vc, &tables, &lens, out_in, ws_in}) device.add(t);
+    for (const at::Tensor* t : more) device.add(t);
+    device.check();
+    out = out_in ? *out_in : fresh(q, q.sizes(), at::kBFloat16);
+    if (rows) ws = ws_in ? *ws_in : fresh(q, {nbytes}, at::kByte);
+    return device.index();
+  }
+};
+
+// prefill_attention(q, k_cache, v_cache, block_tables, context_lens, query_starts, out, workspace, scale) -> out
+PyObject* py_prefill_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    expect_args(n, 9);
+    PagedCall c(a, a[8]);
+    const at::Tensor& starts = tensor(a[5], "query_starts");
+    if (!shaped(starts, at::kInt, {c.batch + 1})) refuse("Expected INT32 query_starts[B+1]");
+    const int device = c.finish(a[6], a[7], {&starts},
+                                nv4_paged_prefill_attention_workspace_bytes(c.rows, c.batch, c.hq, c.hkv));
+    if (c.rows)
+      launch(device, "nv4_paged_prefill_attention", [&](void* stream) {
+        return nv4_paged_prefill_attention(
+            c.q.data_ptr(), c.kc.data_ptr(), c.vc.data_ptr(), static_cast<const int32_t*>(c.tables.data_ptr()),
+            static_cast<const int32_t*>(c.lens.data_ptr()), static_cast<const int32_t*>(starts.data_ptr()),
+            c.out.data_ptr(), c.ws.data_ptr(), static_cast<int64_t>(c.ws.nbytes()), c.rows, c.batch, c.hq, c.hkv, kD,
+            kPage, c.kc.size(0), c.tables.size(1), static_cast<float>(c.scale), stream);
+      });
+    return THPVariable_Wrap(c.out);
+  });
+}
+
+// shared_attention(q, k_cache, v_cache, block_tables, context_lens, group_starts, prefix_lens, out, workspace, scale)
+// -> out
+PyObject* py_shared_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    expect_args(n, 10);
+    PagedCall c(a, a[9]);
+    const at::Tensor &starts = tensor(a[5], "group_starts"), &prefix = tensor(a[6], "prefix_lens");
+    if (c.rows != c.batch) refuse("Expected one query token per request: q[B,Hq,128]");
+    if (prefix.dim() != 1 || prefix.scalar_type() != at::kInt || !shaped(starts, at::kInt, {prefix.size(0) + 1}))
+      refuse("Expected INT32 group_starts[groups+1] and prefix_lens[groups]");
+    const int64_t groups = prefix.size(0);
+    const int device = c.finish(a[7], a[8], {&starts, &prefix},
+                                nv4_shared_prefix_attention_workspace_bytes(c.batch, groups, c.hq, c.hkv));
+    launch(device, "nv4_shared_prefix_attention", [&](void* stream) {
+      return nv4_shared_prefix_attention(
+          c.q.data_ptr(), c.kc.data_ptr(), c.vc.data_ptr(), static_cast<const int32_t*>(c.tables.data_ptr()),
+          static_cast<const int32_t*>(c.lens.data_ptr()), static_cast<const int32_t*>(starts.data_ptr()),
+          groups ? static_cast<const int32_t*>(prefix.data_ptr()) : nullptr, c.out.data_ptr(), c.ws.data_ptr(),
+          static_cast<int64_t>(c.ws.nbytes()), c.batch, groups, c.hq, c.hkv, kD, kPage, c.kc.size(0),
+          c.tables.size(1), static_cast<float>(c.scale), stream);
+    });
+    return THPVariable_Wrap(c.out);
+  });
+}
+
 template <PyObject* (*F)(PyObject*, PyObject* const*, Py_ssize_t)>
 constexpr PyMethodDef method(const char* name) {
   return {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(F)), METH_FASTCALL, nullptr};
@@ -328,7 +478,9 @@ constexpr PyMethodDef method(const char* name) {
 
 PyMethodDef kMethods[] = {method<py_check_cache>("check_cache"), method<py_attention>("attention"),
                           method<py_store>("store"), method<py_step_tables>("step_tables"),
-                          method<py_logprobs>("logprobs"), {nullptr, nullptr, 0, nullptr}};
+                          method<py_logprobs>("logprobs"), method<py_append_kv>("append_kv"),
+                          method<py_prefill_attention>("prefill_attention"),
+                          method<py_shared_attention>("shared_attention"), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_nv4_serving", nullptr, -1, kMethods};
 
 }  // namespace

@@ -42,7 +42,9 @@ EXPORTS = ("nv4_rht_quant_pack", "nv4_rht_quant_i8", "nv4_w4a4_grouped_gemm", "n
            "nv4_paged_decode_attention", "nv4_qk_norm_rope_store", "nv4_w4a16_plan",
            "nv4_qk_norm_rope_store_kv4", "nv4_paged_attention_kv4_workspace_bytes",
            "nv4_paged_decode_attention_kv4", "nv4_step_tables", "nv4_token_logprobs",
-           "nv4_token_logprobs_workspace_bytes")
+           "nv4_token_logprobs_workspace_bytes", "nv4_append_kv", "nv4_paged_prefill_attention",
+           "nv4_paged_prefill_attention_workspace_bytes", "nv4_shared_prefix_attention",
+           "nv4_shared_prefix_attention_workspace_bytes")
 
 
 class NativeLibraryError(RuntimeError):
@@ -150,6 +152,16 @@ def load(path: str | None = None) -> ctypes.CDLL:
         lib.nv4_token_logprobs_workspace_bytes.restype = _i64
         lib.nv4_token_logprobs.argtypes = [_vp, _int] + [_vp] * 7 + [_i64] * 5 + [_vp]
         lib.nv4_token_logprobs.restype = _int
+        lib.nv4_append_kv.argtypes = [_vp] * 11 + [_i64] * 11 + [ctypes.c_float, _vp]
+        lib.nv4_append_kv.restype = _int
+        lib.nv4_paged_prefill_attention_workspace_bytes.argtypes = [_i64] * 4
+        lib.nv4_paged_prefill_attention_workspace_bytes.restype = _i64
+        lib.nv4_paged_prefill_attention.argtypes = [_vp] * 8 + [_i64] * 9 + [ctypes.c_float, _vp]
+        lib.nv4_paged_prefill_attention.restype = _int
+        lib.nv4_shared_prefix_attention_workspace_bytes.argtypes = [_i64] * 4
+        lib.nv4_shared_prefix_attention_workspace_bytes.restype = _i64
+        lib.nv4_shared_prefix_attention.argtypes = [_vp] * 9 + [_i64] * 9 + [ctypes.c_float, _vp]
+        lib.nv4_shared_prefix_attention.restype = _int
         lib.nv4_status_string.argtypes = [_int]
         lib.nv4_status_string.restype = ctypes.c_char_p
         lib.nv4_device_error.argtypes = [ctypes.POINTER(_int)]
@@ -432,3 +444,11 @@ def serving():
 
 def paged_attention_kv4_workspace_bytes(batch: int, num_heads: int, max_pages: int) -> int:
     return int(load().nv4_paged_attention_kv4_workspace_bytes(batch, num_heads, max_pages))
+
+
+def paged_prefill_attention_workspace_bytes(tokens: int, batch: int, num_heads: int, num_kv_heads: int) -> int:
+    return int(load().nv4_paged_prefill_attention_workspace_bytes(tokens, batch, num_heads, num_kv_heads))
+
+
+def shared_prefix_attention_workspace_bytes(batch: int, groups: int, num_heads: int, num_kv_heads: int) -> int:
+    return int(load().nv4_shared_prefix_attention_workspace_bytes(batch, groups, num_heads, num_kv_heads))

@@ -1,0 +1,83 @@
+"""Operators of requests that share cached tokens, over the paged BF16 cache
+(csrc/paged_attention.cu): the append that writes it, the attention of prompts over
+what their requests have cached already, and the decode attention of a batch whose
+requests share a prefix.  (The reference calls flash-attn over its block tables,
+nanovllm/layers/attention.py:59-75, which reads a shared prefix once per request.)
+
+The cache is that of the model runner: BF16 [pages, 256, kv_heads, 128] for K and for
+V, token t of a request in page ``block_tables[request, t // 256]`` at row ``t % 256``.
+Requests share a prefix by naming the same pages; ``step_tables.build_step_tables``
+makes the tables, slots and positions.  Outputs carry no gradient.
+"""
+from __future__ import annotations
+
+import torch
+
+from nanovllm import _native
+
+HEAD_DIM = 128
+PAGE_TOKENS = 256
+
+
+def append_kv(q, k, v, cos_sin, positions, slot_mapping, k_cache, v_cache, *, q_weight=None, k_weight=None,
+              eps: float = 1e-6, q_out=None):
+    """Keys and values written to the cache rows ``slot_mapping`` (page * 256 + offset,
+    each at most once; negative: stores nothing), the rotation applied on the way.
+
+    ``q`` BF16 [T, Hq, 128] (or None), ``k`` and ``v`` BF16 [T, Hkv, 128], each with a
+    token's heads contiguous and any distance between tokens (a multiple of 8
+    channels): separate projections or views of a fused one.  With ``q_weight`` /
+    ``k_weight`` BF16 [128] that side is RMS-normalised first.  ``cos_sin`` FP32
+    [max_position, R] (cos, then sin): of the first R channels (a multiple of 16)
+    c and c + R/2 are rotated.  ``positions`` INT64 [T], ``slot_mapping`` INT32 [T].
+    Everything is FP32 with one rounding at the end (``qk_norm_rope_store`` of the
+    engine rounds three times, as the reference does).  Returns ``q_out`` [T, Hq,
+    128] (may be a contiguous ``q`` itself), None without ``q``.
+    """
+    return _native.serving().append_kv(q, k, v, cos_sin, positions, slot_mapping, k_cache, v_cache, q_weight, k_weight,
+                                       eps, q_out)
+
+
+def prefill_attention_workspace(num_tokens: int, batch: int, num_heads: int, num_kv_heads: int, device) -> torch.Tensor:
+    """Scratch of ``paged_prefill_attention`` for up to so many tokens and requests;
+    calls that may overlap (other streams, graphs) need one each."""
+    nbytes = _native.paged_prefill_attention_workspace_bytes(num_tokens, batch, num_heads, num_kv_heads)
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+
+def paged_prefill_attention(q, k_cache, v_cache, block_tables, context_lens, query_starts, *, scale: float, out=None,
+                            workspace=None):
+    """Attention of the new tokens of several requests, each over the tokens its
+    request has in the cache, the new ones included (causal).
+
+    ``q`` BF16 [T, Hq, 128] (Hq 1 to 16 times the KV heads), ``block_tables`` INT32
+    [B, max_pages], ``context_lens`` INT32 [B], ``query_starts`` INT32 [B + 1], not
+    falling: rows ``query_starts[b]`` to ``query_starts[b + 1] - 1`` are the last
+    tokens of request b's context.  A row that sees no token gets zeros; rows of no
+    request are left as they are.  Returns ``out`` BF16 [T, Hq, 128].
+    """
+    return _native.serving().prefill_attention(q, k_cache, v_cache, block_tables, context_lens, query_starts, out,
+                                               workspace, scale)
+
+
+def shared_prefix_workspace(batch: int, groups: int, num_heads: int, num_kv_heads: int, device) -> torch.Tensor:
+    """Scratch of ``shared_prefix_attention`` for up to so many requests and groups;
+    calls that may overlap (other streams, graphs) need one each."""
+    nbytes = _native.shared_prefix_attention_workspace_bytes(batch, groups, num_heads, num_kv_heads)
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+
+def shared_prefix_attention(q, k_cache, v_cache, block_tables, context_lens, group_starts, prefix_lens, *,
+                            scale: float, out=None, workspace=None):
+    """Attention of one query token per request, each over its whole context, where
+    groups of consecutive requests share a prefix that is read once for the group.
+
+    ``q`` BF16 [B, Hq, 128], ``block_tables`` INT32 [B, max_pages], ``context_lens``
+    INT32 [B] (0: a padding row, whose output is zero).  Requests ``group_starts[g]``
+    to ``group_starts[g + 1] - 1`` have ``prefix_lens[g]`` tokens in common (INT32
+    [groups + 1], not falling, and [groups]); the whole pages of these are read
+    through the first request's table, and the others' tables must name the same.
+    Requests of no group share nothing.  Returns ``out`` BF16 [B, Hq, 128].
+    """
+    return _native.serving().shared_attention(q, k_cache, v_cache, block_tables, context_lens, group_starts,
+                                              prefix_lens, out, workspace, scale)
