@@ -444,9 +444,10 @@ int nv4_paged_prefill_attention(const void* q, const void* k_cache, const void* 
  *   group_starts  int32 [groups + 1], not falling: requests group_starts[g] ..
  *                 group_starts[g + 1] - 1 are a group; requests of none share nothing
  *   prefix_lens   int32 [groups]: tokens that the group has in common.  The whole
- *                 pages of it are read through the first request's block table
- *                 (the others' must name the same pages), the rest, as all other
- *                 tokens, through each request's own
+ *                 pages of it are read through the block table of the group's
+ *                 longest request (the others' must name the same pages, as far as
+ *                 their contexts go), the rest, as all other tokens, through each
+ *                 request's own
  *   context_lens  int32 [batch]; 0 (or less) marks a padding row, whose output is zero
  * Everything else as nv4_paged_prefill_attention; groups may be 0 (then
  * group_starts and prefix_lens may be NULL).

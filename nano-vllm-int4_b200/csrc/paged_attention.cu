@@ -165,103 +165,4 @@ int launch_append_kv(const void* q, const void* k, const void* v, const void* q_
   return launch_kernel(append_kv_kernel, dim3(grid), dim3(kAppendThreads), 0, stream, false, a);
 }
 
-// ------------------------------------------------------------ attention, one warp per (query token, head)
-struct PagedRowsArgs {
-  const uint16_t* q;
-  const uint16_t* k_cache;
-  const uint16_t* v_cache;
-  const int* tables;
-  const int* context;
-  const int* starts;  // query starts [batch + 1], or nullptr: one token per request
-  uint16_t* out;
-  int64_t tokens, num_pages;
-  int batch, Hq, Hkv, max_pages;
-  float scale_log2;
-};
-
-__global__ void __launch_bounds__(256) paged_rows_attention_kernel(const PagedRowsArgs p) {
-  const int64_t row = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
-  const int lane = threadIdx.x & 31;
-  const int64_t t = row / p.Hq;
-  const int h = static_cast<int>(row - t * p.Hq), kvh = h / (p.Hq / p.Hkv);
-  if (t >= p.tokens) return;
-  int64_t b = t, limit;
-  if (p.starts) {
-    // starts count as the running maximum of their values, so that requests do not overlap
-    int64_t at = -1, from = 0, to = 0, top = 0;
-    for (int i = 0; i < p.batch; ++i) {
-      const int64_t lo = max(top, static_cast<int64_t>(p.starts[i]));
-      const int64_t hi = max(lo, static_cast<int64_t>(p.starts[i + 1]));
-      if (t >= lo && t < hi) at = i, from = lo, to = min(hi, p.tokens);
-      top = hi;
-    }
-    if (at < 0) return;
-    b = at;
-    limit = static_cast<int64_t>(p.context[b]) - (to - from) + (t - from) + 1;
-  } else {
-    limit = p.context[b];
-  }
-  limit = min(limit, static_cast<int64_t>(p.max_pages) * kPaPage);
-  const uint2 qr = *reinterpret_cast<const uint2*>(p.q + row * kPaD + lane * 4);
-  const float q[4] = {bf16lo_to_f32(qr.x), bf16hi_to_f32(qr.x), bf16lo_to_f32(qr.y), bf16hi_to_f32(qr.y)};
-  float m = -INFINITY, l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int64_t key = 0; key < limit; ++key) {
-    const int64_t page = p.tables[b * p.max_pages + key / kPaPage];
-    if (page < 0 || page >= p.num_pages) {
-      if (lane == 0) record_index_error(kErrBadPage);
-      continue;
-    }
-    const size_t at = static_cast<size_t>(((page * kPaPage + key % kPaPage) * p.Hkv + kvh) * kPaD + lane * 4);
-    const uint2 kr = *reinterpret_cast<const uint2*>(p.k_cache + at), vr = *reinterpret_cast<const uint2*>(p.v_cache + at);
-    float s = q[0] * bf16lo_to_f32(kr.x) + q[1] * bf16hi_to_f32(kr.x) + q[2] * bf16lo_to_f32(kr.y) +
-              q[3] * bf16hi_to_f32(kr.y);
-#pragma unroll
-    for (int i = 16; i >= 1; i >>= 1) s += __shfl_xor_sync(0xffffffffu, s, i);
-    s *= p.scale_log2;
-    const float m_new = fmaxf(m, s), base = m_new == -INFINITY ? 0.0f : m_new;
-    const float f = exp2f(m - base), e = exp2f(s - base);
-    const float v[4] = {bf16lo_to_f32(vr.x), bf16hi_to_f32(vr.x), bf16lo_to_f32(vr.y), bf16hi_to_f32(vr.y)};
-    l = l * f + e;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = o[i] * f + e * v[i];
-    m = m_new;
-  }
-  const float r = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-  const __nv_bfloat162 a = __floats2bfloat162_rn(o[0] * r, o[1] * r), c = __floats2bfloat162_rn(o[2] * r, o[3] * r);
-  *reinterpret_cast<uint2*>(p.out + row * kPaD + lane * 4) =
-      make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&c));
-}
-
-static int launch_paged_rows(const PagedRowsArgs& a, cudaStream_t stream) {
-  const int64_t blocks = (a.tokens * a.Hq + 7) / 8;
-  return launch_kernel(paged_rows_attention_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, false, a);
-}
-
-int64_t paged_prefill_attention_workspace_bytes(int64_t, int64_t, int64_t, int64_t) { return 16; }
-int64_t shared_prefix_attention_workspace_bytes(int64_t, int64_t, int64_t, int64_t) { return 16; }
-
-int launch_paged_prefill_attention(const void* q, const void* k_cache, const void* v_cache, const int* block_tables,
-                                   const int* context_lens, const int* query_starts, void* out, void*, int64_t tokens,
-                                   int64_t batch, int64_t num_heads, int64_t num_kv_heads, int64_t num_pages,
-                                   int64_t max_pages, float scale, cudaStream_t stream) {
-  return launch_paged_rows({static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k_cache),
-                            static_cast<const uint16_t*>(v_cache), block_tables, context_lens, query_starts,
-                            static_cast<uint16_t*>(out), tokens, num_pages, static_cast<int>(batch),
-                            static_cast<int>(num_heads), static_cast<int>(num_kv_heads), static_cast<int>(max_pages),
-                            scale * 1.4426950408889634f},
-                           stream);
-}
-
-int launch_shared_prefix_attention(const void* q, const void* k_cache, const void* v_cache, const int* block_tables,
-                                   const int* context_lens, const int*, const int*, void* out, void*, int64_t batch,
-                                   int64_t, int64_t num_heads, int64_t num_kv_heads, int64_t num_pages,
-                                   int64_t max_pages, float scale, cudaStream_t stream) {
-  return launch_paged_rows({static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k_cache),
-                            static_cast<const uint16_t*>(v_cache), block_tables, context_lens, nullptr,
-                            static_cast<uint16_t*>(out), batch, num_pages, static_cast<int>(batch),
-                            static_cast<int>(num_heads), static_cast<int>(num_kv_heads), static_cast<int>(max_pages),
-                            scale * 1.4426950408889634f},
-                           stream);
-}
-
 }  // namespace nv4

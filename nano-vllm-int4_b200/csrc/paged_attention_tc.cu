@@ -1,0 +1,1041 @@
+// The two attentions of requests that share cached tokens, on the 5th-generation
+// tensor cores (tcgen05 kind::f16): prompts over what their requests have cached
+// (nv4_paged_prefill_attention) and the decode attention of a batch whose requests
+// share a prefix (nv4_shared_prefix_attention).  BF16 cache, head_dim 128, pages of
+// 256 tokens.
+//
+//   out = sum_t p_t v_t / sum_t p_t,   p_t = 2^(c (s_t - m)),   s_t = q . k_t,
+//   c = scale * log2(e), m a running reference close to the maximum of s.
+//
+// Both are the same work on different rows.  A block is up to 128 rows (TB = 128 / G
+// tokens with the G query heads of a KV head each) that read the same keys:
+//   prompts   TB consecutive new tokens of a request (two such blocks side by side),
+//             over its context up to the last one's own position;
+//   prefix    up to TB requests of a group, over the pages they have in common;
+//   own       one request's token, over what is left of its context.
+// The keys of a block are walked in tiles of 128 (half a page).  All (block, KV head,
+// tile) triples lie in one line that is cut evenly over the workers, whatever the
+// lengths, so that the SMs end together; a block cut by such a border leaves
+// unnormalised outputs with their references and sums, which a last kernel joins in
+// the order of the tiles (the cuts follow from the lengths alone: results are
+// reproducible).  A first kernel of one CTA makes the block table from the lengths on
+// the device, so that captured calls follow new lengths.
+//
+// A CTA (one per SM, 384 threads) has two lanes: Q tile, S and O accumulators in TMEM
+// (128 columns each) and a warpgroup of softmax, one thread per row.  While one
+// lane's warpgroup works on its scores, the tensor cores work for the other.
+//   prompts (pair)  both lanes take the same keys for two blocks of rows: K and V pass
+//                   from L2 to shared memory once for 256 rows;
+//   others (solo)   every lane is a worker of its own.
+//   warp 0     copies K and V tiles (TMA, five slots of 32 KB) in the order of use
+//   warp 1     issues S = Q K^T, O += P V;  V rows behind the last token of a request
+//              are cleared first (0 times an old NaN would be one)
+//   warps 2-3  bring the rows of Q to shared memory (a gather: cp.async)
+//   warps 4-11 softmax of the two lanes; outputs
+// P goes back to TMEM over its scores in two BF16 terms (the upper 16 bits of the FP32
+// value and the rest, 2^-15 of it at most left out), so that the output's own rounding
+// is the only one that shows; one term would cost 1.4 times that error and save a
+// third of the tensor work.  m is moved (and O rescaled) only when a score exceeds it
+// by 2^8, so O is rarely touched.
+#include "nv4_device.cuh"
+#include "nv4_launch.h"
+
+namespace nv4 {
+
+constexpr int kPtRows = 128;    // rows of a block, keys of a tile, head_dim
+constexpr int kPtPage = 256;
+constexpr int kPtMaxCtas = 160;
+constexpr int kPtThreads = 384;
+constexpr int kPtTile = kPtRows * kPtRows * 2;  // bytes of a Q, K or V tile
+constexpr int kPtHalf = kPtTile / 2;            // 64 channels of it: [128 rows][128 bytes], 128-byte swizzle
+constexpr int kPtSlots = 5;
+constexpr int kPtBar = (2 + kPtSlots) * kPtTile;
+constexpr int kPtSmem = kPtBar + 512 + 1024;    // barriers and flags; alignment of the tiles to 1024
+constexpr float kPtSlack = 8.0f;                // log2 units by which a score may pass the reference
+
+enum PtKind : int { kPtPrompt = 0, kPtOwn = 1, kPtPrefix = 2 };
+
+// A block of rows and the keys it walks (for every KV head).
+struct __align__(16) PtBlock {
+  int seq;    // whose block table
+  int tok0;   // first query token
+  int ntok;   // query tokens
+  int tiles;  // key tiles, at least 1
+  int key0;   // first key, a multiple of the page
+  int limit;  // keys that the first token sees, one more each further (prompts); the token's (own)
+  int end;    // keys that exist
+  int kind;
+};
+
+// Where a worker starts, and how many tiles it takes.
+struct __align__(16) PtStart {
+  int block, head, tile, pad;
+  int64_t count, pad2;
+};
+
+struct PtSums {
+  int64_t total, chunk;  // tiles of all blocks and heads; of a worker
+  int blocks, prefix_blocks;
+};
+
+// The scratch: block table and borders, then the outputs of cut blocks.
+struct PtScratch {
+  PtSums* sums;
+  PtStart* starts;   // [workers]
+  PtBlock* blocks;
+  int64_t* before;   // [blocks + 1]: tiles (of one head) before a block
+  int* row_block;    // [batch]: the prefix block of a request, or -1
+  float* part;       // [workers][2][rows][128]: of a worker's first and last block, when cut
+  float* part_ml;    // [..][2]: reference, sum
+  float* row;        // [2][batch * Hq][128]: of own and prefix blocks that are not cut, but joined
+  float* row_ml;
+};
+
+struct PtArgs {
+  const uint16_t* q;
+  const int* tables;
+  const int* context;
+  const int* starts;  // query starts, or group starts
+  const int* prefix;  // of groups, or nullptr: prompts
+  uint16_t* out;
+  PtScratch w;
+  int64_t num_pages;
+  int tokens, batch, groups, Hq, Hkv, G, TB, max_pages, workers, slot_rows;
+  float c;  // scale * log2(e)
+};
+
+// ------------------------------------------------------------ block table
+// Sum over the CTA of values before this thread's; `total` is that of all.
+__device__ __forceinline__ int64_t pt_scan(int64_t v, int64_t* warp_sums, int64_t& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int64_t x = v;
+#pragma unroll
+  for (int m = 1; m < 32; m <<= 1) {
+    const int64_t y = __shfl_up_sync(0xffffffffu, x, m);
+    if (lane >= m) x += y;
+  }
+  __syncthreads();
+  if (lane == 31) warp_sums[warp] = x;
+  __syncthreads();
+  int64_t before = 0;
+  total = 0;
+  for (int i = 0; i < 32; ++i) {
+    if (i < warp) before += warp_sums[i];
+    total += warp_sums[i];
+  }
+  return before + x - v;
+}
+
+// Running maximum up to this thread, `carry` that of the threads before (updated).
+__device__ __forceinline__ int pt_max_scan(int v, int* warp_max, int& carry) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int x = v;
+#pragma unroll
+  for (int m = 1; m < 32; m <<= 1) x = max(x, __shfl_up_sync(0xffffffffu, x, m));
+  __syncthreads();
+  if (lane == 31) warp_max[warp] = x;
+  __syncthreads();
+  int all = carry;
+  x = max(x, carry);
+  for (int i = 0; i < 32; ++i) {
+    if (i < warp) x = max(x, warp_max[i]);
+    all = max(all, warp_max[i]);
+  }
+  carry = all;
+  return x;
+}
+
+__device__ __forceinline__ int pt_tiles(int keys) { return max(1, (keys + kPtRows - 1) / kPtRows); }
+
+constexpr int kPtPlanThreads = 1024;
+constexpr int kPtPlanCached = 2048;  // blocks whose sums are kept in shared memory for the search
+
+__global__ void __launch_bounds__(kPtPlanThreads) pt_plan_kernel(const PtArgs p, const int block_tokens) {
+  __shared__ int64_t sums[32];
+  __shared__ int maxima[32];
+  __shared__ int first[kPtPlanThreads], last[kPtPlanThreads], extra[kPtPlanThreads], which[kPtPlanThreads];
+  __shared__ int table_row[kPtPlanThreads];
+  __shared__ int64_t weight[kPtPlanThreads];
+  __shared__ int64_t cached[kPtPlanCached];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int most = p.max_pages * kPtPage;
+  grid_dependency_wait();
+  grid_dependents_launch();
+  int64_t tiles_before = 0;
+  int blocks = 0, prefix_blocks = 0, carry = 0;
+  auto put = [&](int i, int64_t before, const PtBlock& b) {
+    p.w.blocks[i] = b;
+    p.w.before[i] = before;
+    if (i < kPtPlanCached) cached[i] = before;
+  };
+
+  if (p.prefix == nullptr) {
+    for (int b0 = 0; b0 < p.batch; b0 += kPtPlanThreads) {
+      const int b = b0 + tid;
+      const bool live = b < p.batch;
+      const int at = live ? min(max(p.starts[b], 0), p.tokens) : 0;
+      const int next = live ? min(max(p.starts[b + 1], 0), p.tokens) : 0;
+      const int lo = pt_max_scan(at, maxima, carry);
+      first[tid] = lo;
+      last[tid] = live ? max(lo, next) : lo;
+      extra[tid] = live ? max(p.context[b], 0) : 0;
+      __syncthreads();
+      const int here = min(kPtPlanThreads, p.batch - b0);
+      for (int s = warp; s < here; s += kPtPlanThreads / 32) {
+        const int n = last[s] - first[s], ctx = extra[s], end = min(ctx, most);
+        int64_t sum = 0;
+        for (int j = lane; j * block_tokens < n; j += 32)
+          sum += pt_tiles(min(ctx - n + min(n, (j + 1) * block_tokens), end));
+#pragma unroll
+        for (int m = 16; m >= 1; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
+        if (lane == 0) weight[s] = sum;
+      }
+      __syncthreads();
+      const int mine = live ? (last[tid] - first[tid] + block_tokens - 1) / block_tokens : 0;
+      const int64_t w = live ? weight[tid] : 0;
+      int64_t all_w, all_n;
+      const int64_t wb = tiles_before + pt_scan(w, sums, all_w);
+      which[tid] = blocks + static_cast<int>(pt_scan(mine, sums, all_n));
+      weight[tid] = wb;
+      tiles_before += all_w;
+      blocks += static_cast<int>(all_n);
+      __syncthreads();
+      for (int s = warp; s < here; s += kPtPlanThreads / 32) {
+        const int n = last[s] - first[s], ctx = extra[s], end = min(ctx, most);
+        int64_t before = weight[s];
+        for (int j0 = 0; j0 * block_tokens < n; j0 += 32) {
+          const int j = j0 + lane, i0 = j * block_tokens;
+          const int count = min(n - i0, block_tokens);
+          const int tiles = count > 0 ? pt_tiles(min(ctx - n + i0 + count, end)) : 0;
+          int64_t x = tiles;
+#pragma unroll
+          for (int m = 1; m < 32; m <<= 1) {
+            const int64_t y = __shfl_up_sync(0xffffffffu, x, m);
+            if (lane >= m) x += y;
+          }
+          if (count > 0)
+            put(which[s] + j, before + x - tiles,
+                PtBlock{b0 + s, first[s] + i0, count, tiles, 0, ctx - n + i0 + 1, end, kPtPrompt});
+          before += __shfl_sync(0xffffffffu, x, 31);
+        }
+      }
+      __syncthreads();
+    }
+  } else {
+    for (int b = tid; b < p.batch; b += kPtPlanThreads) p.w.row_block[b] = -1;
+    __syncthreads();
+    for (int g0 = 0; g0 < p.groups; g0 += kPtPlanThreads) {
+      const int g = g0 + tid;
+      const bool live = g < p.groups;
+      const int at = live ? min(max(p.starts[g], 0), p.batch) : 0;
+      const int next = live ? min(max(p.starts[g + 1], 0), p.batch) : 0;
+      const int lo = pt_max_scan(at, maxima, carry);
+      first[tid] = lo;
+      last[tid] = live ? max(lo, next) : lo;
+      extra[tid] = live ? p.prefix[g] : 0;
+      __syncthreads();
+      const int here = min(kPtPlanThreads, p.groups - g0);
+      for (int s = warp; s < here; s += kPtPlanThreads / 32) {
+        // the pages in common, read through the table of the longest request
+        int best = 0, row = first[s], full = 0;
+        for (int r = first[s] + lane; r < last[s]; r += 32) {
+          const int ctx = min(p.context[r], most);
+          if (ctx > best) best = ctx, row = r;
+          full += ctx > 0;
+        }
+#pragma unroll
+        for (int m = 16; m >= 1; m >>= 1) {
+          const int ob = __shfl_xor_sync(0xffffffffu, best, m), orow = __shfl_xor_sync(0xffffffffu, row, m);
+          if (ob > best || (ob == best && orow < row)) best = ob, row = orow;
+          full += __shfl_xor_sync(0xffffffffu, full, m);
+        }
+        if (lane == 0) {
+          extra[s] = full > 1 ? max(min(extra[s], best), 0) / kPtPage * kPtPage : 0;
+          weight[s] = row;
+        }
+      }
+      __syncthreads();
+      const int shared = extra[tid], row = static_cast<int>(weight[tid]);
+      const int mine = live && shared > 0 ? (last[tid] - first[tid] + p.TB - 1) / p.TB : 0;
+      int64_t all_w, all_n;
+      const int64_t wb = tiles_before + pt_scan(static_cast<int64_t>(mine) * (shared / kPtRows), sums, all_w);
+      which[tid] = blocks + static_cast<int>(pt_scan(mine, sums, all_n));
+      __syncthreads();
+      weight[tid] = wb;
+      tiles_before += all_w;
+      blocks += static_cast<int>(all_n);
+      table_row[tid] = row;
+      __syncthreads();
+      for (int s = warp; s < here; s += kPtPlanThreads / 32) {
+        if (extra[s] <= 0) continue;
+        const int n = last[s] - first[s], tiles = extra[s] / kPtRows;
+        for (int j = lane; j * p.TB < n; j += 32)
+          put(which[s] + j, weight[s] + static_cast<int64_t>(j) * tiles,
+              PtBlock{table_row[s], first[s] + j * p.TB, min(p.TB, n - j * p.TB), tiles, 0, 0, extra[s], kPtPrefix});
+        for (int r = lane; r < n; r += 32) p.w.row_block[first[s] + r] = which[s] + r / p.TB;
+      }
+      __syncthreads();
+    }
+    prefix_blocks = blocks;
+    for (int b0 = 0; b0 < p.batch; b0 += kPtPlanThreads) {
+      const int b = b0 + tid;
+      const bool live = b < p.batch;
+      int tiles = 0, shared = 0, end = 0;
+      if (live) {
+        const int of = p.w.row_block[b];
+        shared = of >= 0 ? p.w.blocks[of].end : 0;
+        end = min(max(p.context[b], 0), most);
+        tiles = pt_tiles(end - shared);
+      }
+      int64_t all_w;
+      const int64_t wb = tiles_before + pt_scan(tiles, sums, all_w);
+      if (live) put(blocks + b, wb, PtBlock{b, b, 1, tiles, shared, end, end, kPtOwn});
+      tiles_before += all_w;
+    }
+    blocks += p.batch;
+    __syncthreads();
+  }
+
+  const int64_t total = tiles_before * p.Hkv;
+  const int64_t chunk = max((total + p.workers - 1) / p.workers, static_cast<int64_t>(1));
+  if (tid == 0) {
+    p.w.before[blocks] = tiles_before;
+    *p.w.sums = PtSums{total, chunk, blocks, prefix_blocks};
+  }
+  __syncthreads();
+  const int64_t* before = blocks <= kPtPlanCached ? cached : p.w.before;
+  for (int w = tid; w < p.workers; w += kPtPlanThreads) {
+    PtStart s{0, 0, 0, 0, 0, 0};
+    const int64_t at = w * chunk;
+    s.count = max(min(total - at, chunk), static_cast<int64_t>(0));
+    if (s.count > 0) {
+      int lo = 0, hi = blocks - 1;  // the last block whose tiles start at or before `at`
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) / 2;
+        if (before[mid] * p.Hkv <= at) lo = mid;
+        else hi = mid - 1;
+      }
+      const int64_t into = at - before[lo] * p.Hkv;
+      const int tiles = p.w.blocks[lo].tiles;
+      s.block = lo;
+      s.head = static_cast<int>(into / tiles);
+      s.tile = static_cast<int>(into % tiles);
+    }
+    p.w.starts[w] = s;
+  }
+}
+
+// ------------------------------------------------------------ tensor-core operations
+// Instruction descriptor, BF16 A and B, FP32 accumulator; `b_mn`: B has its N dimension contiguous.
+__host__ __device__ constexpr uint32_t pt_idesc(int m, int n, bool b_mn) {
+  return (1u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(b_mn) << 16) |
+         (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
+}
+// Descriptor of V as the B operand: N (channels) contiguous in 128-byte rows, keys the rows; eight keys are an atom of
+// 1024 bytes (stride offset), the second 64 channels lie a half tile on (leading offset).
+__device__ __forceinline__ uint64_t pt_desc_v(uint32_t addr) {
+  return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | (static_cast<uint64_t>(kPtHalf >> 4) << 16) |
+         (static_cast<uint64_t>(1024u >> 4) << 32) | (static_cast<uint64_t>(1u) << 46) |
+         (static_cast<uint64_t>(2u) << 61);
+}
+__device__ __forceinline__ void pt_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void pt_cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ float pt_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// The tiles of a worker, in order.
+struct PtWalk {
+  const PtBlock* blocks;
+  PtBlock b;
+  int block, head, tile, heads;
+  int64_t left;  // the current one included
+  bool fresh;    // the current tile is the first of this worker in its block and head
+
+  __device__ __forceinline__ void load() {
+    const int4* src = reinterpret_cast<const int4*>(blocks + block);
+    const int4 x = src[0], y = src[1];  // not the read-only path: the kernel before wrote them
+    b = PtBlock{x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+  }
+  __device__ __forceinline__ void start(const PtArgs& p, int worker) {
+    const PtStart s = p.w.starts[worker];
+    blocks = p.w.blocks;
+    block = s.block, head = s.head, tile = s.tile, heads = p.Hkv;
+    left = s.count;
+    fresh = true;
+    if (left > 0) load();
+  }
+  __device__ __forceinline__ bool last() const { return tile + 1 == b.tiles || left == 1; }  // of this worker in it
+  __device__ __forceinline__ void next() {
+    fresh = ++tile == b.tiles;
+    --left;
+    if (!fresh) return;
+    tile = 0;
+    if (++head == heads) {
+      head = 0;
+      ++block;
+      if (left > 0) load();
+    }
+  }
+};
+
+struct PtBars {
+  uint64_t full[kPtSlots], empty[kPtSlots];
+  uint64_t q_full[2], q_free[2], s_full[2], p_full[2], o_full[2], done;
+  uint32_t tmem;
+  int slot_keys[kPtSlots];  // keys of the slot's tile that exist
+  int lane_keys[2];         // of the tile whose scores lie in the lane
+};
+static_assert(sizeof(PtBars) <= 512, "barriers");
+
+// ------------------------------------------------------------ attention
+template <bool kPair>
+__global__ void __launch_bounds__(kPtThreads, 1)
+    pt_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
+                        const PtArgs p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + (((smem_u32(smem_raw) + 1023u) & ~1023u) - smem_u32(smem_raw));
+  uint8_t* ring = smem + 2 * kPtTile;
+  PtBars& bar = *reinterpret_cast<PtBars*>(smem + kPtBar);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kPtSlots; ++s) mbar_init(&bar.full[s], 1), mbar_init(&bar.empty[s], 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bar.q_full[i], 1);
+      mbar_init(&bar.q_free[i], 1);
+      mbar_init(&bar.s_full[i], 2);  // the products' completion, and lane_keys
+      mbar_init(&bar.p_full[i], 4);  // the warps of the lane
+      mbar_init(&bar.o_full[i], 1);
+    }
+    mbar_init(&bar.done, 1);
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(&bar.tmem, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bar.tmem;
+  grid_dependency_wait();  // the block table, and q, from the kernels before
+  grid_dependents_launch();
+
+  // Worker of a lane; in a pair both lanes walk worker blockIdx.x.
+  auto worker = [&](int l) { return static_cast<int>(blockIdx.x) + (kPair ? 0 : l * static_cast<int>(gridDim.x)); };
+  // Does lane l have rows of block b?
+  auto has_rows = [&](int l, const PtBlock& b) { return !kPair || l == 0 || b.ntok > p.TB; };
+  bool ok = true;
+
+  if (warp == 0) {
+    // ---------------- copies of K and V
+    if (lane == 0) {
+      tma_prefetch_desc(&tmap_k);
+      tma_prefetch_desc(&tmap_v);
+      int c = 0;
+      auto load = [&](const CUtensorMap* map, int x, int row, int keys) {
+        const int s = c % kPtSlots;
+        if (c >= kPtSlots && !mbar_wait(&bar.empty[s], ((c / kPtSlots) - 1) & 1, kErrTimeoutEmpty)) return false;
+        bar.slot_keys[s] = keys;
+        mbar_arrive_expect_tx(&bar.full[s], keys > 0 ? kPtTile : 0);
+        if (keys > 0) {
+          tma_load_2d(ring + s * kPtTile, map, &bar.full[s], x, row);
+          tma_load_2d(ring + s * kPtTile + kPtHalf, map, &bar.full[s], x + 64, row);
+        }
+        ++c;
+        return true;
+      };
+      // the cache row and the number of keys of a walk's tile
+      auto place = [&](const PtWalk& w, int& row, int& keys) {
+        const int key = w.b.key0 + w.tile * kPtRows;
+        row = 0;
+        keys = min(max(w.b.end - key, 0), kPtRows);
+        if (keys == 0) return;
+        const int page = __ldg(p.tables + static_cast<int64_t>(w.b.seq) * p.max_pages + key / kPtPage);
+        if (page < 0 || page >= p.num_pages) {
+          record_index_error(kErrBadPage);
+          keys = 0;
+        } else {
+          row = page * kPtPage + key % kPtPage;
+        }
+      };
+      constexpr int kLanes = kPair ? 1 : 2;
+      PtWalk w[kLanes];
+      int row[kLanes], keys[kLanes], x[kLanes];
+#pragma unroll
+      for (int l = 0; l < kLanes; ++l) {
+        w[l].start(p, worker(l));
+        if (w[l].left > 0 && ok) {
+          place(w[l], row[l], keys[l]);
+          x[l] = w[l].head * kPtRows;
+          ok = load(&tmap_k, x[l], row[l], keys[l]);
+        }
+      }
+      while (ok && w[0].left > 0) {
+#pragma unroll
+        for (int l = 0; l < kLanes; ++l) {
+          if (!ok || w[l].left == 0) continue;
+          ok = load(&tmap_v, x[l], row[l], keys[l]);
+          w[l].next();
+          if (!ok || w[l].left == 0) continue;
+          place(w[l], row[l], keys[l]);
+          x[l] = w[l].head * kPtRows;
+          ok = load(&tmap_k, x[l], row[l], keys[l]);
+        }
+      }
+      // every copy issued must land before the CTA may exit
+      for (int i = max(0, c - kPtSlots); i < c; ++i) {
+        const uint64_t start = global_timer_ns();
+        while (!mbar_try_wait(&bar.full[i % kPtSlots], (i / kPtSlots) & 1))
+          if (global_timer_ns() - start > kWaitLimitNs) {
+            record_error(kErrTimeoutDrain);
+            break;
+          }
+      }
+    }
+  } else if (warp == 1) {
+    // ---------------- products; the whole warp walks, lane 0 issues
+    constexpr uint32_t kQk = pt_idesc(kPtRows, kPtRows, false), kPv = pt_idesc(kPtRows, kPtRows, true);
+    int c = 0;                         // ring position
+    int tiles[2] = {0, 0};             // products S of the lane so far
+    int parts[2] = {0, 0};             // blocks of the lane so far
+    bool started[2] = {false, false};  // O holds something of the current block
+    // S = Q K^T of the tile in ring position c
+    auto arrived = [&](uint64_t& b, int phase) {  // the same answer in every lane
+      return __all_sync(0xffffffffu, mbar_wait(&b, phase & 1, kErrTimeoutMma)) != 0;
+    };
+    auto scores = [&](int l, const PtWalk& w, bool release) {
+      const int s = c % kPtSlots;
+      if (!arrived(bar.full[s], c / kPtSlots)) return false;
+      if (w.fresh && !arrived(bar.q_full[l], parts[l]++)) return false;
+      tc_fence_after();
+      if (lane == 0) {
+        bar.lane_keys[l] = bar.slot_keys[s];  // before the slot can be released
+        const uint32_t qa = smem_u32(smem + l * kPtTile), ka = smem_u32(ring + s * kPtTile);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const uint32_t off = (j >> 2) * kPtHalf + (j & 3) * 32;
+          pt_mma_ss(tmem + l * 256, umma_desc_sw128(qa + off), umma_desc_sw128(ka + off), kQk, j > 0);
+        }
+        if (release) umma_commit(&bar.empty[s]);
+        if (w.last()) umma_commit(&bar.q_free[l]);
+        umma_commit(&bar.s_full[l]);
+        mbar_arrive(&bar.s_full[l]);
+      }
+      __syncwarp();
+      ++tiles[l];
+      return true;
+    };
+    // O += P V
+    auto values = [&](int l, const PtWalk& w, bool release) {
+      const int s = c % kPtSlots;
+      if (!arrived(bar.full[s], c / kPtSlots) || !arrived(bar.p_full[l], tiles[l] - 1)) return false;
+      tc_fence_after();
+      const int keys = bar.slot_keys[s], steps = (keys + 15) / 16;
+      __syncwarp();  // all have read it before the slot can be released
+      uint8_t* v = ring + s * kPtTile;
+      if (keys & 15) {  // rows behind the last key: P is zero there, V may be anything
+        for (int i = lane; i < (steps * 16 - keys) * 16; i += 32)
+          *reinterpret_cast<uint4*>(v + (i & 8 ? kPtHalf : 0) + (keys + (i >> 4)) * 128 + (i & 7) * 16) =
+              make_uint4(0, 0, 0, 0);
+        fence_proxy_async_smem();
+        __syncwarp();
+      }
+      if (w.fresh) started[l] = false;
+      if (lane == 0) {
+        const uint32_t o = tmem + l * 256 + 128, pt = tmem + l * 256, va = smem_u32(v);
+        for (int k = 0; k < steps; ++k) {
+          const uint64_t desc = pt_desc_v(va + k * 2048);
+          const uint32_t pk = pt + (k >> 2) * 64 + (k & 3) * 8;
+          umma_bf16_ts(o, pk, desc, kPv, started[l] || k > 0);
+          umma_bf16_ts(o, pk + 32, desc, kPv, 1);
+        }
+        if (release) umma_commit(&bar.empty[s]);
+        if (w.last()) umma_commit(&bar.o_full[l]);
+      }
+      started[l] = started[l] || steps > 0;
+      __syncwarp();
+      return true;
+    };
+    if constexpr (kPair) {
+      PtWalk w;
+      w.start(p, worker(0));
+      if (w.left > 0) {
+        const bool two = has_rows(1, w.b);
+        ok = scores(0, w, !two) && (!two || scores(1, w, true));
+        ++c;
+      }
+      while (ok && w.left > 0) {
+        // ring: V of this tile, then K of the next
+        const bool two = has_rows(1, w.b);
+        PtWalk n = w;
+        n.next();
+        const bool more = n.left > 0, two_next = more && has_rows(1, n.b);
+        ok = values(0, w, !two);
+        if (ok && more) {
+          ++c;
+          ok = scores(0, n, !two_next);
+          --c;
+        }
+        if (ok && two) ok = values(1, w, true);
+        ++c;
+        if (ok && two_next) ok = scores(1, n, true);
+        if (more) ++c;
+        w = n;
+      }
+    } else {
+      PtWalk w[2];
+#pragma unroll
+      for (int l = 0; l < 2; ++l) {
+        w[l].start(p, worker(l));
+        if (w[l].left > 0 && ok) ok = scores(l, w[l], true), ++c;
+      }
+      while (ok && w[0].left > 0) {
+#pragma unroll
+        for (int l = 0; l < 2; ++l) {
+          if (!ok || w[l].left == 0) continue;
+          ok = values(l, w[l], true);
+          ++c;
+          w[l].next();
+          if (!ok || w[l].left == 0) continue;
+          ok = scores(l, w[l], true);
+          ++c;
+        }
+      }
+    }
+    if (lane == 0) {  // all issued products must finish before the TMEM is released
+      umma_commit(&bar.done);
+      const uint64_t start = global_timer_ns();
+      while (!mbar_try_wait(&bar.done, 0))
+        if (global_timer_ns() - start > kWaitLimitNs) {
+          record_error(kErrTimeoutDrain);
+          break;
+        }
+    }
+    __syncwarp();
+  } else if (warp < 4) {
+    // ---------------- rows of Q: row r of a lane is head r % G of its token r / G
+    const int l = warp - 2;
+    uint8_t* dst = smem + l * kPtTile;
+    PtWalk w;
+    w.start(p, worker(l));
+    int part = 0;
+    while (ok && w.left > 0) {
+      if (w.fresh && has_rows(l, w.b)) {
+        if (part > 0) ok = __all_sync(0xffffffffu, mbar_wait(&bar.q_free[l], (part - 1) & 1, kErrTimeoutEmpty));
+        if (!ok) break;
+        const int t0 = kPair ? l * p.TB : 0;
+        const int rows = min(w.b.ntok - t0, p.TB) * p.G;
+        const uint16_t* src = p.q + (static_cast<int64_t>(w.b.tok0 + t0) * p.Hq + w.head * p.G) * kPtRows;
+        for (int i = lane; i < rows * 16; i += 32) {
+          const int r = i >> 4, ch = i & 15, t = r / p.G;
+          pt_cp_async16(smem_u32(dst) + (ch >> 3) * kPtHalf + sw128_offset(r, ch & 7),
+                        src + (static_cast<int64_t>(t) * p.Hq + (r - t * p.G)) * kPtRows + ch * 8);
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar.q_full[l]);
+        ++part;
+      }
+      // to the first tile of the next block
+      const int64_t skip = min(static_cast<int64_t>(w.b.tiles - w.tile), w.left);
+      w.tile += static_cast<int>(skip) - 1;
+      w.left -= skip - 1;
+      w.next();
+    }
+  } else {
+    // ---------------- softmax and outputs: thread = row
+    const int l = (warp - 4) >> 2, r = threadIdx.x & 127;
+    const uint32_t at = tmem + l * 256 + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    const float c = p.c;
+    PtWalk w;
+    w.start(p, worker(l));
+    int64_t part_rows = 0;
+    int tile = 0, part = 0, limit = 0, token = 0, head = 0, from = 0;
+    bool live = false, started = false;
+    float m = -INFINITY, sum = 0.0f;
+    for (; ok && w.left > 0; w.next()) {
+      if (!has_rows(l, w.b)) continue;
+      if (w.fresh) {
+        const int t0 = kPair ? l * p.TB : 0, t = r / p.G;
+        live = r < min(w.b.ntok - t0, p.TB) * p.G;
+        token = w.b.tok0 + t0 + t;
+        head = w.head * p.G + r - t * p.G;
+        limit = 0;
+        if (live)
+          limit = w.b.kind == kPtPrompt ? w.b.limit + t0 + t : w.b.kind == kPtOwn ? w.b.limit : __ldg(p.context + token);
+        m = -INFINITY, sum = 0.0f;
+        started = false;
+        from = w.tile;
+      }
+      const bool busy = __any_sync(0xffffffffu, live);
+      ok = __all_sync(0xffffffffu, mbar_wait(&bar.s_full[l], tile & 1, kErrTimeoutMma));
+      if (!ok) break;
+      tc_fence_after();
+      const int keys = *reinterpret_cast<volatile int*>(&bar.lane_keys[l]);
+      if (busy && keys > 0) {
+        const int seen = min(max(limit - (w.b.key0 + w.tile * kPtRows), 0), keys);
+        const bool edge = __any_sync(0xffffffffu, seen < kPtRows);
+        // scores of keys 64 half .. 64 half + 63; those that the row does not see as -inf
+        auto fetch = [&](int half, uint32_t (&s)[64]) {
+          tmem_ld32(at + 64 * half, s);
+          tmem_ld32(at + 64 * half + 32, s + 32);
+          tmem_wait_ld();
+          if (edge) {
+#pragma unroll
+            for (int j = 0; j < 64; ++j) s[j] = 64 * half + j < seen ? s[j] : 0xFF800000u;
+          }
+        };
+        uint32_t s[64];
+        float top = -INFINITY;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          fetch(half, s);
+#pragma unroll
+          for (int j = 0; j < 64; j += 2)
+            top = fmaxf(top, fmaxf(__uint_as_float(s[j]), __uint_as_float(s[j + 1])));
+        }
+        const bool move = top > m && (m == -INFINITY || (top - m) * c > kPtSlack);
+        if (__any_sync(0xffffffffu, move) && started) {
+          const float f = move ? pt_exp2((m - top) * c) : 1.0f;
+          sum *= f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint32_t o[32];
+            tmem_ld32(at + 128 + 32 * i, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+            tmem_st32(at + 128 + 32 * i, o);
+          }
+        }
+        if (move) m = top;
+        const float base = m == -INFINITY ? 0.0f : m;
+        const uint64_t base2 = pair(base, base), c2 = pair(c, c);
+        uint64_t sums = 0;
+        // 64 keys' probabilities take the columns of their scores: 32 of the upper terms, 32 of the lower
+#pragma unroll
+        for (int half = 1; half >= 0; --half) {
+          if (half == 0) fetch(0, s);
+          uint32_t hi[32], lo[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            float x, y;
+            unpair(mul2(sub2(pair(__uint_as_float(s[2 * j]), __uint_as_float(s[2 * j + 1])), base2), c2), x, y);
+            x = pt_exp2(x), y = pt_exp2(y);
+            const uint64_t e = pair(x, y);
+            sums = add2(sums, e);
+            const uint32_t xb = __float_as_uint(x), yb = __float_as_uint(y);
+            hi[j] = __byte_perm(xb, yb, 0x7632);
+            float u, v;
+            unpair(sub2(e, pair(__uint_as_float(xb & 0xFFFF0000u), __uint_as_float(yb & 0xFFFF0000u))), u, v);
+            const __nv_bfloat162 rest = __floats2bfloat162_rn(u, v);
+            lo[j] = *reinterpret_cast<const uint32_t*>(&rest);
+          }
+          tmem_st32(at + 64 * half, hi);
+          tmem_st32(at + 64 * half + 32, lo);
+        }
+        float x, y;
+        unpair(sums, x, y);
+        sum += x + y;
+        tmem_wait_st();
+      }
+      started = started || keys > 0;
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bar.p_full[l]);
+      ++tile;
+      if (!w.last()) continue;
+
+      // the block's end, or this worker's: outputs
+      ok = __all_sync(0xffffffffu, mbar_wait(&bar.o_full[l], part & 1, kErrTimeoutMma));
+      if (!ok) break;
+      ++part;
+      tc_fence_after();
+      const bool whole = from == 0 && w.tile + 1 == w.b.tiles;
+      const bool final_ = whole && (w.b.kind == kPtPrompt || (w.b.kind == kPtOwn && w.b.key0 == 0));
+      if (busy) {
+        const float f = final_ ? (sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f) : 1.0f;
+        const int64_t row = static_cast<int64_t>(token) * p.Hq + head;
+        float* po;
+        float* pm;
+        if (whole) {
+          const int64_t i = (w.b.kind == kPtPrefix ? static_cast<int64_t>(p.batch) * p.Hq : 0) + row;
+          po = p.w.row + i * kPtRows, pm = p.w.row_ml + i * 2;
+        } else {
+          part_rows = (static_cast<int64_t>(worker(l)) * 2 + (from == 0)) * (kPair ? 2 : 1) + (kPair ? l : 0);
+          const int64_t i = part_rows * p.slot_rows + r;
+          po = p.w.part + i * kPtRows, pm = p.w.part_ml + i * 2;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t o[32];
+          if (started) {
+            tmem_ld32(at + 128 + 32 * i, o);
+            tmem_wait_ld();
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) o[j] = 0u;
+          }
+          if (live && final_) {
+            uint4* dst = reinterpret_cast<uint4*>(p.out + row * kPtRows + 32 * i);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              uint32_t v[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const __nv_bfloat162 b = __floats2bfloat162_rn(__uint_as_float(o[8 * j + 2 * e]) * f,
+                                                               __uint_as_float(o[8 * j + 2 * e + 1]) * f);
+                v[e] = *reinterpret_cast<const uint32_t*>(&b);
+              }
+              dst[j] = make_uint4(v[0], v[1], v[2], v[3]);
+            }
+          } else if (live) {
+            uint4* dst = reinterpret_cast<uint4*>(po + 32 * i);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) dst[j] = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+          }
+          __syncwarp();
+        }
+        if (live && !final_) pm[0] = m, pm[1] = sum;
+      }
+      tc_fence_before();
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// ------------------------------------------------------------ joining
+// out = sum_i w_i O_i / sum_i w_i l_i, w_i = 2^(c (m_i - max m)); a warp per row, four channels a lane.
+struct PtJoin {
+  float m = -INFINITY, l = 0.0f;
+  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+
+  __device__ __forceinline__ void add(const float* po, const float* pm, int lane, float c) {
+    const float pm0 = pm[0], pl = pm[1];
+    const float4 v = *(reinterpret_cast<const float4*>(po) + lane);
+    const float top = fmaxf(m, pm0), base = top == -INFINITY ? 0.0f : top;
+    const float a = pt_exp2((m - base) * c), b = pt_exp2((pm0 - base) * c);
+    l = l * a + pl * b;
+    o.x = o.x * a + v.x * b, o.y = o.y * a + v.y * b, o.z = o.z * a + v.z * b, o.w = o.w * a + v.w * b;
+    m = top;
+  }
+  __device__ __forceinline__ void store(uint16_t* row, int lane) const {
+    const float f = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+    const __nv_bfloat162 x = __floats2bfloat162_rn(o.x * f, o.y * f), y = __floats2bfloat162_rn(o.z * f, o.w * f);
+    *(reinterpret_cast<uint2*>(row) + lane) =
+        make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+  }
+};
+
+constexpr int kPtJoinSplit = 8;  // CTAs that share the rows of a cut block
+
+// Prompts: CTA (i, y) joins the block that worker i starts within, when it began in worker i - 1.
+template <bool kPair>
+__global__ void __launch_bounds__(128) pt_join_prompts_kernel(const PtArgs p) {
+  grid_dependency_wait();
+  grid_dependents_launch();
+  const int i = blockIdx.x + 1, lane = threadIdx.x & 31;
+  const PtStart s = p.w.starts[i];
+  const int64_t chunk = p.w.sums->chunk;
+  if (s.count == 0 || s.tile == 0 || s.tile > chunk) return;
+  const PtBlock b = p.w.blocks[s.block];
+  const int64_t begin = i * chunk - s.tile;
+  const int last = static_cast<int>((begin + b.tiles - 1) / chunk);
+  for (int r = blockIdx.y * 4 + (threadIdx.x >> 5); r < b.ntok * p.G; r += 4 * kPtJoinSplit) {
+    const int per = p.TB * p.G, l = r / per, in = r - l * per;  // lane of a pair, its row
+    PtJoin j;
+    for (int w = i - 1; w <= last; ++w) {
+      const int64_t at = ((static_cast<int64_t>(w) * 2 + (w == i - 1)) * (kPair ? 2 : 1) + l) * p.slot_rows + in;
+      j.add(p.w.part + at * kPtRows, p.w.part_ml + at * 2, lane, p.c);
+    }
+    const int t = r / p.G;
+    j.store(p.out + (static_cast<int64_t>(b.tok0 + t) * p.Hq + s.head * p.G + r - t * p.G) * kPtRows, lane);
+  }
+}
+
+// Decode: CTA (request, KV head) joins what the request's own block and its group's left.
+__global__ void __launch_bounds__(128) pt_join_decode_kernel(const PtArgs p) {
+  grid_dependency_wait();
+  grid_dependents_launch();
+  const int b = blockIdx.x, h = blockIdx.y, lane = threadIdx.x & 31;
+  const PtSums sums = *p.w.sums;
+  const int of = p.w.row_block[b];
+  const int own = sums.prefix_blocks + b;
+  const PtBlock mine = p.w.blocks[own];
+  const int64_t begin = p.w.before[own] * p.Hkv + static_cast<int64_t>(h) * mine.tiles;
+  const bool cut = begin / sums.chunk != (begin + mine.tiles - 1) / sums.chunk;
+  if (!cut && mine.key0 == 0) return;  // the attention wrote it
+  for (int g = threadIdx.x >> 5; g < p.G; g += 4) {
+    PtJoin j;
+    const int64_t row = static_cast<int64_t>(b) * p.Hq + h * p.G + g;
+    auto add = [&](int block, const PtBlock& bl, int in, int64_t area) {
+      const int64_t at0 = p.w.before[block] * p.Hkv + static_cast<int64_t>(h) * bl.tiles;
+      const int first = static_cast<int>(at0 / sums.chunk), last = static_cast<int>((at0 + bl.tiles - 1) / sums.chunk);
+      if (first == last) {
+        const int64_t at = area * p.batch * p.Hq + row;
+        j.add(p.w.row + at * kPtRows, p.w.row_ml + at * 2, lane, p.c);
+        return;
+      }
+      for (int w = first; w <= last; ++w) {
+        const int64_t at = (static_cast<int64_t>(w) * 2 + (w == first)) * p.slot_rows + in;
+        j.add(p.w.part + at * kPtRows, p.w.part_ml + at * 2, lane, p.c);
+      }
+    };
+    if (of >= 0) {
+      const PtBlock shared = p.w.blocks[of];
+      add(of, shared, (b - shared.tok0) * p.G + g, 1);
+    }
+    add(own, mine, g, 0);
+    j.store(p.out + row * kPtRows, lane);
+  }
+}
+
+// ------------------------------------------------------------ host side
+struct PtLayout {
+  PtScratch w;
+  int64_t bytes;
+};
+
+// `blocks` an upper bound; `rows` of a slot; `joined` rows of the decode's uncut blocks.
+static PtLayout pt_layout(char* base, int64_t blocks, int64_t batch, int64_t rows, int64_t joined) {
+  PtLayout l;
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    char* q = base + at;
+    at += (bytes + 255) / 256 * 256;
+    return q;
+  };
+  constexpr int64_t kWorkers = 2 * kPtMaxCtas;
+  l.w.sums = reinterpret_cast<PtSums*>(take(sizeof(PtSums)));
+  l.w.starts = reinterpret_cast<PtStart*>(take(kWorkers * sizeof(PtStart)));
+  l.w.blocks = reinterpret_cast<PtBlock*>(take(blocks * sizeof(PtBlock)));
+  l.w.before = reinterpret_cast<int64_t*>(take((blocks + 1) * 8));
+  l.w.row_block = reinterpret_cast<int*>(take(joined ? batch * 4 : 0));
+  l.w.part = reinterpret_cast<float*>(take(kWorkers * 2 * rows * kPtRows * 4));
+  l.w.part_ml = reinterpret_cast<float*>(take(kWorkers * 2 * rows * 8));
+  l.w.row = reinterpret_cast<float*>(take(joined * kPtRows * 4));
+  l.w.row_ml = reinterpret_cast<float*>(take(joined * 8));
+  l.bytes = at;
+  return l;
+}
+
+static int64_t pt_slot_rows(int64_t tokens, int64_t group) {
+  return std::min<int64_t>(tokens, kPtRows / group) * group;
+}
+
+static PtLayout pt_prefill_layout(char* base, int64_t tokens, int64_t batch, int64_t num_heads, int64_t num_kv_heads) {
+  const int64_t group = num_heads / num_kv_heads;
+  return pt_layout(base, tokens / (kPtRows / group) + batch, batch, pt_slot_rows(tokens, group), 0);
+}
+
+static PtLayout pt_shared_layout(char* base, int64_t batch, int64_t groups, int64_t num_heads, int64_t num_kv_heads) {
+  const int64_t group = num_heads / num_kv_heads;
+  return pt_layout(base, batch / (kPtRows / group) + groups + batch, batch, pt_slot_rows(batch, group),
+                   2 * batch * num_heads);
+}
+
+int64_t paged_prefill_attention_workspace_bytes(int64_t tokens, int64_t batch, int64_t num_heads,
+                                                int64_t num_kv_heads) {
+  return pt_prefill_layout(nullptr, tokens, batch, num_heads, num_kv_heads).bytes;
+}
+
+int64_t shared_prefix_attention_workspace_bytes(int64_t batch, int64_t groups, int64_t num_heads,
+                                                int64_t num_kv_heads) {
+  return pt_shared_layout(nullptr, batch, groups, num_heads, num_kv_heads).bytes;
+}
+
+template <bool kPair>
+static int launch_pt(PtArgs& a, const void* k_cache, const void* v_cache, cudaStream_t stream) {
+  static int done[64] = {};
+  auto* kern = &pt_attention_kernel<kPair>;
+  int rc = ensure_smem_attr(reinterpret_cast<const void*>(kern), kPtSmem, done);
+  if (rc != NV4_OK) return rc;
+  const int sms = std::min(device_sm_count(), kPtMaxCtas);
+  if (sms <= 0) return NV4_ERR_CUDA;
+  CUtensorMap maps[2] = {};
+  const uint64_t rows = static_cast<uint64_t>(a.num_pages) * kPtPage, cols = static_cast<uint64_t>(a.Hkv) * kPtRows;
+  if (!make_tensor_map_2d(&maps[0], CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, k_cache, rows, cols, kPtRows, 64,
+                          CU_TENSOR_MAP_SWIZZLE_128B) ||
+      !make_tensor_map_2d(&maps[1], CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, v_cache, rows, cols, kPtRows, 64,
+                          CU_TENSOR_MAP_SWIZZLE_128B))
+    return NV4_ERR_CUDA;
+  a.workers = kPair ? sms : 2 * sms;
+  rc = launch_kernel(pt_plan_kernel, dim3(1), dim3(kPtPlanThreads), 0, stream, true, a, kPair ? 2 * a.TB : a.TB);
+  if (rc != NV4_OK) return rc;
+  rc = launch_kernel(kern, dim3(sms), dim3(kPtThreads), kPtSmem, stream, true, maps[0], maps[1], a);
+  if (rc != NV4_OK) return rc;
+  if (a.prefix == nullptr)
+    return launch_kernel(pt_join_prompts_kernel<kPair>, dim3(a.workers - 1, kPtJoinSplit), dim3(128), 0, stream, true, a);
+  return launch_kernel(pt_join_decode_kernel, dim3(a.batch, a.Hkv), dim3(128), 0, stream, true, a);
+}
+
+static PtArgs pt_args(const void* q, const int* block_tables, const int* context_lens, const int* starts,
+                      const int* prefix, void* out, const PtScratch& w, int64_t tokens, int64_t batch, int64_t groups,
+                      int64_t num_heads, int64_t num_kv_heads, int64_t num_pages, int64_t max_pages, float scale) {
+  PtArgs a;
+  a.q = static_cast<const uint16_t*>(q);
+  a.tables = block_tables;
+  a.context = context_lens;
+  a.starts = starts;
+  a.prefix = prefix;
+  a.out = static_cast<uint16_t*>(out);
+  a.w = w;
+  a.num_pages = num_pages;
+  a.tokens = static_cast<int>(tokens);
+  a.batch = static_cast<int>(batch);
+  a.groups = static_cast<int>(groups);
+  a.Hq = static_cast<int>(num_heads);
+  a.Hkv = static_cast<int>(num_kv_heads);
+  a.G = a.Hq / a.Hkv;
+  a.TB = kPtRows / a.G;
+  a.max_pages = static_cast<int>(max_pages);
+  a.workers = 0;
+  a.slot_rows = static_cast<int>(pt_slot_rows(tokens, a.G));
+  a.c = scale * 1.4426950408889634f;
+  return a;
+}
+
+int launch_paged_prefill_attention(const void* q, const void* k_cache, const void* v_cache, const int* block_tables,
+                                   const int* context_lens, const int* query_starts, void* out, void* workspace,
+                                   int64_t tokens, int64_t batch, int64_t num_heads, int64_t num_kv_heads,
+                                   int64_t num_pages, int64_t max_pages, float scale, cudaStream_t stream) {
+  const PtLayout l = pt_prefill_layout(static_cast<char*>(workspace), tokens, batch, num_heads, num_kv_heads);
+  PtArgs a = pt_args(q, block_tables, context_lens, query_starts, nullptr, out, l.w, tokens, batch, 0, num_heads,
+                     num_kv_heads, num_pages, max_pages, scale);
+  // Two blocks of rows side by side when the requests have more than one block's rows on average.
+  if (tokens > batch * a.TB) return launch_pt<true>(a, k_cache, v_cache, stream);
+  return launch_pt<false>(a, k_cache, v_cache, stream);
+}
+
+int launch_shared_prefix_attention(const void* q, const void* k_cache, const void* v_cache, const int* block_tables,
+                                   const int* context_lens, const int* group_starts, const int* prefix_lens, void* out,
+                                   void* workspace, int64_t batch, int64_t groups, int64_t num_heads,
+                                   int64_t num_kv_heads, int64_t num_pages, int64_t max_pages, float scale,
+                                   cudaStream_t stream) {
+  const PtLayout l = pt_shared_layout(static_cast<char*>(workspace), batch, groups, num_heads, num_kv_heads);
+  // without groups nothing is read through these two
+  const int* prefix = groups > 0 ? prefix_lens : context_lens;
+  PtArgs a = pt_args(q, block_tables, context_lens, group_starts, prefix, out, l.w, batch, batch, groups, num_heads,
+                     num_kv_heads, num_pages, max_pages, scale);
+  return launch_pt<false>(a, k_cache, v_cache, stream);
+}
+
+}  // namespace nv4

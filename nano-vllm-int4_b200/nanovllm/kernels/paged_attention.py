@@ -76,7 +76,8 @@ def shared_prefix_attention(q, k_cache, v_cache, block_tables, context_lens, gro
     INT32 [B] (0: a padding row, whose output is zero).  Requests ``group_starts[g]``
     to ``group_starts[g + 1] - 1`` have ``prefix_lens[g]`` tokens in common (INT32
     [groups + 1], not falling, and [groups]); the whole pages of these are read
-    through the first request's table, and the others' tables must name the same.
+    through the table of the group's longest request, and the others' tables must
+    name the same pages as far as their contexts go.
     Requests of no group share nothing.  Returns ``out`` BF16 [B, Hq, 128].
     """
     return _native.serving().shared_attention(q, k_cache, v_cache, block_tables, context_lens, group_starts,
