@@ -423,7 +423,8 @@ int nv4_append_kv(const void* q, const void* k, const void* v, const void* q_wei
  * Rows of no request are left as they are.  out and workspace overlap no input nor
  * one another.  Values of the request's own later
  * tokens (masked, but in the cache) must be finite; what lies behind its last
- * token may be anything.  At most NV4_PAGED_MAX_GROUP query heads per KV head.
+ * token may be anything.  At most NV4_PAGED_MAX_GROUP query heads per KV head;
+ * (tokens + 2 * batch) * max_pages * num_kv_heads up to 2^36.
  * Statistics and sums in FP32, the probabilities multiplied in two BF16 terms.
  * All pointers 16-byte aligned (the int32 ones 4).
  */

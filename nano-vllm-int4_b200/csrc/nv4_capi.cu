@@ -95,6 +95,17 @@ bool make_tensor_map_2d(CUtensorMap* map, CUtensorMapDataType dtype, int elem_by
   return r == CUDA_SUCCESS;
 }
 
+// 3-D tensor map of 16-bit elements: dims innermost first, strides (bytes) of the outer two.
+bool make_tensor_map_3d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, const uint64_t (&dims)[3],
+                        const uint64_t (&strides)[2], const uint32_t (&box)[3], CUtensorMapSwizzle swizzle) {
+  EncodeTiledFn enc = encode_fn();
+  if (!enc) return false;
+  const cuuint64_t d[3] = {dims[0], dims[1], dims[2]}, st[2] = {strides[0], strides[1]};
+  const cuuint32_t bx[3] = {box[0], box[1], box[2]}, estr[3] = {1, 1, 1};
+  return enc(map, dtype, 3, const_cast<void*>(base), d, st, bx, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 bool make_tensor_map_u8(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols_bytes, uint32_t box_rows,
                         uint32_t box_cols_bytes, CUtensorMapSwizzle swizzle) {
   return make_tensor_map_2d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, base, rows, cols_bytes, box_rows, box_cols_bytes,
@@ -578,6 +589,8 @@ int check_paged_attention(const void* q, const void* k_cache, const void* v_cach
     return NV4_ERR_INVALID_ARGUMENT;
   if (head_dim != 128 || page_size != 256 || num_heads / num_kv_heads > NV4_PAGED_MAX_GROUP)
     return NV4_ERR_UNSUPPORTED;
+  // key tiles of all blocks of rows and heads: a worker counts its share in 32 bits
+  if ((rows + 2 * batch) * max_pages > (int64_t(1) << 36) / num_kv_heads) return NV4_ERR_UNSUPPORTED;
   if (workspace_bytes < wanted) return NV4_ERR_INVALID_ARGUMENT;
   if (!aligned(q, 16) || !aligned(k_cache, 16) || !aligned(v_cache, 16) || !aligned(out, 16) ||
       !aligned(workspace, 16) || !aligned(block_tables, 4) || !aligned(context_lens, 4))

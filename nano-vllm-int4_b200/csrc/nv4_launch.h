@@ -53,6 +53,9 @@ bool make_tensor_map_u8(CUtensorMap* map, const void* base, uint64_t rows, uint6
 bool make_tensor_map_2d(CUtensorMap* map, CUtensorMapDataType dtype, int elem_bytes, const void* base, uint64_t rows,
                         uint64_t cols, uint32_t box_rows, uint32_t box_cols, CUtensorMapSwizzle swizzle);
 
+bool make_tensor_map_3d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, const uint64_t (&dims)[3],
+                        const uint64_t (&strides)[2], const uint32_t (&box)[3], CUtensorMapSwizzle swizzle);
+
 // ---- launchers (one per kernel family) ----
 // Activation prep; `packed` and/or `codes8` (GEMM-ready INT8 layout) receive the codes.
 int launch_rht_quant(const void* x, const void* signs, void* packed, void* codes8, void* scale, int64_t m, int64_t k,

@@ -30,7 +30,7 @@
 //   warp 0     copies K and V tiles (TMA, five slots of 32 KB) in the order of use
 //   warp 1     issues S = Q K^T, O += P V;  V rows behind the last token of a request
 //              are cleared first (0 times an old NaN would be one)
-//   warps 2-3  bring the rows of Q to shared memory (a gather: cp.async)
+//   warps 2-3  copy the rows of Q of their lane (TMA: [tokens][G heads][128 channels])
 //   warps 4-11 softmax of the two lanes; outputs
 // P goes back to TMEM over its scores in two BF16 terms (the upper 16 bits of the FP32
 // value and the rest, 2^-15 of it at most left out), so that the output's own rounding
@@ -45,7 +45,7 @@ namespace nv4 {
 constexpr int kPtRows = 128;    // rows of a block, keys of a tile, head_dim
 constexpr int kPtPage = 256;
 constexpr int kPtMaxCtas = 160;
-constexpr int kPtThreads = 384;
+constexpr int kPtThreads = 384;  // three warpgroups: copies and products, softmax of the two lanes
 constexpr int kPtTile = kPtRows * kPtRows * 2;  // bytes of a Q, K or V tile
 constexpr int kPtHalf = kPtTile / 2;            // 64 channels of it: [128 rows][128 bytes], 128-byte swizzle
 constexpr int kPtSlots = 5;
@@ -69,8 +69,7 @@ struct __align__(16) PtBlock {
 
 // Where a worker starts, and how many tiles it takes.
 struct __align__(16) PtStart {
-  int block, head, tile, pad;
-  int64_t count, pad2;
+  int block, head, tile, count;
 };
 
 struct PtSums {
@@ -297,29 +296,44 @@ __global__ void __launch_bounds__(kPtPlanThreads) pt_plan_kernel(const PtArgs p,
   }
 
   const int64_t total = tiles_before * p.Hkv;
-  const int64_t chunk = max((total + p.workers - 1) / p.workers, static_cast<int64_t>(1));
+  const bool small = total < (int64_t(1) << 30);  // 64-bit divisions take microseconds here
+  int64_t chunk = small ? (static_cast<uint32_t>(total) + p.workers - 1) / static_cast<uint32_t>(p.workers)
+                        : (total + p.workers - 1) / p.workers;
+  if (chunk < 1) chunk = 1;
   if (tid == 0) {
     p.w.before[blocks] = tiles_before;
     *p.w.sums = PtSums{total, chunk, blocks, prefix_blocks};
   }
   __syncthreads();
-  const int64_t* before = blocks <= kPtPlanCached ? cached : p.w.before;
+  const bool in_smem = blocks <= kPtPlanCached;
   for (int w = tid; w < p.workers; w += kPtPlanThreads) {
-    PtStart s{0, 0, 0, 0, 0, 0};
+    PtStart s{0, 0, 0, 0};
     const int64_t at = w * chunk;
-    s.count = max(min(total - at, chunk), static_cast<int64_t>(0));
+    s.count = static_cast<int>(max(min(total - at, chunk), static_cast<int64_t>(0)));
     if (s.count > 0) {
       int lo = 0, hi = blocks - 1;  // the last block whose tiles start at or before `at`
-      while (lo < hi) {
-        const int mid = (lo + hi + 1) / 2;
-        if (before[mid] * p.Hkv <= at) lo = mid;
-        else hi = mid - 1;
+      if (small && in_smem) {
+        while (lo < hi) {
+          const int mid = (lo + hi + 1) / 2;
+          if (static_cast<int>(cached[mid]) * p.Hkv <= static_cast<int>(at)) lo = mid;
+          else hi = mid - 1;
+        }
+        const uint32_t into = static_cast<uint32_t>(at) - static_cast<uint32_t>(cached[lo]) * p.Hkv;
+        const uint32_t tiles = static_cast<uint32_t>((lo + 1 < blocks ? cached[lo + 1] : tiles_before) - cached[lo]);
+        s.head = static_cast<int>(into / tiles);
+        s.tile = static_cast<int>(into % tiles);
+      } else {
+        while (lo < hi) {
+          const int mid = (lo + hi + 1) / 2;
+          if (p.w.before[mid] * p.Hkv <= at) lo = mid;
+          else hi = mid - 1;
+        }
+        const int64_t into = at - p.w.before[lo] * p.Hkv;
+        const int tiles = p.w.blocks[lo].tiles;
+        s.head = static_cast<int>(into / tiles);
+        s.tile = static_cast<int>(into % tiles);
       }
-      const int64_t into = at - before[lo] * p.Hkv;
-      const int tiles = p.w.blocks[lo].tiles;
       s.block = lo;
-      s.head = static_cast<int>(into / tiles);
-      s.tile = static_cast<int>(into % tiles);
     }
     p.w.starts[w] = s;
   }
@@ -331,22 +345,33 @@ __host__ __device__ constexpr uint32_t pt_idesc(int m, int n, bool b_mn) {
   return (1u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(b_mn) << 16) |
          (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
 }
-// Descriptor of V as the B operand: N (channels) contiguous in 128-byte rows, keys the rows; eight keys are an atom of
-// 1024 bytes (stride offset), the second 64 channels lie a half tile on (leading offset).
-__device__ __forceinline__ uint64_t pt_desc_v(uint32_t addr) {
-  return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | (static_cast<uint64_t>(kPtHalf >> 4) << 16) |
-         (static_cast<uint64_t>(1024u >> 4) << 32) | (static_cast<uint64_t>(1u) << 46) |
-         (static_cast<uint64_t>(2u) << 61);
-}
-__device__ __forceinline__ void pt_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+// Shared-memory descriptors, lower words (address and leading offset, in 16 bytes); the upper word is the same for both:
+// eight rows of 128 bytes are an atom of 1024 (stride offset), 128-byte swizzle.  Q and K have their channels
+// contiguous (K-major; the leading offset counts for nothing), V as the B operand its N dimension: the second 64
+// channels lie a half tile on (leading offset).
+constexpr uint32_t kPtDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+constexpr uint32_t kPtDescK = 1u << 16, kPtDescV = static_cast<uint32_t>(kPtHalf >> 4) << 16;
+constexpr uint32_t kPtHalfLo = kPtHalf >> 4;
+__device__ __forceinline__ void pt_mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      "{\n .reg .pred p;\n .reg .b64 a, b;\n setp.ne.u32 p, %4, 0;\n mov.b64 a, {%1, %5};\n mov.b64 b, {%2, %5};\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "n"(kPtDescHi)
       : "memory");
 }
-__device__ __forceinline__ void pt_cp_async16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+// A in tensor memory
+__device__ __forceinline__ void pt_mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n .reg .b64 b;\n setp.ne.u32 p, %4, 0;\n mov.b64 b, {%2, %5};\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "n"(kPtDescHi)
+      : "memory");
+}
+__device__ __forceinline__ void pt_load_q(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+      ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+      : "memory");
 }
 __device__ __forceinline__ float pt_exp2(float x) {
   float y;
@@ -354,18 +379,43 @@ __device__ __forceinline__ float pt_exp2(float x) {
   return y;
 }
 
-// The tiles of a worker, in order.
+__device__ __forceinline__ void pt_tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+
+// Values of a TMEM load: not used before the wait in front of this.
+__device__ __forceinline__ void pt_pin(uint32_t (&v)[16]) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) asm volatile("" : "+r"(v[i]));
+}
+
+// Registers: 384 threads are launched with 168; the softmax holds a row's 128 scores (216 a thread), what the first
+// warpgroup gives up (72) covers it: 72 + 2 * 216 = 3 * 168.
+__device__ __forceinline__ void pt_registers_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 72;"); }
+__device__ __forceinline__ void pt_registers_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 216;"); }
+
+// The tiles of a worker, in order.  The next block's record is loaded a block ahead.
 struct PtWalk {
   const PtBlock* blocks;
   PtBlock b;
+  int4 ahead[2];
   int block, head, tile, heads;
-  int64_t left;  // the current one included
-  bool fresh;    // the current tile is the first of this worker in its block and head
+  int left;    // the current one included
+  bool fresh;  // the current tile is the first of this worker in its block and head
 
-  __device__ __forceinline__ void load() {
-    const int4* src = reinterpret_cast<const int4*>(blocks + block);
-    const int4 x = src[0], y = src[1];  // not the read-only path: the kernel before wrote them
+  __device__ __forceinline__ void take() {
+    const int4 x = ahead[0], y = ahead[1];
     b = PtBlock{x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+    fetch(block + 1);
+  }
+  __device__ __forceinline__ void fetch(int i) {  // not the read-only path: the kernel before wrote them
+    const int4* src = reinterpret_cast<const int4*>(blocks + i);
+    ahead[0] = src[0], ahead[1] = src[1];
   }
   __device__ __forceinline__ void start(const PtArgs& p, int worker) {
     const PtStart s = p.w.starts[worker];
@@ -373,7 +423,17 @@ struct PtWalk {
     block = s.block, head = s.head, tile = s.tile, heads = p.Hkv;
     left = s.count;
     fresh = true;
-    if (left > 0) load();
+    if (left > 0) {
+      fetch(block);
+      take();
+    }
+  }
+  // To the first tile of the next block and head.
+  __device__ __forceinline__ void skip() {
+    const int n = min(b.tiles - tile, left);
+    tile += n - 1;
+    left -= n - 1;
+    next();
   }
   __device__ __forceinline__ bool last() const { return tile + 1 == b.tiles || left == 1; }  // of this worker in it
   __device__ __forceinline__ void next() {
@@ -384,14 +444,49 @@ struct PtWalk {
     if (++head == heads) {
       head = 0;
       ++block;
-      if (left > 0) load();
+      if (left > 0) take();
+    }
+  }
+};
+
+// The same for the products, which need less of a block.
+struct PtSteps {
+  const PtBlock* blocks;
+  int block, head, tile, heads, left, tiles, ntok, ahead_tiles, ahead_ntok;
+  bool fresh;
+
+  __device__ __forceinline__ void take() {
+    tiles = ahead_tiles, ntok = ahead_ntok;
+    ahead_tiles = blocks[block + 1].tiles, ahead_ntok = blocks[block + 1].ntok;
+  }
+  __device__ __forceinline__ void start(const PtArgs& p, int worker) {
+    const PtStart s = p.w.starts[worker];
+    blocks = p.w.blocks;
+    block = s.block, head = s.head, tile = s.tile, heads = p.Hkv, left = s.count;
+    fresh = true;
+    tiles = ntok = 1;
+    if (left > 0) {
+      ahead_tiles = blocks[block].tiles, ahead_ntok = blocks[block].ntok;
+      take();
+    }
+  }
+  __device__ __forceinline__ bool last() const { return tile + 1 == tiles || left == 1; }
+  __device__ __forceinline__ void next() {
+    fresh = ++tile == tiles;
+    --left;
+    if (!fresh) return;
+    tile = 0;
+    if (++head == heads) {
+      head = 0;
+      ++block;
+      if (left > 0) take();
     }
   }
 };
 
 struct PtBars {
   uint64_t full[kPtSlots], empty[kPtSlots];
-  uint64_t q_full[2], q_free[2], s_full[2], p_full[2], o_full[2], done;
+  uint64_t q_full[2], q_free[2], s_full[2], p_half[2], p_full[2], o_full[2], done;
   uint32_t tmem;
   int slot_keys[kPtSlots];  // keys of the slot's tile that exist
   int lane_keys[2];         // of the tile whose scores lie in the lane
@@ -402,12 +497,13 @@ static_assert(sizeof(PtBars) <= 512, "barriers");
 template <bool kPair>
 __global__ void __launch_bounds__(kPtThreads, 1)
     pt_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
+                        const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_q1,
                         const PtArgs p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + (((smem_u32(smem_raw) + 1023u) & ~1023u) - smem_u32(smem_raw));
   uint8_t* ring = smem + 2 * kPtTile;
   PtBars& bar = *reinterpret_cast<PtBars*>(smem + kPtBar);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kPtSlots; ++s) mbar_init(&bar.full[s], 1), mbar_init(&bar.empty[s], 1);
@@ -415,7 +511,8 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       mbar_init(&bar.q_full[i], 1);
       mbar_init(&bar.q_free[i], 1);
       mbar_init(&bar.s_full[i], 2);  // the products' completion, and lane_keys
-      mbar_init(&bar.p_full[i], 4);  // the warps of the lane
+      mbar_init(&bar.p_half[i], 4);  // the warps of the lane
+      mbar_init(&bar.p_full[i], 4);
       mbar_init(&bar.o_full[i], 1);
     }
     mbar_init(&bar.done, 1);
@@ -428,16 +525,17 @@ __global__ void __launch_bounds__(kPtThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = bar.tmem;
+  const uint32_t tmem = 0;  // all 512 columns are this CTA's: they start at 0
   grid_dependency_wait();  // the block table, and q, from the kernels before
   grid_dependents_launch();
 
   // Worker of a lane; in a pair both lanes walk worker blockIdx.x.
   auto worker = [&](int l) { return static_cast<int>(blockIdx.x) + (kPair ? 0 : l * static_cast<int>(gridDim.x)); };
-  // Does lane l have rows of block b?
+  // Does lane l have rows of block b?  (A pair's second lane: those of the tokens behind the first TB.)
   auto has_rows = [&](int l, const PtBlock& b) { return !kPair || l == 0 || b.ntok > p.TB; };
   bool ok = true;
 
+  if (warp < 4) pt_registers_down();
   if (warp == 0) {
     // ---------------- copies of K and V
     if (lane == 0) {
@@ -505,113 +603,111 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       }
     }
   } else if (warp == 1) {
-    // ---------------- products; the whole warp walks, lane 0 issues
+    // ---------------- products; the whole warp walks, lane 0 issues.  The lanes of the CTA take turns (O += P V of a tile,
+    // then S of the next), in one copy of the code: the softmax streams through the instruction caches beside it.
     constexpr uint32_t kQk = pt_idesc(kPtRows, kPtRows, false), kPv = pt_idesc(kPtRows, kPtRows, true);
-    int c = 0;                         // ring position
-    int tiles[2] = {0, 0};             // products S of the lane so far
-    int parts[2] = {0, 0};             // blocks of the lane so far
-    bool started[2] = {false, false};  // O holds something of the current block
-    // S = Q K^T of the tile in ring position c
-    auto arrived = [&](uint64_t& b, int phase) {  // the same answer in every lane
+    const uint32_t q_lo = (smem_u32(smem) >> 4) + kPtDescK, ring_lo = smem_u32(ring) >> 4;
+    struct Turn {
+      PtSteps w;
+      int l, c;           // lane; ring position (of a pair; else both count in one)
+      uint32_t tiles, parts;  // S products, blocks so far
+      bool begun, started;    // S of the current tile is issued; O holds something of the current block
+    };
+    Turn me, other;
+    me.w.start(p, worker(0)), other.w.start(p, worker(1));
+    me.l = 0, other.l = 1;
+    me.c = other.c = 0;
+    me.tiles = other.tiles = me.parts = other.parts = 0;
+    me.begun = other.begun = me.started = other.started = false;
+    auto arrived = [&](uint64_t& b, uint32_t phase) {  // the same answer in every lane
       return __all_sync(0xffffffffu, mbar_wait(&b, phase & 1, kErrTimeoutMma)) != 0;
     };
-    auto scores = [&](int l, const PtWalk& w, bool release) {
-      const int s = c % kPtSlots;
-      if (!arrived(bar.full[s], c / kPtSlots)) return false;
-      if (w.fresh && !arrived(bar.q_full[l], parts[l]++)) return false;
-      tc_fence_after();
-      if (lane == 0) {
-        bar.lane_keys[l] = bar.slot_keys[s];  // before the slot can be released
-        const uint32_t qa = smem_u32(smem + l * kPtTile), ka = smem_u32(ring + s * kPtTile);
+    // Does the lane have rows in its current block?  The last of a pair's lanes that does releases the slots.
+    auto rows = [&]() { return !kPair || me.l == 0 || me.w.ntok > p.TB; };
+    auto releases = [&]() { return !kPair || me.l == 1 || me.w.ntok <= p.TB; };
+    while (ok && me.w.left > 0) {
+      const int l = me.l;
+      if (me.begun) {
+        if (rows()) {  // O += P V
+          const int s = me.c % kPtSlots;
+          ok = arrived(bar.full[s], me.c / kPtSlots) && arrived(bar.p_half[l], me.tiles - 1);
+          if (!ok) break;
+          tc_fence_after();
+          const int keys = bar.slot_keys[s], steps = (keys + 15) / 16;
+          if (keys & 15) {  // rows behind the last key: P is zero there, V may be anything
+            for (int i = lane; i < (steps * 16 - keys) * 16; i += 32)
+              *reinterpret_cast<uint4*>(ring + s * kPtTile + (i & 8 ? kPtHalf : 0) + (keys + (i >> 4)) * 128 +
+                                        (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+            fence_proxy_async_smem();
+          }
+          if (me.w.fresh) me.started = false;
+          const uint32_t va = ring_lo + s * (kPtTile >> 4) + kPtDescV, o = l * 256 + 128;
+          // 16 keys: their two terms of P against the same rows of V
+          auto step = [&](int k, uint32_t accumulate) {
+            const uint32_t pk = l * 256 + (k >> 1) * 32 + (k & 1) * 8;
+            pt_mma_ts(o, pk, va + k * 128, kPv, accumulate);
+            pt_mma_ts(o, pk + 16, va + k * 128, kPv, 1);
+          };
+          __syncwarp();
+          if (lane == 0) {
+            if (steps >= 4) {
+              step(0, me.started);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const uint32_t off = (j >> 2) * kPtHalf + (j & 3) * 32;
-          pt_mma_ss(tmem + l * 256, umma_desc_sw128(qa + off), umma_desc_sw128(ka + off), kQk, j > 0);
-        }
-        if (release) umma_commit(&bar.empty[s]);
-        if (w.last()) umma_commit(&bar.q_free[l]);
-        umma_commit(&bar.s_full[l]);
-        mbar_arrive(&bar.s_full[l]);
-      }
-      __syncwarp();
-      ++tiles[l];
-      return true;
-    };
-    // O += P V
-    auto values = [&](int l, const PtWalk& w, bool release) {
-      const int s = c % kPtSlots;
-      if (!arrived(bar.full[s], c / kPtSlots) || !arrived(bar.p_full[l], tiles[l] - 1)) return false;
-      tc_fence_after();
-      const int keys = bar.slot_keys[s], steps = (keys + 15) / 16;
-      __syncwarp();  // all have read it before the slot can be released
-      uint8_t* v = ring + s * kPtTile;
-      if (keys & 15) {  // rows behind the last key: P is zero there, V may be anything
-        for (int i = lane; i < (steps * 16 - keys) * 16; i += 32)
-          *reinterpret_cast<uint4*>(v + (i & 8 ? kPtHalf : 0) + (keys + (i >> 4)) * 128 + (i & 7) * 16) =
-              make_uint4(0, 0, 0, 0);
-        fence_proxy_async_smem();
-        __syncwarp();
-      }
-      if (w.fresh) started[l] = false;
-      if (lane == 0) {
-        const uint32_t o = tmem + l * 256 + 128, pt = tmem + l * 256, va = smem_u32(v);
-        for (int k = 0; k < steps; ++k) {
-          const uint64_t desc = pt_desc_v(va + k * 2048);
-          const uint32_t pk = pt + (k >> 2) * 64 + (k & 3) * 8;
-          umma_bf16_ts(o, pk, desc, kPv, started[l] || k > 0);
-          umma_bf16_ts(o, pk + 32, desc, kPv, 1);
-        }
-        if (release) umma_commit(&bar.empty[s]);
-        if (w.last()) umma_commit(&bar.o_full[l]);
-      }
-      started[l] = started[l] || steps > 0;
-      __syncwarp();
-      return true;
-    };
-    if constexpr (kPair) {
-      PtWalk w;
-      w.start(p, worker(0));
-      if (w.left > 0) {
-        const bool two = has_rows(1, w.b);
-        ok = scores(0, w, !two) && (!two || scores(1, w, true));
-        ++c;
-      }
-      while (ok && w.left > 0) {
-        // ring: V of this tile, then K of the next
-        const bool two = has_rows(1, w.b);
-        PtWalk n = w;
-        n.next();
-        const bool more = n.left > 0, two_next = more && has_rows(1, n.b);
-        ok = values(0, w, !two);
-        if (ok && more) {
-          ++c;
-          ok = scores(0, n, !two_next);
-          --c;
-        }
-        if (ok && two) ok = values(1, w, true);
-        ++c;
-        if (ok && two_next) ok = scores(1, n, true);
-        if (more) ++c;
-        w = n;
-      }
-    } else {
-      PtWalk w[2];
+              for (int k = 1; k < 4; ++k) step(k, 1);
+            } else {
+              for (int k = 0; k < steps; ++k) step(k, me.started || k > 0);
+            }
+          }
+          __syncwarp();
+          ok = arrived(bar.p_full[l], me.tiles - 1);
+          if (!ok) break;
+          tc_fence_after();
+          if (lane == 0) {
+            if (steps == 8) {
 #pragma unroll
-      for (int l = 0; l < 2; ++l) {
-        w[l].start(p, worker(l));
-        if (w[l].left > 0 && ok) ok = scores(l, w[l], true), ++c;
-      }
-      while (ok && w[0].left > 0) {
-#pragma unroll
-        for (int l = 0; l < 2; ++l) {
-          if (!ok || w[l].left == 0) continue;
-          ok = values(l, w[l], true);
-          ++c;
-          w[l].next();
-          if (!ok || w[l].left == 0) continue;
-          ok = scores(l, w[l], true);
-          ++c;
+              for (int k = 4; k < 8; ++k) step(k, 1);
+            } else {
+              for (int k = 4; k < steps; ++k) step(k, 1);
+            }
+            if (releases()) umma_commit(&bar.empty[s]);
+            if (me.w.last()) umma_commit(&bar.o_full[l]);
+          }
+          __syncwarp();
+          me.started = me.started || steps > 0;
         }
+        ++me.c;
+        me.w.next();
+      }
+      me.begun = true;
+      if (me.w.left > 0) {
+        if (rows()) {  // S = Q K^T
+          const int s = me.c % kPtSlots;
+          ok = arrived(bar.full[s], me.c / kPtSlots);
+          if (ok && me.w.fresh) ok = arrived(bar.q_full[l], me.parts++);
+          if (!ok) break;
+          tc_fence_after();
+          if (lane == 0) {
+            bar.lane_keys[l] = bar.slot_keys[s];  // before the slot can be released
+            const uint32_t qa = q_lo + l * (kPtTile >> 4), ka = ring_lo + s * (kPtTile >> 4) + kPtDescK;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const uint32_t off = (j >> 2) * kPtHalfLo + (j & 3) * 2;
+              pt_mma_ss(l * 256, qa + off, ka + off, kQk, j > 0);
+            }
+            umma_commit(&bar.s_full[l]);
+            mbar_arrive(&bar.s_full[l]);
+            if (releases()) umma_commit(&bar.empty[s]);
+            if (me.w.last()) umma_commit(&bar.q_free[l]);
+          }
+          __syncwarp();
+          ++me.tiles;
+        }
+        ++me.c;
+      }
+      if (other.w.left > 0 || kPair) {
+        if (!kPair) other.c = me.c;
+        const Turn t = me;
+        me = other, other = t;
       }
     }
     if (lane == 0) {  // all issued products must finish before the TMEM is released
@@ -625,44 +721,42 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     }
     __syncwarp();
   } else if (warp < 4) {
-    // ---------------- rows of Q: row r of a lane is head r % G of its token r / G
-    const int l = warp - 2;
-    uint8_t* dst = smem + l * kPtTile;
-    PtWalk w;
-    w.start(p, worker(l));
-    int part = 0;
-    while (ok && w.left > 0) {
-      if (w.fresh && has_rows(l, w.b)) {
-        if (part > 0) ok = __all_sync(0xffffffffu, mbar_wait(&bar.q_free[l], (part - 1) & 1, kErrTimeoutEmpty));
-        if (!ok) break;
-        const int t0 = kPair ? l * p.TB : 0;
-        const int rows = min(w.b.ntok - t0, p.TB) * p.G;
-        const uint16_t* src = p.q + (static_cast<int64_t>(w.b.tok0 + t0) * p.Hq + w.head * p.G) * kPtRows;
-        for (int i = lane; i < rows * 16; i += 32) {
-          const int r = i >> 4, ch = i & 15, t = r / p.G;
-          pt_cp_async16(smem_u32(dst) + (ch >> 3) * kPtHalf + sw128_offset(r, ch & 7),
-                        src + (static_cast<int64_t>(t) * p.Hq + (r - t * p.G)) * kPtRows + ch * 8);
-        }
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bar.q_full[l]);
+    // ---------------- rows of Q.  The box takes as many tokens as a block can have; rows behind the block's last are
+    // never used.
+    if (lane == 0) {
+      const int l = warp - 2;
+      uint8_t* dst = smem + l * kPtTile;
+      PtWalk w;
+      w.start(p, worker(l));
+      int part = 0;
+      for (; w.left > 0; w.skip()) {
+        if (!has_rows(l, w.b)) continue;
+        if (part > 0 && !mbar_wait(&bar.q_free[l], (part - 1) & 1, kErrTimeoutEmpty)) break;
+        const bool one = w.b.kind == kPtOwn;
+        const CUtensorMap* map = one ? &tmap_q1 : &tmap_q;
+        const int token = w.b.tok0 + (kPair ? l * p.TB : 0);
+        mbar_arrive_expect_tx(&bar.q_full[l], (one ? 1 : p.TB) * p.G * kPtRows * 2);
+        pt_load_q(dst, map, &bar.q_full[l], 0, w.head * p.G, token);
+        pt_load_q(dst + kPtHalf, map, &bar.q_full[l], 64, w.head * p.G, token);
         ++part;
       }
-      // to the first tile of the next block
-      const int64_t skip = min(static_cast<int64_t>(w.b.tiles - w.tile), w.left);
-      w.tile += static_cast<int>(skip) - 1;
-      w.left -= skip - 1;
-      w.next();
+      if (part > 0) {  // the last copy must land before the CTA may exit
+        const uint64_t start = global_timer_ns();
+        while (!mbar_try_wait(&bar.q_full[l], (part - 1) & 1))
+          if (global_timer_ns() - start > kWaitLimitNs) {
+            record_error(kErrTimeoutDrain);
+            break;
+          }
+      }
     }
   } else {
-    // ---------------- softmax and outputs: thread = row
-    const int l = (warp - 4) >> 2, r = threadIdx.x & 127;
-    const uint32_t at = tmem + l * 256 + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    // ---------------- softmax and outputs: thread = row (head r % G of its lane's token r / G)
+    pt_registers_up();
+    const int l = (warp - 4) >> 2, quarter = warp & 3, r = quarter * 32 + lane;
+    const uint32_t at = tmem + l * 256 + (static_cast<uint32_t>(quarter * 32) << 16);
     const float c = p.c;
     PtWalk w;
     w.start(p, worker(l));
-    int64_t part_rows = 0;
     int tile = 0, part = 0, limit = 0, token = 0, head = 0, from = 0;
     bool live = false, started = false;
     float m = -INFINITY, sum = 0.0f;
@@ -688,74 +782,95 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       if (busy && keys > 0) {
         const int seen = min(max(limit - (w.b.key0 + w.tile * kPtRows), 0), keys);
         const bool edge = __any_sync(0xffffffffu, seen < kPtRows);
-        // scores of keys 64 half .. 64 half + 63; those that the row does not see as -inf
-        auto fetch = [&](int half, uint32_t (&s)[64]) {
-          tmem_ld32(at + 64 * half, s);
-          tmem_ld32(at + 64 * half + 32, s + 32);
-          tmem_wait_ld();
-          if (edge) {
+        uint32_t s[kPtRows];
 #pragma unroll
-            for (int j = 0; j < 64; ++j) s[j] = 64 * half + j < seen ? s[j] : 0xFF800000u;
-          }
-        };
-        uint32_t s[64];
-        float top = -INFINITY;
+        for (int i = 0; i < 4; ++i) tmem_ld32(at + 32 * i, s + 32 * i);
+        tmem_wait_ld();
+        if (edge) {  // what the row does not see
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          fetch(half, s);
-#pragma unroll
-          for (int j = 0; j < 64; j += 2)
-            top = fmaxf(top, fmaxf(__uint_as_float(s[j]), __uint_as_float(s[j + 1])));
+          for (int j = 0; j < kPtRows; ++j) s[j] = j < seen ? s[j] : 0xFF800000u;
         }
+        float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int j = 0; j < kPtRows; j += 8)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            t[i] = fmaxf(t[i], fmaxf(__uint_as_float(s[j + 2 * i]), __uint_as_float(s[j + 2 * i + 1])));
+        const float top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
         const bool move = top > m && (m == -INFINITY || (top - m) * c > kPtSlack);
         if (__any_sync(0xffffffffu, move) && started) {
           const float f = move ? pt_exp2((m - top) * c) : 1.0f;
           sum *= f;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint32_t o[32];
-            tmem_ld32(at + 128 + 32 * i, o);
+#pragma unroll 1
+          for (int i = 0; i < 8; ++i) {
+            uint32_t o[16];
+            tmem_ld16(at + 128 + 16 * i, o);
             tmem_wait_ld();
 #pragma unroll
-            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
-            tmem_st32(at + 128 + 32 * i, o);
+            for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+            pt_tmem_st16(at + 128 + 16 * i, o);
           }
         }
         if (move) m = top;
         const float base = m == -INFINITY ? 0.0f : m;
         const uint64_t base2 = pair(base, base), c2 = pair(c, c);
-        uint64_t sums = 0;
-        // 64 keys' probabilities take the columns of their scores: 32 of the upper terms, 32 of the lower
+        uint64_t sums[2] = {0, 0};
+        // 32 keys' probabilities take the columns of their scores: 16 of the upper terms, 16 of the lower.  Rolled, and the
+        // scores loaded again, 16 columns ahead: straight-line code of a whole tile does not stay in the instruction
+        // caches, for this warp and for the one that issues the products.
+        uint32_t va[16], vb[16], hi[16], lo[16];
+        auto probabilities = [&](uint32_t (&v)[16], int here, uint32_t* h, uint32_t* lw) {
+          if (edge) {
 #pragma unroll
-        for (int half = 1; half >= 0; --half) {
-          if (half == 0) fetch(0, s);
-          uint32_t hi[32], lo[32];
+            for (int j = 0; j < 16; ++j) v[j] = j < here ? v[j] : 0xFF800000u;
+          }
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
+          for (int j = 0; j < 8; ++j) {
             float x, y;
-            unpair(mul2(sub2(pair(__uint_as_float(s[2 * j]), __uint_as_float(s[2 * j + 1])), base2), c2), x, y);
+            unpair(mul2(sub2(pair(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1])), base2), c2), x, y);
             x = pt_exp2(x), y = pt_exp2(y);
             const uint64_t e = pair(x, y);
-            sums = add2(sums, e);
+            sums[j & 1] = add2(sums[j & 1], e);
             const uint32_t xb = __float_as_uint(x), yb = __float_as_uint(y);
-            hi[j] = __byte_perm(xb, yb, 0x7632);
-            float u, v;
-            unpair(sub2(e, pair(__uint_as_float(xb & 0xFFFF0000u), __uint_as_float(yb & 0xFFFF0000u))), u, v);
-            const __nv_bfloat162 rest = __floats2bfloat162_rn(u, v);
-            lo[j] = *reinterpret_cast<const uint32_t*>(&rest);
+            h[j] = __byte_perm(xb, yb, 0x7632);
+            float u, w;
+            unpair(sub2(e, pair(__uint_as_float(xb & 0xFFFF0000u), __uint_as_float(yb & 0xFFFF0000u))), u, w);
+            const __nv_bfloat162 rest = __floats2bfloat162_rn(u, w);
+            lw[j] = *reinterpret_cast<const uint32_t*>(&rest);
           }
-          tmem_st32(at + 64 * half, hi);
-          tmem_st32(at + 64 * half + 32, lo);
+        };
+        tmem_ld16(at, va);
+#pragma unroll 1
+        for (int i = 0; i < 4; ++i) {
+          tmem_wait_ld();
+          pt_pin(va);
+          tmem_ld16(at + 32 * i + 16, vb);
+          probabilities(va, seen - 32 * i, hi, lo);
+          tmem_wait_ld();
+          pt_pin(vb);
+          if (i < 3) tmem_ld16(at + 32 * i + 32, va);
+          probabilities(vb, seen - 32 * i - 16, hi + 8, lo + 8);
+          pt_tmem_st16(at + 32 * i, hi);
+          pt_tmem_st16(at + 32 * i + 16, lo);
+          if (i == 1) {  // the products with the first 64 keys may begin
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar.p_half[l]);
+          }
         }
         float x, y;
-        unpair(sums, x, y);
+        unpair(add2(sums[0], sums[1]), x, y);
         sum += x + y;
         tmem_wait_st();
       }
       started = started || keys > 0;
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bar.p_full[l]);
+      if (lane == 0) {
+        if (!busy || keys == 0) mbar_arrive(&bar.p_half[l]);
+        mbar_arrive(&bar.p_full[l]);
+      }
       ++tile;
       if (!w.last()) continue;
 
@@ -769,17 +884,20 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       if (busy) {
         const float f = final_ ? (sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f) : 1.0f;
         const int64_t row = static_cast<int64_t>(token) * p.Hq + head;
-        float* po;
+        // FP32 outputs: of a block that is not cut row after row (for the joining kernel); of a cut one with the rows
+        // beside each other, 16 bytes each, so that a warp's stores are contiguous
+        float4* po;
         float* pm;
+        int stride;
         if (whole) {
           const int64_t i = (w.b.kind == kPtPrefix ? static_cast<int64_t>(p.batch) * p.Hq : 0) + row;
-          po = p.w.row + i * kPtRows, pm = p.w.row_ml + i * 2;
+          po = reinterpret_cast<float4*>(p.w.row) + i * 32, pm = p.w.row_ml + i * 2, stride = 1;
         } else {
-          part_rows = (static_cast<int64_t>(worker(l)) * 2 + (from == 0)) * (kPair ? 2 : 1) + (kPair ? l : 0);
-          const int64_t i = part_rows * p.slot_rows + r;
-          po = p.w.part + i * kPtRows, pm = p.w.part_ml + i * 2;
+          const int64_t slot = (static_cast<int64_t>(worker(l)) * 2 + (from == 0)) * (kPair ? 2 : 1) + (kPair ? l : 0);
+          po = reinterpret_cast<float4*>(p.w.part) + slot * p.slot_rows * 32 + r;
+          pm = p.w.part_ml + (slot * p.slot_rows + r) * 2, stride = p.slot_rows;
         }
-#pragma unroll
+#pragma unroll 1
         for (int i = 0; i < 4; ++i) {
           uint32_t o[32];
           if (started) {
@@ -803,13 +921,14 @@ __global__ void __launch_bounds__(kPtThreads, 1)
               dst[j] = make_uint4(v[0], v[1], v[2], v[3]);
             }
           } else if (live) {
-            uint4* dst = reinterpret_cast<uint4*>(po + 32 * i);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) dst[j] = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+            for (int j = 0; j < 8; ++j)
+              po[(8 * i + j) * stride] = make_float4(__uint_as_float(o[4 * j]), __uint_as_float(o[4 * j + 1]),
+                                                     __uint_as_float(o[4 * j + 2]), __uint_as_float(o[4 * j + 3]));
           }
           __syncwarp();
         }
-        if (live && !final_) pm[0] = m, pm[1] = sum;
+        if (live && !final_) *reinterpret_cast<float2*>(pm) = make_float2(m, sum);
       }
       tc_fence_before();
     }
@@ -818,56 +937,72 @@ __global__ void __launch_bounds__(kPtThreads, 1)
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc(bar.tmem, 512);
   }
 }
 
 // ------------------------------------------------------------ joining
-// out = sum_i w_i O_i / sum_i w_i l_i, w_i = 2^(c (m_i - max m)); a warp per row, four channels a lane.
+// out = sum_i w_i O_i / sum_i w_i l_i, w_i = 2^(c (m_i - max m)), in the order of the pieces.  A CTA of 128 threads
+// takes four rows at a time: thread = four channels (threadIdx / 4) of a row (threadIdx % 4), so that the pieces of a
+// cut block, which have the rows beside each other, are read in whole sectors.
 struct PtJoin {
   float m = -INFINITY, l = 0.0f;
   float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 
-  __device__ __forceinline__ void add(const float* po, const float* pm, int lane, float c) {
-    const float pm0 = pm[0], pl = pm[1];
-    const float4 v = *(reinterpret_cast<const float4*>(po) + lane);
-    const float top = fmaxf(m, pm0), base = top == -INFINITY ? 0.0f : top;
-    const float a = pt_exp2((m - base) * c), b = pt_exp2((pm0 - base) * c);
-    l = l * a + pl * b;
+  __device__ __forceinline__ void fold(const float2& ml, const float4& v, float c) {
+    const float top = fmaxf(m, ml.x), base = top == -INFINITY ? 0.0f : top;
+    const float a = pt_exp2((m - base) * c), b = pt_exp2((ml.x - base) * c);
+    l = l * a + ml.y * b;
     o.x = o.x * a + v.x * b, o.y = o.y * a + v.y * b, o.z = o.z * a + v.z * b, o.w = o.w * a + v.w * b;
     m = top;
   }
-  __device__ __forceinline__ void store(uint16_t* row, int lane) const {
+  // Pieces `first` .. `last` of a cut block: slot 1 of the first worker, 0 of the others; `of_pair` which of a pair's.
+  template <int kPer>
+  __device__ __forceinline__ void pieces(const PtArgs& p, int first, int last, int of_pair, int row, int j) {
+    constexpr int kAhead = 8;  // loads in flight
+    for (int w0 = first; w0 <= last; w0 += kAhead) {
+      float2 ml[kAhead];
+      float4 v[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int w = min(w0 + i, last);
+        const int64_t slot = (static_cast<int64_t>(w) * 2 + (w == first)) * kPer + of_pair;
+        ml[i] = *reinterpret_cast<const float2*>(p.w.part_ml + (slot * p.slot_rows + row) * 2);
+        v[i] = *(reinterpret_cast<const float4*>(p.w.part) + (slot * 32 + j) * p.slot_rows + row);
+      }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i)
+        if (w0 + i <= last) fold(ml[i], v[i], p.c);
+    }
+  }
+  __device__ __forceinline__ void store(uint16_t* row, int j) const {
     const float f = l > 0.0f || l != l ? 1.0f / l : 0.0f;
     const __nv_bfloat162 x = __floats2bfloat162_rn(o.x * f, o.y * f), y = __floats2bfloat162_rn(o.z * f, o.w * f);
-    *(reinterpret_cast<uint2*>(row) + lane) =
+    *(reinterpret_cast<uint2*>(row) + j) =
         make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
   }
 };
 
-constexpr int kPtJoinSplit = 8;  // CTAs that share the rows of a cut block
+constexpr int kPtJoinSplit = 16;  // CTAs that share the rows of a cut block
 
-// Prompts: CTA (i, y) joins the block that worker i starts within, when it began in worker i - 1.
+// Prompts: CTA (i, y) joins the block that worker i + 1 starts within, when it began in worker i.
 template <bool kPair>
 __global__ void __launch_bounds__(128) pt_join_prompts_kernel(const PtArgs p) {
   grid_dependency_wait();
   grid_dependents_launch();
-  const int i = blockIdx.x + 1, lane = threadIdx.x & 31;
+  const int i = blockIdx.x + 1, j = threadIdx.x >> 2;
   const PtStart s = p.w.starts[i];
   const int64_t chunk = p.w.sums->chunk;
   if (s.count == 0 || s.tile == 0 || s.tile > chunk) return;
   const PtBlock b = p.w.blocks[s.block];
-  const int64_t begin = i * chunk - s.tile;
-  const int last = static_cast<int>((begin + b.tiles - 1) / chunk);
-  for (int r = blockIdx.y * 4 + (threadIdx.x >> 5); r < b.ntok * p.G; r += 4 * kPtJoinSplit) {
-    const int per = p.TB * p.G, l = r / per, in = r - l * per;  // lane of a pair, its row
-    PtJoin j;
-    for (int w = i - 1; w <= last; ++w) {
-      const int64_t at = ((static_cast<int64_t>(w) * 2 + (w == i - 1)) * (kPair ? 2 : 1) + l) * p.slot_rows + in;
-      j.add(p.w.part + at * kPtRows, p.w.part_ml + at * 2, lane, p.c);
-    }
+  const int last = i - 1 + static_cast<int>((chunk - s.tile + b.tiles - 1) / chunk);
+  const int per = p.TB * p.G;  // rows of a lane
+  for (int r = blockIdx.y * 4 + (threadIdx.x & 3); r < b.ntok * p.G; r += 4 * kPtJoinSplit) {
+    const int l = kPair && r >= per;
+    PtJoin join;
+    join.pieces<kPair ? 2 : 1>(p, i - 1, last, l, r - l * per, j);
     const int t = r / p.G;
-    j.store(p.out + (static_cast<int64_t>(b.tok0 + t) * p.Hq + s.head * p.G + r - t * p.G) * kPtRows, lane);
+    join.store(p.out + (static_cast<int64_t>(b.tok0 + t) * p.Hq + s.head * p.G + r - t * p.G) * kPtRows, j);
   }
 }
 
@@ -875,36 +1010,39 @@ __global__ void __launch_bounds__(128) pt_join_prompts_kernel(const PtArgs p) {
 __global__ void __launch_bounds__(128) pt_join_decode_kernel(const PtArgs p) {
   grid_dependency_wait();
   grid_dependents_launch();
-  const int b = blockIdx.x, h = blockIdx.y, lane = threadIdx.x & 31;
+  const int b = blockIdx.x, h = blockIdx.y, j = threadIdx.x >> 2;
   const PtSums sums = *p.w.sums;
   const int of = p.w.row_block[b];
   const int own = sums.prefix_blocks + b;
   const PtBlock mine = p.w.blocks[own];
-  const int64_t begin = p.w.before[own] * p.Hkv + static_cast<int64_t>(h) * mine.tiles;
-  const bool cut = begin / sums.chunk != (begin + mine.tiles - 1) / sums.chunk;
-  if (!cut && mine.key0 == 0) return;  // the attention wrote it
-  for (int g = threadIdx.x >> 5; g < p.G; g += 4) {
-    PtJoin j;
+  PtBlock common{};
+  int64_t own_at = p.w.before[own], common_at = 0;
+  if (of >= 0) common = p.w.blocks[of], common_at = p.w.before[of];
+  // the workers of a block: first and last
+  auto workers = [&](int64_t before, int tiles, int& first, int& last) {
+    const int64_t at = before * p.Hkv + static_cast<int64_t>(h) * tiles;
+    first = static_cast<int>(at / sums.chunk);
+    last = first + static_cast<int>((at - first * sums.chunk + tiles - 1) / sums.chunk);
+  };
+  int own_first, own_last, common_first = 0, common_last = 0;
+  workers(own_at, mine.tiles, own_first, own_last);
+  if (of >= 0) workers(common_at, common.tiles, common_first, common_last);
+  if (own_first == own_last && mine.key0 == 0) return;  // the attention wrote it
+  for (int g = threadIdx.x & 3; g < p.G; g += 4) {
+    PtJoin join;
     const int64_t row = static_cast<int64_t>(b) * p.Hq + h * p.G + g;
-    auto add = [&](int block, const PtBlock& bl, int in, int64_t area) {
-      const int64_t at0 = p.w.before[block] * p.Hkv + static_cast<int64_t>(h) * bl.tiles;
-      const int first = static_cast<int>(at0 / sums.chunk), last = static_cast<int>((at0 + bl.tiles - 1) / sums.chunk);
-      if (first == last) {
+    auto add = [&](int first, int last, int in, int64_t area) {
+      if (first < last) {
+        join.pieces<1>(p, first, last, 0, in, j);
+      } else {
         const int64_t at = area * p.batch * p.Hq + row;
-        j.add(p.w.row + at * kPtRows, p.w.row_ml + at * 2, lane, p.c);
-        return;
-      }
-      for (int w = first; w <= last; ++w) {
-        const int64_t at = (static_cast<int64_t>(w) * 2 + (w == first)) * p.slot_rows + in;
-        j.add(p.w.part + at * kPtRows, p.w.part_ml + at * 2, lane, p.c);
+        join.fold(*reinterpret_cast<const float2*>(p.w.row_ml + at * 2),
+                  *(reinterpret_cast<const float4*>(p.w.row + at * kPtRows) + j), p.c);
       }
     };
-    if (of >= 0) {
-      const PtBlock shared = p.w.blocks[of];
-      add(of, shared, (b - shared.tok0) * p.G + g, 1);
-    }
-    add(own, mine, g, 0);
-    j.store(p.out + row * kPtRows, lane);
+    if (of >= 0) add(common_first, common_last, (b - common.tok0) * p.G + g, 1);
+    add(own_first, own_last, g, 0);
+    join.store(p.out + row * kPtRows, j);
   }
 }
 
@@ -926,7 +1064,7 @@ static PtLayout pt_layout(char* base, int64_t blocks, int64_t batch, int64_t row
   constexpr int64_t kWorkers = 2 * kPtMaxCtas;
   l.w.sums = reinterpret_cast<PtSums*>(take(sizeof(PtSums)));
   l.w.starts = reinterpret_cast<PtStart*>(take(kWorkers * sizeof(PtStart)));
-  l.w.blocks = reinterpret_cast<PtBlock*>(take(blocks * sizeof(PtBlock)));
+  l.w.blocks = reinterpret_cast<PtBlock*>(take((blocks + 1) * sizeof(PtBlock)));  // the walks load one ahead
   l.w.before = reinterpret_cast<int64_t*>(take((blocks + 1) * 8));
   l.w.row_block = reinterpret_cast<int*>(take(joined ? batch * 4 : 0));
   l.w.part = reinterpret_cast<float*>(take(kWorkers * 2 * rows * kPtRows * 4));
@@ -970,17 +1108,28 @@ static int launch_pt(PtArgs& a, const void* k_cache, const void* v_cache, cudaSt
   if (rc != NV4_OK) return rc;
   const int sms = std::min(device_sm_count(), kPtMaxCtas);
   if (sms <= 0) return NV4_ERR_CUDA;
-  CUtensorMap maps[2] = {};
+  CUtensorMap maps[4] = {};
   const uint64_t rows = static_cast<uint64_t>(a.num_pages) * kPtPage, cols = static_cast<uint64_t>(a.Hkv) * kPtRows;
   if (!make_tensor_map_2d(&maps[0], CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, k_cache, rows, cols, kPtRows, 64,
                           CU_TENSOR_MAP_SWIZZLE_128B) ||
       !make_tensor_map_2d(&maps[1], CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, v_cache, rows, cols, kPtRows, 64,
                           CU_TENSOR_MAP_SWIZZLE_128B))
     return NV4_ERR_CUDA;
+  // q as [tokens][heads][128]: as many tokens as a block has, or one
+  const uint64_t q_dims[3] = {kPtRows, static_cast<uint64_t>(a.Hq), static_cast<uint64_t>(a.tokens)};
+  const uint64_t q_strides[2] = {kPtRows * 2, static_cast<uint64_t>(a.Hq) * kPtRows * 2};
+  const uint32_t box[3] = {64, static_cast<uint32_t>(a.G), static_cast<uint32_t>(a.TB)};
+  const uint32_t box1[3] = {64, static_cast<uint32_t>(a.G), 1};
+  if (!make_tensor_map_3d(&maps[2], CU_TENSOR_MAP_DATA_TYPE_UINT16, a.q, q_dims, q_strides, box,
+                          CU_TENSOR_MAP_SWIZZLE_128B) ||
+      !make_tensor_map_3d(&maps[3], CU_TENSOR_MAP_DATA_TYPE_UINT16, a.q, q_dims, q_strides, box1,
+                          CU_TENSOR_MAP_SWIZZLE_128B))
+    return NV4_ERR_CUDA;
   a.workers = kPair ? sms : 2 * sms;
   rc = launch_kernel(pt_plan_kernel, dim3(1), dim3(kPtPlanThreads), 0, stream, true, a, kPair ? 2 * a.TB : a.TB);
   if (rc != NV4_OK) return rc;
-  rc = launch_kernel(kern, dim3(sms), dim3(kPtThreads), kPtSmem, stream, true, maps[0], maps[1], a);
+  rc = launch_kernel(kern, dim3(sms), dim3(kPtThreads), kPtSmem, stream, true, maps[0], maps[1], maps[2], maps[3],
+                     a);
   if (rc != NV4_OK) return rc;
   if (a.prefix == nullptr)
     return launch_kernel(pt_join_prompts_kernel<kPair>, dim3(a.workers - 1, kPtJoinSplit), dim3(128), 0, stream, true, a);
