@@ -28,12 +28,13 @@
 //                   from L2 to shared memory once for 256 rows;
 //   others (solo)   every lane is a worker of its own.
 //   warp 0     copies K and V tiles (TMA, five slots of 32 KB) in the order of use
-//   warp 1     issues S = Q K^T, O += P V;  V rows behind the last token of a request
-//              are cleared first (0 times an old NaN would be one)
-//   warps 2-3  copy the rows of Q of their lane (TMA: [tokens][G heads][128 channels])
-//   warps 4-11 softmax of the two lanes; outputs
+//   warps 1-2  issue S = Q K^T, O += P V of a lane each;  V rows behind the last token of
+//              a request are cleared first (0 times an old NaN would be one)
+//   warps 4-11 softmax of the two lanes; outputs; one thread of a lane copies its rows
+//              of Q (TMA: [tokens][G heads][128 channels])
 // P goes back to TMEM over its scores in two BF16 terms (the upper 16 bits of the FP32
-// value and the rest, 2^-15 of it at most left out), so that the output's own rounding
+// value and of the rest, 2^-14 of it at most left out; conversions instructions would
+// share the pipe of the exponentials), so that the output's own rounding
 // is the only one that shows; one term would cost 1.4 times that error and save a
 // third of the tensor work.  m is moved (and O rescaled) only when a score exceeds it
 // by 2^8, so O is rarely touched.
@@ -485,8 +486,10 @@ struct PtSteps {
 };
 
 struct PtBars {
-  uint64_t full[kPtSlots], empty[kPtSlots];
-  uint64_t q_full[2], q_free[2], s_full[2], p_half[2], p_full[2], o_full[2], done;
+  // A slot's arrival is told to the lane that it is for by a barrier of the lane's own (of a pair: one for both): on a
+  // shared one a lane could take the phase before last of a slot, which the other lane has yet to see, for its own.
+  uint64_t full[2][kPtSlots], empty[kPtSlots];
+  uint64_t q_full[2], s_full[2], p_half[2], p_full[2], o_full[2], done;
   uint32_t tmem;
   int slot_keys[kPtSlots];  // keys of the slot's tile that exist
   int lane_keys[2];         // of the tile whose scores lie in the lane
@@ -506,16 +509,19 @@ __global__ void __launch_bounds__(kPtThreads, 1)
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kPtSlots; ++s) mbar_init(&bar.full[s], 1), mbar_init(&bar.empty[s], 1);
+    for (int s = 0; s < kPtSlots; ++s) {
+      mbar_init(&bar.full[0][s], 1);
+      mbar_init(&bar.full[1][s], 1);
+      mbar_init(&bar.empty[s], kPair ? 2 : 1);
+    }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bar.q_full[i], 1);
-      mbar_init(&bar.q_free[i], 1);
       mbar_init(&bar.s_full[i], 2);  // the products' completion, and lane_keys
       mbar_init(&bar.p_half[i], 4);  // the warps of the lane
       mbar_init(&bar.p_full[i], 4);
       mbar_init(&bar.o_full[i], 1);
     }
-    mbar_init(&bar.done, 1);
+    mbar_init(&bar.done, 2);
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -531,8 +537,8 @@ __global__ void __launch_bounds__(kPtThreads, 1)
 
   // Worker of a lane; in a pair both lanes walk worker blockIdx.x.
   auto worker = [&](int l) { return static_cast<int>(blockIdx.x) + (kPair ? 0 : l * static_cast<int>(gridDim.x)); };
-  // Does lane l have rows of block b?  (A pair's second lane: those of the tokens behind the first TB.)
-  auto has_rows = [&](int l, const PtBlock& b) { return !kPair || l == 0 || b.ntok > p.TB; };
+  // Does lane l have rows of a block of so many tokens?  (A pair's second lane: those of the tokens behind the first TB.)
+  auto has_rows = [&](int l, int ntok) { return !kPair || l == 0 || ntok > p.TB; };
   bool ok = true;
 
   if (warp < 4) pt_registers_down();
@@ -541,16 +547,18 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     if (lane == 0) {
       tma_prefetch_desc(&tmap_k);
       tma_prefetch_desc(&tmap_v);
-      int c = 0;
-      auto load = [&](const CUtensorMap* map, int x, int row, int keys) {
-        const int s = c % kPtSlots;
+      uint32_t c = 0, loads[2] = {0, 0};  // ring position; bit s: parity of the lane's loads into slot s
+      auto load = [&](int l, const CUtensorMap* map, int x, int row, int keys) {
+        const uint32_t s = c % kPtSlots;
+        uint64_t* full = &bar.full[l][s];
         if (c >= kPtSlots && !mbar_wait(&bar.empty[s], ((c / kPtSlots) - 1) & 1, kErrTimeoutEmpty)) return false;
         bar.slot_keys[s] = keys;
-        mbar_arrive_expect_tx(&bar.full[s], keys > 0 ? kPtTile : 0);
+        mbar_arrive_expect_tx(full, keys > 0 ? kPtTile : 0);
         if (keys > 0) {
-          tma_load_2d(ring + s * kPtTile, map, &bar.full[s], x, row);
-          tma_load_2d(ring + s * kPtTile + kPtHalf, map, &bar.full[s], x + 64, row);
+          tma_load_2d(ring + s * kPtTile, map, full, x, row);
+          tma_load_2d(ring + s * kPtTile + kPtHalf, map, full, x + 64, row);
         }
+        loads[l] ^= 1u << s;
         ++c;
         return true;
       };
@@ -577,138 +585,141 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         if (w[l].left > 0 && ok) {
           place(w[l], row[l], keys[l]);
           x[l] = w[l].head * kPtRows;
-          ok = load(&tmap_k, x[l], row[l], keys[l]);
+          ok = load(l, &tmap_k, x[l], row[l], keys[l]);
         }
       }
       while (ok && w[0].left > 0) {
 #pragma unroll
         for (int l = 0; l < kLanes; ++l) {
           if (!ok || w[l].left == 0) continue;
-          ok = load(&tmap_v, x[l], row[l], keys[l]);
+          ok = load(l, &tmap_v, x[l], row[l], keys[l]);
           w[l].next();
           if (!ok || w[l].left == 0) continue;
           place(w[l], row[l], keys[l]);
           x[l] = w[l].head * kPtRows;
-          ok = load(&tmap_k, x[l], row[l], keys[l]);
+          ok = load(l, &tmap_k, x[l], row[l], keys[l]);
         }
       }
       // every copy issued must land before the CTA may exit
-      for (int i = max(0, c - kPtSlots); i < c; ++i) {
-        const uint64_t start = global_timer_ns();
-        while (!mbar_try_wait(&bar.full[i % kPtSlots], (i / kPtSlots) & 1))
+      for (int i = 0; i < 2 * kPtSlots; ++i) {
+        const int l = i / kPtSlots, s = i % kPtSlots;
+        const uint64_t start = global_timer_ns();  // (a barrier that was never used is past this parity)
+        while (!mbar_try_wait(&bar.full[l][s], ((loads[l] >> s) & 1) ^ 1))
           if (global_timer_ns() - start > kWaitLimitNs) {
             record_error(kErrTimeoutDrain);
             break;
           }
       }
     }
-  } else if (warp == 1) {
-    // ---------------- products; the whole warp walks, lane 0 issues.  The lanes of the CTA take turns (O += P V of a tile,
-    // then S of the next), in one copy of the code: the softmax streams through the instruction caches beside it.
+  } else if (warp < 3) {
+    // ---------------- products of a lane: S of a tile, O += P V; the whole warp walks, its lane 0 issues.  A warp for
+    // each lane: the tensor cores take few products ahead, so what one waits for in between (two barriers and more at
+    // every tile) is covered by the other's.
     constexpr uint32_t kQk = pt_idesc(kPtRows, kPtRows, false), kPv = pt_idesc(kPtRows, kPtRows, true);
     const uint32_t q_lo = (smem_u32(smem) >> 4) + kPtDescK, ring_lo = smem_u32(ring) >> 4;
-    struct Turn {
-      PtSteps w;
-      int l, c;           // lane; ring position (of a pair; else both count in one)
-      uint32_t tiles, parts;  // S products, blocks so far
-      bool begun, started;    // S of the current tile is issued; O holds something of the current block
+    const int l = warp - 1;
+    PtSteps w;
+    w.start(p, worker(l));
+    const uint32_t others = kPair ? 0 : p.w.starts[worker(1 - l)].count;
+    // Ring position of V of the lane's tile i; K of the next is the one behind it.  Solo: both lanes' first K, then in
+    // turn V of a tile and K of the next, while there are any (the second lane has at most as many tiles).
+    auto v_position = [&](uint32_t i) -> uint32_t {
+      if (kPair) return 2 * i + 1;
+      if (l == 1) return 4 * i + (i + 1 == others ? 3 : 4);
+      return 1 + 2 * i + (others > 0 ? 1 + min(i, others) + min(i, others - 1) : 0);
     };
-    Turn me, other;
-    me.w.start(p, worker(0)), other.w.start(p, worker(1));
-    me.l = 0, other.l = 1;
-    me.c = other.c = 0;
-    me.tiles = other.tiles = me.parts = other.parts = 0;
-    me.begun = other.begun = me.started = other.started = false;
     auto arrived = [&](uint64_t& b, uint32_t phase) {  // the same answer in every lane
       return __all_sync(0xffffffffu, mbar_wait(&b, phase & 1, kErrTimeoutMma)) != 0;
     };
-    // Does the lane have rows in its current block?  The last of a pair's lanes that does releases the slots.
-    auto rows = [&]() { return !kPair || me.l == 0 || me.w.ntok > p.TB; };
-    auto releases = [&]() { return !kPair || me.l == 1 || me.w.ntok <= p.TB; };
-    while (ok && me.w.left > 0) {
-      const int l = me.l;
-      if (me.begun) {
-        if (rows()) {  // O += P V
-          const int s = me.c % kPtSlots;
-          ok = arrived(bar.full[s], me.c / kPtSlots) && arrived(bar.p_half[l], me.tiles - 1);
-          if (!ok) break;
-          tc_fence_after();
-          const int keys = bar.slot_keys[s], steps = (keys + 15) / 16;
-          if (keys & 15) {  // rows behind the last key: P is zero there, V may be anything
-            for (int i = lane; i < (steps * 16 - keys) * 16; i += 32)
-              *reinterpret_cast<uint4*>(ring + s * kPtTile + (i & 8 ? kPtHalf : 0) + (keys + (i >> 4)) * 128 +
-                                        (i & 7) * 16) = make_uint4(0, 0, 0, 0);
-            fence_proxy_async_smem();
-          }
-          if (me.w.fresh) me.started = false;
-          const uint32_t va = ring_lo + s * (kPtTile >> 4) + kPtDescV, o = l * 256 + 128;
-          // 16 keys: their two terms of P against the same rows of V
-          auto step = [&](int k, uint32_t accumulate) {
-            const uint32_t pk = l * 256 + (k >> 1) * 32 + (k & 1) * 8;
-            pt_mma_ts(o, pk, va + k * 128, kPv, accumulate);
-            pt_mma_ts(o, pk + 16, va + k * 128, kPv, 1);
-          };
-          __syncwarp();
-          if (lane == 0) {
-            if (steps >= 4) {
-              step(0, me.started);
+    uint32_t tiles = 0, parts = 0;  // products S, blocks so far
+    bool started = false;           // O holds something of the current block
+    uint32_t c = kPair ? 0 : l;     // ring position
+    uint32_t seen = 0;              // bit s: parity of what this lane has had in slot s
+    auto filled = [&](uint32_t s) {
+      const uint32_t phase = seen >> s;
+      seen ^= 1u << s;
+      return arrived(bar.full[kPair ? 0 : l][s], phase);
+    };
+    for (uint32_t i = 0; ok && w.left > 0; ++i) {
+      const bool rows = has_rows(l, w.ntok);
+      // S = Q K^T
+      uint32_t s = c % kPtSlots;
+      ok = filled(s);
+      if (ok && rows && w.fresh) ok = arrived(bar.q_full[l], parts++);
+      if (!ok) break;
+      tc_fence_after();
+      if (lane == 0) {
+        if (rows) {
+          bar.lane_keys[l] = bar.slot_keys[s];  // before the slot can be released
+          const uint32_t qa = q_lo + l * (kPtTile >> 4), ka = ring_lo + s * (kPtTile >> 4) + kPtDescK;
 #pragma unroll
-              for (int k = 1; k < 4; ++k) step(k, 1);
-            } else {
-              for (int k = 0; k < steps; ++k) step(k, me.started || k > 0);
-            }
+          for (int j = 0; j < 8; ++j) {
+            const uint32_t off = (j >> 2) * kPtHalfLo + (j & 3) * 2;
+            pt_mma_ss(l * 256, qa + off, ka + off, kQk, j > 0);
           }
-          __syncwarp();
-          ok = arrived(bar.p_full[l], me.tiles - 1);
-          if (!ok) break;
-          tc_fence_after();
-          if (lane == 0) {
-            if (steps == 8) {
-#pragma unroll
-              for (int k = 4; k < 8; ++k) step(k, 1);
-            } else {
-              for (int k = 4; k < steps; ++k) step(k, 1);
-            }
-            if (releases()) umma_commit(&bar.empty[s]);
-            if (me.w.last()) umma_commit(&bar.o_full[l]);
-          }
-          __syncwarp();
-          me.started = me.started || steps > 0;
+          umma_commit(&bar.s_full[l]);
+          mbar_arrive(&bar.s_full[l]);
+          umma_commit(&bar.empty[s]);
+        } else {
+          mbar_arrive(&bar.empty[s]);
         }
-        ++me.c;
-        me.w.next();
       }
-      me.begun = true;
-      if (me.w.left > 0) {
-        if (rows()) {  // S = Q K^T
-          const int s = me.c % kPtSlots;
-          ok = arrived(bar.full[s], me.c / kPtSlots);
-          if (ok && me.w.fresh) ok = arrived(bar.q_full[l], me.parts++);
-          if (!ok) break;
-          tc_fence_after();
-          if (lane == 0) {
-            bar.lane_keys[l] = bar.slot_keys[s];  // before the slot can be released
-            const uint32_t qa = q_lo + l * (kPtTile >> 4), ka = ring_lo + s * (kPtTile >> 4) + kPtDescK;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const uint32_t off = (j >> 2) * kPtHalfLo + (j & 3) * 2;
-              pt_mma_ss(l * 256, qa + off, ka + off, kQk, j > 0);
-            }
-            umma_commit(&bar.s_full[l]);
-            mbar_arrive(&bar.s_full[l]);
-            if (releases()) umma_commit(&bar.empty[s]);
-            if (me.w.last()) umma_commit(&bar.q_free[l]);
-          }
-          __syncwarp();
-          ++me.tiles;
+      __syncwarp();
+      tiles += rows;
+      // O += P V
+      c = v_position(i);
+      s = c % kPtSlots;
+      ok = filled(s);
+      if (!ok) break;
+      if (rows) {
+        const int keys = bar.slot_keys[s], steps = (keys + 15) / 16;
+        if (keys & 15) {  // rows behind the last key: P is zero there, V may be anything
+          for (int e = lane; e < (steps * 16 - keys) * 16; e += 32)
+            *reinterpret_cast<uint4*>(ring + s * kPtTile + (e & 8 ? kPtHalf : 0) + (keys + (e >> 4)) * 128 +
+                                      (e & 7) * 16) = make_uint4(0, 0, 0, 0);
+          fence_proxy_async_smem();
         }
-        ++me.c;
+        if (w.fresh) started = false;
+        const uint32_t va = ring_lo + s * (kPtTile >> 4) + kPtDescV, o = l * 256 + 128;
+        // 16 keys: their two terms of P against the same rows of V
+        auto step = [&](int k, uint32_t accumulate) {
+          const uint32_t pk = l * 256 + (k >> 1) * 32 + (k & 1) * 8;
+          pt_mma_ts(o, pk, va + k * 128, kPv, accumulate);
+          pt_mma_ts(o, pk + 16, va + k * 128, kPv, 1);
+        };
+        ok = arrived(bar.p_half[l], tiles - 1);
+        if (!ok) break;
+        tc_fence_after();
+        if (lane == 0) {
+          if (steps >= 4) {
+            step(0, started);
+#pragma unroll
+            for (int k = 1; k < 4; ++k) step(k, 1);
+          } else {
+            for (int k = 0; k < steps; ++k) step(k, started || k > 0);
+          }
+        }
+        __syncwarp();
+        ok = arrived(bar.p_full[l], tiles - 1);
+        if (!ok) break;
+        tc_fence_after();
+        if (lane == 0) {
+          if (steps == 8) {
+#pragma unroll
+            for (int k = 4; k < 8; ++k) step(k, 1);
+          } else {
+            for (int k = 4; k < steps; ++k) step(k, 1);
+          }
+          umma_commit(&bar.empty[s]);
+          if (w.last()) umma_commit(&bar.o_full[l]);
+        }
+        started = started || steps > 0;
+      } else if (lane == 0) {
+        mbar_arrive(&bar.empty[s]);
       }
-      if (other.w.left > 0 || kPair) {
-        if (!kPair) other.c = me.c;
-        const Turn t = me;
-        me = other, other = t;
-      }
+      __syncwarp();
+      ++c;
+      w.next();
     }
     if (lane == 0) {  // all issued products must finish before the TMEM is released
       umma_commit(&bar.done);
@@ -720,36 +731,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         }
     }
     __syncwarp();
-  } else if (warp < 4) {
-    // ---------------- rows of Q.  The box takes as many tokens as a block can have; rows behind the block's last are
-    // never used.
-    if (lane == 0) {
-      const int l = warp - 2;
-      uint8_t* dst = smem + l * kPtTile;
-      PtWalk w;
-      w.start(p, worker(l));
-      int part = 0;
-      for (; w.left > 0; w.skip()) {
-        if (!has_rows(l, w.b)) continue;
-        if (part > 0 && !mbar_wait(&bar.q_free[l], (part - 1) & 1, kErrTimeoutEmpty)) break;
-        const bool one = w.b.kind == kPtOwn;
-        const CUtensorMap* map = one ? &tmap_q1 : &tmap_q;
-        const int token = w.b.tok0 + (kPair ? l * p.TB : 0);
-        mbar_arrive_expect_tx(&bar.q_full[l], (one ? 1 : p.TB) * p.G * kPtRows * 2);
-        pt_load_q(dst, map, &bar.q_full[l], 0, w.head * p.G, token);
-        pt_load_q(dst + kPtHalf, map, &bar.q_full[l], 64, w.head * p.G, token);
-        ++part;
-      }
-      if (part > 0) {  // the last copy must land before the CTA may exit
-        const uint64_t start = global_timer_ns();
-        while (!mbar_try_wait(&bar.q_full[l], (part - 1) & 1))
-          if (global_timer_ns() - start > kWaitLimitNs) {
-            record_error(kErrTimeoutDrain);
-            break;
-          }
-      }
-    }
-  } else {
+  } else if (warp >= 4) {
     // ---------------- softmax and outputs: thread = row (head r % G of its lane's token r / G)
     pt_registers_up();
     const int l = (warp - 4) >> 2, quarter = warp & 3, r = quarter * 32 + lane;
@@ -757,11 +739,28 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     const float c = p.c;
     PtWalk w;
     w.start(p, worker(l));
+    // Rows of Q of the first block at or behind v's with any, copied by one thread.  The box takes as many tokens as a
+    // block can have; rows behind the block's last are never used.
+    const bool copies = quarter == 3 && lane == 0;
+    int copied = 0;
+    auto load_q = [&](PtWalk v) {
+      while (v.left > 0 && !has_rows(l, v.b.ntok)) v.skip();
+      if (v.left <= 0) return;
+      const bool one = v.b.kind == kPtOwn;
+      const CUtensorMap* map = one ? &tmap_q1 : &tmap_q;
+      const int token = v.b.tok0 + (kPair ? l * p.TB : 0);
+      uint8_t* dst = smem + l * kPtTile;
+      mbar_arrive_expect_tx(&bar.q_full[l], (one ? 1 : p.TB) * p.G * kPtRows * 2);
+      pt_load_q(dst, map, &bar.q_full[l], 0, v.head * p.G, token);
+      pt_load_q(dst + kPtHalf, map, &bar.q_full[l], 64, v.head * p.G, token);
+      ++copied;
+    };
+    if (copies && w.left > 0) load_q(w);
     int tile = 0, part = 0, limit = 0, token = 0, head = 0, from = 0;
     bool live = false, started = false;
     float m = -INFINITY, sum = 0.0f;
     for (; ok && w.left > 0; w.next()) {
-      if (!has_rows(l, w.b)) continue;
+      if (!has_rows(l, w.b.ntok)) continue;
       if (w.fresh) {
         const int t0 = kPair ? l * p.TB : 0, t = r / p.G;
         live = r < min(w.b.ntok - t0, p.TB) * p.G;
@@ -779,6 +778,11 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       if (!ok) break;
       tc_fence_after();
       const int keys = *reinterpret_cast<volatile int*>(&bar.lane_keys[l]);
+      if (copies && w.last()) {  // the block's last scores are there: its Q is not needed any more
+        PtWalk v = w;
+        v.skip();
+        load_q(v);
+      }
       if (busy && keys > 0) {
         const int seen = min(max(limit - (w.b.key0 + w.tile * kPtRows), 0), keys);
         const bool edge = __any_sync(0xffffffffu, seen < kPtRows);
@@ -835,8 +839,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
             h[j] = __byte_perm(xb, yb, 0x7632);
             float u, w;
             unpair(sub2(e, pair(__uint_as_float(xb & 0xFFFF0000u), __uint_as_float(yb & 0xFFFF0000u))), u, w);
-            const __nv_bfloat162 rest = __floats2bfloat162_rn(u, w);
-            lw[j] = *reinterpret_cast<const uint32_t*>(&rest);
+            lw[j] = __byte_perm(__float_as_uint(u), __float_as_uint(w), 0x7632);
           }
         };
         tmem_ld16(at, va);
@@ -931,6 +934,14 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         if (live && !final_) *reinterpret_cast<float2*>(pm) = make_float2(m, sum);
       }
       tc_fence_before();
+    }
+    if (copies && copied > 0) {  // the last copy must land before the CTA may exit
+      const uint64_t start = global_timer_ns();
+      while (!mbar_try_wait(&bar.q_full[l], (copied - 1) & 1))
+        if (global_timer_ns() - start > kWaitLimitNs) {
+          record_error(kErrTimeoutDrain);
+          break;
+        }
     }
   }
   tc_fence_before();
