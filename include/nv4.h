@@ -425,8 +425,8 @@ int nv4_append_kv(const void* q, const void* k, const void* v, const void* q_wei
  * tokens (masked, but in the cache) must be finite; what lies behind its last
  * token may be anything.  At most NV4_PAGED_MAX_GROUP query heads per KV head;
  * (tokens + 2 * batch) * max_pages * num_kv_heads up to 2^36.
- * Statistics and sums in FP32, the probabilities multiplied in two BF16 terms.
- * All pointers 16-byte aligned (the int32 ones 4).
+ * Statistics and sums in FP32, the probabilities rounded to BF16 once for the
+ * product with V.  All pointers 16-byte aligned (the int32 ones 4).
  */
 #define NV4_PAGED_MAX_GROUP 16
 #define NV4_PAGED_MAX_TOKENS (1 << 22)
@@ -450,7 +450,8 @@ int nv4_paged_prefill_attention(const void* q, const void* k_cache, const void* 
  *                 their contexts go), the rest, as all other tokens, through each
  *                 request's own
  *   context_lens  int32 [batch]; 0 (or less) marks a padding row, whose output is zero
- * Everything else as nv4_paged_prefill_attention; groups may be 0 (then
+ * The probabilities are multiplied in two BF16 terms.  Everything else as
+ * nv4_paged_prefill_attention; groups may be 0 (then
  * group_starts and prefix_lens may be NULL).
  */
 int64_t nv4_shared_prefix_attention_workspace_bytes(int64_t batch, int64_t groups, int64_t num_heads,

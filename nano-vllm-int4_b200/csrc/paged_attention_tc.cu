@@ -21,23 +21,25 @@
 // reproducible).  A first kernel of one CTA makes the block table from the lengths on
 // the device, so that captured calls follow new lengths.
 //
-// A CTA (one per SM, 384 threads) has two lanes: Q tile, S and O accumulators in TMEM
-// (128 columns each) and a warpgroup of softmax, one thread per row.  While one
-// lane's warpgroup works on its scores, the tensor cores work for the other.
+// A CTA (one per SM, 640 threads) has two lanes: Q tile, S and O accumulators in TMEM
+// (128 columns each) and two warpgroups of softmax, two threads per row.  While one
+// lane's warpgroups work on its scores, the tensor cores work for the other.
 //   prompts (pair)  both lanes take the same keys for two blocks of rows: K and V pass
 //                   from L2 to shared memory once for 256 rows;
 //   others (solo)   every lane is a worker of its own.
 //   warp 0     copies K and V tiles (TMA, five slots of 32 KB) in the order of use
 //   warps 1-2  issue S = Q K^T, O += P V of a lane each;  V rows behind the last token of
 //              a request are cleared first (0 times an old NaN would be one)
-//   warps 4-11 softmax of the two lanes; outputs; one thread of a lane copies its rows
+//   warps 4-19 softmax of the two lanes; outputs; one thread of a lane copies its rows
 //              of Q (TMA: [tokens][G heads][128 channels])
-// P goes back to TMEM over its scores in two BF16 terms (the upper 16 bits of the FP32
-// value and of the rest, 2^-14 of it at most left out; conversions instructions would
-// share the pipe of the exponentials), so that the output's own rounding
-// is the only one that shows; one term would cost 1.4 times that error and save a
-// third of the tensor work.  m is moved (and O rescaled) only when a score exceeds it
-// by 2^8, so O is rarely touched.
+// P goes back to TMEM over its scores.  Decode is bound by the cache's bytes: there P is
+// multiplied in two BF16 terms (the upper 16 bits of the FP32 value and of the rest, 2^-14
+// of it at most left out), so that the output's own rounding
+// is the only one that shows (0.0017 of the norm).  Prompts are bound by the products, and
+// under the power limit by their energy: there P is rounded to BF16 once (0.0023 of the
+// norm; the sum of a row is that of the values before), which
+// saves a third of the products.  m is moved (and O rescaled) only when a score exceeds
+// it by 2^8, so O is rarely touched.
 #include "nv4_device.cuh"
 #include "nv4_launch.h"
 
@@ -46,12 +48,13 @@ namespace nv4 {
 constexpr int kPtRows = 128;    // rows of a block, keys of a tile, head_dim
 constexpr int kPtPage = 256;
 constexpr int kPtMaxCtas = 160;
-constexpr int kPtThreads = 384;  // three warpgroups: copies and products, softmax of the two lanes
+constexpr int kPtThreads = 640;  // a warpgroup for copies and products, two for the softmax of each lane
 constexpr int kPtTile = kPtRows * kPtRows * 2;  // bytes of a Q, K or V tile
 constexpr int kPtHalf = kPtTile / 2;            // 64 channels of it: [128 rows][128 bytes], 128-byte swizzle
 constexpr int kPtSlots = 5;
 constexpr int kPtBar = (2 + kPtSlots) * kPtTile;
-constexpr int kPtSmem = kPtBar + 512 + 1024;    // barriers and flags; alignment of the tiles to 1024
+constexpr int kPtTops = kPtBar + 256;           // after barriers and flags: maxima that the halves of a row exchange
+constexpr int kPtSmem = kPtTops + 2 * 2 * kPtRows * 4;
 constexpr float kPtSlack = 8.0f;                // log2 units by which a score may pass the reference
 
 enum PtKind : int { kPtPrompt = 0, kPtOwn = 1, kPtPrefix = 2 };
@@ -389,17 +392,6 @@ __device__ __forceinline__ void pt_tmem_st16(uint32_t taddr, const uint32_t (&v)
       : "memory");
 }
 
-// Values of a TMEM load: not used before the wait in front of this.
-__device__ __forceinline__ void pt_pin(uint32_t (&v)[16]) {
-#pragma unroll
-  for (int i = 0; i < 16; ++i) asm volatile("" : "+r"(v[i]));
-}
-
-// Registers: 384 threads are launched with 168; the softmax holds a row's 128 scores (216 a thread), what the first
-// warpgroup gives up (72) covers it: 72 + 2 * 216 = 3 * 168.
-__device__ __forceinline__ void pt_registers_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 72;"); }
-__device__ __forceinline__ void pt_registers_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 216;"); }
-
 // The tiles of a worker, in order.  The next block's record is loaded a block ahead.
 struct PtWalk {
   const PtBlock* blocks;
@@ -489,21 +481,20 @@ struct PtBars {
   // A slot's arrival is told to the lane that it is for by a barrier of the lane's own (of a pair: one for both): on a
   // shared one a lane could take the phase before last of a slot, which the other lane has yet to see, for its own.
   uint64_t full[2][kPtSlots], empty[kPtSlots];
-  uint64_t q_full[2], s_full[2], p_half[2], p_full[2], o_full[2], done;
+  uint64_t q_full[2], s_full[2], p_full[2], o_full[2], turn[2], done;
   uint32_t tmem;
   int slot_keys[kPtSlots];  // keys of the slot's tile that exist
   int lane_keys[2];         // of the tile whose scores lie in the lane
 };
-static_assert(sizeof(PtBars) <= 512, "barriers");
+static_assert(sizeof(PtBars) <= 256, "barriers");
 
 // ------------------------------------------------------------ attention
-template <bool kPair>
+template <bool kPair, int kTerms>
 __global__ void __launch_bounds__(kPtThreads, 1)
     pt_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
                         const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_q1,
                         const PtArgs p) {
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = smem_raw + (((smem_u32(smem_raw) + 1023u) & ~1023u) - smem_u32(smem_raw));
+  extern __shared__ __align__(1024) uint8_t smem[];  // the tiles' swizzle wants multiples of 1024
   uint8_t* ring = smem + 2 * kPtTile;
   PtBars& bar = *reinterpret_cast<PtBars*>(smem + kPtBar);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -517,9 +508,9 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bar.q_full[i], 1);
       mbar_init(&bar.s_full[i], 2);  // the products' completion, and lane_keys
-      mbar_init(&bar.p_half[i], 4);  // the warps of the lane
-      mbar_init(&bar.p_full[i], 4);
+      mbar_init(&bar.p_full[i], 8);  // the warps of the lane
       mbar_init(&bar.o_full[i], 1);
+      mbar_init(&bar.turn[i], 1);
     }
     mbar_init(&bar.done, 2);
     fence_mbar_init();
@@ -531,7 +522,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = 0;  // all 512 columns are this CTA's: they start at 0
+  // TMEM: all 512 columns are this CTA's, so they start at 0: lane l has S (then P) at l * 256, O at l * 256 + 128.
   grid_dependency_wait();  // the block table, and q, from the kernels before
   grid_dependents_launch();
 
@@ -541,7 +532,6 @@ __global__ void __launch_bounds__(kPtThreads, 1)
   auto has_rows = [&](int l, int ntok) { return !kPair || l == 0 || ntok > p.TB; };
   bool ok = true;
 
-  if (warp < 4) pt_registers_down();
   if (warp == 0) {
     // ---------------- copies of K and V
     if (lane == 0) {
@@ -613,8 +603,9 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     }
   } else if (warp < 3) {
     // ---------------- products of a lane: S of a tile, O += P V; the whole warp walks, its lane 0 issues.  A warp for
-    // each lane: the tensor cores take few products ahead, so what one waits for in between (two barriers and more at
-    // every tile) is covered by the other's.
+    // each lane: the tensor cores take few products ahead, so what one waits for in between is covered by the other's.
+    // The lanes of a pair take turns at O += P V of a tile with S of the next: left to themselves they fall into step,
+    // both at their exponentials (the pipe of these then takes 2048 cycles) and both at their products in turn.
     constexpr uint32_t kQk = pt_idesc(kPtRows, kPtRows, false), kPv = pt_idesc(kPtRows, kPtRows, true);
     const uint32_t q_lo = (smem_u32(smem) >> 4) + kPtDescK, ring_lo = smem_u32(ring) >> 4;
     const int l = warp - 1;
@@ -663,6 +654,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         } else {
           mbar_arrive(&bar.empty[s]);
         }
+        if (kPair && i > 0) mbar_arrive(&bar.turn[1 - l]);
       }
       __syncwarp();
       tiles += rows;
@@ -681,45 +673,36 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         }
         if (w.fresh) started = false;
         const uint32_t va = ring_lo + s * (kPtTile >> 4) + kPtDescV, o = l * 256 + 128;
-        // 16 keys: their two terms of P against the same rows of V
+        // 16 keys: the terms of P against the same rows of V
         auto step = [&](int k, uint32_t accumulate) {
-          const uint32_t pk = l * 256 + (k >> 1) * 32 + (k & 1) * 8;
+          const uint32_t pk = l * 256 + (kTerms == 1 ? (k >> 2) * 64 + (k & 3) * 8 : (k >> 1) * 32 + (k & 1) * 8);
           pt_mma_ts(o, pk, va + k * 128, kPv, accumulate);
-          pt_mma_ts(o, pk + 16, va + k * 128, kPv, 1);
+          if (kTerms == 2) pt_mma_ts(o, pk + 16, va + k * 128, kPv, 1);
         };
-        ok = arrived(bar.p_half[l], tiles - 1);
-        if (!ok) break;
-        tc_fence_after();
-        if (lane == 0) {
-          if (steps >= 4) {
-            step(0, started);
-#pragma unroll
-            for (int k = 1; k < 4; ++k) step(k, 1);
-          } else {
-            for (int k = 0; k < steps; ++k) step(k, started || k > 0);
-          }
-        }
-        __syncwarp();
         ok = arrived(bar.p_full[l], tiles - 1);
+        if (kPair && ok && l + i > 0) ok = arrived(bar.turn[l], i - 1 + l);
         if (!ok) break;
         tc_fence_after();
         if (lane == 0) {
           if (steps == 8) {
+            step(0, started);
 #pragma unroll
-            for (int k = 4; k < 8; ++k) step(k, 1);
+            for (int k = 1; k < 8; ++k) step(k, 1);
           } else {
-            for (int k = 4; k < steps; ++k) step(k, 1);
+            for (int k = 0; k < steps; ++k) step(k, started || k > 0);
           }
           umma_commit(&bar.empty[s]);
           if (w.last()) umma_commit(&bar.o_full[l]);
         }
         started = started || steps > 0;
-      } else if (lane == 0) {
-        mbar_arrive(&bar.empty[s]);
+      } else {
+        if (kPair && l + i > 0) ok = arrived(bar.turn[l], i - 1 + l);
+        if (lane == 0) mbar_arrive(&bar.empty[s]);
       }
       __syncwarp();
       ++c;
       w.next();
+      if (kPair && w.left == 0 && lane == 0) mbar_arrive(&bar.turn[1 - l]);
     }
     if (lane == 0) {  // all issued products must finish before the TMEM is released
       umma_commit(&bar.done);
@@ -732,16 +715,20 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     }
     __syncwarp();
   } else if (warp >= 4) {
-    // ---------------- softmax and outputs: thread = row (head r % G of its lane's token r / G)
-    pt_registers_up();
-    const int l = (warp - 4) >> 2, quarter = warp & 3, r = quarter * 32 + lane;
-    const uint32_t at = tmem + l * 256 + (static_cast<uint32_t>(quarter * 32) << 16);
+    // ---------------- softmax and outputs: two threads a row (head r % G of its lane's token r / G), each with half of a
+    // tile's keys, and of the output's channels at the end.  (With one thread a row the two warps of a scheduler left
+    // two thirds of its issue slots empty.)
+    const int l = (warp - 4) >> 3, half = ((warp - 4) >> 2) & 1, quarter = warp & 3, r = quarter * 32 + lane;
+    const uint32_t at = l * 256 + half * 64 + (static_cast<uint32_t>(quarter * 32) << 16);
+    float* const mine = reinterpret_cast<float*>(smem + kPtTops) + (l * 2 + half) * kPtRows + r;
+    const float* const others = reinterpret_cast<float*>(smem + kPtTops) + (l * 2 + 1 - half) * kPtRows + r;
+    const int pairing = 1 + l * 4 + quarter;  // named barrier of the two warps that share rows
     const float c = p.c;
     PtWalk w;
     w.start(p, worker(l));
     // Rows of Q of the first block at or behind v's with any, copied by one thread.  The box takes as many tokens as a
     // block can have; rows behind the block's last are never used.
-    const bool copies = quarter == 3 && lane == 0;
+    const bool copies = half == 1 && quarter == 3 && lane == 0;
     int copied = 0;
     auto load_q = [&](PtWalk v) {
       while (v.left > 0 && !has_rows(l, v.b.ntok)) v.skip();
@@ -759,7 +746,8 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     int tile = 0, part = 0, limit = 0, token = 0, head = 0, from = 0;
     bool live = false, started = false;
     float m = -INFINITY, sum = 0.0f;
-    for (; ok && w.left > 0; w.next()) {
+    // A wait that gave up does not end the walk (the two warps of a row meet at barriers): later ones are not waited for.
+    for (; w.left > 0; w.next()) {
       if (!has_rows(l, w.b.ntok)) continue;
       if (w.fresh) {
         const int t0 = kPair ? l * p.TB : 0, t = r / p.G;
@@ -774,8 +762,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         from = w.tile;
       }
       const bool busy = __any_sync(0xffffffffu, live);
-      ok = __all_sync(0xffffffffu, mbar_wait(&bar.s_full[l], tile & 1, kErrTimeoutMma));
-      if (!ok) break;
+      ok = ok && __all_sync(0xffffffffu, mbar_wait(&bar.s_full[l], tile & 1, kErrTimeoutMma));
       tc_fence_after();
       const int keys = *reinterpret_cast<volatile int*>(&bar.lane_keys[l]);
       if (copies && w.last()) {  // the block's last scores are there: its Q is not needed any more
@@ -786,27 +773,31 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       if (busy && keys > 0) {
         const int seen = min(max(limit - (w.b.key0 + w.tile * kPtRows), 0), keys);
         const bool edge = __any_sync(0xffffffffu, seen < kPtRows);
-        uint32_t s[kPtRows];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) tmem_ld32(at + 32 * i, s + 32 * i);
+        uint32_t s[64];
+        tmem_ld32(at, s);
+        tmem_ld32(at + 32, s + 32);
         tmem_wait_ld();
         if (edge) {  // what the row does not see
+          const int here = seen - 64 * half;
 #pragma unroll
-          for (int j = 0; j < kPtRows; ++j) s[j] = j < seen ? s[j] : 0xFF800000u;
+          for (int j = 0; j < 64; ++j) s[j] = j < here ? s[j] : 0xFF800000u;
         }
         float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int j = 0; j < kPtRows; j += 8)
+        for (int j = 0; j < 64; j += 8)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             t[i] = fmaxf(t[i], fmaxf(__uint_as_float(s[j + 2 * i]), __uint_as_float(s[j + 2 * i + 1])));
-        const float top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+        float top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+        *mine = top;
+        named_barrier_sync(pairing, 64);
+        top = fmaxf(top, *others);
         const bool move = top > m && (m == -INFINITY || (top - m) * c > kPtSlack);
         if (__any_sync(0xffffffffu, move) && started) {
           const float f = move ? pt_exp2((m - top) * c) : 1.0f;
           sum *= f;
 #pragma unroll 1
-          for (int i = 0; i < 8; ++i) {
+          for (int i = 0; i < 4; ++i) {
             uint32_t o[16];
             tmem_ld16(at + 128 + 16 * i, o);
             tmem_wait_ld();
@@ -819,48 +810,31 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         const float base = m == -INFINITY ? 0.0f : m;
         const uint64_t base2 = pair(base, base), c2 = pair(c, c);
         uint64_t sums[2] = {0, 0};
-        // 32 keys' probabilities take the columns of their scores: 16 of the upper terms, 16 of the lower.  Rolled, and the
-        // scores loaded again, 16 columns ahead: straight-line code of a whole tile does not stay in the instruction
-        // caches, for this warp and for the one that issues the products.
-        uint32_t va[16], vb[16], hi[16], lo[16];
-        auto probabilities = [&](uint32_t (&v)[16], int here, uint32_t* h, uint32_t* lw) {
-          if (edge) {
+        // The probabilities take columns of their own scores: of 32 keys 16 of the upper terms and 16 of the lower, or 16
 #pragma unroll
-            for (int j = 0; j < 16; ++j) v[j] = j < here ? v[j] : 0xFF800000u;
-          }
+        for (int i = 0; i < 2; ++i) {
+          uint32_t hi[16], lo[16];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
+          for (int j = 0; j < 16; ++j) {
             float x, y;
-            unpair(mul2(sub2(pair(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1])), base2), c2), x, y);
+            unpair(mul2(sub2(pair(__uint_as_float(s[32 * i + 2 * j]), __uint_as_float(s[32 * i + 2 * j + 1])), base2), c2),
+                   x, y);
             x = pt_exp2(x), y = pt_exp2(y);
             const uint64_t e = pair(x, y);
             sums[j & 1] = add2(sums[j & 1], e);
-            const uint32_t xb = __float_as_uint(x), yb = __float_as_uint(y);
-            h[j] = __byte_perm(xb, yb, 0x7632);
-            float u, w;
-            unpair(sub2(e, pair(__uint_as_float(xb & 0xFFFF0000u), __uint_as_float(yb & 0xFFFF0000u))), u, w);
-            lw[j] = __byte_perm(__float_as_uint(u), __float_as_uint(w), 0x7632);
+            if constexpr (kTerms == 1) {
+              const __nv_bfloat162 b = __floats2bfloat162_rn(x, y);
+              hi[j] = *reinterpret_cast<const uint32_t*>(&b);
+            } else {
+              const uint32_t xb = __float_as_uint(x), yb = __float_as_uint(y);
+              hi[j] = __byte_perm(xb, yb, 0x7632);
+              float u, w;
+              unpair(sub2(e, pair(__uint_as_float(xb & 0xFFFF0000u), __uint_as_float(yb & 0xFFFF0000u))), u, w);
+              lo[j] = __byte_perm(__float_as_uint(u), __float_as_uint(w), 0x7632);
+            }
           }
-        };
-        tmem_ld16(at, va);
-#pragma unroll 1
-        for (int i = 0; i < 4; ++i) {
-          tmem_wait_ld();
-          pt_pin(va);
-          tmem_ld16(at + 32 * i + 16, vb);
-          probabilities(va, seen - 32 * i, hi, lo);
-          tmem_wait_ld();
-          pt_pin(vb);
-          if (i < 3) tmem_ld16(at + 32 * i + 32, va);
-          probabilities(vb, seen - 32 * i - 16, hi + 8, lo + 8);
-          pt_tmem_st16(at + 32 * i, hi);
-          pt_tmem_st16(at + 32 * i + 16, lo);
-          if (i == 1) {  // the products with the first 64 keys may begin
-            tmem_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&bar.p_half[l]);
-          }
+          pt_tmem_st16(at + 16 * kTerms * i, hi);
+          if constexpr (kTerms == 2) pt_tmem_st16(at + 32 * i + 16, lo);
         }
         float x, y;
         unpair(add2(sums[0], sums[1]), x, y);
@@ -870,21 +844,22 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       started = started || keys > 0;
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) {
-        if (!busy || keys == 0) mbar_arrive(&bar.p_half[l]);
-        mbar_arrive(&bar.p_full[l]);
-      }
+      if (lane == 0) mbar_arrive(&bar.p_full[l]);
       ++tile;
       if (!w.last()) continue;
 
       // the block's end, or this worker's: outputs
-      ok = __all_sync(0xffffffffu, mbar_wait(&bar.o_full[l], part & 1, kErrTimeoutMma));
-      if (!ok) break;
+      ok = ok && __all_sync(0xffffffffu, mbar_wait(&bar.o_full[l], part & 1, kErrTimeoutMma));
       ++part;
       tc_fence_after();
       const bool whole = from == 0 && w.tile + 1 == w.b.tiles;
       const bool final_ = whole && (w.b.kind == kPtPrompt || (w.b.kind == kPtOwn && w.b.key0 == 0));
       if (busy) {
+        *mine = sum;
+        named_barrier_sync(pairing, 64);
+        const float other = *others;
+        named_barrier_sync(pairing, 64);  // read before the next block's maxima take their place
+        sum = half == 0 ? sum + other : other + sum;
         const float f = final_ ? (sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f) : 1.0f;
         const int64_t row = static_cast<int64_t>(token) * p.Hq + head;
         // FP32 outputs: of a block that is not cut row after row (for the joining kernel); of a cut one with the rows
@@ -894,14 +869,14 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         int stride;
         if (whole) {
           const int64_t i = (w.b.kind == kPtPrefix ? static_cast<int64_t>(p.batch) * p.Hq : 0) + row;
-          po = reinterpret_cast<float4*>(p.w.row) + i * 32, pm = p.w.row_ml + i * 2, stride = 1;
+          po = reinterpret_cast<float4*>(p.w.row) + i * 32 + half * 16, pm = p.w.row_ml + i * 2, stride = 1;
         } else {
           const int64_t slot = (static_cast<int64_t>(worker(l)) * 2 + (from == 0)) * (kPair ? 2 : 1) + (kPair ? l : 0);
-          po = reinterpret_cast<float4*>(p.w.part) + slot * p.slot_rows * 32 + r;
+          po = reinterpret_cast<float4*>(p.w.part) + (slot * 32 + half * 16) * p.slot_rows + r;
           pm = p.w.part_ml + (slot * p.slot_rows + r) * 2, stride = p.slot_rows;
         }
 #pragma unroll 1
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 2; ++i) {
           uint32_t o[32];
           if (started) {
             tmem_ld32(at + 128 + 32 * i, o);
@@ -911,7 +886,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
             for (int j = 0; j < 32; ++j) o[j] = 0u;
           }
           if (live && final_) {
-            uint4* dst = reinterpret_cast<uint4*>(p.out + row * kPtRows + 32 * i);
+            uint4* dst = reinterpret_cast<uint4*>(p.out + row * kPtRows + half * 64 + 32 * i);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               uint32_t v[4];
@@ -931,7 +906,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           }
           __syncwarp();
         }
-        if (live && !final_) *reinterpret_cast<float2*>(pm) = make_float2(m, sum);
+        if (live && !final_ && half == 0) *reinterpret_cast<float2*>(pm) = make_float2(m, sum);
       }
       tc_fence_before();
     }
@@ -1111,10 +1086,10 @@ int64_t shared_prefix_attention_workspace_bytes(int64_t batch, int64_t groups, i
   return pt_shared_layout(nullptr, batch, groups, num_heads, num_kv_heads).bytes;
 }
 
-template <bool kPair>
+template <bool kPair, int kTerms>
 static int launch_pt(PtArgs& a, const void* k_cache, const void* v_cache, cudaStream_t stream) {
   static int done[64] = {};
-  auto* kern = &pt_attention_kernel<kPair>;
+  auto* kern = &pt_attention_kernel<kPair, kTerms>;
   int rc = ensure_smem_attr(reinterpret_cast<const void*>(kern), kPtSmem, done);
   if (rc != NV4_OK) return rc;
   const int sms = std::min(device_sm_count(), kPtMaxCtas);
@@ -1181,8 +1156,8 @@ int launch_paged_prefill_attention(const void* q, const void* k_cache, const voi
   PtArgs a = pt_args(q, block_tables, context_lens, query_starts, nullptr, out, l.w, tokens, batch, 0, num_heads,
                      num_kv_heads, num_pages, max_pages, scale);
   // Two blocks of rows side by side when the requests have more than one block's rows on average.
-  if (tokens > batch * a.TB) return launch_pt<true>(a, k_cache, v_cache, stream);
-  return launch_pt<false>(a, k_cache, v_cache, stream);
+  if (tokens > batch * a.TB) return launch_pt<true, 1>(a, k_cache, v_cache, stream);
+  return launch_pt<false, 1>(a, k_cache, v_cache, stream);
 }
 
 int launch_shared_prefix_attention(const void* q, const void* k_cache, const void* v_cache, const int* block_tables,
@@ -1195,7 +1170,7 @@ int launch_shared_prefix_attention(const void* q, const void* k_cache, const voi
   const int* prefix = groups > 0 ? prefix_lens : context_lens;
   PtArgs a = pt_args(q, block_tables, context_lens, group_starts, prefix, out, l.w, batch, batch, groups, num_heads,
                      num_kv_heads, num_pages, max_pages, scale);
-  return launch_pt<false>(a, k_cache, v_cache, stream);
+  return launch_pt<false, 2>(a, k_cache, v_cache, stream);
 }
 
 }  // namespace nv4

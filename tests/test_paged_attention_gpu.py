@@ -167,6 +167,10 @@ def prefill_case(lens, hq, hkv, device, seed=0, extra_rows=0, spare_pages=2):
     return q, k_cache, v_cache, tables, context, starts
 
 
+def close_prompt(got, want, size):
+    ref.assert_attention_close(got, want, size, terms=1)
+
+
 def run_prefill(q, k_cache, v_cache, tables, context, starts, **kw):
     dev = q.device
     return paged_prefill_attention(q, k_cache, v_cache, i32(tables, dev), i32(context, dev), i32(starts, dev),
@@ -187,7 +191,7 @@ def test_prefill(cuda_device, lens, hq, hkv):
     out = run_prefill(*case)
     want, size, rows = ref.prefill(*case, SCALE)
     assert rows.all()
-    ref.assert_attention_close(out, want, size)
+    close_prompt(out, want, size)
     assert _native.device_error() == 0
 
 
@@ -195,7 +199,7 @@ def test_prefill(cuda_device, lens, hq, hkv):
                                          ([(100 * i, 37 * i % 90) for i in range(70)], 8, 1)])
 def test_prefill_larger(cuda_device, lens, hq, hkv):
     case = prefill_case(lens, hq, hkv, cuda_device)
-    ref.assert_attention_close(run_prefill(*case), *ref.prefill(*case, SCALE)[:2])
+    close_prompt(run_prefill(*case), *ref.prefill(*case, SCALE)[:2])
 
 
 def test_prefill_ignores_what_lies_behind_the_last_token(cuda_device):
@@ -210,7 +214,7 @@ def test_prefill_ignores_what_lies_behind_the_last_token(cuda_device):
     for fill in (float("nan"), float("inf"), -float("inf")):
         k_cache[~live] = fill
         v_cache[~live] = fill
-        ref.assert_attention_close(run_prefill(q, k_cache, v_cache, tables, context, starts), want, size)
+        close_prompt(run_prefill(q, k_cache, v_cache, tables, context, starts), want, size)
 
 
 def test_prefill_later_tokens_do_not_matter(cuda_device):
@@ -234,7 +238,7 @@ def test_prefill_rows_of_no_request_and_rows_that_see_nothing(cuda_device):
     out = torch.full_like(q, 7.0)
     assert run_prefill(q, k_cache, v_cache, tables, context, starts, out=out) is out
     want, size, rows = ref.prefill(q, k_cache, v_cache, tables, context, starts, SCALE)
-    ref.assert_attention_close(out[rows], want[rows], size[rows])
+    close_prompt(out[rows], want[rows], size[rows])
     assert (out[~rows] == 7).all() and (~rows).sum() == 9
     assert (out[starts[1]:starts[1] + 7] == 0).all() and (out[starts[2]:starts[3]] == 0).all()
 
@@ -245,7 +249,7 @@ def test_prefill_starts_that_fall_or_pass_the_end(cuda_device):
     q, k_cache, v_cache, tables, context, starts = prefill_case([(10, 20), (30, 20), (5, 20)], 4, 2, dev)
     out = run_prefill(q, k_cache, v_cache, tables, context, [-3, 20, 10, 1 << 30])
     want, size, rows = ref.prefill(q, k_cache, v_cache, tables, context, [0, 20, 20, 60], SCALE)
-    ref.assert_attention_close(out, want, size)
+    close_prompt(out, want, size)
 
 
 def test_prefill_bad_pages_and_narrow_tables(cuda_device):
@@ -255,7 +259,7 @@ def test_prefill_bad_pages_and_narrow_tables(cuda_device):
     tables[0][1], tables[1][0] = pages, -1
     out = run_prefill(q, k_cache, v_cache, tables, context, starts)
     assert _native.device_error() == 6
-    ref.assert_attention_close(out, *ref.prefill(q, k_cache, v_cache, tables, context, starts, SCALE)[:2])
+    close_prompt(out, *ref.prefill(q, k_cache, v_cache, tables, context, starts, SCALE)[:2])
     tables = [[1 << 30] * 3, [pages + 7] * 3]
     assert (run_prefill(q, k_cache, v_cache, tables, context, starts) == 0).all()
     assert _native.device_error() == 6
@@ -263,7 +267,7 @@ def test_prefill_bad_pages_and_narrow_tables(cuda_device):
     q, k_cache, v_cache, tables, context, starts = prefill_case([(600, 40)], 4, 1, dev)
     narrow = [tables[0][:1]]
     out = run_prefill(q, k_cache, v_cache, narrow, context, starts)
-    ref.assert_attention_close(out, *ref.prefill(q, k_cache, v_cache, narrow, context, starts, SCALE)[:2])
+    close_prompt(out, *ref.prefill(q, k_cache, v_cache, narrow, context, starts, SCALE)[:2])
     _native.device_error()
 
 
@@ -275,7 +279,7 @@ def test_prefill_extreme_scores(cuda_device, factor):
     q.copy_(torch.sign(q.float()) * 2)
     k_cache.copy_(torch.round(k_cache.float()).clamp(-3, 3) * factor)
     out = run_prefill(q, k_cache, v_cache, tables, context, starts)
-    ref.assert_attention_close(out, *ref.prefill(q, k_cache, v_cache, tables, context, starts, SCALE)[:2])
+    close_prompt(out, *ref.prefill(q, k_cache, v_cache, tables, context, starts, SCALE)[:2])
 
 
 def test_prefill_scores_that_rise_along_the_context(cuda_device):
@@ -286,14 +290,16 @@ def test_prefill_scores_that_rise_along_the_context(cuda_device):
         k_cache[tables[0][t // PAGE], t % PAGE] = (t // 4) / 8  # exact in BF16
     for scale in (SCALE, 0.001):
         out = run_prefill(q, k_cache, v_cache, tables, context, starts, scale=scale)
-        ref.assert_attention_close(out, *ref.prefill(q, k_cache, v_cache, tables, context, starts, scale)[:2])
+        close_prompt(out, *ref.prefill(q, k_cache, v_cache, tables, context, starts, scale)[:2])
 
 
-def test_prefill_error_is_the_outputs_rounding(cuda_device):
+def test_prefill_error_is_two_roundings(cuda_device):
+    """Each probability's rounding is as large, relative to its share, as the output's own
+    and independent of it: together sqrt(2) = 1.414 of the latter, 1.45 with what is left of chance."""
     case = prefill_case([(300, 500)], 8, 2, cuda_device)
     want = ref.prefill(*case, SCALE)[0]
     rounded = (want.bfloat16().double() - want).norm()
-    assert (run_prefill(*case).double() - want).norm() <= 1.02 * rounded
+    assert (run_prefill(*case).double() - want).norm() <= 1.45 * rounded
 
 
 def test_prefill_same_whatever_is_beside_it(cuda_device):
@@ -305,7 +311,7 @@ def test_prefill_same_whatever_is_beside_it(cuda_device):
         alone = run_prefill(q[lo:hi].contiguous(), k_cache, v_cache, [tables[b]], [context[b]], [0, hi - lo])
         seen = range(context[b] - (hi - lo) + 1, context[b] + 1)
         want, size = ref.attend(q[lo:hi], k_cache, v_cache, tables[b], seen, SCALE)
-        ref.assert_attention_close(alone, want, size)
+        close_prompt(alone, want, size)
         assert (alone.double() - together[lo:hi].double()).norm() <= 2.0 ** -8 * want.norm()
 
 
@@ -468,7 +474,7 @@ def test_conversation_over_a_shared_prefix(cuda_device):
             out = shared_prefix_attention(q, k_cache, v_cache, tab.block_tables, tab.context_lens, i32(groups[0], dev),
                                           i32(groups[1], dev), scale=SCALE)
             want = ref.decode(q, k_cache, v_cache, lists, [c + 1 for c in cached], SCALE)
-        ref.assert_attention_close(out, want[0], want[1])
+        ref.assert_attention_close(out, want[0], want[1], terms=1 if groups is None else 2)
         expected, size = ref.norm_rope(k, kw, cos_sin, tab.positions, 1e-6)
         ref.assert_rows_close(k_cache.flatten(0, 1)[tab.slot_mapping.long()], expected, size)
 
@@ -524,7 +530,7 @@ def test_streams_and_graphs(cuda_device):
     torch.cuda.synchronize()
     ref.assert_attention_close(captured[1], *ref.decode(*case[:4], context.tolist(), SCALE))
     want, size, rows = ref.prefill(*pre[:4], pcontext.tolist(), pstarts.tolist(), SCALE)
-    ref.assert_attention_close(captured[2], want, size)
+    close_prompt(captured[2], want, size)
     assert _native.device_error() == 0
 
 
