@@ -77,7 +77,7 @@ struct __align__(16) PtStart {
 };
 
 struct PtSums {
-  int64_t total, chunk;  // tiles of all blocks and heads; of a worker
+  int64_t total, chunk;  // cost of all blocks and heads; of a worker's share
   int blocks, prefix_blocks;
 };
 
@@ -86,7 +86,7 @@ struct PtScratch {
   PtSums* sums;
   PtStart* starts;   // [workers]
   PtBlock* blocks;
-  int64_t* before;   // [blocks + 1]: tiles (of one head) before a block
+  int64_t* before;   // [blocks + 1]: cost (of one head) of what lies before a block
   int* row_block;    // [batch]: the prefix block of a request, or -1
   float* part;       // [workers][2][rows][128]: of a worker's first and last block, when cut
   float* part_ml;    // [..][2]: reference, sum
@@ -149,6 +149,9 @@ __device__ __forceinline__ int pt_max_scan(int v, int* warp_max, int& carry) {
 }
 
 __device__ __forceinline__ int pt_tiles(int keys) { return max(1, (keys + kPtRows - 1) / kPtRows); }
+// A block counts for its tiles and as much as one more for its beginning and end (its outputs, mostly).
+constexpr int kPtBlockCost = 1;
+__device__ __forceinline__ int pt_cost(int tiles) { return tiles + kPtBlockCost; }
 
 constexpr int kPtPlanThreads = 1024;
 constexpr int kPtPlanCached = 2048;  // blocks whose sums are kept in shared memory for the search
@@ -188,7 +191,7 @@ __global__ void __launch_bounds__(kPtPlanThreads) pt_plan_kernel(const PtArgs p,
         const int n = last[s] - first[s], ctx = extra[s], end = min(ctx, most);
         int64_t sum = 0;
         for (int j = lane; j * block_tokens < n; j += 32)
-          sum += pt_tiles(min(ctx - n + min(n, (j + 1) * block_tokens), end));
+          sum += pt_cost(pt_tiles(min(ctx - n + min(n, (j + 1) * block_tokens), end)));
 #pragma unroll
         for (int m = 16; m >= 1; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
         if (lane == 0) weight[s] = sum;
@@ -210,14 +213,15 @@ __global__ void __launch_bounds__(kPtPlanThreads) pt_plan_kernel(const PtArgs p,
           const int j = j0 + lane, i0 = j * block_tokens;
           const int count = min(n - i0, block_tokens);
           const int tiles = count > 0 ? pt_tiles(min(ctx - n + i0 + count, end)) : 0;
-          int64_t x = tiles;
+          const int cost = count > 0 ? pt_cost(tiles) : 0;
+          int64_t x = cost;
 #pragma unroll
           for (int m = 1; m < 32; m <<= 1) {
             const int64_t y = __shfl_up_sync(0xffffffffu, x, m);
             if (lane >= m) x += y;
           }
           if (count > 0)
-            put(which[s] + j, before + x - tiles,
+            put(which[s] + j, before + x - cost,
                 PtBlock{b0 + s, first[s] + i0, count, tiles, 0, ctx - n + i0 + 1, end, kPtPrompt});
           before += __shfl_sync(0xffffffffu, x, 31);
         }
@@ -261,7 +265,7 @@ __global__ void __launch_bounds__(kPtPlanThreads) pt_plan_kernel(const PtArgs p,
       const int shared = extra[tid], row = static_cast<int>(weight[tid]);
       const int mine = live && shared > 0 ? (last[tid] - first[tid] + p.TB - 1) / p.TB : 0;
       int64_t all_w, all_n;
-      const int64_t wb = tiles_before + pt_scan(static_cast<int64_t>(mine) * (shared / kPtRows), sums, all_w);
+      const int64_t wb = tiles_before + pt_scan(static_cast<int64_t>(mine) * pt_cost(shared / kPtRows), sums, all_w);
       which[tid] = blocks + static_cast<int>(pt_scan(mine, sums, all_n));
       __syncthreads();
       weight[tid] = wb;
@@ -273,7 +277,7 @@ __global__ void __launch_bounds__(kPtPlanThreads) pt_plan_kernel(const PtArgs p,
         if (extra[s] <= 0) continue;
         const int n = last[s] - first[s], tiles = extra[s] / kPtRows;
         for (int j = lane; j * p.TB < n; j += 32)
-          put(which[s] + j, weight[s] + static_cast<int64_t>(j) * tiles,
+          put(which[s] + j, weight[s] + static_cast<int64_t>(j) * pt_cost(tiles),
               PtBlock{table_row[s], first[s] + j * p.TB, min(p.TB, n - j * p.TB), tiles, 0, 0, extra[s], kPtPrefix});
         for (int r = lane; r < n; r += 32) p.w.row_block[first[s] + r] = which[s] + r / p.TB;
       }
@@ -291,7 +295,7 @@ __global__ void __launch_bounds__(kPtPlanThreads) pt_plan_kernel(const PtArgs p,
         tiles = pt_tiles(end - shared);
       }
       int64_t all_w;
-      const int64_t wb = tiles_before + pt_scan(tiles, sums, all_w);
+      const int64_t wb = tiles_before + pt_scan(live ? pt_cost(tiles) : 0, sums, all_w);
       if (live) put(blocks + b, wb, PtBlock{b, b, 1, tiles, shared, end, end, kPtOwn});
       tiles_before += all_w;
     }
@@ -310,34 +314,48 @@ __global__ void __launch_bounds__(kPtPlanThreads) pt_plan_kernel(const PtArgs p,
   }
   __syncthreads();
   const bool in_smem = blocks <= kPtPlanCached;
-  for (int w = tid; w < p.workers; w += kPtPlanThreads) {
-    PtStart s{0, 0, 0, 0};
-    const int64_t at = w * chunk;
-    s.count = static_cast<int>(max(min(total - at, chunk), static_cast<int64_t>(0)));
-    if (s.count > 0) {
-      int lo = 0, hi = blocks - 1;  // the last block whose tiles start at or before `at`
-      if (small && in_smem) {
-        while (lo < hi) {
-          const int mid = (lo + hi + 1) / 2;
-          if (static_cast<int>(cached[mid]) * p.Hkv <= static_cast<int>(at)) lo = mid;
-          else hi = mid - 1;
-        }
-        const uint32_t into = static_cast<uint32_t>(at) - static_cast<uint32_t>(cached[lo]) * p.Hkv;
-        const uint32_t tiles = static_cast<uint32_t>((lo + 1 < blocks ? cached[lo + 1] : tiles_before) - cached[lo]);
-        s.head = static_cast<int>(into / tiles);
-        s.tile = static_cast<int>(into % tiles);
-      } else {
-        while (lo < hi) {
-          const int mid = (lo + hi + 1) / 2;
-          if (p.w.before[mid] * p.Hkv <= at) lo = mid;
-          else hi = mid - 1;
-        }
-        const int64_t into = at - p.w.before[lo] * p.Hkv;
-        const int tiles = p.w.blocks[lo].tiles;
-        s.head = static_cast<int>(into / tiles);
-        s.tile = static_cast<int>(into % tiles);
+  // The border at `at`: block, head and tile, and the tiles (without the costs) of all before it within the block.
+  auto border = [&](int64_t at, PtStart& s) {
+    int lo = 0, hi = blocks - 1, cost;  // the last block that starts at or before `at`
+    if (small && in_smem) {
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) / 2;
+        if (static_cast<int>(cached[mid]) * p.Hkv <= static_cast<int>(at)) lo = mid;
+        else hi = mid - 1;
       }
-      s.block = lo;
+      const uint32_t into = static_cast<uint32_t>(at) - static_cast<uint32_t>(cached[lo]) * p.Hkv;
+      cost = static_cast<int>((lo + 1 < blocks ? cached[lo + 1] : tiles_before) - cached[lo]);
+      s.head = static_cast<int>(into / static_cast<uint32_t>(cost));
+      s.tile = static_cast<int>(into % static_cast<uint32_t>(cost));
+    } else {
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) / 2;
+        if (p.w.before[mid] * p.Hkv <= at) lo = mid;
+        else hi = mid - 1;
+      }
+      const int64_t into = at - p.w.before[lo] * p.Hkv;
+      cost = pt_cost(p.w.blocks[lo].tiles);
+      s.head = static_cast<int>(into / cost);
+      s.tile = static_cast<int>(into % cost);
+    }
+    s.block = lo;
+    const int tiles = cost - kPtBlockCost;
+    // tiles before the border: what lies before it less the costs of the blocks begun (and ended) there
+    const int64_t begun = static_cast<int64_t>(lo) * p.Hkv + s.head;
+    const int64_t real = at - begun * kPtBlockCost - max(s.tile - tiles, 0);
+    if (s.tile >= tiles) {  // in the block's cost: the next one begins
+      s.tile = 0;
+      if (++s.head == p.Hkv) s.head = 0, ++s.block;
+    }
+    return real;
+  };
+  const int64_t end = total - static_cast<int64_t>(blocks) * p.Hkv * kPtBlockCost;  // tiles of all
+  for (int w = tid; w < p.workers; w += kPtPlanThreads) {
+    PtStart s{0, 0, 0, 0}, next;
+    const int64_t at = w * chunk;
+    if (at < total) {
+      const int64_t from = border(at, s);
+      s.count = static_cast<int>((at + chunk < total ? border(at + chunk, next) : end) - from);
     }
     p.w.starts[w] = s;
   }
@@ -390,6 +408,12 @@ __device__ __forceinline__ void pt_tmem_st16(uint32_t taddr, const uint32_t (&v)
       "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
       "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
       : "memory");
+}
+
+// Takes a lock in shared memory; after a while without it too (it only orders the lanes).
+__device__ __forceinline__ void pt_lock(uint32_t* lock) {
+  for (int i = 0; i < 100000; ++i)
+    if (atomicCAS(lock, 0u, 1u) == 0) return;
 }
 
 // The tiles of a worker, in order.  The next block's record is loaded a block ahead.
@@ -481,8 +505,8 @@ struct PtBars {
   // A slot's arrival is told to the lane that it is for by a barrier of the lane's own (of a pair: one for both): on a
   // shared one a lane could take the phase before last of a slot, which the other lane has yet to see, for its own.
   uint64_t full[2][kPtSlots], empty[kPtSlots];
-  uint64_t q_full[2], s_full[2], p_full[2], o_full[2], turn[2], done;
-  uint32_t tmem;
+  uint64_t q_full[2], s_full[2], p_full[2], o_full[2], done;
+  uint32_t tmem, lock;
   int slot_keys[kPtSlots];  // keys of the slot's tile that exist
   int lane_keys[2];         // of the tile whose scores lie in the lane
 };
@@ -510,9 +534,9 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       mbar_init(&bar.s_full[i], 2);  // the products' completion, and lane_keys
       mbar_init(&bar.p_full[i], 8);  // the warps of the lane
       mbar_init(&bar.o_full[i], 1);
-      mbar_init(&bar.turn[i], 1);
     }
     mbar_init(&bar.done, 2);
+    bar.lock = 0;
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -578,7 +602,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           ok = load(l, &tmap_k, x[l], row[l], keys[l]);
         }
       }
-      while (ok && w[0].left > 0) {
+      while (ok && (w[0].left > 0 || w[kLanes - 1].left > 0)) {
 #pragma unroll
         for (int l = 0; l < kLanes; ++l) {
           if (!ok || w[l].left == 0) continue;
@@ -604,8 +628,8 @@ __global__ void __launch_bounds__(kPtThreads, 1)
   } else if (warp < 3) {
     // ---------------- products of a lane: S of a tile, O += P V; the whole warp walks, its lane 0 issues.  A warp for
     // each lane: the tensor cores take few products ahead, so what one waits for in between is covered by the other's.
-    // The lanes of a pair take turns at O += P V of a tile with S of the next: left to themselves they fall into step,
-    // both at their exponentials (the pipe of these then takes 2048 cycles) and both at their products in turn.
+    // Of a pair's lanes one at a time has O += P V of a tile and S of the next: left to themselves they fall into step,
+    // both at their exponentials (the pipe of these then takes 2048 cycles) and both at their products.
     constexpr uint32_t kQk = pt_idesc(kPtRows, kPtRows, false), kPv = pt_idesc(kPtRows, kPtRows, true);
     const uint32_t q_lo = (smem_u32(smem) >> 4) + kPtDescK, ring_lo = smem_u32(ring) >> 4;
     const int l = warp - 1;
@@ -613,18 +637,20 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     w.start(p, worker(l));
     const uint32_t others = kPair ? 0 : p.w.starts[worker(1 - l)].count;
     // Ring position of V of the lane's tile i; K of the next is the one behind it.  Solo: both lanes' first K, then in
-    // turn V of a tile and K of the next, while there are any (the second lane has at most as many tiles).
+    // turn V of a tile and K of the next, while a lane has any.
     auto v_position = [&](uint32_t i) -> uint32_t {
       if (kPair) return 2 * i + 1;
-      if (l == 1) return 4 * i + (i + 1 == others ? 3 : 4);
-      return 1 + 2 * i + (others > 0 ? 1 + min(i, others) + min(i, others - 1) : 0);
+      const uint32_t j = i + l;  // turns that the other lane had
+      return 1 + 2 * i + (others > 0 ? 1 + min(j, others) + min(j, others - 1) : 0);
     };
     auto arrived = [&](uint64_t& b, uint32_t phase) {  // the same answer in every lane
       return __all_sync(0xffffffffu, mbar_wait(&b, phase & 1, kErrTimeoutMma)) != 0;
     };
     uint32_t tiles = 0, parts = 0;  // products S, blocks so far
     bool started = false;           // O holds something of the current block
-    uint32_t c = kPair ? 0 : l;     // ring position
+    uint32_t c = !kPair && l == 1 && others > 0;  // ring position
+    bool held = false;              // the lock on the products
+    bool ahead = false;             // K of the next tile is known to be there
     uint32_t seen = 0;              // bit s: parity of what this lane has had in slot s
     auto filled = [&](uint32_t s) {
       const uint32_t phase = seen >> s;
@@ -635,7 +661,8 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       const bool rows = has_rows(l, w.ntok);
       // S = Q K^T
       uint32_t s = c % kPtSlots;
-      ok = filled(s);
+      ok = ahead || filled(s);
+      ahead = false;
       if (ok && rows && w.fresh) ok = arrived(bar.q_full[l], parts++);
       if (!ok) break;
       tc_fence_after();
@@ -654,9 +681,10 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         } else {
           mbar_arrive(&bar.empty[s]);
         }
-        if (kPair && i > 0) mbar_arrive(&bar.turn[1 - l]);
+        if (held) atomicExch(&bar.lock, 0u);
       }
       __syncwarp();
+      held = false;
       tiles += rows;
       // O += P V
       c = v_position(i);
@@ -680,8 +708,15 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           if (kTerms == 2) pt_mma_ts(o, pk + 16, va + k * 128, kPv, 1);
         };
         ok = arrived(bar.p_full[l], tiles - 1);
-        if (kPair && ok && l + i > 0) ok = arrived(bar.turn[l], i - 1 + l);
         if (!ok) break;
+        if (kPair) {  // held until S of the next tile is issued
+          // its K first: it may have to wait for a slot that the other lane has yet to release
+          if (w.left > 1) ok = ahead = filled((c + 1) % kPtSlots);
+          if (!ok) break;
+          if (lane == 0) pt_lock(&bar.lock);
+          __syncwarp();
+          held = true;
+        }
         tc_fence_after();
         if (lane == 0) {
           if (steps == 8) {
@@ -695,14 +730,17 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           if (w.last()) umma_commit(&bar.o_full[l]);
         }
         started = started || steps > 0;
-      } else {
-        if (kPair && l + i > 0) ok = arrived(bar.turn[l], i - 1 + l);
-        if (lane == 0) mbar_arrive(&bar.empty[s]);
+      } else if (lane == 0) {
+        mbar_arrive(&bar.empty[s]);
       }
       __syncwarp();
       ++c;
       w.next();
-      if (kPair && w.left == 0 && lane == 0) mbar_arrive(&bar.turn[1 - l]);
+      // (not over a wait for rows of Q, which come when the block before has its scores)
+      if (held && (w.left == 0 || w.fresh)) {
+        if (lane == 0) atomicExch(&bar.lock, 0u);
+        held = false;
+      }
     }
     if (lane == 0) {  // all issued products must finish before the TMEM is released
       umma_commit(&bar.done);
@@ -979,9 +1017,9 @@ __global__ void __launch_bounds__(128) pt_join_prompts_kernel(const PtArgs p) {
   const int i = blockIdx.x + 1, j = threadIdx.x >> 2;
   const PtStart s = p.w.starts[i];
   const int64_t chunk = p.w.sums->chunk;
-  if (s.count == 0 || s.tile == 0 || s.tile > chunk) return;
+  if (s.tile == 0 || s.tile > chunk) return;
   const PtBlock b = p.w.blocks[s.block];
-  const int last = i - 1 + static_cast<int>((chunk - s.tile + b.tiles - 1) / chunk);
+  const int last = i - 1 + static_cast<int>((chunk - s.tile + b.tiles - 1) / chunk);  // with the last tile
   const int per = p.TB * p.G;  // rows of a lane
   for (int r = blockIdx.y * 4 + (threadIdx.x & 3); r < b.ntok * p.G; r += 4 * kPtJoinSplit) {
     const int l = kPair && r >= per;
@@ -1006,7 +1044,7 @@ __global__ void __launch_bounds__(128) pt_join_decode_kernel(const PtArgs p) {
   if (of >= 0) common = p.w.blocks[of], common_at = p.w.before[of];
   // the workers of a block: first and last
   auto workers = [&](int64_t before, int tiles, int& first, int& last) {
-    const int64_t at = before * p.Hkv + static_cast<int64_t>(h) * tiles;
+    const int64_t at = before * p.Hkv + static_cast<int64_t>(h) * pt_cost(tiles);
     first = static_cast<int>(at / sums.chunk);
     last = first + static_cast<int>((at - first * sums.chunk + tiles - 1) / sums.chunk);
   };
