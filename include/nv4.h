@@ -426,7 +426,7 @@ int nv4_append_kv(const void* q, const void* k, const void* v, const void* q_wei
  * token may be anything.  At most NV4_PAGED_MAX_GROUP query heads per KV head;
  * (tokens + 2 * batch) * max_pages * num_kv_heads up to 2^36.
  * Statistics and sums in FP32, the probabilities rounded to BF16 once for the
- * product with V.  All pointers 16-byte aligned (the int32 ones 4).
+ * product with V.  All pointers 16-byte aligned (out 32, the int32 ones 4).
  */
 #define NV4_PAGED_MAX_GROUP 16
 #define NV4_PAGED_MAX_TOKENS (1 << 22)

@@ -592,7 +592,7 @@ int check_paged_attention(const void* q, const void* k_cache, const void* v_cach
   // key tiles of all blocks of rows and heads: a worker counts its share in 32 bits
   if ((rows + 2 * batch) * max_pages > (int64_t(1) << 36) / num_kv_heads) return NV4_ERR_UNSUPPORTED;
   if (workspace_bytes < wanted) return NV4_ERR_INVALID_ARGUMENT;
-  if (!aligned(q, 16) || !aligned(k_cache, 16) || !aligned(v_cache, 16) || !aligned(out, 16) ||
+  if (!aligned(q, 16) || !aligned(k_cache, 16) || !aligned(v_cache, 16) || !aligned(out, 32) ||
       !aligned(workspace, 16) || !aligned(block_tables, 4) || !aligned(context_lens, 4))
     return NV4_ERR_ALIGNMENT;
   // q and the cache are read again after other rows were written

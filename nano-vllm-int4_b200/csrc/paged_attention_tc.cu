@@ -30,8 +30,8 @@
 //   warp 0     copies K and V tiles (TMA, five slots of 32 KB) in the order of use
 //   warps 1-2  issue S = Q K^T, O += P V of a lane each;  V rows behind the last token of
 //              a request are cleared first (0 times an old NaN would be one)
-//   warps 4-19 softmax of the two lanes; outputs; one thread of a lane copies its rows
-//              of Q (TMA: [tokens][G heads][128 channels])
+//   warp 3     copies the lanes' rows of Q (TMA: [tokens][G heads][128 channels])
+//   warps 4-19 softmax of the two lanes; outputs
 // P goes back to TMEM over its scores.  Decode is bound by the cache's bytes: there P is
 // multiplied in two BF16 terms (the upper 16 bits of the FP32 value and of the rest, 2^-14
 // of it at most left out), so that the output's own rounding
@@ -416,6 +416,22 @@ __device__ __forceinline__ void pt_lock(uint32_t* lock) {
     if (atomicCAS(lock, 0u, 1u) == 0) return;
 }
 
+__device__ __forceinline__ bool pt_passed(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// 32 bytes in one store
+__device__ __forceinline__ void pt_store32(void* dst, const uint32_t (&v)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+
 // The tiles of a worker, in order.  The next block's record is loaded a block ahead.
 struct PtWalk {
   const PtBlock* blocks;
@@ -505,7 +521,7 @@ struct PtBars {
   // A slot's arrival is told to the lane that it is for by a barrier of the lane's own (of a pair: one for both): on a
   // shared one a lane could take the phase before last of a slot, which the other lane has yet to see, for its own.
   uint64_t full[2][kPtSlots], empty[kPtSlots];
-  uint64_t q_full[2], s_full[2], p_full[2], o_full[2], done;
+  uint64_t q_full[2], q_free[2], s_full[2], p_full[2], o_full[2], done;
   uint32_t tmem, lock;
   int slot_keys[kPtSlots];  // keys of the slot's tile that exist
   int lane_keys[2];         // of the tile whose scores lie in the lane
@@ -531,6 +547,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bar.q_full[i], 1);
+      mbar_init(&bar.q_free[i], 1);
       mbar_init(&bar.s_full[i], 2);  // the products' completion, and lane_keys
       mbar_init(&bar.p_full[i], 8);  // the warps of the lane
       mbar_init(&bar.o_full[i], 1);
@@ -626,99 +643,87 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       }
     }
   } else if (warp < 3) {
-    // ---------------- products of a lane: S of a tile, O += P V; the whole warp walks, its lane 0 issues.  A warp for
-    // each lane: the tensor cores take few products ahead, so what one waits for in between is covered by the other's.
-    // Of a pair's lanes one at a time has O += P V of a tile and S of the next: left to themselves they fall into step,
-    // both at their exponentials (the pipe of these then takes 2048 cycles) and both at their products.
-    constexpr uint32_t kQk = pt_idesc(kPtRows, kPtRows, false), kPv = pt_idesc(kPtRows, kPtRows, true);
-    const uint32_t q_lo = (smem_u32(smem) >> 4) + kPtDescK, ring_lo = smem_u32(ring) >> 4;
-    const int l = warp - 1;
-    PtSteps w;
-    w.start(p, worker(l));
-    const uint32_t others = kPair ? 0 : p.w.starts[worker(1 - l)].count;
-    // Ring position of V of the lane's tile i; K of the next is the one behind it.  Solo: both lanes' first K, then in
-    // turn V of a tile and K of the next, while a lane has any.
-    auto v_position = [&](uint32_t i) -> uint32_t {
-      if (kPair) return 2 * i + 1;
-      const uint32_t j = i + l;  // turns that the other lane had
-      return 1 + 2 * i + (others > 0 ? 1 + min(j, others) + min(j, others - 1) : 0);
-    };
-    auto arrived = [&](uint64_t& b, uint32_t phase) {  // the same answer in every lane
-      return __all_sync(0xffffffffu, mbar_wait(&b, phase & 1, kErrTimeoutMma)) != 0;
-    };
-    uint32_t tiles = 0, parts = 0;  // products S, blocks so far
-    bool started = false;           // O holds something of the current block
-    uint32_t c = !kPair && l == 1 && others > 0;  // ring position
-    bool held = false;              // the lock on the products
-    bool ahead = false;             // K of the next tile is known to be there
-    uint32_t seen = 0;              // bit s: parity of what this lane has had in slot s
-    auto filled = [&](uint32_t s) {
-      const uint32_t phase = seen >> s;
-      seen ^= 1u << s;
-      return arrived(bar.full[kPair ? 0 : l][s], phase);
-    };
-    for (uint32_t i = 0; ok && w.left > 0; ++i) {
-      const bool rows = has_rows(l, w.ntok);
+    // ---------------- products of a lane: S of a tile, O += P V, all by one thread.  A warp for each lane: the tensor
+    // cores take few products ahead, so what one waits for in between is covered by the other's.  Of a pair's lanes one at
+    // a time has its O += P V with the next S: left to themselves they fall into step, both at their exponentials (the
+    // pipe of these then takes 2048 cycles) and both at their products (a tile of both 5200 cycles instead of 4000).
+    if (lane == 0) {
+      constexpr uint32_t kQk = pt_idesc(kPtRows, kPtRows, false), kPv = pt_idesc(kPtRows, kPtRows, true);
+      const uint32_t q_lo = (smem_u32(smem) >> 4) + kPtDescK, ring_lo = smem_u32(ring) >> 4;
+      const int l = warp - 1;
+      PtSteps w;
+      w.start(p, worker(l));
+      const uint32_t others = kPair ? 0 : p.w.starts[worker(1 - l)].count;
+      // Ring position of V of the lane's tile i; K of the next is the one behind it.  Solo: both lanes' first K, then in
+      // turn V of a tile and K of the next, while a lane has any.
+      auto v_position = [&](uint32_t i) -> uint32_t {
+        if (kPair) return 2 * i + 1;
+        const uint32_t j = i + l;  // turns that the other lane had
+        return 1 + 2 * i + (others > 0 ? 1 + min(j, others) + min(j, others - 1) : 0);
+      };
+      auto arrived = [&](uint64_t& b, uint32_t phase) { return mbar_wait(&b, phase & 1, kErrTimeoutMma); };
+      uint32_t parts = 0, seen = 0;  // blocks so far; bit s: parity of what this lane has had in slot s
+      auto filled = [&](uint32_t s) {
+        const uint32_t phase = seen >> s;
+        seen ^= 1u << s;
+        return arrived(bar.full[kPair ? 0 : l][s], phase);
+      };
+      // K of the walk's tile, in slot s, and with a block's first tile its rows of Q
+      auto ready = [&](uint32_t s, bool rows) { return filled(s) && (!rows || !w.fresh || arrived(bar.q_full[l], parts++)); };
       // S = Q K^T
-      uint32_t s = c % kPtSlots;
-      ok = ahead || filled(s);
-      ahead = false;
-      if (ok && rows && w.fresh) ok = arrived(bar.q_full[l], parts++);
-      if (!ok) break;
-      tc_fence_after();
-      if (lane == 0) {
-        if (rows) {
-          bar.lane_keys[l] = bar.slot_keys[s];  // before the slot can be released
-          const uint32_t qa = q_lo + l * (kPtTile >> 4), ka = ring_lo + s * (kPtTile >> 4) + kPtDescK;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const uint32_t off = (j >> 2) * kPtHalfLo + (j & 3) * 2;
-            pt_mma_ss(l * 256, qa + off, ka + off, kQk, j > 0);
-          }
-          umma_commit(&bar.s_full[l]);
-          mbar_arrive(&bar.s_full[l]);
-          umma_commit(&bar.empty[s]);
-        } else {
+      auto scores = [&](uint32_t s, bool rows) {
+        if (!rows) {
           mbar_arrive(&bar.empty[s]);
-        }
-        if (held) atomicExch(&bar.lock, 0u);
-      }
-      __syncwarp();
-      held = false;
-      tiles += rows;
-      // O += P V
-      c = v_position(i);
-      s = c % kPtSlots;
-      ok = filled(s);
-      if (!ok) break;
-      if (rows) {
-        const int keys = bar.slot_keys[s], steps = (keys + 15) / 16;
-        if (keys & 15) {  // rows behind the last key: P is zero there, V may be anything
-          for (int e = lane; e < (steps * 16 - keys) * 16; e += 32)
-            *reinterpret_cast<uint4*>(ring + s * kPtTile + (e & 8 ? kPtHalf : 0) + (keys + (e >> 4)) * 128 +
-                                      (e & 7) * 16) = make_uint4(0, 0, 0, 0);
-          fence_proxy_async_smem();
-        }
-        if (w.fresh) started = false;
-        const uint32_t va = ring_lo + s * (kPtTile >> 4) + kPtDescV, o = l * 256 + 128;
-        // 16 keys: the terms of P against the same rows of V
-        auto step = [&](int k, uint32_t accumulate) {
-          const uint32_t pk = l * 256 + (kTerms == 1 ? (k >> 2) * 64 + (k & 3) * 8 : (k >> 1) * 32 + (k & 1) * 8);
-          pt_mma_ts(o, pk, va + k * 128, kPv, accumulate);
-          if (kTerms == 2) pt_mma_ts(o, pk + 16, va + k * 128, kPv, 1);
-        };
-        ok = arrived(bar.p_full[l], tiles - 1);
-        if (!ok) break;
-        if (kPair) {  // held until S of the next tile is issued
-          // its K first: it may have to wait for a slot that the other lane has yet to release
-          if (w.left > 1) ok = ahead = filled((c + 1) % kPtSlots);
-          if (!ok) break;
-          if (lane == 0) pt_lock(&bar.lock);
-          __syncwarp();
-          held = true;
+          return;
         }
         tc_fence_after();
-        if (lane == 0) {
+        bar.lane_keys[l] = bar.slot_keys[s];  // before the slot can be released
+        const uint32_t qa = q_lo + l * (kPtTile >> 4), ka = ring_lo + s * (kPtTile >> 4) + kPtDescK;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const uint32_t off = (j >> 2) * kPtHalfLo + (j & 3) * 2;
+          pt_mma_ss(l * 256, qa + off, ka + off, kQk, j > 0);
+        }
+        umma_commit(&bar.s_full[l]);
+        mbar_arrive(&bar.s_full[l]);
+        umma_commit(&bar.empty[s]);
+        if (w.last()) umma_commit(&bar.q_free[l]);
+      };
+      bool rows = has_rows(l, w.ntok), started = false;  // started: O holds something of the current block
+      uint32_t tiles = 0;                                // with rows, so far
+      uint32_t c = !kPair && l == 1 && others > 0;       // ring position
+      if (w.left > 0) {
+        ok = ready(c % kPtSlots, rows);
+        if (ok) scores(c % kPtSlots, rows);
+      }
+      for (uint32_t i = 0; ok && w.left > 0; ++i) {
+        // what O += P V and the next S need besides P
+        c = v_position(i);
+        const uint32_t s = c % kPtSlots, next = (c + 1) % kPtSlots;
+        const bool fresh = w.fresh, last = w.last(), now = rows;
+        if (!filled(s)) break;
+        w.next();
+        rows = has_rows(l, w.ntok);
+        if (w.left > 0 && !ready(next, rows)) break;
+        if (now) {
+          const int keys = bar.slot_keys[s], steps = (keys + 15) / 16;
+          if (keys & 15) {  // rows behind the last key: P is zero there, V may be anything
+            for (int e = 0; e < (steps * 16 - keys) * 16; ++e)
+              *reinterpret_cast<uint4*>(ring + s * kPtTile + (e & 8 ? kPtHalf : 0) + (keys + (e >> 4)) * 128 +
+                                        (e & 7) * 16) = make_uint4(0, 0, 0, 0);
+            fence_proxy_async_smem();
+          }
+          if (fresh) started = false;
+          const uint32_t va = ring_lo + s * (kPtTile >> 4) + kPtDescV, o = l * 256 + 128;
+          // 16 keys: the terms of P against the same rows of V
+          auto step = [&](int k, uint32_t accumulate) {
+            const uint32_t pk = l * 256 + (kTerms == 1 ? (k >> 2) * 64 + (k & 3) * 8 : (k >> 1) * 32 + (k & 1) * 8);
+            pt_mma_ts(o, pk, va + k * 128, kPv, accumulate);
+            if (kTerms == 2) pt_mma_ts(o, pk + 16, va + k * 128, kPv, 1);
+          };
+          if (!arrived(bar.p_full[l], tiles++)) break;
+          if (kPair) pt_lock(&bar.lock);
+          tc_fence_after();
           if (steps == 8) {
             step(0, started);
 #pragma unroll
@@ -727,23 +732,15 @@ __global__ void __launch_bounds__(kPtThreads, 1)
             for (int k = 0; k < steps; ++k) step(k, started || k > 0);
           }
           umma_commit(&bar.empty[s]);
-          if (w.last()) umma_commit(&bar.o_full[l]);
+          if (last) umma_commit(&bar.o_full[l]);
+          started = started || steps > 0;
+        } else {
+          mbar_arrive(&bar.empty[s]);
         }
-        started = started || steps > 0;
-      } else if (lane == 0) {
-        mbar_arrive(&bar.empty[s]);
+        if (w.left > 0) scores(next, rows);
+        if (kPair && now) atomicExch(&bar.lock, 0u);
       }
-      __syncwarp();
-      ++c;
-      w.next();
-      // (not over a wait for rows of Q, which come when the block before has its scores)
-      if (held && (w.left == 0 || w.fresh)) {
-        if (lane == 0) atomicExch(&bar.lock, 0u);
-        held = false;
-      }
-    }
-    if (lane == 0) {  // all issued products must finish before the TMEM is released
-      umma_commit(&bar.done);
+      umma_commit(&bar.done);  // all issued products must finish before the TMEM is released
       const uint64_t start = global_timer_ns();
       while (!mbar_try_wait(&bar.done, 0))
         if (global_timer_ns() - start > kWaitLimitNs) {
@@ -752,7 +749,57 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         }
     }
     __syncwarp();
-  } else if (warp >= 4) {
+  } else if (warp < 4) {
+    // ---------------- rows of Q of both lanes, by one thread.  The box takes as many tokens as a block can have; rows
+    // behind the block's last are never used.
+    if (lane == 0) {
+      PtWalk w[2];
+      int copied[2] = {0, 0};
+#pragma unroll
+      for (int l = 0; l < 2; ++l) {
+        w[l].start(p, worker(l));
+        while (w[l].left > 0 && !has_rows(l, w[l].b.ntok)) w[l].skip();
+      }
+      uint64_t start = global_timer_ns();
+      while (w[0].left > 0 || w[1].left > 0) {
+        bool any = false;
+#pragma unroll
+        for (int l = 0; l < 2; ++l) {
+          if (w[l].left <= 0 || (copied[l] > 0 && !pt_passed(&bar.q_free[l], (copied[l] - 1) & 1))) continue;
+          const bool one = w[l].b.kind == kPtOwn;
+          const CUtensorMap* map = one ? &tmap_q1 : &tmap_q;
+          const int token = w[l].b.tok0 + (kPair ? l * p.TB : 0);
+          uint8_t* dst = smem + l * kPtTile;
+          mbar_arrive_expect_tx(&bar.q_full[l], (one ? 1 : p.TB) * p.G * kPtRows * 2);
+          pt_load_q(dst, map, &bar.q_full[l], 0, w[l].head * p.G, token);
+          pt_load_q(dst + kPtHalf, map, &bar.q_full[l], 64, w[l].head * p.G, token);
+          ++copied[l];
+          do w[l].skip();
+          while (w[l].left > 0 && !has_rows(l, w[l].b.ntok));
+          any = true;
+        }
+        if (any) {
+          start = global_timer_ns();
+        } else {
+          __nanosleep(100);
+          if (error_raised()) break;
+          if (global_timer_ns() - start > kWaitLimitNs) {
+            record_error(kErrTimeoutEmpty);
+            break;
+          }
+        }
+      }
+#pragma unroll
+      for (int l = 0; l < 2; ++l) {  // the last copies must land before the CTA may exit
+        start = global_timer_ns();
+        while (copied[l] > 0 && !mbar_try_wait(&bar.q_full[l], (copied[l] - 1) & 1))
+          if (global_timer_ns() - start > kWaitLimitNs) {
+            record_error(kErrTimeoutDrain);
+            break;
+          }
+      }
+    }
+  } else {
     // ---------------- softmax and outputs: two threads a row (head r % G of its lane's token r / G), each with half of a
     // tile's keys, and of the output's channels at the end.  (With one thread a row the two warps of a scheduler left
     // two thirds of its issue slots empty.)
@@ -764,23 +811,6 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     const float c = p.c;
     PtWalk w;
     w.start(p, worker(l));
-    // Rows of Q of the first block at or behind v's with any, copied by one thread.  The box takes as many tokens as a
-    // block can have; rows behind the block's last are never used.
-    const bool copies = half == 1 && quarter == 3 && lane == 0;
-    int copied = 0;
-    auto load_q = [&](PtWalk v) {
-      while (v.left > 0 && !has_rows(l, v.b.ntok)) v.skip();
-      if (v.left <= 0) return;
-      const bool one = v.b.kind == kPtOwn;
-      const CUtensorMap* map = one ? &tmap_q1 : &tmap_q;
-      const int token = v.b.tok0 + (kPair ? l * p.TB : 0);
-      uint8_t* dst = smem + l * kPtTile;
-      mbar_arrive_expect_tx(&bar.q_full[l], (one ? 1 : p.TB) * p.G * kPtRows * 2);
-      pt_load_q(dst, map, &bar.q_full[l], 0, v.head * p.G, token);
-      pt_load_q(dst + kPtHalf, map, &bar.q_full[l], 64, v.head * p.G, token);
-      ++copied;
-    };
-    if (copies && w.left > 0) load_q(w);
     int tile = 0, part = 0, limit = 0, token = 0, head = 0, from = 0;
     bool live = false, started = false;
     float m = -INFINITY, sum = 0.0f;
@@ -803,11 +833,6 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       ok = ok && __all_sync(0xffffffffu, mbar_wait(&bar.s_full[l], tile & 1, kErrTimeoutMma));
       tc_fence_after();
       const int keys = *reinterpret_cast<volatile int*>(&bar.lane_keys[l]);
-      if (copies && w.last()) {  // the block's last scores are there: its Q is not needed any more
-        PtWalk v = w;
-        v.skip();
-        load_q(v);
-      }
       if (busy && keys > 0) {
         const int seen = min(max(limit - (w.b.key0 + w.tile * kPtRows), 0), keys);
         const bool edge = __any_sync(0xffffffffu, seen < kPtRows);
@@ -924,17 +949,17 @@ __global__ void __launch_bounds__(kPtThreads, 1)
             for (int j = 0; j < 32; ++j) o[j] = 0u;
           }
           if (live && final_) {
-            uint4* dst = reinterpret_cast<uint4*>(p.out + row * kPtRows + half * 64 + 32 * i);
+            uint16_t* dst = p.out + row * kPtRows + half * 64 + 32 * i;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              uint32_t v[4];
+            for (int j = 0; j < 2; ++j) {
+              uint32_t v[8];
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const __nv_bfloat162 b = __floats2bfloat162_rn(__uint_as_float(o[8 * j + 2 * e]) * f,
-                                                               __uint_as_float(o[8 * j + 2 * e + 1]) * f);
+              for (int e = 0; e < 8; ++e) {
+                const __nv_bfloat162 b = __floats2bfloat162_rn(__uint_as_float(o[16 * j + 2 * e]) * f,
+                                                               __uint_as_float(o[16 * j + 2 * e + 1]) * f);
                 v[e] = *reinterpret_cast<const uint32_t*>(&b);
               }
-              dst[j] = make_uint4(v[0], v[1], v[2], v[3]);
+              pt_store32(dst + 16 * j, v);
             }
           } else if (live) {
 #pragma unroll
@@ -947,14 +972,6 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         if (live && !final_ && half == 0) *reinterpret_cast<float2*>(pm) = make_float2(m, sum);
       }
       tc_fence_before();
-    }
-    if (copies && copied > 0) {  // the last copy must land before the CTA may exit
-      const uint64_t start = global_timer_ns();
-      while (!mbar_try_wait(&bar.q_full[l], (copied - 1) & 1))
-        if (global_timer_ns() - start > kWaitLimitNs) {
-          record_error(kErrTimeoutDrain);
-          break;
-        }
     }
   }
   tc_fence_before();
