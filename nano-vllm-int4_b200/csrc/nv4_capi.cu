@@ -543,6 +543,7 @@ int nv4_append_kv(const void* q, const void* k, const void* v, const void* q_wei
     return NV4_ERR_INVALID_ARGUMENT;
   if (head_dim != 128 || page_size != 256 || rotary_dim < 16 || rotary_dim > 128 || rotary_dim % 16)
     return NV4_ERR_UNSUPPORTED;
+  if (tokens * (num_heads + 2 * num_kv_heads) > int64_t(1) << 34) return NV4_ERR_INVALID_ARGUMENT;
   const int64_t most = int64_t(1) << 32;
   if (k_stride < num_kv_heads * 128 || v_stride < num_kv_heads * 128 || (q && q_stride < num_heads * 128) ||
       k_stride > most || v_stride > most || (q && q_stride > most))

@@ -15,9 +15,8 @@ constexpr int kPaPage = 256;
 // With y = x * rsqrt(mean(x^2) + eps) * w (or x without a norm), channels c and c +
 // R/2 of the first R are rotated, (a, b) -> (a cos - b sin, b cos + a sin); FP32
 // throughout, one rounding to BF16.  The lane of channel c + R/2 is R/16 lanes on.
-// A CTA takes a token, its half warps the heads in turn, so that cos and sin are
-// loaded once a lane; four rows are in flight a half warp.  Bound by HBM for long
-// prompts, by launch and one chain of loads (position, cos) for few tokens.
+// A half warp takes kRows rows of a token: their loads go out first, then the position
+// and slot, then cos and sin, so that two loads in a row are what a warp waits for.
 struct AppendArgs {
   const uint16_t* q;
   const uint16_t* k;
@@ -36,102 +35,101 @@ struct AppendArgs {
 };
 
 constexpr int kAppendThreads = 256;
-constexpr int kAppendRows = 4;  // rows in flight of a half warp
 
 __device__ __forceinline__ void unpack8(const uint4& r, float (&x)[8]) {
   x[0] = bf16lo_to_f32(r.x), x[1] = bf16hi_to_f32(r.x), x[2] = bf16lo_to_f32(r.y), x[3] = bf16hi_to_f32(r.y);
   x[4] = bf16lo_to_f32(r.z), x[5] = bf16hi_to_f32(r.z), x[6] = bf16lo_to_f32(r.w), x[7] = bf16hi_to_f32(r.w);
 }
 
-__global__ void __launch_bounds__(kAppendThreads) append_kv_kernel(const AppendArgs p) {
-  const int half = threadIdx.x >> 4, lane = threadIdx.x & 15;
+template <int kRows>
+__global__ void __launch_bounds__(kAppendThreads, 4) append_kv_kernel(const AppendArgs p) {
+  const int lane = threadIdx.x & 15;
   const int heads = p.Hq + 2 * p.Hkv, hl = p.half_lanes;
+  const uint32_t groups = (heads + kRows - 1) / kRows;
+  const int64_t unit = (static_cast<int64_t>(blockIdx.x) * kAppendThreads + threadIdx.x) >> 4;
+  // a half warp behind the last row works on it once more (every lane takes part in the shuffles) and stores nothing
+  const bool live = unit < p.tokens * groups;
+  const int64_t t = live ? unit / groups : p.tokens - 1;
+  const int h0 = static_cast<int>(live ? unit - t * groups : 0) * kRows;
+  uint4 raw[kRows];
+#pragma unroll
+  for (int j = 0; j < kRows; ++j) {
+    const int h = min(h0 + j, heads - 1);
+    const uint16_t* src = h < p.Hq           ? p.q + t * p.q_stride + h * kPaD
+                          : h < p.Hq + p.Hkv ? p.k + t * p.k_stride + (h - p.Hq) * kPaD
+                                             : p.v + t * p.v_stride + (h - p.Hq - p.Hkv) * kPaD;
+    raw[j] = *(reinterpret_cast<const uint4*>(src) + lane);
+  }
+  const int64_t pos = p.positions[t];
+  const int64_t slot = p.slots[t];
+  const bool known = pos >= 0 && pos < p.max_position, store = slot >= 0 && slot < p.num_slots;
+  if (live && h0 == 0 && lane == 0) {
+    if (!known) record_index_error(kErrBadPosition);
+    if (slot >= p.num_slots) record_index_error(kErrBadSlot);
+  }
   const bool first = lane < hl, turned = lane < 2 * hl;
   const int partner = (threadIdx.x & 16) + (first ? lane + hl : lane - hl);
-  float qw[8], kw[8];
+  float c[8], s[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) qw[i] = kw[i] = 1.0f;
-  if (p.q_weight) unpack8(__ldg(reinterpret_cast<const uint4*>(p.q_weight) + lane), qw);
-  if (p.k_weight) unpack8(__ldg(reinterpret_cast<const uint4*>(p.k_weight) + lane), kw);
-  for (int64_t t = blockIdx.x; t < p.tokens; t += gridDim.x) {
-    const int64_t pos = p.positions[t];
-    const int64_t slot = p.slots ? p.slots[t] : -1;
-    const bool known = pos >= 0 && pos < p.max_position;
-    if (threadIdx.x == 0) {
-      if (!known) record_index_error(kErrBadPosition);
-      if (slot >= p.num_slots) record_index_error(kErrBadSlot);
-    }
-    const bool store = slot >= 0 && slot < p.num_slots;
-    float c[8], s[8];
-    {
-      const int at = (first ? lane : lane - hl) * 8;
+  for (int i = 0; i < 8; ++i) c[i] = known ? 1.0f : __int_as_float(0x7FFFFFFF), s[i] = 0.0f;
+  if (turned && known && h0 < p.Hq + p.Hkv) {
+    const float4* row =
+        reinterpret_cast<const float4*>(p.cos_sin + pos * (16 * hl) + (first ? lane : lane - hl) * 8);
+    const float4 c0 = __ldg(row), c1 = __ldg(row + 1), s0 = __ldg(row + 2 * hl), s1 = __ldg(row + 2 * hl + 1);
+    c[0] = c0.x, c[1] = c0.y, c[2] = c0.z, c[3] = c0.w, c[4] = c1.x, c[5] = c1.y, c[6] = c1.z, c[7] = c1.w;
+    s[0] = s0.x, s[1] = s0.y, s[2] = s0.z, s[3] = s0.w, s[4] = s1.x, s[5] = s1.y, s[6] = s1.z, s[7] = s1.w;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) c[i] = 1.0f, s[i] = 0.0f;
-      if (turned && known) {
-        const float4* row = reinterpret_cast<const float4*>(p.cos_sin + pos * (16 * hl) + at);
-        const float4 c0 = __ldg(row), c1 = __ldg(row + 1), s0 = __ldg(row + 2 * hl), s1 = __ldg(row + 2 * hl + 1);
-        c[0] = c0.x, c[1] = c0.y, c[2] = c0.z, c[3] = c0.w, c[4] = c1.x, c[5] = c1.y, c[6] = c1.z, c[7] = c1.w;
-        s[0] = s0.x, s[1] = s0.y, s[2] = s0.z, s[3] = s0.w, s[4] = s1.x, s[5] = s1.y, s[6] = s1.z, s[7] = s1.w;
-        if (first) {
+    for (int i = 0; i < 8; ++i) s[i] = first ? -s[i] : s[i];
+  }
 #pragma unroll
-          for (int i = 0; i < 8; ++i) s[i] = -s[i];
-        }
-      }
-      if (!known) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) c[i] = __int_as_float(0x7FFFFFFF);
-      }
-    }
-    for (int h0 = half; h0 < heads; h0 += kAppendRows * (kAppendThreads / 16)) {
-      uint4 raw[kAppendRows];
-#pragma unroll
-      for (int j = 0; j < kAppendRows; ++j) {
-        const int h = h0 + j * (kAppendThreads / 16);
-        if (h >= heads) continue;
-        const uint16_t* src = h < p.Hq           ? p.q + t * p.q_stride + h * kPaD
-                              : h < p.Hq + p.Hkv ? p.k + t * p.k_stride + (h - p.Hq) * kPaD
-                                                 : p.v + t * p.v_stride + (h - p.Hq - p.Hkv) * kPaD;
-        raw[j] = *(reinterpret_cast<const uint4*>(src) + lane);
-      }
-#pragma unroll
-      for (int j = 0; j < kAppendRows; ++j) {
-        const int h = h0 + j * (kAppendThreads / 16);
-        const bool live = h < heads;  // the two rows of a warp may differ: every lane takes part in the shuffles
-        const bool is_q = h < p.Hq, is_v = h >= p.Hq + p.Hkv;
-        if (!__any_sync(0xffffffffu, live)) break;
-        float x[8];
-        unpack8(live ? raw[j] : make_uint4(0, 0, 0, 0), x);
-        const bool normed = is_q ? p.q_weight != nullptr : p.k_weight != nullptr;
+  for (int j = 0; j < kRows; ++j) {
+    const int h = h0 + j;
+    const bool is_q = h < p.Hq, is_v = h >= p.Hq + p.Hkv;
+    uint4 out = raw[j];
+    if (__any_sync(0xffffffffu, !is_v)) {
+      float x[8];
+      unpack8(raw[j], x);
+      const uint16_t* weight = is_q ? p.q_weight : p.k_weight;
+      if (p.q_weight || p.k_weight) {
         float ss = 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
 #pragma unroll
         for (int m = 8; m >= 1; m >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
-        const float r = normed ? rsqrtf(ss * (1.0f / kPaD) + p.eps) : 1.0f;
-        uint32_t packed[4];
-        float y[8];
+        if (weight) {
+          const float r = rsqrtf(ss * (1.0f / kPaD) + p.eps);
+          float w[8];
+          unpack8(__ldg(reinterpret_cast<const uint4*>(weight) + lane), w);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float a = x[i] * r * (is_q ? qw[i] : kw[i]);
-          const float b = __shfl_sync(0xffffffffu, a, partner);
-          y[i] = turned ? fmaf(a, c[i], b * s[i]) : a * c[i];
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const __nv_bfloat162 o = __floats2bfloat162_rn(y[2 * i], y[2 * i + 1]);
-          packed[i] = *reinterpret_cast<const uint32_t*>(&o);
-        }
-        if (!live) continue;
-        const uint4 out = is_v ? raw[j] : make_uint4(packed[0], packed[1], packed[2], packed[3]);
-        if (is_q) {
-          *(reinterpret_cast<uint4*>(p.q_out + (t * p.Hq + h) * kPaD) + lane) = out;
-        } else if (store) {
-          const int kh = h - p.Hq - (is_v ? p.Hkv : 0);
-          *(reinterpret_cast<uint4*>((is_v ? p.v_cache : p.k_cache) + (slot * p.Hkv + kh) * kPaD) + lane) = out;
+          for (int i = 0; i < 8; ++i) x[i] = x[i] * r * w[i];
         }
       }
+      uint32_t packed[4];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float b = __shfl_sync(0xffffffffu, x[i], partner);
+        const float y = turned ? fmaf(x[i], c[i], b * s[i]) : x[i] * c[i];
+        const uint32_t bits = __bfloat16_as_ushort(__float2bfloat16_rn(y));
+        packed[i / 2] = i % 2 ? packed[i / 2] | bits << 16 : bits;
+      }
+      if (!is_v) out = make_uint4(packed[0], packed[1], packed[2], packed[3]);
+    }
+    if (!live || h >= heads) continue;
+    if (is_q) {
+      *(reinterpret_cast<uint4*>(p.q_out + (t * p.Hq + h) * kPaD) + lane) = out;
+    } else if (store) {
+      const int kh = h - p.Hq - (is_v ? p.Hkv : 0);
+      *(reinterpret_cast<uint4*>((is_v ? p.v_cache : p.k_cache) + (slot * p.Hkv + kh) * kPaD) + lane) = out;
     }
   }
+}
+
+template <int kRows>
+static int launch_append_rows(const AppendArgs& a, cudaStream_t stream) {
+  const int64_t units = a.tokens * ((a.Hq + 2 * a.Hkv + kRows - 1) / kRows);
+  const int64_t blocks = (units * 16 + kAppendThreads - 1) / kAppendThreads;
+  return launch_kernel(append_kv_kernel<kRows>, dim3(static_cast<unsigned>(blocks)), dim3(kAppendThreads), 0, stream,
+                       false, a);
 }
 
 int launch_append_kv(const void* q, const void* k, const void* v, const void* q_weight, const void* k_weight,
@@ -161,8 +159,10 @@ int launch_append_kv(const void* q, const void* k, const void* v, const void* q_
   a.Hkv = static_cast<int>(num_kv_heads);
   a.half_lanes = static_cast<int>(rotary_dim / 16);
   a.eps = eps;
-  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(tokens, int64_t(1) << 30));
-  return launch_kernel(append_kv_kernel, dim3(grid), dim3(kAppendThreads), 0, stream, false, a);
+  // One row a half warp while these fit the SMs twice over (shorter chains), else four (fewer loads of cos and sin).
+  const int64_t rows = tokens * (a.Hq + 2 * num_kv_heads);
+  return rows <= 2 * 148 * 4 * (kAppendThreads / 16) ? launch_append_rows<1>(a, stream)
+                                                     : launch_append_rows<4>(a, stream);
 }
 
 }  // namespace nv4

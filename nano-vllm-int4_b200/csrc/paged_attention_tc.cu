@@ -704,7 +704,8 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         if (!filled(s)) break;
         w.next();
         rows = has_rows(l, w.ntok);
-        if (w.left > 0 && !ready(next, rows)) break;
+        // (solo: K may be on its way from memory, and the slot of V is wanted)
+        if (kPair && w.left > 0 && !ready(next, rows)) break;
         if (now) {
           const int keys = bar.slot_keys[s], steps = (keys + 15) / 16;
           if (keys & 15) {  // rows behind the last key: P is zero there, V may be anything
@@ -737,6 +738,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         } else {
           mbar_arrive(&bar.empty[s]);
         }
+        if (!kPair && w.left > 0 && !ready(next, rows)) break;
         if (w.left > 0) scores(next, rows);
         if (kPair && now) atomicExch(&bar.lock, 0u);
       }
@@ -781,7 +783,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         if (any) {
           start = global_timer_ns();
         } else {
-          __nanosleep(100);
+          __nanosleep(20);
           if (error_raised()) break;
           if (global_timer_ns() - start > kWaitLimitNs) {
             record_error(kErrTimeoutEmpty);
