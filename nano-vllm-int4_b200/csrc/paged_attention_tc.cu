@@ -108,43 +108,48 @@ struct PtArgs {
 };
 
 // ------------------------------------------------------------ block table
-// Sum over the CTA of values before this thread's; `total` is that of all.
-__device__ __forceinline__ int64_t pt_scan(int64_t v, int64_t* warp_sums, int64_t& total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int64_t x = v;
+// The block table is made by one CTA, whose time is latency: few warps, sums of warps by shuffles.
+constexpr int kPtPlanThreads = 512;
+constexpr int kPtPlanWarps = kPtPlanThreads / 32;
+constexpr int kPtPlanCached = 2048;  // blocks whose sums are kept in shared memory for the search
+
+__device__ __forceinline__ int64_t pt_warp_scan(int64_t x) {
+  const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int m = 1; m < 32; m <<= 1) {
     const int64_t y = __shfl_up_sync(0xffffffffu, x, m);
     if (lane >= m) x += y;
   }
+  return x;
+}
+
+// Sums over the CTA of values before this thread's (two at once); `all` those of all threads.
+__device__ __forceinline__ longlong2 pt_scan(int64_t v, int64_t w, int64_t (&sums)[2][kPtPlanWarps], longlong2& all) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t x = pt_warp_scan(v), y = pt_warp_scan(w);
   __syncthreads();
-  if (lane == 31) warp_sums[warp] = x;
+  if (lane == 31) sums[0][warp] = x, sums[1][warp] = y;
   __syncthreads();
-  int64_t before = 0;
-  total = 0;
-  for (int i = 0; i < 32; ++i) {
-    if (i < warp) before += warp_sums[i];
-    total += warp_sums[i];
-  }
-  return before + x - v;
+  const int64_t a = pt_warp_scan(lane < kPtPlanWarps ? sums[0][lane] : 0);
+  const int64_t b = pt_warp_scan(lane < kPtPlanWarps ? sums[1][lane] : 0);
+  all.x = __shfl_sync(0xffffffffu, a, 31), all.y = __shfl_sync(0xffffffffu, b, 31);
+  const int64_t before = __shfl_sync(0xffffffffu, a, max(warp - 1, 0)), before2 = __shfl_sync(0xffffffffu, b, max(warp - 1, 0));
+  return make_longlong2((warp ? before : 0) + x - v, (warp ? before2 : 0) + y - w);
 }
 
 // Running maximum up to this thread, `carry` that of the threads before (updated).
-__device__ __forceinline__ int pt_max_scan(int v, int* warp_max, int& carry) {
+__device__ __forceinline__ int pt_max_scan(int v, int (&maxima)[kPtPlanWarps], int& carry) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int x = v;
 #pragma unroll
   for (int m = 1; m < 32; m <<= 1) x = max(x, __shfl_up_sync(0xffffffffu, x, m));
   __syncthreads();
-  if (lane == 31) warp_max[warp] = x;
+  if (lane == 31) maxima[warp] = x;
   __syncthreads();
-  int all = carry;
-  x = max(x, carry);
-  for (int i = 0; i < 32; ++i) {
-    if (i < warp) x = max(x, warp_max[i]);
-    all = max(all, warp_max[i]);
-  }
-  carry = all;
+  const int m = lane < kPtPlanWarps ? maxima[lane] : 0;
+  const int before = __reduce_max_sync(0xffffffffu, lane < warp ? m : 0);
+  x = max(max(x, before), carry);
+  carry = max(carry, __reduce_max_sync(0xffffffffu, m));
   return x;
 }
 
@@ -153,12 +158,9 @@ __device__ __forceinline__ int pt_tiles(int keys) { return max(1, (keys + kPtRow
 constexpr int kPtBlockCost = 1;
 __device__ __forceinline__ int pt_cost(int tiles) { return tiles + kPtBlockCost; }
 
-constexpr int kPtPlanThreads = 1024;
-constexpr int kPtPlanCached = 2048;  // blocks whose sums are kept in shared memory for the search
-
 __global__ void __launch_bounds__(kPtPlanThreads) pt_plan_kernel(const PtArgs p, const int block_tokens) {
-  __shared__ int64_t sums[32];
-  __shared__ int maxima[32];
+  __shared__ int64_t sums[2][kPtPlanWarps];
+  __shared__ int maxima[kPtPlanWarps];
   __shared__ int first[kPtPlanThreads], last[kPtPlanThreads], extra[kPtPlanThreads], which[kPtPlanThreads];
   __shared__ int table_row[kPtPlanThreads];
   __shared__ int64_t weight[kPtPlanThreads];
@@ -187,7 +189,7 @@ __global__ void __launch_bounds__(kPtPlanThreads) pt_plan_kernel(const PtArgs p,
       extra[tid] = live ? max(p.context[b], 0) : 0;
       __syncthreads();
       const int here = min(kPtPlanThreads, p.batch - b0);
-      for (int s = warp; s < here; s += kPtPlanThreads / 32) {
+      for (int s = warp; s < here; s += kPtPlanWarps) {
         const int n = last[s] - first[s], ctx = extra[s], end = min(ctx, most);
         int64_t sum = 0;
         for (int j = lane; j * block_tokens < n; j += 32)
@@ -199,14 +201,14 @@ __global__ void __launch_bounds__(kPtPlanThreads) pt_plan_kernel(const PtArgs p,
       __syncthreads();
       const int mine = live ? (last[tid] - first[tid] + block_tokens - 1) / block_tokens : 0;
       const int64_t w = live ? weight[tid] : 0;
-      int64_t all_w, all_n;
-      const int64_t wb = tiles_before + pt_scan(w, sums, all_w);
-      which[tid] = blocks + static_cast<int>(pt_scan(mine, sums, all_n));
-      weight[tid] = wb;
-      tiles_before += all_w;
-      blocks += static_cast<int>(all_n);
+      longlong2 all;
+      const longlong2 before = pt_scan(w, mine, sums, all);
+      which[tid] = blocks + static_cast<int>(before.y);
+      weight[tid] = tiles_before + before.x;
+      tiles_before += all.x;
+      blocks += static_cast<int>(all.y);
       __syncthreads();
-      for (int s = warp; s < here; s += kPtPlanThreads / 32) {
+      for (int s = warp; s < here; s += kPtPlanWarps) {
         const int n = last[s] - first[s], ctx = extra[s], end = min(ctx, most);
         int64_t before = weight[s];
         for (int j0 = 0; j0 * block_tokens < n; j0 += 32) {
@@ -214,12 +216,7 @@ __global__ void __launch_bounds__(kPtPlanThreads) pt_plan_kernel(const PtArgs p,
           const int count = min(n - i0, block_tokens);
           const int tiles = count > 0 ? pt_tiles(min(ctx - n + i0 + count, end)) : 0;
           const int cost = count > 0 ? pt_cost(tiles) : 0;
-          int64_t x = cost;
-#pragma unroll
-          for (int m = 1; m < 32; m <<= 1) {
-            const int64_t y = __shfl_up_sync(0xffffffffu, x, m);
-            if (lane >= m) x += y;
-          }
+          const int64_t x = pt_warp_scan(cost);
           if (count > 0)
             put(which[s] + j, before + x - cost,
                 PtBlock{b0 + s, first[s] + i0, count, tiles, 0, ctx - n + i0 + 1, end, kPtPrompt});
@@ -242,7 +239,7 @@ __global__ void __launch_bounds__(kPtPlanThreads) pt_plan_kernel(const PtArgs p,
       extra[tid] = live ? p.prefix[g] : 0;
       __syncthreads();
       const int here = min(kPtPlanThreads, p.groups - g0);
-      for (int s = warp; s < here; s += kPtPlanThreads / 32) {
+      for (int s = warp; s < here; s += kPtPlanWarps) {
         // the pages in common, read through the table of the longest request
         int best = 0, row = first[s], full = 0;
         for (int r = first[s] + lane; r < last[s]; r += 32) {
@@ -264,16 +261,15 @@ __global__ void __launch_bounds__(kPtPlanThreads) pt_plan_kernel(const PtArgs p,
       __syncthreads();
       const int shared = extra[tid], row = static_cast<int>(weight[tid]);
       const int mine = live && shared > 0 ? (last[tid] - first[tid] + p.TB - 1) / p.TB : 0;
-      int64_t all_w, all_n;
-      const int64_t wb = tiles_before + pt_scan(static_cast<int64_t>(mine) * pt_cost(shared / kPtRows), sums, all_w);
-      which[tid] = blocks + static_cast<int>(pt_scan(mine, sums, all_n));
-      __syncthreads();
-      weight[tid] = wb;
-      tiles_before += all_w;
-      blocks += static_cast<int>(all_n);
+      longlong2 all;
+      const longlong2 before = pt_scan(static_cast<int64_t>(mine) * pt_cost(shared / kPtRows), mine, sums, all);
+      which[tid] = blocks + static_cast<int>(before.y);
+      weight[tid] = tiles_before + before.x;  // (the scan waited for all to have read it)
+      tiles_before += all.x;
+      blocks += static_cast<int>(all.y);
       table_row[tid] = row;
       __syncthreads();
-      for (int s = warp; s < here; s += kPtPlanThreads / 32) {
+      for (int s = warp; s < here; s += kPtPlanWarps) {
         if (extra[s] <= 0) continue;
         const int n = last[s] - first[s], tiles = extra[s] / kPtRows;
         for (int j = lane; j * p.TB < n; j += 32)
@@ -294,10 +290,10 @@ __global__ void __launch_bounds__(kPtPlanThreads) pt_plan_kernel(const PtArgs p,
         end = min(max(p.context[b], 0), most);
         tiles = pt_tiles(end - shared);
       }
-      int64_t all_w;
-      const int64_t wb = tiles_before + pt_scan(live ? pt_cost(tiles) : 0, sums, all_w);
-      if (live) put(blocks + b, wb, PtBlock{b, b, 1, tiles, shared, end, end, kPtOwn});
-      tiles_before += all_w;
+      longlong2 all;
+      const longlong2 before = pt_scan(live ? pt_cost(tiles) : 0, 0, sums, all);
+      if (live) put(blocks + b, tiles_before + before.x, PtBlock{b, b, 1, tiles, shared, end, end, kPtOwn});
+      tiles_before += all.x;
     }
     blocks += p.batch;
     __syncthreads();
@@ -350,14 +346,15 @@ __global__ void __launch_bounds__(kPtPlanThreads) pt_plan_kernel(const PtArgs p,
     return real;
   };
   const int64_t end = total - static_cast<int64_t>(blocks) * p.Hkv * kPtBlockCost;  // tiles of all
-  for (int w = tid; w < p.workers; w += kPtPlanThreads) {
-    PtStart s{0, 0, 0, 0}, next;
-    const int64_t at = w * chunk;
-    if (at < total) {
-      const int64_t from = border(at, s);
-      s.count = static_cast<int>((at + chunk < total ? border(at + chunk, next) : end) - from);
-    }
-    p.w.starts[w] = s;
+  static_assert(2 * kPtMaxCtas <= kPtPlanThreads, "a thread for every worker");
+  __syncthreads();  // weight is free
+  PtStart s{0, 0, 0, 0};
+  const int64_t from = tid < p.workers && tid * chunk < total ? border(tid * chunk, s) : end;
+  weight[tid] = from;
+  __syncthreads();
+  if (tid < p.workers) {
+    s.count = static_cast<int>((tid + 1 < p.workers ? weight[tid + 1] : end) - from);
+    p.w.starts[tid] = s;
   }
 }
 
@@ -571,6 +568,9 @@ __global__ void __launch_bounds__(kPtThreads, 1)
   auto worker = [&](int l) { return static_cast<int>(blockIdx.x) + (kPair ? 0 : l * static_cast<int>(gridDim.x)); };
   // Does lane l have rows of a block of so many tokens?  (A pair's second lane: those of the tokens behind the first TB.)
   auto has_rows = [&](int l, int ntok) { return !kPair || l == 0 || ntok > p.TB; };
+  // Tokens by which lane 1's rows lie further on in its tile (solo), where they fit: few rows of both lanes would
+  // otherwise be the work of one of the SM's four schedulers.
+  auto shift = [&](int l, int ntok) { return !kPair && l == 1 && ntok <= p.TB / 2 ? p.TB / 2 : 0; };
   bool ok = true;
 
   if (warp == 0) {
@@ -753,7 +753,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     __syncwarp();
   } else if (warp < 4) {
     // ---------------- rows of Q of both lanes, by one thread.  The box takes as many tokens as a block can have; rows
-    // behind the block's last are never used.
+    // behind the block's last (and, with a shift, before its first) are never used.
     if (lane == 0) {
       PtWalk w[2];
       int copied[2] = {0, 0};
@@ -770,8 +770,9 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           if (w[l].left <= 0 || (copied[l] > 0 && !pt_passed(&bar.q_free[l], (copied[l] - 1) & 1))) continue;
           const bool one = w[l].b.kind == kPtOwn;
           const CUtensorMap* map = one ? &tmap_q1 : &tmap_q;
-          const int token = w[l].b.tok0 + (kPair ? l * p.TB : 0);
-          uint8_t* dst = smem + l * kPtTile;
+          const int ahead = shift(l, w[l].b.ntok);
+          const int token = w[l].b.tok0 + (kPair ? l * p.TB : 0) - (one ? 0 : ahead);
+          uint8_t* dst = smem + l * kPtTile + (one ? ahead * p.G * 128 : 0);
           mbar_arrive_expect_tx(&bar.q_full[l], (one ? 1 : p.TB) * p.G * kPtRows * 2);
           pt_load_q(dst, map, &bar.q_full[l], 0, w[l].head * p.G, token);
           pt_load_q(dst + kPtHalf, map, &bar.q_full[l], 64, w[l].head * p.G, token);
@@ -813,17 +814,18 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     const float c = p.c;
     PtWalk w;
     w.start(p, worker(l));
-    int tile = 0, part = 0, limit = 0, token = 0, head = 0, from = 0;
+    int tile = 0, part = 0, row_in = 0, limit = 0, token = 0, head = 0, from = 0;
     bool live = false, started = false;
     float m = -INFINITY, sum = 0.0f;
     // A wait that gave up does not end the walk (the two warps of a row meet at barriers): later ones are not waited for.
     for (; w.left > 0; w.next()) {
       if (!has_rows(l, w.b.ntok)) continue;
       if (w.fresh) {
-        const int t0 = kPair ? l * p.TB : 0, t = r / p.G;
-        live = r < min(w.b.ntok - t0, p.TB) * p.G;
+        row_in = r - shift(l, w.b.ntok) * p.G;
+        const int t0 = kPair ? l * p.TB : 0, t = max(row_in, 0) / p.G;
+        live = row_in >= 0 && row_in < min(w.b.ntok - t0, p.TB) * p.G;
         token = w.b.tok0 + t0 + t;
-        head = w.head * p.G + r - t * p.G;
+        head = w.head * p.G + row_in - t * p.G;
         limit = 0;
         if (live)
           limit = w.b.kind == kPtPrompt ? w.b.limit + t0 + t : w.b.kind == kPtOwn ? w.b.limit : __ldg(p.context + token);
@@ -837,7 +839,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       const int keys = *reinterpret_cast<volatile int*>(&bar.lane_keys[l]);
       if (busy && keys > 0) {
         const int seen = min(max(limit - (w.b.key0 + w.tile * kPtRows), 0), keys);
-        const bool edge = __any_sync(0xffffffffu, seen < kPtRows);
+        const bool edge = __any_sync(0xffffffffu, live && seen < kPtRows);  // other rows may come to anything
         uint32_t s[64];
         tmem_ld32(at, s);
         tmem_ld32(at + 32, s + 32);
@@ -857,7 +859,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         *mine = top;
         named_barrier_sync(pairing, 64);
         top = fmaxf(top, *others);
-        const bool move = top > m && (m == -INFINITY || (top - m) * c > kPtSlack);
+        const bool move = live && top > m && (m == -INFINITY || (top - m) * c > kPtSlack);
         if (__any_sync(0xffffffffu, move) && started) {
           const float f = move ? pt_exp2((m - top) * c) : 1.0f;
           sum *= f;
@@ -882,8 +884,8 @@ __global__ void __launch_bounds__(kPtThreads, 1)
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
             float x, y;
-            unpair(mul2(sub2(pair(__uint_as_float(s[32 * i + 2 * j]), __uint_as_float(s[32 * i + 2 * j + 1])), base2), c2),
-                   x, y);
+            const int k = 32 * i + 2 * j;
+            unpair(mul2(sub2(pair(__uint_as_float(s[k]), __uint_as_float(s[k + 1])), base2), c2), x, y);
             x = pt_exp2(x), y = pt_exp2(y);
             const uint64_t e = pair(x, y);
             sums[j & 1] = add2(sums[j & 1], e);
@@ -937,8 +939,8 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           po = reinterpret_cast<float4*>(p.w.row) + i * 32 + half * 16, pm = p.w.row_ml + i * 2, stride = 1;
         } else {
           const int64_t slot = (static_cast<int64_t>(worker(l)) * 2 + (from == 0)) * (kPair ? 2 : 1) + (kPair ? l : 0);
-          po = reinterpret_cast<float4*>(p.w.part) + (slot * 32 + half * 16) * p.slot_rows + r;
-          pm = p.w.part_ml + (slot * p.slot_rows + r) * 2, stride = p.slot_rows;
+          po = reinterpret_cast<float4*>(p.w.part) + (slot * 32 + half * 16) * p.slot_rows + row_in;
+          pm = p.w.part_ml + (slot * p.slot_rows + row_in) * 2, stride = p.slot_rows;
         }
 #pragma unroll 1
         for (int i = 0; i < 2; ++i) {
@@ -1002,13 +1004,14 @@ struct PtJoin {
   // Pieces `first` .. `last` of a cut block: slot 1 of the first worker, 0 of the others; `of_pair` which of a pair's.
   template <int kPer>
   __device__ __forceinline__ void pieces(const PtArgs& p, int first, int last, int of_pair, int row, int j) {
-    constexpr int kAhead = 8;  // loads in flight
+    constexpr int kAhead = 4;  // loads in flight
     for (int w0 = first; w0 <= last; w0 += kAhead) {
       float2 ml[kAhead];
       float4 v[kAhead];
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
-        const int w = min(w0 + i, last);
+        const int w = w0 + i;
+        if (w > last) break;
         const int64_t slot = (static_cast<int64_t>(w) * 2 + (w == first)) * kPer + of_pair;
         ml[i] = *reinterpret_cast<const float2*>(p.w.part_ml + (slot * p.slot_rows + row) * 2);
         v[i] = *(reinterpret_cast<const float4*>(p.w.part) + (slot * 32 + j) * p.slot_rows + row);
