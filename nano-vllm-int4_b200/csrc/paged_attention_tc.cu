@@ -28,10 +28,10 @@
 //                   from L2 to shared memory once for 256 rows;
 //   others (solo)   every lane is a worker of its own.
 //   warp 0     copies K and V tiles (TMA, five slots of 32 KB) in the order of use
-//   warps 1-2  issue S = Q K^T, O += P V of a lane each;  V rows behind the last token of
-//              a request are cleared first (0 times an old NaN would be one)
+//   warps 1-2  issue S = Q K^T, O += P V of a lane each
 //   warp 3     copies the lanes' rows of Q (TMA: [tokens][G heads][128 channels])
-//   warps 4-19 softmax of the two lanes; outputs
+//   warps 4-19 softmax of the two lanes; outputs.  They also clear the V rows behind the last
+//              token of a request (0 times an old NaN would be one)
 // P goes back to TMEM over its scores.  Decode is bound by the cache's bytes: there P is
 // multiplied in two BF16 terms (the upper 16 bits of the FP32 value and of the rest, 2^-14
 // of it at most left out), so that the output's own rounding
@@ -522,6 +522,7 @@ struct PtBars {
   uint32_t tmem, lock;
   int slot_keys[kPtSlots];  // keys of the slot's tile that exist
   int lane_keys[2];         // of the tile whose scores lie in the lane
+  uint32_t lane_v[2];       // its V: slot, parity of its arrival
 };
 static_assert(sizeof(PtBars) <= 256, "barriers");
 
@@ -671,13 +672,15 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       // K of the walk's tile, in slot s, and with a block's first tile its rows of Q
       auto ready = [&](uint32_t s, bool rows) { return filled(s) && (!rows || !w.fresh || arrived(bar.q_full[l], parts++)); };
       // S = Q K^T
-      auto scores = [&](uint32_t s, bool rows) {
+      auto scores = [&](uint32_t i, uint32_t s, bool rows) {
         if (!rows) {
           mbar_arrive(&bar.empty[s]);
           return;
         }
         tc_fence_after();
         bar.lane_keys[l] = bar.slot_keys[s];  // before the slot can be released
+        const uint32_t vs = v_position(i) % kPtSlots;
+        bar.lane_v[l] = vs << 1 | ((seen >> vs) & 1);
         const uint32_t qa = q_lo + l * (kPtTile >> 4), ka = ring_lo + s * (kPtTile >> 4) + kPtDescK;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -694,7 +697,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       uint32_t c = !kPair && l == 1 && others > 0;       // ring position
       if (w.left > 0) {
         ok = ready(c % kPtSlots, rows);
-        if (ok) scores(c % kPtSlots, rows);
+        if (ok) scores(0, c % kPtSlots, rows);
       }
       for (uint32_t i = 0; ok && w.left > 0; ++i) {
         // what O += P V and the next S need besides P
@@ -708,12 +711,6 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         if (kPair && w.left > 0 && !ready(next, rows)) break;
         if (now) {
           const int keys = bar.slot_keys[s], steps = (keys + 15) / 16;
-          if (keys & 15) {  // rows behind the last key: P is zero there, V may be anything
-            for (int e = 0; e < (steps * 16 - keys) * 16; ++e)
-              *reinterpret_cast<uint4*>(ring + s * kPtTile + (e & 8 ? kPtHalf : 0) + (keys + (e >> 4)) * 128 +
-                                        (e & 7) * 16) = make_uint4(0, 0, 0, 0);
-            fence_proxy_async_smem();
-          }
           if (fresh) started = false;
           const uint32_t va = ring_lo + s * (kPtTile >> 4) + kPtDescV, o = l * 256 + 128;
           // 16 keys: the terms of P against the same rows of V
@@ -739,7 +736,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           mbar_arrive(&bar.empty[s]);
         }
         if (!kPair && w.left > 0 && !ready(next, rows)) break;
-        if (w.left > 0) scores(next, rows);
+        if (w.left > 0) scores(i + 1, next, rows);
         if (kPair && now) atomicExch(&bar.lock, 0u);
       }
       umma_commit(&bar.done);  // all issued products must finish before the TMEM is released
@@ -909,6 +906,15 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         tmem_wait_st();
       }
       started = started || keys > 0;
+      if (keys & 15) {  // V rows behind the last key are cleared: P is zero there, they may be anything
+        const uint32_t v = *reinterpret_cast<volatile uint32_t*>(&bar.lane_v[l]);
+        ok = ok && __all_sync(0xffffffffu, mbar_wait(&bar.full[kPair ? 0 : l][v >> 1], v & 1, kErrTimeoutFull));
+        const int e = (half * 4 + quarter) * 32 + lane, row = keys + (e >> 4);
+        if (row < ((keys + 15) & ~15))
+          *reinterpret_cast<uint4*>(ring + (v >> 1) * kPtTile + (e & 8 ? kPtHalf : 0) + row * 128 + (e & 7) * 16) =
+              make_uint4(0, 0, 0, 0);
+        fence_proxy_async_smem();
+      }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bar.p_full[l]);
@@ -916,64 +922,67 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       if (!w.last()) continue;
 
       // the block's end, or this worker's: outputs
-      ok = ok && __all_sync(0xffffffffu, mbar_wait(&bar.o_full[l], part & 1, kErrTimeoutMma));
-      ++part;
-      tc_fence_after();
       const bool whole = from == 0 && w.tile + 1 == w.b.tiles;
       const bool final_ = whole && (w.b.kind == kPtPrompt || (w.b.kind == kPtOwn && w.b.key0 == 0));
+      // BF16 rows; or FP32 ones, of a block that is not cut row after row (for the joining kernel), of a cut one with the
+      // rows beside each other, 16 bytes each, so that a warp's stores are contiguous
+      const int64_t row = static_cast<int64_t>(token) * p.Hq + head;
+      uint4* dst;
+      int64_t stride = 1;
+      float2* ml = nullptr;
+      float f = 1.0f;
       if (busy) {
+        named_barrier_sync(pairing, 64);  // the last tile's maxima are read
         *mine = sum;
         named_barrier_sync(pairing, 64);
         const float other = *others;
-        named_barrier_sync(pairing, 64);  // read before the next block's maxima take their place
+        named_barrier_sync(pairing, 64);
         sum = half == 0 ? sum + other : other + sum;
-        const float f = final_ ? (sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f) : 1.0f;
-        const int64_t row = static_cast<int64_t>(token) * p.Hq + head;
-        // FP32 outputs: of a block that is not cut row after row (for the joining kernel); of a cut one with the rows
-        // beside each other, 16 bytes each, so that a warp's stores are contiguous
-        float4* po;
-        float* pm;
-        int stride;
-        if (whole) {
+        if (final_) {
+          f = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
+          dst = reinterpret_cast<uint4*>(p.out + row * kPtRows) + half * 8;
+        } else if (whole) {
           const int64_t i = (w.b.kind == kPtPrefix ? static_cast<int64_t>(p.batch) * p.Hq : 0) + row;
-          po = reinterpret_cast<float4*>(p.w.row) + i * 32 + half * 16, pm = p.w.row_ml + i * 2, stride = 1;
+          dst = reinterpret_cast<uint4*>(p.w.row) + i * 32 + half * 16;
+          ml = reinterpret_cast<float2*>(p.w.row_ml) + i;
         } else {
           const int64_t slot = (static_cast<int64_t>(worker(l)) * 2 + (from == 0)) * (kPair ? 2 : 1) + (kPair ? l : 0);
-          po = reinterpret_cast<float4*>(p.w.part) + (slot * 32 + half * 16) * p.slot_rows + row_in;
-          pm = p.w.part_ml + (slot * p.slot_rows + row_in) * 2, stride = p.slot_rows;
+          stride = p.slot_rows;
+          dst = reinterpret_cast<uint4*>(p.w.part) + (slot * 32 + half * 16) * stride + row_in;
+          ml = reinterpret_cast<float2*>(p.w.part_ml) + slot * stride + row_in;
         }
+      }
+      ok = ok && __all_sync(0xffffffffu, mbar_wait(&bar.o_full[l], part & 1, kErrTimeoutMma));
+      ++part;
+      tc_fence_after();
+      if (busy) {
 #pragma unroll 1
-        for (int i = 0; i < 2; ++i) {
-          uint32_t o[32];
+        for (int i = 0; i < 4; ++i) {
+          uint32_t o[16];
           if (started) {
-            tmem_ld32(at + 128 + 32 * i, o);
+            tmem_ld16(at + 128 + 16 * i, o);
             tmem_wait_ld();
           } else {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) o[j] = 0u;
+            for (int j = 0; j < 16; ++j) o[j] = 0u;
           }
           if (live && final_) {
-            uint16_t* dst = p.out + row * kPtRows + half * 64 + 32 * i;
+            uint32_t v[8];
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              uint32_t v[8];
-#pragma unroll
-              for (int e = 0; e < 8; ++e) {
-                const __nv_bfloat162 b = __floats2bfloat162_rn(__uint_as_float(o[16 * j + 2 * e]) * f,
-                                                               __uint_as_float(o[16 * j + 2 * e + 1]) * f);
-                v[e] = *reinterpret_cast<const uint32_t*>(&b);
-              }
-              pt_store32(dst + 16 * j, v);
+            for (int j = 0; j < 8; ++j) {
+              const __nv_bfloat162 b =
+                  __floats2bfloat162_rn(__uint_as_float(o[2 * j]) * f, __uint_as_float(o[2 * j + 1]) * f);
+              v[j] = *reinterpret_cast<const uint32_t*>(&b);
             }
+            pt_store32(dst, v);
+            dst += 2;
           } else if (live) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-              po[(8 * i + j) * stride] = make_float4(__uint_as_float(o[4 * j]), __uint_as_float(o[4 * j + 1]),
-                                                     __uint_as_float(o[4 * j + 2]), __uint_as_float(o[4 * j + 3]));
+            for (int j = 0; j < 4; ++j, dst += stride) *dst = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
           }
           __syncwarp();
         }
-        if (live && !final_ && half == 0) *reinterpret_cast<float2*>(pm) = make_float2(m, sum);
+        if (live && !final_ && half == 0) *ml = make_float2(m, sum);
       }
       tc_fence_before();
     }
