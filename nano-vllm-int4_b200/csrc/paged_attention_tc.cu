@@ -407,6 +407,11 @@ __device__ __forceinline__ void pt_tmem_st16(uint32_t taddr, const uint32_t (&v)
       : "memory");
 }
 
+// Registers: 640 threads are launched with 96; what the first warpgroup gives up goes to the four of the softmax, which
+// hold 64 scores a thread: 64 + 4 * 104 = 5 * 96.
+__device__ __forceinline__ void pt_registers_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 64;"); }
+__device__ __forceinline__ void pt_registers_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 104;"); }
+
 // Takes a lock in shared memory; after a while without it too (it only orders the lanes).
 __device__ __forceinline__ void pt_lock(uint32_t* lock) {
   for (int i = 0; i < 100000; ++i)
@@ -574,6 +579,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
   auto shift = [&](int l, int ntok) { return !kPair && l == 1 && ntok <= p.TB / 2 ? p.TB / 2 : 0; };
   bool ok = true;
 
+  if (warp < 4) pt_registers_down();
   if (warp == 0) {
     // ---------------- copies of K and V
     if (lane == 0) {
@@ -803,6 +809,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     // ---------------- softmax and outputs: two threads a row (head r % G of its lane's token r / G), each with half of a
     // tile's keys, and of the output's channels at the end.  (With one thread a row the two warps of a scheduler left
     // two thirds of its issue slots empty.)
+    pt_registers_up();
     const int l = (warp - 4) >> 3, half = ((warp - 4) >> 2) & 1, quarter = warp & 3, r = quarter * 32 + lane;
     const uint32_t at = l * 256 + half * 64 + (static_cast<uint32_t>(quarter * 32) << 16);
     float* const mine = reinterpret_cast<float*>(smem + kPtTops) + (l * 2 + half) * kPtRows + r;
