@@ -26,7 +26,11 @@
 // lane's warpgroups work on its scores, the tensor cores work for the other.
 //   prompts (pair)  both lanes take the same keys for two blocks of rows: K and V pass
 //                   from L2 to shared memory once for 256 rows;
-//   others (solo)   every lane is a worker of its own.
+//   others (solo)   every lane is a worker of its own.  A decode block of up to 32 rows is
+//                   spread: its rows of Q stand four times in the tile, in each quarter of
+//                   the TMEM lanes, and P of quarter 2 h + t is term t of the keys of half
+//                   h, zero elsewhere.  So the four schedulers share a row's exponentials,
+//                   and one product does for both terms; the four parts of O are joined.
 //   warp 0     copies K and V tiles (TMA, five slots of 32 KB) in the order of use
 //   warps 1-2  issue S = Q K^T, O += P V of a lane each
 //   warp 3     copies the lanes' rows of Q (TMA: [tokens][G heads][128 channels])
@@ -90,7 +94,7 @@ struct PtScratch {
   int* row_block;    // [batch]: the prefix block of a request, or -1
   float* part;       // [workers][2][rows][128]: of a worker's first and last block, when cut
   float* part_ml;    // [..][2]: reference, sum
-  float* row;        // [2][batch * Hq][128]: of own and prefix blocks that are not cut, but joined
+  float* row;        // [2][batch * Hq][4][128]: of own and prefix blocks that are not cut; four parts when spread
   float* row_ml;
 };
 
@@ -157,6 +161,8 @@ __device__ __forceinline__ int pt_tiles(int keys) { return max(1, (keys + kPtRow
 // A block counts for its tiles and as much as one more for its beginning and end (its outputs, mostly).
 constexpr int kPtBlockCost = 1;
 __device__ __forceinline__ int pt_cost(int tiles) { return tiles + kPtBlockCost; }
+// A decode block of up to 32 rows is spread: its rows stand four times in the tile.
+__device__ __forceinline__ bool pt_spread(const PtArgs& p, int ntok) { return ntok <= p.TB / 4; }
 
 __global__ void __launch_bounds__(kPtPlanThreads) pt_plan_kernel(const PtArgs p, const int block_tokens) {
   __shared__ int64_t sums[2][kPtPlanWarps];
@@ -536,7 +542,7 @@ template <bool kPair, int kTerms>
 __global__ void __launch_bounds__(kPtThreads, 1)
     pt_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
                         const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_q1,
-                        const PtArgs p) {
+                        const __grid_constant__ CUtensorMap tmap_q4, const PtArgs p) {
   extern __shared__ __align__(1024) uint8_t smem[];  // the tiles' swizzle wants multiples of 1024
   uint8_t* ring = smem + 2 * kPtTile;
   PtBars& bar = *reinterpret_cast<PtBars*>(smem + kPtBar);
@@ -574,9 +580,11 @@ __global__ void __launch_bounds__(kPtThreads, 1)
   auto worker = [&](int l) { return static_cast<int>(blockIdx.x) + (kPair ? 0 : l * static_cast<int>(gridDim.x)); };
   // Does lane l have rows of a block of so many tokens?  (A pair's second lane: those of the tokens behind the first TB.)
   auto has_rows = [&](int l, int ntok) { return !kPair || l == 0 || ntok > p.TB; };
+  // Is a block of so many tokens spread (see above)?
+  auto spread_out = [&](int ntok) { return kTerms == 2 && pt_spread(p, ntok); };
   // Tokens by which lane 1's rows lie further on in its tile (solo), where they fit: few rows of both lanes would
   // otherwise be the work of one of the SM's four schedulers.
-  auto shift = [&](int l, int ntok) { return !kPair && l == 1 && ntok <= p.TB / 2 ? p.TB / 2 : 0; };
+  auto shift = [&](int l, int ntok) { return !kPair && l == 1 && !spread_out(ntok) && ntok <= p.TB / 2 ? p.TB / 2 : 0; };
   bool ok = true;
 
   if (warp < 4) pt_registers_down();
@@ -709,7 +717,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         // what O += P V and the next S need besides P
         c = v_position(i);
         const uint32_t s = c % kPtSlots, next = (c + 1) % kPtSlots;
-        const bool fresh = w.fresh, last = w.last(), now = rows;
+        const bool fresh = w.fresh, last = w.last(), now = rows, spread = spread_out(w.ntok);
         if (!filled(s)) break;
         w.next();
         rows = has_rows(l, w.ntok);
@@ -719,11 +727,15 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           const int keys = bar.slot_keys[s], steps = (keys + 15) / 16;
           if (fresh) started = false;
           const uint32_t va = ring_lo + s * (kPtTile >> 4) + kPtDescV, o = l * 256 + 128;
-          // 16 keys: the terms of P against the same rows of V
+          // 16 keys: P, or its two terms against the same rows of V
           auto step = [&](int k, uint32_t accumulate) {
-            const uint32_t pk = l * 256 + (kTerms == 1 ? (k >> 2) * 64 + (k & 3) * 8 : (k >> 1) * 32 + (k & 1) * 8);
-            pt_mma_ts(o, pk, va + k * 128, kPv, accumulate);
-            if (kTerms == 2) pt_mma_ts(o, pk + 16, va + k * 128, kPv, 1);
+            if (kTerms == 1 || spread) {
+              pt_mma_ts(o, l * 256 + (k >> 2) * 64 + (k & 3) * 8, va + k * 128, kPv, accumulate);
+            } else {
+              const uint32_t pk = l * 256 + (k >> 1) * 32 + (k & 1) * 8;
+              pt_mma_ts(o, pk, va + k * 128, kPv, accumulate);
+              pt_mma_ts(o, pk + 16, va + k * 128, kPv, 1);
+            }
           };
           if (!arrived(bar.p_full[l], tiles++)) break;
           if (kPair) pt_lock(&bar.lock);
@@ -771,14 +783,16 @@ __global__ void __launch_bounds__(kPtThreads, 1)
 #pragma unroll
         for (int l = 0; l < 2; ++l) {
           if (w[l].left <= 0 || (copied[l] > 0 && !pt_passed(&bar.q_free[l], (copied[l] - 1) & 1))) continue;
-          const bool one = w[l].b.kind == kPtOwn;
-          const CUtensorMap* map = one ? &tmap_q1 : &tmap_q;
-          const int ahead = shift(l, w[l].b.ntok);
+          const bool one = w[l].b.kind == kPtOwn, spread = spread_out(w[l].b.ntok);
+          const CUtensorMap* map = one ? &tmap_q1 : spread ? &tmap_q4 : &tmap_q;
+          const int ahead = shift(l, w[l].b.ntok), copies = spread ? 4 : 1;
           const int token = w[l].b.tok0 + (kPair ? l * p.TB : 0) - (one ? 0 : ahead);
           uint8_t* dst = smem + l * kPtTile + (one ? ahead * p.G * 128 : 0);
-          mbar_arrive_expect_tx(&bar.q_full[l], (one ? 1 : p.TB) * p.G * kPtRows * 2);
-          pt_load_q(dst, map, &bar.q_full[l], 0, w[l].head * p.G, token);
-          pt_load_q(dst + kPtHalf, map, &bar.q_full[l], 64, w[l].head * p.G, token);
+          mbar_arrive_expect_tx(&bar.q_full[l], copies * (one ? 1 : spread ? p.TB / 4 : p.TB) * p.G * kPtRows * 2);
+          for (int i = 0; i < copies; ++i, dst += 32 * 128) {
+            pt_load_q(dst, map, &bar.q_full[l], 0, w[l].head * p.G, token);
+            pt_load_q(dst + kPtHalf, map, &bar.q_full[l], 64, w[l].head * p.G, token);
+          }
           ++copied[l];
           do w[l].skip();
           while (w[l].left > 0 && !has_rows(l, w[l].b.ntok));
@@ -812,9 +826,12 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     pt_registers_up();
     const int l = (warp - 4) >> 3, half = ((warp - 4) >> 2) & 1, quarter = warp & 3, r = quarter * 32 + lane;
     const uint32_t at = l * 256 + half * 64 + (static_cast<uint32_t>(quarter * 32) << 16);
-    float* const mine = reinterpret_cast<float*>(smem + kPtTops) + (l * 2 + half) * kPtRows + r;
-    const float* const others = reinterpret_cast<float*>(smem + kPtTops) + (l * 2 + 1 - half) * kPtRows + r;
-    const int pairing = 1 + l * 4 + quarter;  // named barrier of the two warps that share rows
+    float* const tops = reinterpret_cast<float*>(smem + kPtTops) + l * 2 * kPtRows;
+    // Spread, a row is the work of four warps, one in each quarter: of quarter 2 h + t those of half h, for term t.
+    const bool works = half == quarter >> 1;
+    bool spread = false;
+    float *mine = nullptr, *others = nullptr;  // the maxima of the two halves of a row
+    int pairing = 0, paired = 0;               // named barrier of the warps that share rows, and its threads
     const float c = p.c;
     PtWalk w;
     w.start(p, worker(l));
@@ -825,7 +842,10 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     for (; w.left > 0; w.next()) {
       if (!has_rows(l, w.b.ntok)) continue;
       if (w.fresh) {
-        row_in = r - shift(l, w.b.ntok) * p.G;
+        spread = spread_out(w.b.ntok);
+        row_in = spread ? lane : r - shift(l, w.b.ntok) * p.G;
+        mine = tops + half * kPtRows + (spread ? lane : r), others = tops + (1 - half) * kPtRows + (spread ? lane : r);
+        pairing = spread ? 9 + l : 1 + l * 4 + quarter, paired = spread ? 128 : 64;
         const int t0 = kPair ? l * p.TB : 0, t = max(row_in, 0) / p.G;
         live = row_in >= 0 && row_in < min(w.b.ntok - t0, p.TB) * p.G;
         token = w.b.tok0 + t0 + t;
@@ -841,7 +861,16 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       ok = ok && __all_sync(0xffffffffu, mbar_wait(&bar.s_full[l], tile & 1, kErrTimeoutMma));
       tc_fence_after();
       const int keys = *reinterpret_cast<volatile int*>(&bar.lane_keys[l]);
-      if (busy && keys > 0) {
+      if (spread && !works) {  // keys that are not this quarter's
+        if (keys > 0) {
+          uint32_t zero[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) zero[i] = 0u;
+          pt_tmem_st16(at, zero);
+          pt_tmem_st16(at + 16, zero);
+          tmem_wait_st();
+        }
+      } else if (busy && keys > 0) {
         const int seen = min(max(limit - (w.b.key0 + w.tile * kPtRows), 0), keys);
         const bool edge = __any_sync(0xffffffffu, live && seen < kPtRows);  // other rows may come to anything
         uint32_t s[64];
@@ -860,21 +889,22 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           for (int i = 0; i < 4; ++i)
             t[i] = fmaxf(t[i], fmaxf(__uint_as_float(s[j + 2 * i]), __uint_as_float(s[j + 2 * i + 1])));
         float top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
-        *mine = top;
-        named_barrier_sync(pairing, 64);
+        *mine = top;  // (spread, two warps write the same)
+        named_barrier_sync(pairing, paired);
         top = fmaxf(top, *others);
         const bool move = live && top > m && (m == -INFINITY || (top - m) * c > kPtSlack);
         if (__any_sync(0xffffffffu, move) && started) {
           const float f = move ? pt_exp2((m - top) * c) : 1.0f;
           sum *= f;
 #pragma unroll 1
-          for (int i = 0; i < 4; ++i) {
+          for (int i = 0; i < (spread ? 8 : 4); ++i) {  // half of the row's channels, or all
+            const uint32_t ao = (spread ? at - half * 64 : at) + 128 + 16 * i;
             uint32_t o[16];
-            tmem_ld16(at + 128 + 16 * i, o);
+            tmem_ld16(ao, o);
             tmem_wait_ld();
 #pragma unroll
             for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
-            pt_tmem_st16(at + 128 + 16 * i, o);
+            pt_tmem_st16(ao, o);
           }
         }
         if (move) m = top;
@@ -904,8 +934,16 @@ __global__ void __launch_bounds__(kPtThreads, 1)
               lo[j] = __byte_perm(__float_as_uint(u), __float_as_uint(w), 0x7632);
             }
           }
-          pt_tmem_st16(at + 16 * kTerms * i, hi);
-          if constexpr (kTerms == 2) pt_tmem_st16(at + 32 * i + 16, lo);
+          if (kTerms == 1) {
+            pt_tmem_st16(at + 16 * i, hi);
+          } else if (!spread) {
+            pt_tmem_st16(at + 32 * i, hi);
+            pt_tmem_st16(at + 32 * i + 16, lo);
+          } else if (quarter & 1) {
+            pt_tmem_st16(at + 16 * i, lo);
+          } else {
+            pt_tmem_st16(at + 16 * i, hi);
+          }
         }
         float x, y;
         unpair(add2(sums[0], sums[1]), x, y);
@@ -930,7 +968,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
 
       // the block's end, or this worker's: outputs
       const bool whole = from == 0 && w.tile + 1 == w.b.tiles;
-      const bool final_ = whole && (w.b.kind == kPtPrompt || (w.b.kind == kPtOwn && w.b.key0 == 0));
+      const bool final_ = kTerms == 1 && whole;
       // BF16 rows; or FP32 ones, of a block that is not cut row after row (for the joining kernel), of a cut one with the
       // rows beside each other, 16 bytes each, so that a warp's stores are contiguous
       const int64_t row = static_cast<int64_t>(token) * p.Hq + head;
@@ -939,24 +977,28 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       float2* ml = nullptr;
       float f = 1.0f;
       if (busy) {
-        named_barrier_sync(pairing, 64);  // the last tile's maxima are read
-        *mine = sum;
-        named_barrier_sync(pairing, 64);
-        const float other = *others;
-        named_barrier_sync(pairing, 64);
-        sum = half == 0 ? sum + other : other + sum;
+        if (!spread) {
+          named_barrier_sync(pairing, paired);  // the last tile's maxima are read
+          *mine = sum;
+          named_barrier_sync(pairing, paired);
+          const float other = *others;
+          named_barrier_sync(pairing, paired);
+          sum = half == 0 ? sum + other : other + sum;
+        }
         if (final_) {
           f = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
           dst = reinterpret_cast<uint4*>(p.out + row * kPtRows) + half * 8;
         } else if (whole) {
-          const int64_t i = (w.b.kind == kPtPrefix ? static_cast<int64_t>(p.batch) * p.Hq : 0) + row;
+          const int64_t i =
+              ((w.b.kind == kPtPrefix ? static_cast<int64_t>(p.batch) * p.Hq : 0) + row) * 4 + (spread ? quarter : 0);
           dst = reinterpret_cast<uint4*>(p.w.row) + i * 32 + half * 16;
           ml = reinterpret_cast<float2*>(p.w.row_ml) + i;
         } else {
           const int64_t slot = (static_cast<int64_t>(worker(l)) * 2 + (from == 0)) * (kPair ? 2 : 1) + (kPair ? l : 0);
           stride = p.slot_rows;
-          dst = reinterpret_cast<uint4*>(p.w.part) + (slot * 32 + half * 16) * stride + row_in;
-          ml = reinterpret_cast<float2*>(p.w.part_ml) + slot * stride + row_in;
+          const int at_row = spread ? r : row_in;
+          dst = reinterpret_cast<uint4*>(p.w.part) + (slot * 32 + half * 16) * stride + at_row;
+          ml = reinterpret_cast<float2*>(p.w.part_ml) + slot * stride + at_row;
         }
       }
       ok = ok && __all_sync(0xffffffffu, mbar_wait(&bar.o_full[l], part & 1, kErrTimeoutMma));
@@ -989,7 +1031,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           }
           __syncwarp();
         }
-        if (live && !final_ && half == 0) *ml = make_float2(m, sum);
+        if (live && !final_ && (spread ? works : half == 0)) *ml = make_float2(m, spread && (quarter & 1) ? 0.0f : sum);
       }
       tc_fence_before();
     }
@@ -1019,22 +1061,23 @@ struct PtJoin {
   }
   // Pieces `first` .. `last` of a cut block: slot 1 of the first worker, 0 of the others; `of_pair` which of a pair's.
   template <int kPer>
-  __device__ __forceinline__ void pieces(const PtArgs& p, int first, int last, int of_pair, int row, int j) {
-    constexpr int kAhead = 4;  // loads in flight
-    for (int w0 = first; w0 <= last; w0 += kAhead) {
+  __device__ __forceinline__ void pieces(const PtArgs& p, int first, int last, int of_pair, int row, int j, int parts = 1) {
+    constexpr int kAhead = 4;  // loads in flight: of four workers, or of the four parts of a spread row
+    for (int w0 = first; w0 <= last; w0 += parts == 1 ? kAhead : 1) {
       float2 ml[kAhead];
       float4 v[kAhead];
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
-        const int w = w0 + i;
+        const int w = parts == 1 ? w0 + i : w0;
         if (w > last) break;
         const int64_t slot = (static_cast<int64_t>(w) * 2 + (w == first)) * kPer + of_pair;
-        ml[i] = *reinterpret_cast<const float2*>(p.w.part_ml + (slot * p.slot_rows + row) * 2);
-        v[i] = *(reinterpret_cast<const float4*>(p.w.part) + (slot * 32 + j) * p.slot_rows + row);
+        const int at = row + (parts == 1 ? 0 : 32 * i);
+        ml[i] = *reinterpret_cast<const float2*>(p.w.part_ml + (slot * p.slot_rows + at) * 2);
+        v[i] = *(reinterpret_cast<const float4*>(p.w.part) + (slot * 32 + j) * p.slot_rows + at);
       }
 #pragma unroll
       for (int i = 0; i < kAhead; ++i)
-        if (w0 + i <= last) fold(ml[i], v[i], p.c);
+        if (parts != 1 || w0 + i <= last) fold(ml[i], v[i], p.c);
     }
   }
   __device__ __forceinline__ void store(uint16_t* row, int j) const {
@@ -1089,21 +1132,29 @@ __global__ void __launch_bounds__(128) pt_join_decode_kernel(const PtArgs p) {
   int own_first, own_last, common_first = 0, common_last = 0;
   workers(own_at, mine.tiles, own_first, own_last);
   if (of >= 0) workers(common_at, common.tiles, common_first, common_last);
-  if (own_first == own_last && mine.key0 == 0) return;  // the attention wrote it
   for (int g = threadIdx.x & 3; g < p.G; g += 4) {
     PtJoin join;
     const int64_t row = static_cast<int64_t>(b) * p.Hq + h * p.G + g;
-    auto add = [&](int first, int last, int in, int64_t area) {
+    auto add = [&](int first, int last, int in, int64_t area, bool spread) {
       if (first < last) {
-        join.pieces<1>(p, first, last, 0, in, j);
-      } else {
-        const int64_t at = area * p.batch * p.Hq + row;
-        join.fold(*reinterpret_cast<const float2*>(p.w.row_ml + at * 2),
-                  *(reinterpret_cast<const float4*>(p.w.row + at * kPtRows) + j), p.c);
+        join.pieces<1>(p, first, last, 0, in, j, spread ? 4 : 1);
+        return;
       }
+      const int64_t at = (area * p.batch * p.Hq + row) * 4;
+      float2 ml[4];
+      float4 v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (i == 0 || spread) {
+          ml[i] = *reinterpret_cast<const float2*>(p.w.row_ml + (at + i) * 2);
+          v[i] = *(reinterpret_cast<const float4*>(p.w.row + (at + i) * kPtRows) + j);
+        }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (i == 0 || spread) join.fold(ml[i], v[i], p.c);
     };
-    if (of >= 0) add(common_first, common_last, (b - common.tok0) * p.G + g, 1);
-    add(own_first, own_last, g, 0);
+    if (of >= 0) add(common_first, common_last, (b - common.tok0) * p.G + g, 1, pt_spread(p, common.ntok));
+    add(own_first, own_last, g, 0, pt_spread(p, 1));
     join.store(p.out + row * kPtRows, j);
   }
 }
@@ -1148,8 +1199,7 @@ static PtLayout pt_prefill_layout(char* base, int64_t tokens, int64_t batch, int
 
 static PtLayout pt_shared_layout(char* base, int64_t batch, int64_t groups, int64_t num_heads, int64_t num_kv_heads) {
   const int64_t group = num_heads / num_kv_heads;
-  return pt_layout(base, batch / (kPtRows / group) + groups + batch, batch, pt_slot_rows(batch, group),
-                   2 * batch * num_heads);
+  return pt_layout(base, batch / (kPtRows / group) + groups + batch, batch, kPtRows, 8 * batch * num_heads);
 }
 
 int64_t paged_prefill_attention_workspace_bytes(int64_t tokens, int64_t batch, int64_t num_heads,
@@ -1170,28 +1220,31 @@ static int launch_pt(PtArgs& a, const void* k_cache, const void* v_cache, cudaSt
   if (rc != NV4_OK) return rc;
   const int sms = std::min(device_sm_count(), kPtMaxCtas);
   if (sms <= 0) return NV4_ERR_CUDA;
-  CUtensorMap maps[4] = {};
+  CUtensorMap maps[5] = {};
   const uint64_t rows = static_cast<uint64_t>(a.num_pages) * kPtPage, cols = static_cast<uint64_t>(a.Hkv) * kPtRows;
   if (!make_tensor_map_2d(&maps[0], CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, k_cache, rows, cols, kPtRows, 64,
                           CU_TENSOR_MAP_SWIZZLE_128B) ||
       !make_tensor_map_2d(&maps[1], CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, v_cache, rows, cols, kPtRows, 64,
                           CU_TENSOR_MAP_SWIZZLE_128B))
     return NV4_ERR_CUDA;
-  // q as [tokens][heads][128]: as many tokens as a block has, or one
+  // q as [tokens][heads][128]: as many tokens as a block has, one, or those of a spread block
   const uint64_t q_dims[3] = {kPtRows, static_cast<uint64_t>(a.Hq), static_cast<uint64_t>(a.tokens)};
   const uint64_t q_strides[2] = {kPtRows * 2, static_cast<uint64_t>(a.Hq) * kPtRows * 2};
   const uint32_t box[3] = {64, static_cast<uint32_t>(a.G), static_cast<uint32_t>(a.TB)};
   const uint32_t box1[3] = {64, static_cast<uint32_t>(a.G), 1};
+  const uint32_t box4[3] = {64, static_cast<uint32_t>(a.G), static_cast<uint32_t>(a.TB / 4)};
   if (!make_tensor_map_3d(&maps[2], CU_TENSOR_MAP_DATA_TYPE_UINT16, a.q, q_dims, q_strides, box,
                           CU_TENSOR_MAP_SWIZZLE_128B) ||
       !make_tensor_map_3d(&maps[3], CU_TENSOR_MAP_DATA_TYPE_UINT16, a.q, q_dims, q_strides, box1,
+                          CU_TENSOR_MAP_SWIZZLE_128B) ||
+      !make_tensor_map_3d(&maps[4], CU_TENSOR_MAP_DATA_TYPE_UINT16, a.q, q_dims, q_strides, box4,
                           CU_TENSOR_MAP_SWIZZLE_128B))
     return NV4_ERR_CUDA;
   a.workers = kPair ? sms : 2 * sms;
   rc = launch_kernel(pt_plan_kernel, dim3(1), dim3(kPtPlanThreads), 0, stream, true, a, kPair ? 2 * a.TB : a.TB);
   if (rc != NV4_OK) return rc;
   rc = launch_kernel(kern, dim3(sms), dim3(kPtThreads), kPtSmem, stream, true, maps[0], maps[1], maps[2], maps[3],
-                     a);
+                     maps[4], a);
   if (rc != NV4_OK) return rc;
   if (a.prefix == nullptr)
     return launch_kernel(pt_join_prompts_kernel<kPair>, dim3(a.workers - 1, kPtJoinSplit), dim3(128), 0, stream, true, a);
@@ -1219,7 +1272,7 @@ static PtArgs pt_args(const void* q, const int* block_tables, const int* context
   a.TB = kPtRows / a.G;
   a.max_pages = static_cast<int>(max_pages);
   a.workers = 0;
-  a.slot_rows = static_cast<int>(pt_slot_rows(tokens, a.G));
+  a.slot_rows = static_cast<int>(prefix ? kPtRows : pt_slot_rows(tokens, a.G));
   a.c = scale * 1.4426950408889634f;
   return a;
 }
