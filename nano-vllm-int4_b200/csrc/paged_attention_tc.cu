@@ -1060,25 +1060,38 @@ struct PtJoin {
     m = top;
   }
   // Pieces `first` .. `last` of a cut block: slot 1 of the first worker, 0 of the others; `of_pair` which of a pair's.
-  template <int kPer>
-  __device__ __forceinline__ void pieces(const PtArgs& p, int first, int last, int of_pair, int row, int j, int parts = 1) {
-    constexpr int kAhead = 4;  // loads in flight: of four workers, or of the four parts of a spread row
-    for (int w0 = first; w0 <= last; w0 += parts == 1 ? kAhead : 1) {
+  // kParts parts of each (of a spread row, 32 rows apart).
+  template <int kPer, int kParts>
+  __device__ __forceinline__ void pieces(const PtArgs& p, int first, int last, int of_pair, int row, int j) {
+    constexpr int kAhead = 4;  // loads in flight
+    for (int w0 = first; w0 <= last; w0 += kAhead / kParts) {
       float2 ml[kAhead];
       float4 v[kAhead];
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
-        const int w = parts == 1 ? w0 + i : w0;
+        const int w = w0 + i / kParts, at = row + 32 * (i % kParts);
         if (w > last) break;
         const int64_t slot = (static_cast<int64_t>(w) * 2 + (w == first)) * kPer + of_pair;
-        const int at = row + (parts == 1 ? 0 : 32 * i);
         ml[i] = *reinterpret_cast<const float2*>(p.w.part_ml + (slot * p.slot_rows + at) * 2);
         v[i] = *(reinterpret_cast<const float4*>(p.w.part) + (slot * 32 + j) * p.slot_rows + at);
       }
 #pragma unroll
       for (int i = 0; i < kAhead; ++i)
-        if (parts != 1 || w0 + i <= last) fold(ml[i], v[i], p.c);
+        if (w0 + i / kParts <= last) fold(ml[i], v[i], p.c);
     }
+  }
+  // kParts parts of a row of a block that is not cut.
+  template <int kParts>
+  __device__ __forceinline__ void uncut(const PtArgs& p, int64_t at, int j) {
+    float2 ml[kParts];
+    float4 v[kParts];
+#pragma unroll
+    for (int i = 0; i < kParts; ++i) {
+      ml[i] = *reinterpret_cast<const float2*>(p.w.row_ml + (at + i) * 2);
+      v[i] = *(reinterpret_cast<const float4*>(p.w.row + (at + i) * kPtRows) + j);
+    }
+#pragma unroll
+    for (int i = 0; i < kParts; ++i) fold(ml[i], v[i], p.c);
   }
   __device__ __forceinline__ void store(uint16_t* row, int j) const {
     const float f = l > 0.0f || l != l ? 1.0f / l : 0.0f;
@@ -1105,57 +1118,82 @@ __global__ void __launch_bounds__(128) pt_join_prompts_kernel(const PtArgs p) {
   for (int r = blockIdx.y * 4 + (threadIdx.x & 3); r < b.ntok * p.G; r += 4 * kPtJoinSplit) {
     const int l = kPair && r >= per;
     PtJoin join;
-    join.pieces<kPair ? 2 : 1>(p, i - 1, last, l, r - l * per, j);
+    join.pieces<kPair ? 2 : 1, 1>(p, i - 1, last, l, r - l * per, j);
     const int t = r / p.G;
     join.store(p.out + (static_cast<int64_t>(b.tok0 + t) * p.Hq + s.head * p.G + r - t * p.G) * kPtRows, j);
   }
 }
 
-// Decode: CTA (request, KV head) joins what the request's own block and its group's left.
-__global__ void __launch_bounds__(128) pt_join_decode_kernel(const PtArgs p) {
+// Decode: CTA (request, KV head) joins what the request's own block and its group's left.  `kWide`: 128 threads as above
+// for each of the four parts of spread rows (a row that is not spread is all in the first), which are joined last: 4
+// requests over 900 tokens 18 us instead of 21.  With more CTAs than fit at once the other way (256 requests: 184 us
+// instead of 190).
+template <bool kWide>
+__global__ void __launch_bounds__(kWide ? 512 : 128, kWide ? 2 : 4) pt_join_decode_kernel(const PtArgs p) {
+  __shared__ float parts[kWide ? 3 : 1][6][128];
   grid_dependency_wait();
   grid_dependents_launch();
-  const int b = blockIdx.x, h = blockIdx.y, j = threadIdx.x >> 2;
+  const int b = blockIdx.x, h = blockIdx.y, part = threadIdx.x >> 7, in_part = threadIdx.x & 127, j = in_part >> 2;
   const PtSums sums = *p.w.sums;
   const int of = p.w.row_block[b];
   const int own = sums.prefix_blocks + b;
-  const PtBlock mine = p.w.blocks[own];
-  PtBlock common{};
-  int64_t own_at = p.w.before[own], common_at = 0;
-  if (of >= 0) common = p.w.blocks[of], common_at = p.w.before[of];
   // the workers of a block: first and last
   auto workers = [&](int64_t before, int tiles, int& first, int& last) {
     const int64_t at = before * p.Hkv + static_cast<int64_t>(h) * pt_cost(tiles);
-    first = static_cast<int>(at / sums.chunk);
-    last = first + static_cast<int>((at - first * sums.chunk + tiles - 1) / sums.chunk);
+    if (sums.total < (int64_t(1) << 30)) {  // (64-bit divisions take long)
+      const uint32_t chunk = static_cast<uint32_t>(sums.chunk), a = static_cast<uint32_t>(at);
+      first = static_cast<int>(a / chunk);
+      last = static_cast<int>((a + tiles - 1) / chunk);
+    } else {
+      first = static_cast<int>(at / sums.chunk);
+      last = static_cast<int>((at + tiles - 1) / sums.chunk);
+    }
   };
   int own_first, own_last, common_first = 0, common_last = 0;
-  workers(own_at, mine.tiles, own_first, own_last);
-  if (of >= 0) workers(common_at, common.tiles, common_first, common_last);
-  for (int g = threadIdx.x & 3; g < p.G; g += 4) {
+  workers(p.w.before[own], p.w.blocks[own].tiles, own_first, own_last);
+  int common_row = 0;
+  bool common_spread = false;
+  if (of >= 0) {
+    const PtBlock common = p.w.blocks[of];
+    workers(p.w.before[of], common.tiles, common_first, common_last);
+    common_row = b - common.tok0;
+    common_spread = pt_spread(p, common.ntok);
+  }
+  for (int g0 = 0; g0 < p.G; g0 += 4) {
+    const int g = min(g0 + (in_part & 3), p.G - 1);
     PtJoin join;
     const int64_t row = static_cast<int64_t>(b) * p.Hq + h * p.G + g;
     auto add = [&](int first, int last, int in, int64_t area, bool spread) {
-      if (first < last) {
-        join.pieces<1>(p, first, last, 0, in, j, spread ? 4 : 1);
-        return;
+      if (part > 0 && !spread) return;
+      const int64_t at = (area * p.batch * p.Hq + row) * 4 + part;
+      if (kWide || !spread) {
+        if (first < last) join.pieces<1, 1>(p, first, last, 0, in + 32 * part, j);
+        else join.uncut<1>(p, at, j);
+      } else {
+        if (first < last) join.pieces<1, 4>(p, first, last, 0, in, j);
+        else join.uncut<4>(p, at, j);
       }
-      const int64_t at = (area * p.batch * p.Hq + row) * 4;
-      float2 ml[4];
-      float4 v[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (i == 0 || spread) {
-          ml[i] = *reinterpret_cast<const float2*>(p.w.row_ml + (at + i) * 2);
-          v[i] = *(reinterpret_cast<const float4*>(p.w.row + (at + i) * kPtRows) + j);
-        }
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (i == 0 || spread) join.fold(ml[i], v[i], p.c);
     };
-    if (of >= 0) add(common_first, common_last, (b - common.tok0) * p.G + g, 1, pt_spread(p, common.ntok));
-    add(own_first, own_last, g, 0, pt_spread(p, 1));
-    join.store(p.out + row * kPtRows, j);
+#pragma unroll 1
+    for (int i = of >= 0 ? 0 : 1; i < 2; ++i)  // in one copy of the code: registers
+      add(i ? own_first : common_first, i ? own_last : common_last, i ? g : common_row * p.G + g, 1 - i,
+          i ? pt_spread(p, 1) : common_spread);
+    if constexpr (kWide) {
+      __syncthreads();
+      if (part > 0) {
+        const float v[6] = {join.m, join.l, join.o.x, join.o.y, join.o.z, join.o.w};
+#pragma unroll
+        for (int i = 0; i < 6; ++i) parts[part - 1][i][in_part] = v[i];
+      }
+      __syncthreads();
+      if (part > 0) continue;
+#pragma unroll
+      for (int i = 0; i < 3; ++i) {
+        const auto v = [&](int k) { return parts[i][k][in_part]; };
+        join.fold(make_float2(v(0), v(1)), make_float4(v(2), v(3), v(4), v(5)), p.c);
+      }
+    }
+    if (g == g0 + (in_part & 3)) join.store(p.out + row * kPtRows, j);
   }
 }
 
@@ -1248,7 +1286,9 @@ static int launch_pt(PtArgs& a, const void* k_cache, const void* v_cache, cudaSt
   if (rc != NV4_OK) return rc;
   if (a.prefix == nullptr)
     return launch_kernel(pt_join_prompts_kernel<kPair>, dim3(a.workers - 1, kPtJoinSplit), dim3(128), 0, stream, true, a);
-  return launch_kernel(pt_join_decode_kernel, dim3(a.batch, a.Hkv), dim3(128), 0, stream, true, a);
+  if (static_cast<int64_t>(a.batch) * a.Hkv <= 2 * sms)
+    return launch_kernel(pt_join_decode_kernel<true>, dim3(a.batch, a.Hkv), dim3(512), 0, stream, true, a);
+  return launch_kernel(pt_join_decode_kernel<false>, dim3(a.batch, a.Hkv), dim3(128), 0, stream, true, a);
 }
 
 static PtArgs pt_args(const void* q, const int* block_tables, const int* context_lens, const int* starts,
