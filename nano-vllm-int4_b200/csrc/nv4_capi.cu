@@ -578,7 +578,8 @@ int nv4_append_kv(const void* q, const void* k, const void* v, const void* q_wei
 namespace {
 // The checks that the two attentions over shared cached tokens have in common.
 int check_paged_attention(const void* q, const void* k_cache, const void* v_cache, const void* block_tables,
-                          const void* context_lens, const void* out, const void* workspace, int64_t workspace_bytes,
+                          const void* context_lens, Span starts, Span prefix, const void* out, const void* workspace,
+                          int64_t workspace_bytes,
                           int64_t wanted, int64_t rows, int64_t batch, int64_t num_heads, int64_t num_kv_heads,
                           int64_t head_dim, int64_t page_size, int64_t num_pages, int64_t max_pages, float scale) {
   if (!q || !k_cache || !v_cache || !block_tables || !context_lens || !out || !workspace)
@@ -598,10 +599,10 @@ int check_paged_attention(const void* q, const void* k_cache, const void* v_cach
     return NV4_ERR_ALIGNMENT;
   // q and the cache are read again after other rows were written
   const int64_t cache = num_pages * 256 * num_kv_heads * 256, row_bytes = rows * num_heads * 256;
-  const Span spans[7] = {{out, row_bytes}, {workspace, wanted}, {q, row_bytes}, {k_cache, cache}, {v_cache, cache},
-                         {block_tables, batch * max_pages * 4}, {context_lens, batch * 4}};
+  const Span spans[9] = {{out, row_bytes}, {workspace, wanted}, {q, row_bytes}, {k_cache, cache}, {v_cache, cache},
+                         {block_tables, batch * max_pages * 4}, {context_lens, batch * 4}, starts, prefix};
   for (int i = 0; i < 2; ++i)
-    for (int j = i + 1; j < 7; ++j)
+    for (int j = i + 1; j < 9; ++j)
       if (overlap(spans[i], spans[j])) return NV4_ERR_INVALID_ARGUMENT;
   return NV4_OK;
 }
@@ -623,8 +624,8 @@ int nv4_paged_prefill_attention(const void* q, const void* k_cache, const void* 
                                 int64_t max_pages, float scale, void* stream) {
   if (!query_starts) return NV4_ERR_INVALID_ARGUMENT;
   const int rc = check_paged_attention(
-      q, k_cache, v_cache, block_tables, context_lens, out, workspace, workspace_bytes,
-      nv4_paged_prefill_attention_workspace_bytes(tokens, batch, num_heads, num_kv_heads), tokens, batch, num_heads,
+      q, k_cache, v_cache, block_tables, context_lens, Span{query_starts, (batch + 1) * 4}, Span{nullptr, 0}, out,
+      workspace, workspace_bytes, nv4_paged_prefill_attention_workspace_bytes(tokens, batch, num_heads, num_kv_heads), tokens, batch, num_heads,
       num_kv_heads, head_dim, page_size, num_pages, max_pages, scale);
   if (rc != NV4_OK) return rc;
   if (!aligned(query_starts, 4)) return NV4_ERR_ALIGNMENT;
@@ -650,7 +651,8 @@ int nv4_shared_prefix_attention(const void* q, const void* k_cache, const void* 
                                 int64_t num_pages, int64_t max_pages, float scale, void* stream) {
   if (groups < 0 || groups > 65535 || (groups > 0 && (!group_starts || !prefix_lens))) return NV4_ERR_INVALID_ARGUMENT;
   const int rc = check_paged_attention(
-      q, k_cache, v_cache, block_tables, context_lens, out, workspace, workspace_bytes,
+      q, k_cache, v_cache, block_tables, context_lens, Span{group_starts, groups > 0 ? (groups + 1) * 4 : 0},
+      Span{prefix_lens, groups * 4}, out, workspace, workspace_bytes,
       nv4_shared_prefix_attention_workspace_bytes(batch, groups, num_heads, num_kv_heads), batch, batch, num_heads,
       num_kv_heads, head_dim, page_size, num_pages, max_pages, scale);
   if (rc != NV4_OK) return rc;

@@ -39,8 +39,8 @@ def append_kv(q, k, v, cos_sin, positions, slot_mapping, k_cache, v_cache, *, q_
 
 
 def prefill_attention_workspace(num_tokens: int, batch: int, num_heads: int, num_kv_heads: int, device) -> torch.Tensor:
-    """Scratch of ``paged_prefill_attention`` for up to so many tokens and requests;
-    calls that may overlap (other streams, graphs) need one each."""
+    """Scratch of ``paged_prefill_attention`` for up to so many tokens and requests (up to
+    43 MB); calls that may overlap (other streams, graphs) need one each."""
     nbytes = _native.paged_prefill_attention_workspace_bytes(num_tokens, batch, num_heads, num_kv_heads)
     return torch.empty(nbytes, dtype=torch.uint8, device=device)
 
@@ -54,15 +54,18 @@ def paged_prefill_attention(q, k_cache, v_cache, block_tables, context_lens, que
     [B, max_pages], ``context_lens`` INT32 [B], ``query_starts`` INT32 [B + 1], not
     falling: rows ``query_starts[b]`` to ``query_starts[b + 1] - 1`` are the last
     tokens of request b's context.  A row that sees no token gets zeros; rows of no
-    request are left as they are.  Returns ``out`` BF16 [T, Hq, 128].
+    request are left as they are.  What the cache holds behind a request's last token
+    may be anything, its own tokens' values must be finite.  Probabilities are rounded to
+    BF16 once.  Returns ``out`` BF16 [T, Hq, 128] (32-byte aligned; over no input).
     """
     return _native.serving().prefill_attention(q, k_cache, v_cache, block_tables, context_lens, query_starts, out,
                                                workspace, scale)
 
 
 def shared_prefix_workspace(batch: int, groups: int, num_heads: int, num_kv_heads: int, device) -> torch.Tensor:
-    """Scratch of ``shared_prefix_attention`` for up to so many requests and groups;
-    calls that may overlap (other streams, graphs) need one each."""
+    """Scratch of ``shared_prefix_attention`` for up to so many requests and groups (43 MB
+    and 4 KB for every request and query head); calls that may overlap (other streams,
+    graphs) need one each."""
     nbytes = _native.shared_prefix_attention_workspace_bytes(batch, groups, num_heads, num_kv_heads)
     return torch.empty(nbytes, dtype=torch.uint8, device=device)
 
@@ -78,7 +81,9 @@ def shared_prefix_attention(q, k_cache, v_cache, block_tables, context_lens, gro
     [groups + 1], not falling, and [groups]); the whole pages of these are read
     through the table of the group's longest request, and the others' tables must
     name the same pages as far as their contexts go.
-    Requests of no group share nothing.  Returns ``out`` BF16 [B, Hq, 128].
+    Requests of no group share nothing.  Probabilities are multiplied in two BF16 terms,
+    so that the output's rounding is the only one that shows.  Returns ``out`` BF16 [B,
+    Hq, 128] (32-byte aligned; over no input).
     """
     return _native.serving().shared_attention(q, k_cache, v_cache, block_tables, context_lens, group_starts,
                                               prefix_lens, out, workspace, scale)
