@@ -137,8 +137,8 @@ __device__ __forceinline__ longlong2 pt_scan(int64_t v, int64_t w, int64_t (&sum
   const int64_t a = pt_warp_scan(lane < kPtPlanWarps ? sums[0][lane] : 0);
   const int64_t b = pt_warp_scan(lane < kPtPlanWarps ? sums[1][lane] : 0);
   all.x = __shfl_sync(0xffffffffu, a, 31), all.y = __shfl_sync(0xffffffffu, b, 31);
-  const int64_t before = __shfl_sync(0xffffffffu, a, max(warp - 1, 0)), before2 = __shfl_sync(0xffffffffu, b, max(warp - 1, 0));
-  return make_longlong2((warp ? before : 0) + x - v, (warp ? before2 : 0) + y - w);
+  const int64_t u = __shfl_sync(0xffffffffu, a, max(warp - 1, 0)), t = __shfl_sync(0xffffffffu, b, max(warp - 1, 0));
+  return make_longlong2((warp ? u : 0) + x - v, (warp ? t : 0) + y - w);
 }
 
 // Running maximum up to this thread, `carry` that of the threads before (updated).
@@ -370,8 +370,8 @@ __host__ __device__ constexpr uint32_t pt_idesc(int m, int n, bool b_mn) {
   return (1u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(b_mn) << 16) |
          (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
 }
-// Shared-memory descriptors, lower words (address and leading offset, in 16 bytes); the upper word is the same for both:
-// eight rows of 128 bytes are an atom of 1024 (stride offset), 128-byte swizzle.  Q and K have their channels
+// Shared-memory descriptors, lower words (address and leading offset, in 16 bytes); the upper word is the same for
+// both: eight rows of 128 bytes are an atom of 1024 (stride offset), 128-byte swizzle.  Q and K have their channels
 // contiguous (K-major; the leading offset counts for nothing), V as the B operand its N dimension: the second 64
 // channels lie a half tile on (leading offset).
 constexpr uint32_t kPtDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
@@ -578,13 +578,15 @@ __global__ void __launch_bounds__(kPtThreads, 1)
 
   // Worker of a lane; in a pair both lanes walk worker blockIdx.x.
   auto worker = [&](int l) { return static_cast<int>(blockIdx.x) + (kPair ? 0 : l * static_cast<int>(gridDim.x)); };
-  // Does lane l have rows of a block of so many tokens?  (A pair's second lane: those of the tokens behind the first TB.)
+  // Does lane l have rows of a block of so many tokens?  (A pair's second lane has those of the tokens behind TB.)
   auto has_rows = [&](int l, int ntok) { return !kPair || l == 0 || ntok > p.TB; };
   // Is a block of so many tokens spread (see above)?
   auto spread_out = [&](int ntok) { return kTerms == 2 && pt_spread(p, ntok); };
   // Tokens by which lane 1's rows lie further on in its tile (solo), where they fit: few rows of both lanes would
   // otherwise be the work of one of the SM's four schedulers.
-  auto shift = [&](int l, int ntok) { return !kPair && l == 1 && !spread_out(ntok) && ntok <= p.TB / 2 ? p.TB / 2 : 0; };
+  auto shift = [&](int l, int ntok) {
+    return !kPair && l == 1 && !spread_out(ntok) && ntok <= p.TB / 2 ? p.TB / 2 : 0;
+  };
   bool ok = true;
 
   if (warp < 4) pt_registers_down();
@@ -659,9 +661,9 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     }
   } else if (warp < 3) {
     // ---------------- products of a lane: S of a tile, O += P V, all by one thread.  A warp for each lane: the tensor
-    // cores take few products ahead, so what one waits for in between is covered by the other's.  Of a pair's lanes one at
-    // a time has its O += P V with the next S: left to themselves they fall into step, both at their exponentials (the
-    // pipe of these then takes 2048 cycles) and both at their products (a tile of both 5200 cycles instead of 4000).
+    // cores take few products ahead, so what one waits for in between is covered by the other's.  Of a pair's lanes one
+    // at a time has its O += P V with the next S: left to themselves they fall into step, both at their exponentials
+    // (the pipe of these then takes 2048 cycles) and both at their products (5200 cycles a tile of both, not 4170).
     if (lane == 0) {
       constexpr uint32_t kQk = pt_idesc(kPtRows, kPtRows, false), kPv = pt_idesc(kPtRows, kPtRows, true);
       const uint32_t q_lo = (smem_u32(smem) >> 4) + kPtDescK, ring_lo = smem_u32(ring) >> 4;
@@ -669,8 +671,8 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       PtSteps w;
       w.start(p, worker(l));
       const uint32_t others = kPair ? 0 : p.w.starts[worker(1 - l)].count;
-      // Ring position of V of the lane's tile i; K of the next is the one behind it.  Solo: both lanes' first K, then in
-      // turn V of a tile and K of the next, while a lane has any.
+      // Ring position of V of the lane's tile i; K of the next is the one behind it.  Solo: both lanes' first K, then
+      // in turn V of a tile and K of the next, while a lane has any.
       auto v_position = [&](uint32_t i) -> uint32_t {
         if (kPair) return 2 * i + 1;
         const uint32_t j = i + l;  // turns that the other lane had
@@ -684,7 +686,9 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         return arrived(bar.full[kPair ? 0 : l][s], phase);
       };
       // K of the walk's tile, in slot s, and with a block's first tile its rows of Q
-      auto ready = [&](uint32_t s, bool rows) { return filled(s) && (!rows || !w.fresh || arrived(bar.q_full[l], parts++)); };
+      auto ready = [&](uint32_t s, bool rows) {
+        return filled(s) && (!rows || !w.fresh || arrived(bar.q_full[l], parts++));
+      };
       // S = Q K^T
       auto scores = [&](uint32_t i, uint32_t s, bool rows) {
         if (!rows) {
@@ -820,8 +824,8 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       }
     }
   } else {
-    // ---------------- softmax and outputs: two threads a row (head r % G of its lane's token r / G), each with half of a
-    // tile's keys, and of the output's channels at the end.  (With one thread a row the two warps of a scheduler left
+    // ---------------- softmax and outputs: two threads a row (head r % G of its lane's token r / G), each with half of
+    // a tile's keys, and of the output's channels at the end.  (With one thread a row the two warps of a scheduler left
     // two thirds of its issue slots empty.)
     pt_registers_up();
     const int l = (warp - 4) >> 3, half = ((warp - 4) >> 2) & 1, quarter = warp & 3, r = quarter * 32 + lane;
@@ -838,7 +842,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     int tile = 0, part = 0, row_in = 0, limit = 0, token = 0, head = 0, from = 0;
     bool live = false, started = false;
     float m = -INFINITY, sum = 0.0f;
-    // A wait that gave up does not end the walk (the two warps of a row meet at barriers): later ones are not waited for.
+    // A wait that gave up does not end the walk (the warps of a row meet at barriers): later ones are not waited for.
     for (; w.left > 0; w.next()) {
       if (!has_rows(l, w.b.ntok)) continue;
       if (w.fresh) {
@@ -852,7 +856,9 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         head = w.head * p.G + row_in - t * p.G;
         limit = 0;
         if (live)
-          limit = w.b.kind == kPtPrompt ? w.b.limit + t0 + t : w.b.kind == kPtOwn ? w.b.limit : __ldg(p.context + token);
+          limit = w.b.kind == kPtPrompt ? w.b.limit + t0 + t
+                  : w.b.kind == kPtOwn  ? w.b.limit
+                                        : __ldg(p.context + token);
         m = -INFINITY, sum = 0.0f;
         started = false;
         from = w.tile;
@@ -911,7 +917,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         const float base = m == -INFINITY ? 0.0f : m;
         const uint64_t base2 = pair(base, base), c2 = pair(c, c);
         uint64_t sums[2] = {0, 0};
-        // The probabilities take columns of their own scores: of 32 keys 16 of the upper terms and 16 of the lower, or 16
+        // The probabilities take columns of their scores: of 32 keys 16, or 16 of the upper and 16 of the lower terms
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           uint32_t hi[16], lo[16];
@@ -969,7 +975,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       // the block's end, or this worker's: outputs
       const bool whole = from == 0 && w.tile + 1 == w.b.tiles;
       const bool final_ = kTerms == 1 && whole;
-      // BF16 rows; or FP32 ones, of a block that is not cut row after row (for the joining kernel), of a cut one with the
+      // BF16 rows; or FP32 ones for the joining kernel, of a block that is not cut row after row, of a cut one with the
       // rows beside each other, 16 bytes each, so that a warp's stores are contiguous
       const int64_t row = static_cast<int64_t>(token) * p.Hq + head;
       uint4* dst;
@@ -1027,7 +1033,8 @@ __global__ void __launch_bounds__(kPtThreads, 1)
             dst += 2;
           } else if (live) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j, dst += stride) *dst = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+            for (int j = 0; j < 4; ++j, dst += stride)
+              *dst = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
           }
           __syncwarp();
         }
@@ -1060,10 +1067,9 @@ struct PtJoin {
     m = top;
   }
   // Pieces `first` .. `last` of a cut block: slot 1 of the first worker, 0 of the others; `of_pair` which of a pair's.
-  // kParts parts of each (of a spread row, 32 rows apart).
-  template <int kPer, int kParts>
+  // kParts parts of each (of a spread row, 32 rows apart); kAhead loads in flight.
+  template <int kPer, int kParts, int kAhead>
   __device__ __forceinline__ void pieces(const PtArgs& p, int first, int last, int of_pair, int row, int j) {
-    constexpr int kAhead = 4;  // loads in flight
     for (int w0 = first; w0 <= last; w0 += kAhead / kParts) {
       float2 ml[kAhead];
       float4 v[kAhead];
@@ -1101,7 +1107,7 @@ struct PtJoin {
   }
 };
 
-constexpr int kPtJoinSplit = 16;  // CTAs that share the rows of a cut block
+constexpr int kPtJoinSplit = 32;  // CTAs that share the rows of a cut block
 
 // Prompts: CTA (i, y) joins the block that worker i + 1 starts within, when it began in worker i.
 template <bool kPair>
@@ -1118,16 +1124,16 @@ __global__ void __launch_bounds__(128) pt_join_prompts_kernel(const PtArgs p) {
   for (int r = blockIdx.y * 4 + (threadIdx.x & 3); r < b.ntok * p.G; r += 4 * kPtJoinSplit) {
     const int l = kPair && r >= per;
     PtJoin join;
-    join.pieces<kPair ? 2 : 1, 1>(p, i - 1, last, l, r - l * per, j);
+    join.pieces<kPair ? 2 : 1, 1, 8>(p, i - 1, last, l, r - l * per, j);
     const int t = r / p.G;
     join.store(p.out + (static_cast<int64_t>(b.tok0 + t) * p.Hq + s.head * p.G + r - t * p.G) * kPtRows, j);
   }
 }
 
-// Decode: CTA (request, KV head) joins what the request's own block and its group's left.  `kWide`: 128 threads as above
-// for each of the four parts of spread rows (a row that is not spread is all in the first), which are joined last: 4
-// requests over 900 tokens 18 us instead of 21.  With more CTAs than fit at once the other way (256 requests: 184 us
-// instead of 190).
+// Decode: CTA (request, KV head) joins what the request's own block and its group's left.  `kWide`: 128 threads as
+// above for each of the four parts of spread rows (a row that is not spread is all in the first), which are joined
+// last: 4 requests over 900 tokens 18 us instead of 21.  With more CTAs than fit at once the other way (256 requests:
+// 184 us instead of 190).
 template <bool kWide>
 __global__ void __launch_bounds__(kWide ? 512 : 128, kWide ? 2 : 4) pt_join_decode_kernel(const PtArgs p) {
   __shared__ float parts[kWide ? 3 : 1][6][128];
@@ -1167,10 +1173,10 @@ __global__ void __launch_bounds__(kWide ? 512 : 128, kWide ? 2 : 4) pt_join_deco
       if (part > 0 && !spread) return;
       const int64_t at = (area * p.batch * p.Hq + row) * 4 + part;
       if (kWide || !spread) {
-        if (first < last) join.pieces<1, 1>(p, first, last, 0, in + 32 * part, j);
+        if (first < last) join.pieces<1, 1, 4>(p, first, last, 0, in + 32 * part, j);
         else join.uncut<1>(p, at, j);
       } else {
-        if (first < last) join.pieces<1, 4>(p, first, last, 0, in, j);
+        if (first < last) join.pieces<1, 4, 4>(p, first, last, 0, in, j);
         else join.uncut<4>(p, at, j);
       }
     };
@@ -1285,7 +1291,8 @@ static int launch_pt(PtArgs& a, const void* k_cache, const void* v_cache, cudaSt
                      maps[4], a);
   if (rc != NV4_OK) return rc;
   if (a.prefix == nullptr)
-    return launch_kernel(pt_join_prompts_kernel<kPair>, dim3(a.workers - 1, kPtJoinSplit), dim3(128), 0, stream, true, a);
+    return launch_kernel(pt_join_prompts_kernel<kPair>, dim3(a.workers - 1, kPtJoinSplit), dim3(128), 0, stream, true,
+                         a);
   if (static_cast<int64_t>(a.batch) * a.Hkv <= 2 * sms)
     return launch_kernel(pt_join_decode_kernel<true>, dim3(a.batch, a.Hkv), dim3(512), 0, stream, true, a);
   return launch_kernel(pt_join_decode_kernel<false>, dim3(a.batch, a.Hkv), dim3(128), 0, stream, true, a);

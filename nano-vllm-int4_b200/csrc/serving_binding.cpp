@@ -1,9 +1,10 @@
 // Python binding of the 4-bit cache, step table, log-probability and shared-token
 // entry points (nanovllm/kernels/{kv4_cache,step_tables,token_logprobs,
-// paged_attention}.py), whose kernels take 3 to 15 us when short: the checks of the arguments, the outputs' allocation and the
-// call itself.  The same through Python and ctypes took 17 to 22 us of host time
-// a call, most of it in new tensors (2.5 us each there, 0.9 us here) and checks;
-// here it is 4 to 8 us in a loop of one call (x.add_(1) takes 4.4), 6 to 12 among others.
+// paged_attention}.py), whose kernels take 3 to 15 us when short: the checks of
+// the arguments, the outputs' allocation and the call itself.  The same through
+// Python and ctypes took 17 to 22 us of host time a call, most of it in new tensors
+// (2.5 us each there, 0.9 us here) and checks; here it is 4 to 8 us in a loop of one
+// call (x.add_(1) takes 4.4), 6 to 12 among others.
 // Every output has storage of its own: parts of one allocation would save 3 us of
 // the step tables' 9, but could not be saved together and would keep one another alive.
 // The calls go to the C ABI of include/nv4.h.
@@ -354,7 +355,8 @@ PyObject* py_append_kv(PyObject*, PyObject* const* a, Py_ssize_t n) {
         k.scalar_type() != at::kBFloat16 || v.scalar_type() != at::kBFloat16)
       refuse("Expected BF16 k and v[T,Hkv,128] with the cache's KV heads");
     const int64_t t = k.size(0);
-    if (q && (q->dim() != 3 || q->size(0) != t || q->size(1) < 1 || q->size(2) != kD || q->scalar_type() != at::kBFloat16))
+    if (q && (q->dim() != 3 || q->size(0) != t || q->size(1) < 1 || q->size(2) != kD ||
+              q->scalar_type() != at::kBFloat16))
       refuse("Expected BF16 q[T,Hq,128]");
     const int64_t hq = q ? q->size(1) : 1;
     for (const at::Tensor* w : {qw, kw})
