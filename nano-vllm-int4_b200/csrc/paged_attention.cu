@@ -1,7 +1,5 @@
-// Operators of requests that share cached tokens, over the paged BF16 cache of
-// attention.cu ([pages, 256, Hkv, 128]): the append that writes it from q, k and
-// v of their own, the attention of prompts over what their requests have cached,
-// and the decode attention of a batch whose requests share a prefix's pages.
+// The append that writes the paged BF16 cache of attention.cu ([pages, 256, Hkv, 128])
+// from q, k and v of their own; paged_attention_tc.cu has the two attentions over it.
 #include "nv4_device.cuh"
 #include "nv4_launch.h"
 
@@ -17,6 +15,10 @@ constexpr int kPaPage = 256;
 // throughout, one rounding to BF16.  The lane of channel c + R/2 is R/16 lanes on.
 // A half warp takes kRows rows of a token: their loads go out first, then the position
 // and slot, then cos and sin, so that two loads in a row are what a warp waits for.
+//
+// A token's heads are read once and written once: bound by that for long prompts (16,384
+// tokens, 32 / 8 heads: 411 MB in 96 us, 4.3 TB/s), by one such chain of loads for a
+// decode batch (32 tokens: 2.2 us).  4 CTAs an SM: 3 and 5 take 110 and 115 us there.
 struct AppendArgs {
   const uint16_t* q;
   const uint16_t* k;
@@ -36,9 +38,10 @@ struct AppendArgs {
 
 constexpr int kAppendThreads = 256;
 
-__device__ __forceinline__ void unpack8(const uint4& r, float (&x)[8]) {
-  x[0] = bf16lo_to_f32(r.x), x[1] = bf16hi_to_f32(r.x), x[2] = bf16lo_to_f32(r.y), x[3] = bf16hi_to_f32(r.y);
-  x[4] = bf16lo_to_f32(r.z), x[5] = bf16hi_to_f32(r.z), x[6] = bf16lo_to_f32(r.w), x[7] = bf16hi_to_f32(r.w);
+// Eight BF16 values as four pairs of FP32.
+__device__ __forceinline__ void unpack8(const uint4& r, uint64_t (&x)[4]) {
+  x[0] = pair(bf16lo_to_f32(r.x), bf16hi_to_f32(r.x)), x[1] = pair(bf16lo_to_f32(r.y), bf16hi_to_f32(r.y));
+  x[2] = pair(bf16lo_to_f32(r.z), bf16hi_to_f32(r.z)), x[3] = pair(bf16lo_to_f32(r.w), bf16hi_to_f32(r.w));
 }
 
 template <int kRows>
@@ -69,17 +72,19 @@ __global__ void __launch_bounds__(kAppendThreads, 4) append_kv_kernel(const Appe
   }
   const bool first = lane < hl, turned = lane < 2 * hl;
   const int partner = (threadIdx.x & 16) + (first ? lane + hl : lane - hl);
-  float c[8], s[8];
+  uint64_t c[4], s[4];  // (a, b) -> (a c + b s): one and zero where nothing is turned, NaN at an unknown position
 #pragma unroll
-  for (int i = 0; i < 8; ++i) c[i] = known ? 1.0f : __int_as_float(0x7FFFFFFF), s[i] = 0.0f;
+  for (int i = 0; i < 4; ++i) {
+    const float one = known ? 1.0f : __int_as_float(0x7FFFFFFF);
+    c[i] = pair(one, one), s[i] = 0;
+  }
   if (turned && known && h0 < p.Hq + p.Hkv) {
-    const float4* row =
-        reinterpret_cast<const float4*>(p.cos_sin + pos * (16 * hl) + (first ? lane : lane - hl) * 8);
-    const float4 c0 = __ldg(row), c1 = __ldg(row + 1), s0 = __ldg(row + 2 * hl), s1 = __ldg(row + 2 * hl + 1);
-    c[0] = c0.x, c[1] = c0.y, c[2] = c0.z, c[3] = c0.w, c[4] = c1.x, c[5] = c1.y, c[6] = c1.z, c[7] = c1.w;
-    s[0] = s0.x, s[1] = s0.y, s[2] = s0.z, s[3] = s0.w, s[4] = s1.x, s[5] = s1.y, s[6] = s1.z, s[7] = s1.w;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) s[i] = first ? -s[i] : s[i];
+    const ulonglong2* row =
+        reinterpret_cast<const ulonglong2*>(p.cos_sin + pos * (16 * hl) + (first ? lane : lane - hl) * 8);
+    const ulonglong2 c0 = __ldg(row), c1 = __ldg(row + 1), s0 = __ldg(row + 2 * hl), s1 = __ldg(row + 2 * hl + 1);
+    c[0] = c0.x, c[1] = c0.y, c[2] = c1.x, c[3] = c1.y;
+    const uint64_t sign = first ? 0x8000000080000000ull : 0;
+    s[0] = s0.x ^ sign, s[1] = s0.y ^ sign, s[2] = s1.x ^ sign, s[3] = s1.y ^ sign;
   }
 #pragma unroll
   for (int j = 0; j < kRows; ++j) {
@@ -87,30 +92,32 @@ __global__ void __launch_bounds__(kAppendThreads, 4) append_kv_kernel(const Appe
     const bool is_q = h < p.Hq, is_v = h >= p.Hq + p.Hkv;
     uint4 out = raw[j];
     if (__any_sync(0xffffffffu, !is_v)) {
-      float x[8];
+      uint64_t x[4];
       unpack8(raw[j], x);
       const uint16_t* weight = is_q ? p.q_weight : p.k_weight;
       if (p.q_weight || p.k_weight) {
-        float ss = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
+        float ss, odd;
+        unpair(fma2(x[3], x[3], fma2(x[2], x[2], fma2(x[1], x[1], mul2(x[0], x[0])))), ss, odd);
+        ss += odd;
 #pragma unroll
         for (int m = 8; m >= 1; m >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
         if (weight) {
           const float r = rsqrtf(ss * (1.0f / kPaD) + p.eps);
-          float w[8];
+          uint64_t w[4];
           unpack8(__ldg(reinterpret_cast<const uint4*>(weight) + lane), w);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] = x[i] * r * w[i];
+          for (int i = 0; i < 4; ++i) x[i] = mul2(mul2(x[i], pair(r, r)), w[i]);
         }
       }
       uint32_t packed[4];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float b = __shfl_sync(0xffffffffu, x[i], partner);
-        const float y = turned ? fmaf(x[i], c[i], b * s[i]) : x[i] * c[i];
-        const uint32_t bits = __bfloat16_as_ushort(__float2bfloat16_rn(y));
-        packed[i / 2] = i % 2 ? packed[i / 2] | bits << 16 : bits;
+      for (int i = 0; i < 4; ++i) {
+        float a, b, u, v;
+        unpair(x[i], a, b);
+        const float pa = __shfl_sync(0xffffffffu, a, partner), pb = __shfl_sync(0xffffffffu, b, partner);
+        unpair(turned ? fma2(x[i], c[i], mul2(pair(pa, pb), s[i])) : mul2(x[i], c[i]), u, v);
+        const __nv_bfloat162 y = __floats2bfloat162_rn(u, v);
+        packed[i] = *reinterpret_cast<const uint32_t*>(&y);
       }
       if (!is_v) out = make_uint4(packed[0], packed[1], packed[2], packed[3]);
     }
@@ -159,10 +166,10 @@ int launch_append_kv(const void* q, const void* k, const void* v, const void* q_
   a.Hkv = static_cast<int>(num_kv_heads);
   a.half_lanes = static_cast<int>(rotary_dim / 16);
   a.eps = eps;
-  // One row a half warp while these fit the SMs twice over (shorter chains), else four (fewer loads of cos and sin).
+  // One row a half warp while there are few (a shorter chain; 32 / 8 heads, 128 tokens: 2.6 us, 3.5 with four), else
+  // four (fewer loads of cos and sin; 301 tokens: 4.2 us, 4.5 with one, 3.9 with two; 2400: 16.1, 24.7, 18.4 us).
   const int64_t rows = tokens * (a.Hq + 2 * num_kv_heads);
-  return rows <= 2 * 148 * 4 * (kAppendThreads / 16) ? launch_append_rows<1>(a, stream)
-                                                     : launch_append_rows<4>(a, stream);
+  return rows <= 8192 ? launch_append_rows<1>(a, stream) : launch_append_rows<4>(a, stream);
 }
 
 }  // namespace nv4
