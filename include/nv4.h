@@ -421,9 +421,9 @@ int nv4_append_kv(const void* q, const void* k, const void* v, const void* q_wei
  *   workspace     nv4_paged_prefill_attention_workspace_bytes(...) bytes of
  *                 scratch; calls that may overlap need one each
  * Rows of no request are left as they are.  out and workspace overlap no input nor
- * one another.  Values of the request's own later
- * tokens (masked, but in the cache) must be finite; what lies behind its last
- * token may be anything.  At most NV4_PAGED_MAX_GROUP query heads per KV head;
+ * one another.  Values of the request's own later tokens (masked, but in the cache)
+ * must be finite, since they meet probabilities of zero; what lies behind its last
+ * token may be anything, and so may masked keys.  At most NV4_PAGED_MAX_GROUP query heads per KV head;
  * (tokens + 2 * batch) * max_pages * num_kv_heads up to 2^36.
  * Statistics and sums in FP32, the probabilities rounded to BF16 once for the
  * product with V.  All pointers 16-byte aligned (out 32, the int32 ones 4).
@@ -450,9 +450,10 @@ int nv4_paged_prefill_attention(const void* q, const void* k_cache, const void* 
  *                 their contexts go), the rest, as all other tokens, through each
  *                 request's own
  *   context_lens  int32 [batch]; 0 (or less) marks a padding row, whose output is zero
- * The probabilities are multiplied in two BF16 terms.  Everything else as
- * nv4_paged_prefill_attention; groups may be 0 (then
- * group_starts and prefix_lens may be NULL).
+ * Values of the pages in common must be finite as far as the longest request goes,
+ * also those behind a shorter one's last token.  The probabilities are multiplied in
+ * two BF16 terms.  Everything else as nv4_paged_prefill_attention; groups may be 0
+ * (then group_starts and prefix_lens may be NULL).
  */
 int64_t nv4_shared_prefix_attention_workspace_bytes(int64_t batch, int64_t groups, int64_t num_heads,
                                                     int64_t num_kv_heads);

@@ -535,7 +535,8 @@ int nv4_append_kv(const void* q, const void* k, const void* v, const void* q_wei
                   void* k_cache, void* v_cache, int64_t tokens, int64_t num_heads, int64_t num_kv_heads,
                   int64_t head_dim, int64_t q_stride, int64_t k_stride, int64_t v_stride, int64_t rotary_dim,
                   int64_t page_size, int64_t num_pages, int64_t max_position, float eps, void* stream) {
-  if (!k || !v || !cos_sin || !positions || !slot_mapping || !k_cache || !v_cache || (q != nullptr) != (q_out != nullptr))
+  if (!k || !v || !cos_sin || !positions || !slot_mapping || !k_cache || !v_cache ||
+      (q != nullptr) != (q_out != nullptr))
     return NV4_ERR_INVALID_ARGUMENT;
   if (tokens < 1 || tokens > (int64_t(1) << 30) || num_heads < 1 || num_heads > 65535 || num_kv_heads < 1 ||
       num_kv_heads > 65535 || num_pages < 1 || num_pages > (int64_t(1) << 23) - 1 || max_position < 1 ||
@@ -579,9 +580,9 @@ namespace {
 // The checks that the two attentions over shared cached tokens have in common.
 int check_paged_attention(const void* q, const void* k_cache, const void* v_cache, const void* block_tables,
                           const void* context_lens, Span starts, Span prefix, const void* out, const void* workspace,
-                          int64_t workspace_bytes,
-                          int64_t wanted, int64_t rows, int64_t batch, int64_t num_heads, int64_t num_kv_heads,
-                          int64_t head_dim, int64_t page_size, int64_t num_pages, int64_t max_pages, float scale) {
+                          int64_t workspace_bytes, int64_t wanted, int64_t rows, int64_t batch, int64_t num_heads,
+                          int64_t num_kv_heads, int64_t head_dim, int64_t page_size, int64_t num_pages,
+                          int64_t max_pages, float scale) {
   if (!q || !k_cache || !v_cache || !block_tables || !context_lens || !out || !workspace)
     return NV4_ERR_INVALID_ARGUMENT;
   if (rows < 1 || rows > NV4_PAGED_MAX_TOKENS || batch < 1 || batch > 65535 || num_kv_heads < 1 ||
@@ -625,8 +626,8 @@ int nv4_paged_prefill_attention(const void* q, const void* k_cache, const void* 
   if (!query_starts) return NV4_ERR_INVALID_ARGUMENT;
   const int rc = check_paged_attention(
       q, k_cache, v_cache, block_tables, context_lens, Span{query_starts, (batch + 1) * 4}, Span{nullptr, 0}, out,
-      workspace, workspace_bytes, nv4_paged_prefill_attention_workspace_bytes(tokens, batch, num_heads, num_kv_heads), tokens, batch, num_heads,
-      num_kv_heads, head_dim, page_size, num_pages, max_pages, scale);
+      workspace, workspace_bytes, nv4_paged_prefill_attention_workspace_bytes(tokens, batch, num_heads, num_kv_heads),
+      tokens, batch, num_heads, num_kv_heads, head_dim, page_size, num_pages, max_pages, scale);
   if (rc != NV4_OK) return rc;
   if (!aligned(query_starts, 4)) return NV4_ERR_ALIGNMENT;
   if (!device_is_sm100()) return NV4_ERR_DEVICE;

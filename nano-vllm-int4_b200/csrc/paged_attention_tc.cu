@@ -108,6 +108,7 @@ struct PtArgs {
   PtScratch w;
   int64_t num_pages;
   int tokens, batch, groups, Hq, Hkv, G, TB, max_pages, workers, slot_rows;
+  int block_cost;  // a block counts for its tiles and so many more, for its beginning and end
   float c;  // scale * log2(e)
 };
 
@@ -158,9 +159,7 @@ __device__ __forceinline__ int pt_max_scan(int v, int (&maxima)[kPtPlanWarps], i
 }
 
 __device__ __forceinline__ int pt_tiles(int keys) { return max(1, (keys + kPtRows - 1) / kPtRows); }
-// A block counts for its tiles and as much as one more for its beginning and end (its outputs, mostly).
-constexpr int kPtBlockCost = 1;
-__device__ __forceinline__ int pt_cost(int tiles) { return tiles + kPtBlockCost; }
+__device__ __forceinline__ int pt_cost(const PtArgs& p, int tiles) { return tiles + p.block_cost; }
 // A decode block of up to 32 rows is spread: its rows stand four times in the tile.
 __device__ __forceinline__ bool pt_spread(const PtArgs& p, int ntok) { return ntok <= p.TB / 4; }
 
@@ -199,7 +198,7 @@ __global__ void __launch_bounds__(kPtPlanThreads) pt_plan_kernel(const PtArgs p,
         const int n = last[s] - first[s], ctx = extra[s], end = min(ctx, most);
         int64_t sum = 0;
         for (int j = lane; j * block_tokens < n; j += 32)
-          sum += pt_cost(pt_tiles(min(ctx - n + min(n, (j + 1) * block_tokens), end)));
+          sum += pt_cost(p, pt_tiles(min(ctx - n + min(n, (j + 1) * block_tokens), end)));
 #pragma unroll
         for (int m = 16; m >= 1; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
         if (lane == 0) weight[s] = sum;
@@ -221,7 +220,7 @@ __global__ void __launch_bounds__(kPtPlanThreads) pt_plan_kernel(const PtArgs p,
           const int j = j0 + lane, i0 = j * block_tokens;
           const int count = min(n - i0, block_tokens);
           const int tiles = count > 0 ? pt_tiles(min(ctx - n + i0 + count, end)) : 0;
-          const int cost = count > 0 ? pt_cost(tiles) : 0;
+          const int cost = count > 0 ? pt_cost(p, tiles) : 0;
           const int64_t x = pt_warp_scan(cost);
           if (count > 0)
             put(which[s] + j, before + x - cost,
@@ -268,7 +267,7 @@ __global__ void __launch_bounds__(kPtPlanThreads) pt_plan_kernel(const PtArgs p,
       const int shared = extra[tid], row = static_cast<int>(weight[tid]);
       const int mine = live && shared > 0 ? (last[tid] - first[tid] + p.TB - 1) / p.TB : 0;
       longlong2 all;
-      const longlong2 before = pt_scan(static_cast<int64_t>(mine) * pt_cost(shared / kPtRows), mine, sums, all);
+      const longlong2 before = pt_scan(static_cast<int64_t>(mine) * pt_cost(p, shared / kPtRows), mine, sums, all);
       which[tid] = blocks + static_cast<int>(before.y);
       weight[tid] = tiles_before + before.x;  // (the scan waited for all to have read it)
       tiles_before += all.x;
@@ -279,7 +278,7 @@ __global__ void __launch_bounds__(kPtPlanThreads) pt_plan_kernel(const PtArgs p,
         if (extra[s] <= 0) continue;
         const int n = last[s] - first[s], tiles = extra[s] / kPtRows;
         for (int j = lane; j * p.TB < n; j += 32)
-          put(which[s] + j, weight[s] + static_cast<int64_t>(j) * pt_cost(tiles),
+          put(which[s] + j, weight[s] + static_cast<int64_t>(j) * pt_cost(p, tiles),
               PtBlock{table_row[s], first[s] + j * p.TB, min(p.TB, n - j * p.TB), tiles, 0, 0, extra[s], kPtPrefix});
         for (int r = lane; r < n; r += 32) p.w.row_block[first[s] + r] = which[s] + r / p.TB;
       }
@@ -297,7 +296,7 @@ __global__ void __launch_bounds__(kPtPlanThreads) pt_plan_kernel(const PtArgs p,
         tiles = pt_tiles(end - shared);
       }
       longlong2 all;
-      const longlong2 before = pt_scan(live ? pt_cost(tiles) : 0, 0, sums, all);
+      const longlong2 before = pt_scan(live ? pt_cost(p, tiles) : 0, 0, sums, all);
       if (live) put(blocks + b, tiles_before + before.x, PtBlock{b, b, 1, tiles, shared, end, end, kPtOwn});
       tiles_before += all.x;
     }
@@ -336,22 +335,22 @@ __global__ void __launch_bounds__(kPtPlanThreads) pt_plan_kernel(const PtArgs p,
         else hi = mid - 1;
       }
       const int64_t into = at - p.w.before[lo] * p.Hkv;
-      cost = pt_cost(p.w.blocks[lo].tiles);
+      cost = pt_cost(p, p.w.blocks[lo].tiles);
       s.head = static_cast<int>(into / cost);
       s.tile = static_cast<int>(into % cost);
     }
     s.block = lo;
-    const int tiles = cost - kPtBlockCost;
+    const int tiles = cost - p.block_cost;
     // tiles before the border: what lies before it less the costs of the blocks begun (and ended) there
     const int64_t begun = static_cast<int64_t>(lo) * p.Hkv + s.head;
-    const int64_t real = at - begun * kPtBlockCost - max(s.tile - tiles, 0);
+    const int64_t real = at - begun * p.block_cost - max(s.tile - tiles, 0);
     if (s.tile >= tiles) {  // in the block's cost: the next one begins
       s.tile = 0;
       if (++s.head == p.Hkv) s.head = 0, ++s.block;
     }
     return real;
   };
-  const int64_t end = total - static_cast<int64_t>(blocks) * p.Hkv * kPtBlockCost;  // tiles of all
+  const int64_t end = total - static_cast<int64_t>(blocks) * p.Hkv * p.block_cost;  // tiles of all
   static_assert(2 * kPtMaxCtas <= kPtPlanThreads, "a thread for every worker");
   __syncthreads();  // weight is free
   PtStart s{0, 0, 0, 0};
@@ -789,9 +788,9 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           if (w[l].left <= 0 || (copied[l] > 0 && !pt_passed(&bar.q_free[l], (copied[l] - 1) & 1))) continue;
           const bool one = w[l].b.kind == kPtOwn, spread = spread_out(w[l].b.ntok);
           const CUtensorMap* map = one ? &tmap_q1 : spread ? &tmap_q4 : &tmap_q;
-          const int ahead = shift(l, w[l].b.ntok), copies = spread ? 4 : 1;
-          const int token = w[l].b.tok0 + (kPair ? l * p.TB : 0) - (one ? 0 : ahead);
-          uint8_t* dst = smem + l * kPtTile + (one ? ahead * p.G * 128 : 0);
+          const int copies = spread ? 4 : 1;  // (an own block is spread: one token, up to 16 rows)
+          const int token = w[l].b.tok0 + (kPair ? l * p.TB : 0) - shift(l, w[l].b.ntok);
+          uint8_t* dst = smem + l * kPtTile;
           mbar_arrive_expect_tx(&bar.q_full[l], copies * (one ? 1 : spread ? p.TB / 4 : p.TB) * p.G * kPtRows * 2);
           for (int i = 0; i < copies; ++i, dst += 32 * 128) {
             pt_load_q(dst, map, &bar.q_full[l], 0, w[l].head * p.G, token);
@@ -1145,7 +1144,7 @@ __global__ void __launch_bounds__(kWide ? 512 : 128, kWide ? 2 : 4) pt_join_deco
   const int own = sums.prefix_blocks + b;
   // the workers of a block: first and last
   auto workers = [&](int64_t before, int tiles, int& first, int& last) {
-    const int64_t at = before * p.Hkv + static_cast<int64_t>(h) * pt_cost(tiles);
+    const int64_t at = before * p.Hkv + static_cast<int64_t>(h) * pt_cost(p, tiles);
     if (sums.total < (int64_t(1) << 30)) {  // (64-bit divisions take long)
       const uint32_t chunk = static_cast<uint32_t>(sums.chunk), a = static_cast<uint32_t>(at);
       first = static_cast<int>(a / chunk);
@@ -1319,6 +1318,9 @@ static PtArgs pt_args(const void* q, const int* block_tables, const int* context
   a.TB = kPtRows / a.G;
   a.max_pages = static_cast<int>(max_pages);
   a.workers = 0;
+  // Prompts' blocks (4 x 4096: 662 us, 730 with none and 665 with two); a decode block's beginning is covered by the
+  // other lane's products (256 over 2k: 174 us, 181 with one and 186 with two).
+  a.block_cost = prefix ? 0 : 1;
   a.slot_rows = static_cast<int>(prefix ? kPtRows : pt_slot_rows(tokens, a.G));
   a.c = scale * 1.4426950408889634f;
   return a;
@@ -1331,8 +1333,11 @@ int launch_paged_prefill_attention(const void* q, const void* k_cache, const voi
   const PtLayout l = pt_prefill_layout(static_cast<char*>(workspace), tokens, batch, num_heads, num_kv_heads);
   PtArgs a = pt_args(q, block_tables, context_lens, query_starts, nullptr, out, l.w, tokens, batch, 0, num_heads,
                      num_kv_heads, num_pages, max_pages, scale);
-  // Two blocks of rows side by side when the requests have more than one block's rows on average.
-  if (tokens > batch * a.TB) return launch_pt<true, 1>(a, k_cache, v_cache, stream);
+  // Two blocks of rows side by side when the requests have more than one block's rows on average (32 / 8 heads, 64
+  // requests of 64 tokens over 2000: 206 us, 256 otherwise), or when there are few blocks, which make fewer pieces
+  // then (one of 32 over 3000: 19.3 us, 25.6 otherwise, over 30,000 46 and 50; but 4 of 32 over 20,000: 89 us, 80
+  // otherwise).
+  if (tokens > batch * a.TB || batch * num_kv_heads <= 16) return launch_pt<true, 1>(a, k_cache, v_cache, stream);
   return launch_pt<false, 1>(a, k_cache, v_cache, stream);
 }
 

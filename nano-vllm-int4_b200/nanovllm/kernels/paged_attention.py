@@ -1,5 +1,5 @@
 """Operators of requests that share cached tokens, over the paged BF16 cache
-(csrc/paged_attention.cu): the append that writes it, the attention of prompts over
+(csrc/paged_attention.cu, csrc/paged_attention_tc.cu): the append that writes it, the attention of prompts over
 what their requests have cached already, and the decode attention of a batch whose
 requests share a prefix.  (The reference calls flash-attn over its block tables,
 nanovllm/layers/attention.py:59-75, which reads a shared prefix once per request.)
@@ -80,10 +80,11 @@ def shared_prefix_attention(q, k_cache, v_cache, block_tables, context_lens, gro
     to ``group_starts[g + 1] - 1`` have ``prefix_lens[g]`` tokens in common (INT32
     [groups + 1], not falling, and [groups]); the whole pages of these are read
     through the table of the group's longest request, and the others' tables must
-    name the same pages as far as their contexts go.
-    Requests of no group share nothing.  Probabilities are multiplied in two BF16 terms,
-    so that the output's rounding is the only one that shows.  Returns ``out`` BF16 [B,
-    Hq, 128] (32-byte aligned; over no input).
+    name the same pages as far as their contexts go (and the values there must be finite,
+    also those behind a shorter request's last token).  Requests of no group share
+    nothing.  Probabilities are multiplied in two BF16 terms, so that the output's
+    rounding is the only one that shows.  Returns ``out`` BF16 [B, Hq, 128] (32-byte
+    aligned; over no input).
     """
     return _native.serving().shared_attention(q, k_cache, v_cache, block_tables, context_lens, group_starts,
                                               prefix_lens, out, workspace, scale)

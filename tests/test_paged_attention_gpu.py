@@ -202,6 +202,22 @@ def test_prefill_larger(cuda_device, lens, hq, hkv):
     close_prompt(run_prefill(*case), *ref.prefill(*case, SCALE)[:2])
 
 
+@pytest.mark.parametrize("hq,hkv", [(32, 8), (5, 1), (16, 1), (9, 3), (2, 2)])
+@pytest.mark.parametrize("new,cached", [(1, 0), (3, 700), (6, 250), (8, 3000)])
+def test_prefill_many_requests_with_few_new_tokens(cuda_device, new, cached, hq, hkv):
+    """Up to one block of rows each, ragged, with requests that have none, and NaN behind the last ones."""
+    lens = [(max(0, cached - 37 * i) + 128 * (i % 3), (new + i) % (new + 2)) for i in range(21)]
+    q, k_cache, v_cache, tables, context, starts = prefill_case(lens, hq, hkv, cuda_device, seed=new)
+    live = torch.zeros(k_cache.shape[:2], dtype=torch.bool, device=cuda_device)
+    for t, n in zip(tables, context):
+        for i in range(-(-n // PAGE)):
+            live[t[i], :min(PAGE, n - i * PAGE)] = True
+    want, size, _ = ref.prefill(q, k_cache, v_cache, tables, context, starts, SCALE)
+    k_cache[~live] = v_cache[~live] = float("nan")
+    close_prompt(run_prefill(q, k_cache, v_cache, tables, context, starts), want, size)
+    assert _native.device_error() == 0
+
+
 def test_prefill_ignores_what_lies_behind_the_last_token(cuda_device):
     """NaN and infinities behind the context (in its last page, in pages of no request)."""
     lens, dev = [(130, 7), (0, 300), (255, 1), (256, 9)], cuda_device
