@@ -9,16 +9,18 @@ constexpr int kPaD = 128;
 constexpr int kPaPage = 256;
 
 // ------------------------------------------------------------ append
-// Sixteen lanes per row (one head of one token), eight channels (16 bytes) a lane.
+// Sixteen lanes per row (one head of one token), eight channels a lane: of the first R four
+// and those R/2 on, which are rotated with them, so that no lane needs another's; of the
+// rest eight in a row.
 // With y = x * rsqrt(mean(x^2) + eps) * w (or x without a norm), channels c and c +
 // R/2 of the first R are rotated, (a, b) -> (a cos - b sin, b cos + a sin); FP32
-// throughout, one rounding to BF16.  The lane of channel c + R/2 is R/16 lanes on.
+// throughout, one rounding to BF16.
 // A half warp takes kRows rows of a token: their loads go out first, then the position
 // and slot, then cos and sin, so that two loads in a row are what a warp waits for.
 //
-// A token's heads are read once and written once: bound by that for long prompts (16,384
-// tokens, 32 / 8 heads: 411 MB in 96 us, 4.3 TB/s), by one such chain of loads for a
-// decode batch (32 tokens: 2.2 us).  4 CTAs an SM: 3 and 5 take 110 and 115 us there.
+// A token's heads are read once and written once: bound by that and by the instructions for
+// long prompts (16,384 tokens, 32 / 8 heads: 411 MB in 84 us, 4.9 TB/s), by one such chain of
+// loads for a decode batch (32 tokens: 2.1 us).  5 CTAs an SM: 4 take 92 us there, 6 104 us.
 struct AppendArgs {
   const uint16_t* q;
   const uint16_t* k;
@@ -38,14 +40,20 @@ struct AppendArgs {
 
 constexpr int kAppendThreads = 256;
 
-// Eight BF16 values as four pairs of FP32.
-__device__ __forceinline__ void unpack8(const uint4& r, uint64_t (&x)[4]) {
-  x[0] = pair(bf16lo_to_f32(r.x), bf16hi_to_f32(r.x)), x[1] = pair(bf16lo_to_f32(r.y), bf16hi_to_f32(r.y));
-  x[2] = pair(bf16lo_to_f32(r.z), bf16hi_to_f32(r.z)), x[3] = pair(bf16lo_to_f32(r.w), bf16hi_to_f32(r.w));
+// Two times four BF16 values as pairs of FP32.
+__device__ __forceinline__ void unpack8(const uint2& a, const uint2& b, uint64_t (&x)[4]) {
+  x[0] = pair(bf16lo_to_f32(a.x), bf16hi_to_f32(a.x)), x[1] = pair(bf16lo_to_f32(a.y), bf16hi_to_f32(a.y));
+  x[2] = pair(bf16lo_to_f32(b.x), bf16hi_to_f32(b.x)), x[3] = pair(bf16lo_to_f32(b.y), bf16hi_to_f32(b.y));
+}
+__device__ __forceinline__ uint32_t pack2(uint64_t x) {
+  float a, b;
+  unpair(x, a, b);
+  const __nv_bfloat162 y = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&y);
 }
 
 template <int kRows>
-__global__ void __launch_bounds__(kAppendThreads, 4) append_kv_kernel(const AppendArgs p) {
+__global__ void __launch_bounds__(kAppendThreads, 5) append_kv_kernel(const AppendArgs p) {
   const int lane = threadIdx.x & 15;
   const int heads = p.Hq + 2 * p.Hkv, hl = p.half_lanes;
   const uint32_t groups = (heads + kRows - 1) / kRows;
@@ -54,14 +62,17 @@ __global__ void __launch_bounds__(kAppendThreads, 4) append_kv_kernel(const Appe
   const bool live = unit < p.tokens * groups;
   const int64_t t = live ? unit / groups : p.tokens - 1;
   const int h0 = static_cast<int>(live ? unit - t * groups : 0) * kRows;
-  uint4 raw[kRows];
+  const bool turned = lane < 2 * hl;
+  const int at = (turned ? 4 : 8) * lane, at2 = at + (turned ? 8 * hl : 4);  // channels
+  uint2 raw[kRows], raw2[kRows];
 #pragma unroll
   for (int j = 0; j < kRows; ++j) {
     const int h = min(h0 + j, heads - 1);
     const uint16_t* src = h < p.Hq           ? p.q + t * p.q_stride + h * kPaD
                           : h < p.Hq + p.Hkv ? p.k + t * p.k_stride + (h - p.Hq) * kPaD
                                              : p.v + t * p.v_stride + (h - p.Hq - p.Hkv) * kPaD;
-    raw[j] = *(reinterpret_cast<const uint4*>(src) + lane);
+    raw[j] = *reinterpret_cast<const uint2*>(src + at);
+    raw2[j] = *reinterpret_cast<const uint2*>(src + at2);
   }
   const int64_t pos = p.positions[t];
   const int64_t slot = p.slots[t];
@@ -70,30 +81,24 @@ __global__ void __launch_bounds__(kAppendThreads, 4) append_kv_kernel(const Appe
     if (!known) record_index_error(kErrBadPosition);
     if (slot >= p.num_slots) record_index_error(kErrBadSlot);
   }
-  const bool first = lane < hl, turned = lane < 2 * hl;
-  const int partner = (threadIdx.x & 16) + (first ? lane + hl : lane - hl);
-  uint64_t c[4], s[4];  // (a, b) -> (a c + b s): one and zero where nothing is turned, NaN at an unknown position
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float one = known ? 1.0f : __int_as_float(0x7FFFFFFF);
-    c[i] = pair(one, one), s[i] = 0;
-  }
+  // (a, b) -> (a c - b s, b c + a s); an unknown position makes all of it NaN
+  uint64_t c[2], s[2] = {0, 0};
+  const float one = known ? 1.0f : __int_as_float(0x7FFFFFFF);
+  c[0] = c[1] = pair(one, one);
   if (turned && known && h0 < p.Hq + p.Hkv) {
-    const ulonglong2* row =
-        reinterpret_cast<const ulonglong2*>(p.cos_sin + pos * (16 * hl) + (first ? lane : lane - hl) * 8);
-    const ulonglong2 c0 = __ldg(row), c1 = __ldg(row + 1), s0 = __ldg(row + 2 * hl), s1 = __ldg(row + 2 * hl + 1);
-    c[0] = c0.x, c[1] = c0.y, c[2] = c1.x, c[3] = c1.y;
-    const uint64_t sign = first ? 0x8000000080000000ull : 0;
-    s[0] = s0.x ^ sign, s[1] = s0.y ^ sign, s[2] = s1.x ^ sign, s[3] = s1.y ^ sign;
+    const float* row = p.cos_sin + pos * (16 * hl) + at;
+    const ulonglong2 cs = __ldg(reinterpret_cast<const ulonglong2*>(row));
+    const ulonglong2 sn = __ldg(reinterpret_cast<const ulonglong2*>(row + 8 * hl));
+    c[0] = cs.x, c[1] = cs.y, s[0] = sn.x, s[1] = sn.y;
   }
 #pragma unroll
   for (int j = 0; j < kRows; ++j) {
     const int h = h0 + j;
     const bool is_q = h < p.Hq, is_v = h >= p.Hq + p.Hkv;
-    uint4 out = raw[j];
+    uint2 out = raw[j], out2 = raw2[j];
     if (__any_sync(0xffffffffu, !is_v)) {
       uint64_t x[4];
-      unpack8(raw[j], x);
+      unpack8(raw[j], raw2[j], x);
       const uint16_t* weight = is_q ? p.q_weight : p.k_weight;
       if (p.q_weight || p.k_weight) {
         float ss, odd;
@@ -104,30 +109,33 @@ __global__ void __launch_bounds__(kAppendThreads, 4) append_kv_kernel(const Appe
         if (weight) {
           const float r = rsqrtf(ss * (1.0f / kPaD) + p.eps);
           uint64_t w[4];
-          unpack8(__ldg(reinterpret_cast<const uint4*>(weight) + lane), w);
+          unpack8(__ldg(reinterpret_cast<const uint2*>(weight + at)),
+                  __ldg(reinterpret_cast<const uint2*>(weight + at2)), w);
 #pragma unroll
           for (int i = 0; i < 4; ++i) x[i] = mul2(mul2(x[i], pair(r, r)), w[i]);
         }
       }
-      uint32_t packed[4];
+      if (turned) {
+        constexpr uint64_t kSigns = 0x8000000080000000ull;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float a, b, u, v;
-        unpair(x[i], a, b);
-        const float pa = __shfl_sync(0xffffffffu, a, partner), pb = __shfl_sync(0xffffffffu, b, partner);
-        unpair(turned ? fma2(x[i], c[i], mul2(pair(pa, pb), s[i])) : mul2(x[i], c[i]), u, v);
-        const __nv_bfloat162 y = __floats2bfloat162_rn(u, v);
-        packed[i] = *reinterpret_cast<const uint32_t*>(&y);
+        for (int i = 0; i < 2; ++i) {
+          const uint64_t a = x[i], b = x[i + 2];
+          x[i] = fma2(a, c[i], mul2(b, s[i] ^ kSigns));
+          x[i + 2] = fma2(b, c[i], mul2(a, s[i]));
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = mul2(x[i], c[0]);
       }
-      if (!is_v) out = make_uint4(packed[0], packed[1], packed[2], packed[3]);
+      if (!is_v) out = make_uint2(pack2(x[0]), pack2(x[1])), out2 = make_uint2(pack2(x[2]), pack2(x[3]));
     }
     if (!live || h >= heads) continue;
-    if (is_q) {
-      *(reinterpret_cast<uint4*>(p.q_out + (t * p.Hq + h) * kPaD) + lane) = out;
-    } else if (store) {
-      const int kh = h - p.Hq - (is_v ? p.Hkv : 0);
-      *(reinterpret_cast<uint4*>((is_v ? p.v_cache : p.k_cache) + (slot * p.Hkv + kh) * kPaD) + lane) = out;
-    }
+    uint16_t* dst = nullptr;
+    if (is_q) dst = p.q_out + (t * p.Hq + h) * kPaD;
+    else if (store) dst = (is_v ? p.v_cache : p.k_cache) + (slot * p.Hkv + (h - p.Hq - (is_v ? p.Hkv : 0))) * kPaD;
+    if (!dst) continue;
+    *reinterpret_cast<uint2*>(dst + at) = out;
+    *reinterpret_cast<uint2*>(dst + at2) = out2;
   }
 }
 
@@ -166,10 +174,11 @@ int launch_append_kv(const void* q, const void* k, const void* v, const void* q_
   a.Hkv = static_cast<int>(num_kv_heads);
   a.half_lanes = static_cast<int>(rotary_dim / 16);
   a.eps = eps;
-  // One row a half warp while there are few (a shorter chain; 32 / 8 heads, 128 tokens: 2.6 us, 3.5 with four), else
-  // four (fewer loads of cos and sin; 301 tokens: 4.2 us, 4.5 with one, 3.9 with two; 2400: 16.1, 24.7, 18.4 us).
+  // One row a half warp while there are few (a shorter chain; 32 / 8 heads, 128 tokens: 2.4 us, 3.5 with four), else
+  // four (fewer loads of cos and sin; 301 tokens: 4.1 us, 3.9 with one; 600: 5.5 and 5.6; 16384: 84 and 135, 101 with
+  // two).
   const int64_t rows = tokens * (a.Hq + 2 * num_kv_heads);
-  return rows <= 8192 ? launch_append_rows<1>(a, stream) : launch_append_rows<4>(a, stream);
+  return rows <= 16384 ? launch_append_rows<1>(a, stream) : launch_append_rows<4>(a, stream);
 }
 
 }  // namespace nv4
