@@ -569,6 +569,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     }
     mbar_init(&bar.done, 2);
     bar.lock = 0;
+    for (int i = 0; i < 2; ++i) bar.lane_keys[i] = 0, bar.lane_v[i] = 0;
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -849,6 +850,8 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     bool live = false, started = false;
     float m = -INFINITY, sum = 0.0f;
     // A wait that gave up does not end the walk (the warps of a row meet at barriers): later ones are not waited for.
+    // From there on lane_keys may be of another tile, and differ between the warps of a row: which barriers a warp
+    // meets follows from the walk alone, and V is touched by warps whose waits all ended well.
     for (; w.left > 0; w.next()) {
       if (!has_rows(l, w.b.ntok)) continue;
       if (w.fresh) {
@@ -872,7 +875,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       const bool busy = __any_sync(0xffffffffu, live);
       ok = ok && __all_sync(0xffffffffu, mbar_wait(&bar.s_full[l], tile & 1, kErrTimeoutMma));
       tc_fence_after();
-      const int keys = *reinterpret_cast<volatile int*>(&bar.lane_keys[l]);
+      const int keys = __shfl_sync(0xffffffffu, *reinterpret_cast<volatile int*>(&bar.lane_keys[l]), 0);
       if (spread && !works) {  // keys that are not this quarter's
         if (keys > 0) {
           uint32_t zero[16];
@@ -882,7 +885,9 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           pt_tmem_st16(at + 16, zero);
           tmem_wait_st();
         }
-      } else if (busy && keys > 0) {
+      } else if (busy && keys <= 0) {  // no page, or a request without tokens
+        named_barrier_sync(pairing, paired);
+      } else if (busy) {
         const int seen = min(max(limit - (w.b.key0 + w.tile * kPtRows), 0), keys);
         const bool edge = __any_sync(0xffffffffu, live && seen < kPtRows);  // other rows may come to anything
         uint32_t s[64];
@@ -967,7 +972,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         const uint32_t v = *reinterpret_cast<volatile uint32_t*>(&bar.lane_v[l]);
         ok = ok && __all_sync(0xffffffffu, mbar_wait(&bar.full[kPair ? 0 : l][v >> 1], v & 1, kErrTimeoutFull));
         const int e = (half * 4 + quarter) * 32 + lane, row = keys + (e >> 4);
-        if (row < ((keys + 15) & ~15))
+        if (ok && row < ((keys + 15) & ~15))
           *reinterpret_cast<uint4*>(ring + (v >> 1) * kPtTile + (e & 8 ? kPtHalf : 0) + row * 128 + (e & 7) * 16) =
               make_uint4(0, 0, 0, 0);
         fence_proxy_async_smem();
