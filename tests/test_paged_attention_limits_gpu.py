@@ -3,8 +3,9 @@ does not go: waits that give up, and the sizes at which the kernels take other b
 import pytest
 import torch
 
+import paged_reference as ref
 from nanovllm import _native
-from test_paged_attention_gpu import PAGE, prefill_case, run_prefill, run_shared, shared_case
+from test_paged_attention_gpu import PAGE, SCALE, prefill_case, run_prefill, run_shared, shared_case
 
 pytestmark = pytest.mark.gpu
 
@@ -50,3 +51,34 @@ def test_a_wait_that_gave_up_ends_the_call(cuda_device, name):
             _native.peer_buffer_free(b, cuda_device)
     assert all(torch.equal(call(*c), w) for c, w in zip(cases, want))
     assert _native.device_error() == 6
+
+
+# ------------------------------------------------------------------ many requests and heads
+def check_shared(case):
+    out = run_shared(*case)
+    ref.assert_attention_close(out, *ref.decode(*case[:5], SCALE))
+    assert _native.device_error() == 0
+
+
+RAGGED = [(1000, [5, 90, 3, 700]), (700, [1 + 7 * i for i in range(40)]), (2000, [4, 4]), (100, [3, 600, 2]),
+          (256, [1 + 3 * i % 50 for i in range(70)]), (3000, [10, 300, 20])]
+
+
+@pytest.mark.parametrize("hq,hkv,copies", [(32, 8, 1), (8, 8, 1), (48, 3, 1), (10, 2, 2)])
+def test_shared_join_of_many_rows(cuda_device, hq, hkv, copies):
+    """More (request, KV head) pairs than are joined by 512 threads each: groups of at most a quarter of a block's
+    rows and larger ones, cut and whole blocks, padding, requests of no group."""
+    case = shared_case(RAGGED * copies, hq, hkv, cuda_device, seed=hq, before=3, after=6)
+    assert len(case[4]) * hkv > 2 * 160
+    for b in (0, 9, 20, len(case[4]) - 1):
+        case[4][b] = 0
+    check_shared(case)
+
+
+@pytest.mark.parametrize("hq,hkv", [(32, 8), (48, 3)])
+def test_shared_join_of_many_rows_in_whole_blocks(cuda_device, hq, hkv):
+    """Blocks of a tile or two: most are not cut."""
+    case = shared_case([(256, [1 + (i + j) % 40 for i in range(2 + j % 5)]) for j in range(30)], hq, hkv, cuda_device)
+    assert len(case[4]) * hkv > 2 * 160
+    check_shared(case)
+
