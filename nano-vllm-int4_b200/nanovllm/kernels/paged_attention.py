@@ -40,7 +40,8 @@ def append_kv(q, k, v, cos_sin, positions, slot_mapping, k_cache, v_cache, *, q_
 
 def prefill_attention_workspace(num_tokens: int, batch: int, num_heads: int, num_kv_heads: int, device) -> torch.Tensor:
     """Scratch of ``paged_prefill_attention`` for up to so many tokens and requests (up to
-    43 MB); calls that may overlap (other streams, graphs) need one each."""
+    43 MB, and 40 bytes for every request and every block of up to 128 query rows of a KV
+    head); calls that may overlap (other streams, graphs) need one each."""
     nbytes = _native.paged_prefill_attention_workspace_bytes(num_tokens, batch, num_heads, num_kv_heads)
     return torch.empty(nbytes, dtype=torch.uint8, device=device)
 
@@ -63,9 +64,9 @@ def paged_prefill_attention(q, k_cache, v_cache, block_tables, context_lens, que
 
 
 def shared_prefix_workspace(batch: int, groups: int, num_heads: int, num_kv_heads: int, device) -> torch.Tensor:
-    """Scratch of ``shared_prefix_attention`` for up to so many requests and groups (43 MB
-    and 4 KB for every request and query head); calls that may overlap (other streams,
-    graphs) need one each."""
+    """Scratch of ``shared_prefix_attention`` for up to so many requests and groups (43 MB,
+    4160 bytes for every request and query head, and less than 100 for every request and
+    group); calls that may overlap (other streams, graphs) need one each."""
     nbytes = _native.shared_prefix_attention_workspace_bytes(batch, groups, num_heads, num_kv_heads)
     return torch.empty(nbytes, dtype=torch.uint8, device=device)
 
