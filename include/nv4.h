@@ -391,8 +391,8 @@ int nv4_paged_decode_attention_kv4(const void* q, const void* k_codes, const voi
  *   q, k, v    bf16 [tokens, heads, 128], a token's heads contiguous, tokens
  *              *_stride elements apart (a multiple of 8); q NULL with q_out NULL
  *   q_weight, k_weight  bf16 [128] or NULL (no norm of that side)
- *   cos_sin    float32 [max_position, rotary_dim]: cos in the first half, sin in
- *              the second; channels c and c + rotary_dim / 2 of the first
+ *   cos_sin    float32 [max_position, rotary_dim], up to 2^48 positions: cos in the
+ *              first half, sin in the second; channels c and c + rotary_dim / 2 of the first
  *              rotary_dim (a multiple of 16 up to 128) are rotated
  *   positions  int64 [tokens]; one outside [0, max_position) makes q and k NaN and
  *              records error 8 (nv4_device_error)

@@ -540,7 +540,7 @@ int nv4_append_kv(const void* q, const void* k, const void* v, const void* q_wei
     return NV4_ERR_INVALID_ARGUMENT;
   if (tokens < 1 || tokens > (int64_t(1) << 30) || num_heads < 1 || num_heads > 65535 || num_kv_heads < 1 ||
       num_kv_heads > 65535 || num_pages < 1 || num_pages > (int64_t(1) << 23) - 1 || max_position < 1 ||
-      !(eps >= 0.0f) || !(eps < 1.0f))
+      max_position > int64_t(1) << 48 /* its bytes are counted in 64 bits */ || !(eps >= 0.0f) || !(eps < 1.0f))
     return NV4_ERR_INVALID_ARGUMENT;
   if (head_dim != 128 || page_size != 256 || rotary_dim < 16 || rotary_dim > 128 || rotary_dim % 16)
     return NV4_ERR_UNSUPPORTED;
