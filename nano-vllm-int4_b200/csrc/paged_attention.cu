@@ -19,8 +19,9 @@ constexpr int kPaPage = 256;
 // and slot, then cos and sin, so that two loads in a row are what a warp waits for.
 //
 // A token's heads are read once and written once: bound by that and by the instructions for
-// long prompts (16,384 tokens, 32 / 8 heads: 411 MB in 84 us, 4.9 TB/s), by one such chain of
-// loads for a decode batch (32 tokens: 2.1 us).  5 CTAs an SM: 4 take 92 us there, 6 104 us.
+// long prompts (16,384 tokens, 32 / 8 heads: 411 MB in 84 us, 4.9 TB/s, 0.75 instructions a
+// cycle and scheduler), by one such chain of loads for a decode batch (32 tokens: 2.1 us).
+// 5 CTAs an SM: 4 take 92 us there, 6 104 us.
 struct AppendArgs {
   const uint16_t* q;
   const uint16_t* k;
@@ -174,9 +175,12 @@ int launch_append_kv(const void* q, const void* k, const void* v, const void* q_
   a.Hkv = static_cast<int>(num_kv_heads);
   a.half_lanes = static_cast<int>(rotary_dim / 16);
   a.eps = eps;
-  // One row a half warp while there are few (a shorter chain; 32 / 8 heads, 128 tokens: 2.4 us, 3.5 with four), else
-  // four (fewer loads of cos and sin; 301 tokens: 4.1 us, 3.9 with one; 600: 5.5 and 5.6; 16384: 84 and 135, 101 with
-  // two).
+  // One row a half warp while there are few (a shorter chain), else four (fewer loads of cos and sin).  Timed in graphs
+  // with 32 / 8, 40 / 8, 64 / 8, 16 / 2, 8 / 1 and 5 / 1 heads; us with one and with four rows, 32 / 8 heads, norm and
+  // 128 channels turned: 6144 rows 2.4 and 3.5, 14,448 (301 tokens) 3.9 and 4.1, 16,384 4.15 both, 20,480 4.4 and 4.6,
+  // 28,800 5.6 and 5.4, 786,432 135 and 85 (101 with two).  Without a norm, 64 turned, four are ahead from 14,448 on
+  // (3.6 and 3.3); with 8 / 1 or 5 / 1 heads, whose last four are not all there, the two draw level at about 57,600
+  // (20,480: 4.5 and 5.0).
   const int64_t rows = tokens * (a.Hq + 2 * num_kv_heads);
   return rows <= 16384 ? launch_append_rows<1>(a, stream) : launch_append_rows<4>(a, stream);
 }

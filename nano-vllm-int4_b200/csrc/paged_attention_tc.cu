@@ -43,12 +43,14 @@
 // under the power limit by their energy: there P is rounded to BF16 once (0.0023 of the
 // norm; the sum of a row is that of the values before), which
 // saves a third of the products.  m is moved (and O rescaled) only when a score exceeds
-// it by 2^8, so O is rarely touched.
+// it by 2^8, so O is rarely touched.  (Two tiles of queries that take turns, and the
+// accumulator rescaled past a slack only, are published methods of attention for these
+// tensor cores.)
 //
-// Measured (32 / 8 heads, the three launches): 4 prompts of 4096 tokens 665 us, 824 TFLOP/s
-// (334 us at the rate of a large product); 2048 over 14,336 cached 583 us; 37 over 3100
-// 22 us.  Decode of 12 groups of 8 over up to 16,384 shared tokens 143 us, 4.2 TB/s (92 us
-// at the copy rate; the attention alone 111); 256 requests over 2000 176 us; 4 over 900
+// Measured (32 / 8 heads, the three launches): 4 prompts of 4096 tokens 656 us, 838 TFLOP/s
+// (334 us at the rate of a large product); 2048 over 14,336 cached 573 us; 37 over 3100
+// 22 us.  Decode of 12 groups of 8 over up to 16,384 shared tokens 135 us, 4.5 TB/s (92 us
+// at the copy rate; the attention alone 111); 256 requests over 2000 168 us; 4 over 900
 // 18 us, which is the three launches' latency.
 #include "nv4_device.cuh"
 #include "nv4_launch.h"
@@ -124,8 +126,8 @@ struct PtArgs {
 constexpr int kPtPlanThreads = 512;
 constexpr int kPtPlanWarps = kPtPlanThreads / 32;
 constexpr int kPtPlanCached = 2048;  // blocks whose sums are kept in shared memory for the search
-// Costs of all blocks below it are divided in 32 bits: 256 requests over 2000 take 151 us, 152.5 with divisions in 64 (4
-// over 900 17.3 and 17.7); what costs more takes milliseconds.
+// Costs of all blocks below it are divided in 32 bits: in a graph 256 requests over 2000 take 151 us, 152.5 with
+// divisions in 64 (4 over 900 17.3 and 17.7); what costs more takes milliseconds.
 constexpr int64_t kPtNarrow = 1 << 20;
 
 __device__ __forceinline__ int64_t pt_warp_scan(int64_t x) {
@@ -673,7 +675,8 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     // ---------------- products of a lane: S of a tile, O += P V, all by one thread.  A warp for each lane: the tensor
     // cores take few products ahead, so what one waits for in between is covered by the other's.  Of a pair's lanes one
     // at a time has its O += P V with the next S: left to themselves they fall into step, both at their exponentials
-    // (the pipe of these then takes 2048 cycles) and both at their products (5200 cycles a tile of both, not 4170).
+    // (the pipe of these then takes 2048 cycles) and both at their products (2048 over 14,336: 511 us in a graph, 613
+    // without the lock; 4 x 4096 630 and 691, 8 ragged prompts 165 and 197).
     if (lane == 0) {
       constexpr uint32_t kQk = pt_idesc(kPtRows, kPtRows, false), kPv = pt_idesc(kPtRows, kPtRows, true);
       const uint32_t q_lo = (smem_u32(smem) >> 4) + kPtDescK, ring_lo = smem_u32(ring) >> 4;
@@ -1348,10 +1351,15 @@ int launch_paged_prefill_attention(const void* q, const void* k_cache, const voi
   const PtLayout l = pt_prefill_layout(static_cast<char*>(workspace), tokens, batch, num_heads, num_kv_heads);
   PtArgs a = pt_args(q, block_tables, context_lens, query_starts, nullptr, out, l.w, tokens, batch, 0, num_heads,
                      num_kv_heads, num_pages, max_pages, scale);
-  // Two blocks of rows side by side when the requests have more than one block's rows on average (32 / 8 heads, 64
-  // requests of 64 tokens over 2000: 206 us, 256 otherwise), or when there are few blocks, which make fewer pieces
-  // then (one of 32 over 3000: 19.3 us, 25.6 otherwise, over 30,000 46 and 50; but 4 of 32 over 20,000: 89 us, 80
-  // otherwise).
+  // Two blocks of rows side by side when the requests have more than one block's rows on average, or when there are few
+  // blocks, which make fewer pieces then.  Both forms timed in graphs at 4 / 1 to 64 / 8 heads (us, side by side and
+  // not):
+  //   33 tokens over 20,000, 4 requests of 32 / 8 heads 98 and 124, 32 of 4 / 1 heads 100 and 126; over 500 20 and 25;
+  //   single tokens of as many requests as make 16 blocks, over 500, 3000, 20,000 tokens: 15 and 19, 19 and 22, 52 and
+  //   45, of 32 blocks 17 and 20, 25 and 25, 87 and 69, with 1, 2 and 8 KV heads alike: it goes by the blocks, and by
+  //   the contexts, which the host does not know;
+  //   a prompt of 2048 among 31 single tokens over 2000: 192 and 202 with 32 / 8 heads, 46 and 53 with 4 / 1; where the
+  //   average misleads (700 among 63 over 3000, 16 / 1 heads) 50 and 43.
   if (tokens > batch * a.TB || batch * num_kv_heads <= 16) return launch_pt<true, 1>(a, k_cache, v_cache, stream);
   return launch_pt<false, 1>(a, k_cache, v_cache, stream);
 }

@@ -86,6 +86,9 @@ def shared_prefix_attention(q, k_cache, v_cache, block_tables, context_lens, gro
     nothing.  Probabilities are multiplied in two BF16 terms, so that the output's
     rounding is the only one that shows.  Returns ``out`` BF16 [B, Hq, 128] (32-byte
     aligned; over no input).
+
+    It pays from about 16 requests over 900 common tokens, 8 over 4096 and 4 over 16,384;
+    smaller groups are faster row by row (``_native.paged_decode_attention``).
     """
     return _native.serving().shared_attention(q, k_cache, v_cache, block_tables, context_lens, group_starts,
                                               prefix_lens, out, workspace, scale)
